@@ -22,9 +22,7 @@ Tuning &tuning() {
     return t;
 }
 
-namespace {
-
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
 int fail(int code, const char *fmt, ...) {
     char buf[512];
@@ -45,6 +43,8 @@ int hip_status(hipError_t e, const char *what) {
     if (e != hipSuccess) return fail(KR_E_HIP, "%s: %s", what, hipGetErrorString(e));
     return ok();
 }
+
+namespace {
 
 bool aligned(const void *p, size_t a) { return ((uintptr_t)p % a) == 0; }
 

@@ -10,6 +10,11 @@
 
 namespace kr {
 
+// The C ABI's status: a message for kr_last_error() and the code back (kr_api.hip).
+int fail(int code, const char *fmt, ...);
+int ok();
+int hip_status(hipError_t e, const char *what);
+
 // Epilogues of the m == 1 GEMV.
 enum GemvEpilogue : int {
     kStoreF32 = 0,
@@ -312,5 +317,78 @@ hipError_t launch_gemv_tokens(const Q4Mat &a, const Q4Mat *b, const uint16_t *x,
                               int epilogue, int act, const uint16_t *bias, hipStream_t s);
 hipError_t launch_gemv(const Q4Mat &a, const Q4Mat *b, const uint16_t *x, void *out, int epilogue,
                        int activation, const uint16_t *bias, hipStream_t s);
+
+// ---- rotary positions (rope.hip)
+constexpr uint32_t kRopeMaxDim = 256;       // of a table
+constexpr uint32_t kRopeMaxHeadDim = 1024;
+struct RopeTurns {
+    double turns[kRopeMaxDim / 2];  // frequencies in turns a position
+};
+struct RopeArgs {  // rotary_dim even, rows of the table 8-byte aligned
+    const float *cos_sin;           // [rows, rotary_dim / 2, 2]
+    const uint32_t *positions;
+    uint32_t rows, rotary_dim;
+    int interleaved, inverse;
+};
+// Whether heads of D elements at 16-byte aligned rows can be turned 8 dims a load.
+inline bool rope_units_ok(const RopeArgs &a, uint32_t D) {
+    return a.rotary_dim % 16 == 0 && D % 8 == 0 && (uintptr_t)a.cos_sin % 16 == 0;
+}
+hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, uint32_t count, float gain,
+                             float *cos_sin, hipStream_t s);
+hipError_t launch_rope_apply(const RopeArgs &a, const void *x, size_t xs, void *y, size_t ys, int f32, uint32_t tokens,
+                             uint32_t heads, uint32_t D, hipStream_t s);
+
+// ---- 8-bit key/value cache (kv8_cache.hip, kv8_attention.hip; layout in include/kriya_kv8.h)
+constexpr uint32_t kKv8Block = 32;
+struct Kv8 {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    uint16_t *ko, *vo;
+    uint32_t batch, heads, D, max_ctx, blocks;
+    int e4m3;
+};
+struct Kv8Step {             // the new tokens of a step
+    const uint32_t *starts;  // [batch + 1], nullptr: one token each
+    const uint32_t *lengths; // [batch]
+    uint32_t batch, tokens;
+};
+struct Kv8AppendArgs {
+    Kv8 c;
+    Kv8Step step;
+    RopeArgs rope;           // cos_sin == nullptr: none
+    int rope_units;          // the rotation in 8-dim units (rope_units_ok)
+    const uint16_t *k, *v, *q;
+    uint16_t *q_out;
+    size_t kv_stride, q_stride;
+    uint32_t q_heads;
+};
+hipError_t launch_kv8_append(const Kv8AppendArgs &a, hipStream_t s);
+hipError_t launch_kv8_dequant(const Kv8 &c, const uint32_t *lengths, const uint32_t *first, uint32_t count, void *k_out,
+                              void *v_out, int f32, hipStream_t s);
+struct Kv8AttnArgs {
+    Kv8 c;
+    Kv8Step step;
+    const uint16_t *q;
+    size_t q_stride;
+    uint32_t q_heads, group;
+    float scale_log2;        // softmax scale times log2 e
+    uint16_t *out;
+    float *lse;              // may be nullptr (attention); in (weights)
+    float *part;             // workspace
+    float decay, *weight;    // weights
+};
+size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens);
+hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s);
+hipError_t launch_kv8_weight(const Kv8AttnArgs &a, hipStream_t s);
+struct Kv8EvictArgs {
+    Kv8 from, to;
+    const uint32_t *lengths;
+    const float *weight;
+    uint32_t budget, sink, recent;
+    float *to_weight;
+    uint32_t *kept, *to_lengths;
+};
+hipError_t launch_kv8_evict(const Kv8EvictArgs &a, hipStream_t s);
 
 }  // namespace kr

@@ -1,0 +1,35 @@
+"""Checks of tensors, and the device and stream that a call on them runs on."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+_here = contextlib.nullcontext()
+
+
+def at(t: torch.Tensor):
+    """The device of t made current for a call (nothing to do where it is)."""
+    return _here if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor, stream):
+    """The raw stream of a call: the given one, else the current one of t's device."""
+    if stream is None:
+        return torch.cuda.current_stream(t.device).cuda_stream
+    return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+
+
+def checked(name: str, t: torch.Tensor, dtype, shape=None, like=None) -> torch.Tensor:
+    """t, after a check of its type, its shape (where one is given), its contiguity and its device."""
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, strides are {t.stride()}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on the GPU")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {like.device}")
+    return t

@@ -178,6 +178,273 @@ __global__ __launch_bounds__(256) void kv8_attention_kernel(Kv8AttnArgs a, uint3
         }
 }
 
+// ---- few rows: the context split over workgroups
+//
+// A workgroup takes one tile of 16 query rows and one part of the sequence's blocks, its four waves every fourth block of
+// the part; each wave keeps its own m, l and O, and they are joined in LDS. With more than one part the normalised
+// O_s and (m_s, l_s) go to the workspace and kv8_join_kernel joins the parts in order:
+//   out = sum_s 2^(m_s - M) l_s O_s / L,   L = sum_s 2^(m_s - M) l_s
+// On v_mfma_f32_16x16x32_f16: lane (column l & 15, g = l >> 4) holds slots 16 t + 4 g + j after the first product, and
+// needs of dim d the slots 16 s + 4 g + j for the second, eight bytes of v's order (h = g & 1, a = g >> 1).
+constexpr uint32_t kFewRows = 16, kFewWaves = 4;
+
+struct FewPart {
+    uint32_t first, end, parts;  // blocks of this part; parts in use
+};
+// Blocks of part `part` of `most` parts: all parts in use but the last have the same number, at least one a wave.
+__device__ __forceinline__ FewPart few_part(uint32_t blocks, uint32_t most, uint32_t part) {
+    const uint32_t per = max((blocks + most - 1) / most, kFewWaves);
+    return FewPart{min(part * per, blocks), min((part + 1) * per, blocks), (blocks + per - 1) / per};
+}
+
+template <int NS>
+__device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, const uint16_t *row, bool live, float scale_log2) {
+    const uint32_t lane = __lane_id(), g = lane >> 4;
+    u32x4 raw[NS];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        raw[i] = u32x4{0, 0, 0, 0};
+        // steps 2 j, 2 j + 1 cover 64 dims, 16 a lane; the last of an odd number 32, 8 a lane
+        const uint32_t d = (NS & 1) && i == NS - 1 ? 32 * i + 8 * g : 64 * (i / 2) + 16 * g + 8 * (i & 1);
+        if (live) raw[i] = *reinterpret_cast<const u32x4 *>(row + d);
+        top = max(top, bf16_unit_max_bits(raw[i]));
+    }
+    top = max(top, (uint32_t)__float_as_uint(xchg32(__uint_as_float(top), lane)));
+    top = max(top, (uint32_t)__float_as_uint(xchg16(__uint_as_float(top), lane)));
+    const int e = row_stage_exp(top, 14, 14, 14);
+    const float up = exp2_int(e);
+    c = scale_log2 * exp2_int(-e);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const uint32_t W[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            f[i][2 * x] = (_Float16)(__uint_as_float(W[x] << 16) * up);
+            f[i][2 * x + 1] = (_Float16)(__uint_as_float(W[x] & 0xFFFF0000u) * up);
+        }
+    }
+}
+
+// The bytes of one block as a wave's lanes take them.
+template <int NS>
+struct FewBlock {
+    u32x4 k[2][NS / 2 > 0 ? NS / 2 : 1];  // [half of the slots][64 dims]
+    u32x2 ke[2];                          // the last 32 dims of an odd number
+    u32x2 v[2 * NS];                      // [16 dims]
+    float ks, vs;
+};
+template <int NS>
+__device__ __forceinline__ void load_few(FewBlock<NS> &f, const uint8_t *k, const uint8_t *v, const float *ks, const float *vs,
+                                         uint32_t blk) {
+    const uint32_t lane = __lane_id(), r = lane & 15, g = lane >> 4;
+    k += (size_t)blk * (1024 * NS);
+    v += (size_t)blk * (1024 * NS);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int j = 0; j < NS / 2; ++j)
+            f.k[t][j] = *reinterpret_cast<const u32x4 *>(k + 512 * (4 * j + g) + 16 * (16 * t + r));
+        if constexpr (NS & 1)
+            f.ke[t] = *reinterpret_cast<const u32x2 *>(k + 512 * (2 * (NS - 1) + g / 2) + 16 * (16 * t + r) + 8 * (g & 1));
+    }
+#pragma unroll
+    for (int d = 0; d < 2 * NS; ++d)
+        f.v[d] = *reinterpret_cast<const u32x2 *>(v + 1024 * (d / 2) + 512 * (g & 1) + 16 * (16 * (d & 1) + r) + 8 * (g >> 1));
+    f.ks = ks[blk];
+    f.vs = vs[blk];
+}
+
+template <int NS, int E4M3>
+__global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t parts) {
+    constexpr uint32_t D = 32 * NS;
+    __shared__ float sm[kFewWaves][kFewRows], sl[kFewWaves][kFewRows];
+    __shared__ float so[kFewWaves][kFewRows][D + 4];
+    const uint32_t lane = __lane_id(), r16 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const uint32_t head = blockIdx.y, item = blockIdx.x / parts, part = blockIdx.x % parts;
+    uint32_t b, tile;
+    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kFewRows - 1) / kFewRows; }, b, tile)) return;
+    const Kv8Span s = kv8_span(a.step, b);
+    const uint32_t rows = s.m * a.group, r = kFewRows * tile + r16;
+    const bool live = r < rows;
+    const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
+    const uint32_t most = row_limit(s, min(kFewRows * tile + kFewRows, rows) - 1, a.group, a.c.max_ctx);
+    const uint32_t least = row_limit(s, kFewRows * tile, a.group, a.c.max_ctx);
+    const FewPart w = few_part((most + 31) / 32, parts, part);
+    if (part > 0 && part >= w.parts) return;
+    const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
+    f16x8_t q[NS];
+    float qc;
+    load_query16<NS>(q, qc, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
+    const size_t bh = (size_t)b * a.c.heads + head;
+    const uint8_t *k = a.c.k + bh * a.c.blocks * (size_t)(32 * D), *v = a.c.v + bh * a.c.blocks * (size_t)(32 * D);
+    const float *ks = a.c.ks + bh * a.c.blocks, *vs = a.c.vs + bh * a.c.blocks;
+    f32x4 o[2 * NS];
+#pragma unroll
+    for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f, vref = 0.0f;
+    uint32_t blk = w.first + wave;
+    FewBlock<NS> f;
+    if (blk < w.end) load_few<NS>(f, k, v, ks, vs, blk);
+    for (; blk < w.end; blk += kFewWaves) {
+        f32x4 p[2] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) {
+                p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.k[h][j].x, f.k[h][j].y), q[2 * j], p[h], 0, 0, 0);
+                p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.k[h][j].z, f.k[h][j].w), q[2 * j + 1], p[h], 0, 0, 0);
+            }
+            if constexpr (NS & 1)
+                p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.ke[h].x, f.ke[h].y), q[NS - 1], p[h], 0, 0, 0);
+        }
+        f16x8_t vf[2 * NS];
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) vf[d] = kv8_operand<E4M3>(f.v[d].x, f.v[d].y);
+        const float c = qc * f.ks, vscale = f.vs;
+        if (blk + kFewWaves < w.end) load_few<NS>(f, k, v, ks, vs, blk + kFewWaves);
+        const bool edge = blk * 32 + 32 > least;
+        const uint32_t room = limit > blk * 32 ? limit - blk * 32 : 0u;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float x = p[i >> 2][i & 3] * c;
+            if (edge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = -INFINITY;
+            p[i >> 2][i & 3] = x;
+            top = fmaxf(top, x);
+        }
+        top = fmaxf(top, xchg32(top, lane));
+        top = fmaxf(top, xchg16(top, lane));
+        const float m1 = fmaxf(m, top);
+        const float base = m1 == -INFINITY ? 0.0f : m1;
+        float down = __builtin_amdgcn_exp2f(m - base);
+        m = m1;
+        l *= down;
+        if (vscale > vref && vscale < INFINITY) {
+            down *= vref / vscale;
+            vref = vscale;
+        }
+        const float vrel = vref > 0.0f ? vscale / vref : (vscale == 0.0f ? 0.0f : vscale);
+        f16x8_t pf;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(p[i >> 2][i & 3] - base);
+            l += e;
+            float x = e * vrel;
+            if (edge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = 0.0f;
+            pf[i] = (_Float16)x;
+        }
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] *= down;
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf, o[d], 0, 0, 0);
+        }
+    }
+    l += xchg32(l, lane);
+    l += xchg16(l, lane);
+    const float norm = l == 0.0f ? 0.0f : vref / l;
+    if (g == 0) {
+        sm[wave][r16] = m;
+        sl[wave][r16] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < 2 * NS; ++d)
+        *reinterpret_cast<f32x4 *>(&so[wave][r16][16 * d + 4 * g]) = o[d] * norm;
+    __syncthreads();
+    // four dims of a row a thread
+    for (uint32_t i = threadIdx.x; i < kFewRows * (D / 4); i += 256) {
+        const uint32_t row = i / (D / 4), d = i % (D / 4) * 4, rr = kFewRows * tile + row;
+        if (rr >= rows) continue;
+        float M = sm[0][row], L = 0.0f;
+#pragma unroll
+        for (uint32_t x = 1; x < kFewWaves; ++x) M = fmaxf(M, sm[x][row]);
+        f32x4 acc = {0, 0, 0, 0};
+        bool nan = false;
+#pragma unroll
+        for (uint32_t x = 0; x < kFewWaves; ++x) {
+            const float lx = sl[x][row];
+            nan |= lx != lx;
+            if (lx > 0.0f) {  // a wave that saw no slot has nothing to add
+                const float wx = lx * __builtin_amdgcn_exp2f(sm[x][row] - M);
+                L += wx;
+                acc += wx * *reinterpret_cast<const f32x4 *>(&so[x][row][d]);
+            }
+        }
+        if (nan) L = __builtin_nanf("");
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        acc *= inv;
+        if (parts == 1) {
+            const uint32_t tt = s.t0 + rr / a.group, hh = head * a.group + rr % a.group;
+            const size_t at = (size_t)tt * a.q_heads + hh;
+            const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
+            *reinterpret_cast<u32x2 *>(a.out + at * D + d) = y;
+            if (a.lse && d == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
+        } else {
+            const size_t at = (((size_t)item * a.c.heads + head) * parts + part) * kFewRows + row;
+            *reinterpret_cast<f32x4 *>(a.part + at * D + d) = acc;
+            if (d == 0) {
+                float *ml = a.part + (size_t)gridDim.x * a.c.heads * kFewRows * D + 2 * at;
+                ml[0] = M;
+                ml[1] = L;
+            }
+        }
+    }
+}
+
+// A workgroup per query row: thread (i, j) adds up parts i, i + n, ... of four dims, then the n sums are joined.
+template <int NS>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts) {
+    constexpr uint32_t D = 32 * NS, kQuads = D / 4, kWays = 256 / kQuads;
+    __shared__ float red[4], wl[512];
+    __shared__ f32x4 so[kWays][kQuads];
+    const uint32_t head = blockIdx.y, item = blockIdx.x / kFewRows, row = blockIdx.x % kFewRows;
+    uint32_t b, tile;
+    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kFewRows - 1) / kFewRows; }, b, tile)) return;
+    const Kv8Span s = kv8_span(a.step, b);
+    const uint32_t rows = s.m * a.group, r = kFewRows * tile + row;
+    if (r >= rows) return;
+    const uint32_t most = row_limit(s, min(kFewRows * tile + kFewRows, rows) - 1, a.group, a.c.max_ctx);
+    const uint32_t used = max(few_part((most + 31) / 32, parts, 0).parts, 1u);
+    const size_t at = ((size_t)item * a.c.heads + head) * parts * kFewRows + row;  // part p: at + p kFewRows
+    const float *ml = a.part + (size_t)items * parts * a.c.heads * kFewRows * D;
+    // weights of the parts, relative to the largest m
+    const uint32_t tid = threadIdx.x;
+    float mx = -INFINITY;
+    for (uint32_t p = tid; p < used; p += 256) mx = fmaxf(mx, ml[2 * (at + (size_t)p * kFewRows)]);
+    mx = wave_max(mx);
+    if ((tid & 63) == 0) red[tid >> 6] = mx;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    for (uint32_t p = tid; p < used; p += 256) {
+        const float *x = ml + 2 * (at + (size_t)p * kFewRows);
+        const float lx = x[1];
+        wl[p] = lx == 0.0f ? 0.0f : lx * __builtin_amdgcn_exp2f(x[0] - M);  // NaN stays
+    }
+    __syncthreads();
+    float L = 0.0f;
+    for (uint32_t p = 0; p < used; ++p) L += wl[p];
+    const uint32_t way = tid / kQuads, quad = tid % kQuads;
+    if (way < kWays) {
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+        for (uint32_t p = way; p < used; p += kWays)
+            acc += wl[p] * *reinterpret_cast<const f32x4 *>(a.part + (at + (size_t)p * kFewRows) * D + 4 * quad);
+        so[way][quad] = acc;
+    }
+    __syncthreads();
+    if (tid < kQuads) {
+        f32x4 acc = so[0][tid];
+#pragma unroll
+        for (uint32_t i = 1; i < kWays; ++i) acc += so[i][tid];
+        acc *= L == 0.0f ? 0.0f : 1.0f / L;
+        const size_t to = (size_t)(s.t0 + r / a.group) * a.q_heads + head * a.group + r % a.group;
+        const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
+        *reinterpret_cast<u32x2 *>(a.out + to * D + 4 * tid) = y;
+        if (a.lse && tid == 0) a.lse[to] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
+    }
+}
+
 // A wave per block of 32 slots of one sequence and kv head: its keys stay in registers, the query rows that see it
 // pass by in tiles of 32, and lane (column, h) adds up its own rows' probabilities of slots 8 i + 4 h + j; the 32
 // columns are summed at the end.
@@ -229,8 +496,27 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a) {
     }
 }
 
+namespace {
+
+// Whether a step has few query rows a sequence: then the context is split, a tile of 16 rows at a time.
+bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
+
+uint32_t few_items(uint32_t batch, uint32_t group, uint32_t tokens) {
+    return (uint32_t)((uint64_t)tokens * group / kFewRows) + std::min(batch, tokens);
+}
+
+// Parts of a context: enough workgroups for the card.
+uint32_t few_parts(uint32_t items, uint32_t kv_heads) {
+    const uint64_t tiles = (uint64_t)items * kv_heads;
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512, 1024 / tiles));
+}
+
+}  // namespace
+
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
-    return 0;
+    if (!few_rows(batch, group, tokens)) return 0;
+    const uint32_t items = few_items(batch, group, tokens), parts = few_parts(items, kv_heads);
+    return parts == 1 ? 0 : (size_t)items * kv_heads * parts * kFewRows * (D + 2) * sizeof(float);
 }
 
 namespace {
@@ -252,6 +538,16 @@ hipError_t by_shape(const Kv8 &c, F &&f) {
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
+    if (few_rows(a.c.batch, a.group, a.step.tokens)) {
+        const uint32_t n = few_items(a.c.batch, a.group, a.step.tokens), parts = few_parts(n, a.c.heads);
+        return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
+            kv8_few_kernel<decltype(ns)::value, decltype(e4m3)::value><<<dim3(n * parts, a.c.heads), 256, 0, s>>>(a, parts);
+            if (hipError_t e = hipGetLastError()) return e;
+            if (parts == 1) return hipSuccess;
+            kv8_join_kernel<decltype(ns)::value><<<dim3(n * kFewRows, a.c.heads), 256, 0, s>>>(a, n, parts);
+            return hipGetLastError();
+        });
+    }
     // 32-row tiles of every sequence: at most one that is not full each
     const uint32_t items = (uint32_t)((uint64_t)a.step.tokens * a.group / 32) + std::min(a.c.batch, a.step.tokens);
     return by_shape(a.c, [&](auto ns, auto e4m3) {

@@ -87,95 +87,190 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
     return min(s.n - s.m + i + 1, max_ctx);
 }
 
+// A part of a context that is split over workgroups: its blocks, and the parts in use.
+struct Part {
+    uint32_t first, end, parts;
+};
+// All parts in use but the last have the same number of blocks, a multiple of `unit`.
+__device__ __forceinline__ Part part_of(uint32_t blocks, uint32_t most, uint32_t part, uint32_t unit) {
+    const uint32_t per = max(((blocks + most - 1) / most + unit - 1) / unit * unit, unit);
+    return Part{min(part * per, blocks), min((part + 1) * per, blocks), (blocks + per - 1) / per};
+}
+
+// Where a part's normalised O of a query row lies in the workspace, in rows; its m and l in pairs behind all of them.
+__device__ __forceinline__ size_t part_at(uint32_t item, uint32_t heads, uint32_t head, uint32_t parts, uint32_t part,
+                                          uint32_t tile_rows, uint32_t row) {
+    return (((size_t)item * heads + head) * parts + part) * tile_rows + row;
+}
+
+constexpr uint32_t kMostParts = 512;
+
 __device__ __forceinline__ uint32_t wave_max_uniform(uint32_t v) { return wave_max_u32(v); }
 __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_max_u32(~v); }
 
 }  // namespace
 
-// A wave per tile of 32 query rows of one kv head, over all blocks of its sequence.
+// ---- many rows: prompts and chunks
+//
+// A workgroup of four waves takes 128 query rows, 32 a wave, and walks the blocks that they see, kTileBlocks<NS> at a time:
+// every wave turns its share of the bytes into fp16 operands in LDS once for all four (a wave unpacking for itself would
+// spend more vector cycles on it than the matrix cores take), each as the 16 bytes a lane that an operand load takes.
+constexpr uint32_t kManyRows = 128;
+template <int NS>
+constexpr int kTileBlocks = NS <= 2 ? 4 : (NS <= 4 ? 2 : 1);
+
 template <int NS, int E4M3>
-__global__ __launch_bounds__(256) void kv8_attention_kernel(Kv8AttnArgs a, uint32_t items) {
+__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts) {
     constexpr uint32_t D = 32 * NS;
-    const uint32_t lane = __lane_id(), h = lane >> 5;
-    const uint32_t head = blockIdx.y, idx = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (idx >= items) return;
+    constexpr int SB = kTileBlocks<NS>, kUnits = SB * 2 * NS / 4;  // 1 KB pieces of a tile that a wave takes
+    static_assert(SB * 2 * NS % 4 == 0, "whole pieces a wave");
+    __shared__ u32x4 lds[SB][2][2 * NS][64];
+    const uint32_t lane = __lane_id(), h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Work order: heads side by side (with eight of them each XCD's L2 keeps one), a sequence's last tiles, which see the most,
+    // first; every second round of 256 workgroups reversed, so that a compute unit's workgroups add up to about the same.
+    uint32_t idx = blockIdx.x;
+    const uint32_t round = idx / 256, whole = gridDim.x / 256;
+    if ((round & 1) && round < whole) idx = round * 256 + 255 - idx % 256;
+    const uint32_t head = idx % a.c.heads, rest = idx / a.c.heads, part = rest % parts, item = rest / parts;
     uint32_t b, tile;
-    if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + 31) / 32; }, b, tile)) return;
+    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kManyRows - 1) / kManyRows; }, b, tile)) return;
     const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t r = 32 * tile + (lane & 31);
-    const bool live = r < s.m * a.group;
+    const uint32_t rows = s.m * a.group, tiles = (rows + kManyRows - 1) / kManyRows;
+    const uint32_t tile_in_work = tile;
+    tile = tiles - 1 - tile_in_work;
+    const uint32_t r0 = kManyRows * tile, r = r0 + 32 * wave + (lane & 31);
+    const bool live = r < rows;
+    const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
+    const uint32_t most = row_limit(s, min(r0 + kManyRows, rows) - 1, a.group, a.c.max_ctx);
+    const uint32_t wave_most = wave_max_uniform(limit), wave_least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);
+    const Part w = part_of((most + 31) / 32, parts, part, SB);
+    if (part > 0 && part >= w.parts) return;
     const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     QueryRow<NS> q;
     load_query<NS>(q, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
-    const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-    const uint32_t most = wave_max_uniform(limit), least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);
     const size_t bh = (size_t)b * a.c.heads + head;
     const uint8_t *k = a.c.k + bh * a.c.blocks * (size_t)(32 * D), *v = a.c.v + bh * a.c.blocks * (size_t)(32 * D);
     const float *ks = a.c.ks + bh * a.c.blocks, *vs = a.c.vs + bh * a.c.blocks;
     f32x16 o[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) o[i] = f32x16{};
-    float m = -INFINITY, l = 0.0f, vref = 0.0f;
-    for (uint32_t blk = 0; blk * 32 < most; ++blk) {
-        u32x4 kw[NS], vw[NS];
-        load_units<NS>(kw, k + (size_t)blk * (32 * D));
-        load_units<NS>(vw, v + (size_t)blk * (32 * D));
-        const float kscale = ks[blk], vscale = vs[blk];
-        f32x16 p = key_product<NS, E4M3>(kw, q);
-        const float c = q.c * kscale;
-        const bool edge = blk * 32 + 32 > least;
-        const uint32_t room = limit > blk * 32 ? limit - blk * 32 : 0u;  // slots of this block that the row sees
-        float top = -INFINITY;
+    float base = -1e38f, l = 0.0f, vref = 0.0f;
+    u32x4 piece[kUnits];
+    const auto fetch = [&](uint32_t blk) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            p[i] *= c;
-            if (edge && 8 * (i >> 2) + 4 * h + (i & 3) >= room) p[i] = -INFINITY;
-            top = fmaxf(top, p[i]);
+        for (int i = 0; i < kUnits; ++i) {
+            const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
+            if (blk + sb < w.end)
+                piece[i] = *reinterpret_cast<const u32x4 *>((kv ? v : k) + (size_t)(blk + sb) * (32 * D) + 1024 * j + 16 * lane);
         }
-        top = fmaxf(top, xchg32(top, lane));
-        const float m1 = fmaxf(m, top);
-        const float base = m1 == -INFINITY ? 0.0f : m1;  // nothing seen yet: every 2^(-inf - 0) is 0
-        float down = __builtin_amdgcn_exp2f(m - base);
-        m = m1;
-        // the values' scale relative to the largest so far: what enters the product in fp16 stays within [0, 1]
-        float sum = 0.0f;
-        l *= down;
-        if (vscale > vref && vscale < INFINITY) {
-            down *= vref / vscale;
-            vref = vscale;
+    };
+    fetch(w.first);
+    for (uint32_t blk = w.first; blk < w.end; blk += SB) {
+        __syncthreads();  // the tile before has been read
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
+            lds[sb][kv][2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].x, piece[i].y));
+            lds[sb][kv][2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].z, piece[i].w));
         }
-        const float vrel = vref > 0.0f ? vscale / vref : (vscale == 0.0f ? 0.0f : vscale);
-        f16x8_t pf[2];
+        __syncthreads();
+        if (blk + SB < w.end) fetch(blk + SB);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(p[i] - base);
-            sum += e;
-            float w = e * vrel;
-            if (edge && 8 * (i >> 2) + 4 * h + (i & 3) >= room) w = 0.0f;  // also where the block stands for NaN
-            pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)w;
-        }
-        l += sum;
+        for (int sb = 0; sb < SB; ++sb) {
+            const uint32_t p0 = (blk + sb) * 32;
+            if (blk + sb >= w.end || p0 >= wave_most) break;
+            f32x16 p = {};
 #pragma unroll
-        for (int d = 0; d < NS; ++d) {
+            for (int j = 0; j < 2 * NS; ++j)
+                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][0][j][lane]), q.f[j], p, 0, 0, 0);
+            float c = q.c * ks[blk + sb];
+            const float vscale = vs[blk + sb];
+            const bool finite = vscale < INFINITY;
+            // blocks that some row sees in part, or that stand for NaN: the scores masked one by one
+            const bool edge = p0 + 32 > wave_least || !finite;
+            const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
+            if (edge) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= down;
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kv8_operand<E4M3>(vw[d].x, vw[d].y), pf[0], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kv8_operand<E4M3>(vw[d].z, vw[d].w), pf[1], o[d], 0, 0, 0);
+                for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
+                c = 1.0f;
+            }
+            float top = fmaxf(fmaxf(p[0], p[1]), p[2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
+            top = fmaxf(top, p[15]) * c;
+            top = fmaxf(top, xchg32(top, lane));
+            // The base of the exponents follows the maximum only when it is passed by 2^8: the probabilities stay within fp16, and
+            // O is scaled down a few times in all.  The values' scale relative to the largest so far joins the exponent: what
+            // enters the second product stays in range, and l takes it out again.
+            if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
+                const float base1 = fmaxf(base, top);
+                float down = __builtin_amdgcn_exp2f(base - base1);
+                base = base1;
+                l *= down;
+                if (finite && vscale > vref) {
+                    down *= vref / vscale;
+                    vref = vscale;
+                }
+#pragma unroll
+                for (int d = 0; d < NS; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= down;
+            }
+            // a block of zeros (scale 0) has no values to keep in range; below 2^-30 of the largest the scale is held there
+            const float shift = finite && vscale > 0.0f ? fmaxf(__log2f(vscale / vref), -30.0f) : 0.0f;
+            const float from = base - shift;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
+                sum += p[i];
+            }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+            if (edge && !finite) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i >> 2) + 4 * h + (i & 3) < room) p[i] = __builtin_nanf("");
+            }
+            f16x8_t pf[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)p[i];
+#pragma unroll
+            for (int d = 0; d < NS; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][1][2 * d][lane]), pf[0], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][1][2 * d + 1][lane]), pf[1], o[d], 0, 0, 0);
+            }
         }
     }
     if (!live) return;
     l += xchg32(l, lane);
-    if (a.lse && h == 0) a.lse[(size_t)t * a.q_heads + qh] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
-    const float w = l == 0.0f ? 0.0f : vref / l;
-    uint16_t *out = a.out + ((size_t)t * a.q_heads + qh) * D;
+    const float norm = l == 0.0f ? 0.0f : vref / l;
+    if (parts == 1) {
+        const size_t at = (size_t)t * a.q_heads + qh;
+        if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
+        uint16_t *out = a.out + at * D;
 #pragma unroll
-    for (int d = 0; d < NS; ++d)
+        for (int d = 0; d < NS; ++d)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u32x2 y = {pack_bf16_rne(o[d][4 * i] * w, o[d][4 * i + 1] * w),
-                             pack_bf16_rne(o[d][4 * i + 2] * w, o[d][4 * i + 3] * w)};
-            *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
+            for (int i = 0; i < 4; ++i) {
+                const u32x2 y = {pack_bf16_rne(o[d][4 * i] * norm, o[d][4 * i + 1] * norm),
+                                 pack_bf16_rne(o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm)};
+                *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
+            }
+    } else {
+        // the workspace is in the order of the tiles, not of the work
+        const size_t at = part_at(item - tile_in_work + tile, a.c.heads, head, parts, part, kManyRows, r - r0);
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
+                    f32x4{o[d][4 * i] * norm, o[d][4 * i + 1] * norm, o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm};
+        if (h == 0) {
+            float *ml = a.part + (size_t)items * parts * a.c.heads * kManyRows * D + 2 * at;
+            ml[0] = base;
+            ml[1] = l;
         }
+    }
 }
 
 // ---- few rows: the context split over workgroups
@@ -187,15 +282,6 @@ __global__ __launch_bounds__(256) void kv8_attention_kernel(Kv8AttnArgs a, uint3
 // On v_mfma_f32_16x16x32_f16: lane (column l & 15, g = l >> 4) holds slots 16 t + 4 g + j after the first product, and
 // needs of dim d the slots 16 s + 4 g + j for the second, eight bytes of v's order (h = g & 1, a = g >> 1).
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
-
-struct FewPart {
-    uint32_t first, end, parts;  // blocks of this part; parts in use
-};
-// Blocks of part `part` of `most` parts: all parts in use but the last have the same number, at least one a wave.
-__device__ __forceinline__ FewPart few_part(uint32_t blocks, uint32_t most, uint32_t part) {
-    const uint32_t per = max((blocks + most - 1) / most, kFewWaves);
-    return FewPart{min(part * per, blocks), min((part + 1) * per, blocks), (blocks + per - 1) / per};
-}
 
 template <int NS>
 __device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, const uint16_t *row, bool live, float scale_log2) {
@@ -270,7 +356,7 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
     const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
     const uint32_t most = row_limit(s, min(kFewRows * tile + kFewRows, rows) - 1, a.group, a.c.max_ctx);
     const uint32_t least = row_limit(s, kFewRows * tile, a.group, a.c.max_ctx);
-    const FewPart w = few_part((most + 31) / 32, parts, part);
+    const Part w = part_of((most + 31) / 32, parts, part, kFewWaves);
     if (part > 0 && part >= w.parts) return;
     const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     f16x8_t q[NS];
@@ -381,7 +467,7 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
             *reinterpret_cast<u32x2 *>(a.out + at * D + d) = y;
             if (a.lse && d == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
         } else {
-            const size_t at = (((size_t)item * a.c.heads + head) * parts + part) * kFewRows + row;
+            const size_t at = part_at(item, a.c.heads, head, parts, part, kFewRows, row);
             *reinterpret_cast<f32x4 *>(a.part + at * D + d) = acc;
             if (d == 0) {
                 float *ml = a.part + (size_t)gridDim.x * a.c.heads * kFewRows * D + 2 * at;
@@ -394,30 +480,31 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
 
 // A workgroup per query row: thread (i, j) adds up parts i, i + n, ... of four dims, then the n sums are joined.
 template <int NS>
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts) {
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts, uint32_t tile_rows,
+                                                       uint32_t unit) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kWays = 256 / kQuads;
-    __shared__ float red[4], wl[512];
+    __shared__ float red[4], wl[kMostParts];
     __shared__ f32x4 so[kWays][kQuads];
-    const uint32_t head = blockIdx.y, item = blockIdx.x / kFewRows, row = blockIdx.x % kFewRows;
+    const uint32_t head = blockIdx.y, item = blockIdx.x / tile_rows, row = blockIdx.x % tile_rows;
     uint32_t b, tile;
-    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kFewRows - 1) / kFewRows; }, b, tile)) return;
+    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + tile_rows - 1) / tile_rows; }, b, tile)) return;
     const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t rows = s.m * a.group, r = kFewRows * tile + row;
+    const uint32_t rows = s.m * a.group, r = tile_rows * tile + row;
     if (r >= rows) return;
-    const uint32_t most = row_limit(s, min(kFewRows * tile + kFewRows, rows) - 1, a.group, a.c.max_ctx);
-    const uint32_t used = max(few_part((most + 31) / 32, parts, 0).parts, 1u);
-    const size_t at = ((size_t)item * a.c.heads + head) * parts * kFewRows + row;  // part p: at + p kFewRows
-    const float *ml = a.part + (size_t)items * parts * a.c.heads * kFewRows * D;
+    const uint32_t most = row_limit(s, min(tile_rows * tile + tile_rows, rows) - 1, a.group, a.c.max_ctx);
+    const uint32_t used = max(part_of((most + 31) / 32, parts, 0, unit).parts, 1u);
+    const size_t at = part_at(item, a.c.heads, head, parts, 0, tile_rows, row);  // part p: at + p tile_rows
+    const float *ml = a.part + (size_t)items * parts * a.c.heads * tile_rows * D;
     // weights of the parts, relative to the largest m
     const uint32_t tid = threadIdx.x;
     float mx = -INFINITY;
-    for (uint32_t p = tid; p < used; p += 256) mx = fmaxf(mx, ml[2 * (at + (size_t)p * kFewRows)]);
+    for (uint32_t p = tid; p < used; p += 256) mx = fmaxf(mx, ml[2 * (at + (size_t)p * tile_rows)]);
     mx = wave_max(mx);
     if ((tid & 63) == 0) red[tid >> 6] = mx;
     __syncthreads();
     const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     for (uint32_t p = tid; p < used; p += 256) {
-        const float *x = ml + 2 * (at + (size_t)p * kFewRows);
+        const float *x = ml + 2 * (at + (size_t)p * tile_rows);
         const float lx = x[1];
         wl[p] = lx == 0.0f ? 0.0f : lx * __builtin_amdgcn_exp2f(x[0] - M);  // NaN stays
     }
@@ -429,7 +516,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, uint32_t i
         f32x4 acc = {0, 0, 0, 0};
 #pragma unroll 4
         for (uint32_t p = way; p < used; p += kWays)
-            acc += wl[p] * *reinterpret_cast<const f32x4 *>(a.part + (at + (size_t)p * kFewRows) * D + 4 * quad);
+            acc += wl[p] * *reinterpret_cast<const f32x4 *>(a.part + (at + (size_t)p * tile_rows) * D + 4 * quad);
         so[way][quad] = acc;
     }
     __syncthreads();
@@ -498,25 +585,28 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a) {
 
 namespace {
 
-// Whether a step has few query rows a sequence: then the context is split, a tile of 16 rows at a time.
-bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
-
-uint32_t few_items(uint32_t batch, uint32_t group, uint32_t tokens) {
-    return (uint32_t)((uint64_t)tokens * group / kFewRows) + std::min(batch, tokens);
-}
-
-// Parts of a context: enough workgroups for the card.
-uint32_t few_parts(uint32_t items, uint32_t kv_heads) {
-    const uint64_t tiles = (uint64_t)items * kv_heads;
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512, 1024 / tiles));
+// How a step is launched: tiles of 16 rows where the sequences have few query rows (one or two tokens of a group of
+// heads), else of 128; and the parts that a context is split into, so that there are workgroups for the whole card.
+struct AttnPlan {
+    bool few;
+    uint32_t rows, items, parts;
+};
+AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens) {
+    AttnPlan p;
+    p.few = (uint64_t)tokens * group <= 32ull * batch;
+    p.rows = p.few ? kFewRows : kManyRows;
+    // tiles of every sequence: at most one that is not full each
+    p.items = (uint32_t)((uint64_t)tokens * group / p.rows) + std::min(batch, tokens);
+    const uint64_t tiles = (uint64_t)p.items * kv_heads, want = p.few ? 1024 : 512;
+    p.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kMostParts, want / tiles));
+    return p;
 }
 
 }  // namespace
 
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
-    if (!few_rows(batch, group, tokens)) return 0;
-    const uint32_t items = few_items(batch, group, tokens), parts = few_parts(items, kv_heads);
-    return parts == 1 ? 0 : (size_t)items * kv_heads * parts * kFewRows * (D + 2) * sizeof(float);
+    const AttnPlan p = plan_of(batch, kv_heads, group, tokens);
+    return p.parts == 1 ? 0 : (size_t)p.items * kv_heads * p.parts * p.rows * (D + 2) * sizeof(float);
 }
 
 namespace {
@@ -538,21 +628,17 @@ hipError_t by_shape(const Kv8 &c, F &&f) {
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
-    if (few_rows(a.c.batch, a.group, a.step.tokens)) {
-        const uint32_t n = few_items(a.c.batch, a.group, a.step.tokens), parts = few_parts(n, a.c.heads);
-        return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
-            kv8_few_kernel<decltype(ns)::value, decltype(e4m3)::value><<<dim3(n * parts, a.c.heads), 256, 0, s>>>(a, parts);
-            if (hipError_t e = hipGetLastError()) return e;
-            if (parts == 1) return hipSuccess;
-            kv8_join_kernel<decltype(ns)::value><<<dim3(n * kFewRows, a.c.heads), 256, 0, s>>>(a, n, parts);
-            return hipGetLastError();
-        });
-    }
-    // 32-row tiles of every sequence: at most one that is not full each
-    const uint32_t items = (uint32_t)((uint64_t)a.step.tokens * a.group / 32) + std::min(a.c.batch, a.step.tokens);
-    return by_shape(a.c, [&](auto ns, auto e4m3) {
-        kv8_attention_kernel<decltype(ns)::value, decltype(e4m3)::value>
-            <<<dim3((items + 3) / 4, a.c.heads), 256, 0, s>>>(a, items);
+    const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.step.tokens);
+    return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
+        constexpr int NS = decltype(ns)::value, E4M3 = decltype(e4m3)::value;
+        if (p.few)
+            kv8_few_kernel<NS, E4M3><<<dim3(p.items * p.parts, a.c.heads), 256, 0, s>>>(a, p.parts);
+        else
+            kv8_many_kernel<NS, E4M3><<<dim3(p.items * p.parts * a.c.heads), 256, 0, s>>>(a, p.items, p.parts);
+        if (hipError_t e = hipGetLastError()) return e;
+        if (p.parts == 1) return hipSuccess;
+        kv8_join_kernel<NS><<<dim3(p.items * p.rows, a.c.heads), 256, 0, s>>>(a, p.items, p.parts, p.rows,
+                                                                             p.few ? kFewWaves : kTileBlocks<NS>);
         return hipGetLastError();
     });
 }

@@ -105,6 +105,11 @@ __device__ __forceinline__ size_t part_at(uint32_t item, uint32_t heads, uint32_
 
 constexpr uint32_t kMostParts = 512;
 
+// A value that every lane holds, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
+
 __device__ __forceinline__ uint32_t wave_max_uniform(uint32_t v) { return wave_max_u32(v); }
 __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_max_u32(~v); }
 
@@ -129,8 +134,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     // Work order: heads side by side (with eight of them each XCD's L2 keeps one), a sequence's last tiles, which see the most,
     // first; every second round of 256 workgroups reversed, so that a compute unit's workgroups add up to about the same.
     uint32_t idx = blockIdx.x;
-    const uint32_t round = idx / 256, whole = gridDim.x / 256;
-    if ((round & 1) && round < whole) idx = round * 256 + 255 - idx % 256;
+    const uint32_t round = idx / 256;
+    if (round & 1) idx = round * 256 + min(gridDim.x - round * 256, 256u) - 1 - idx % 256;
     const uint32_t head = idx % a.c.heads, rest = idx / a.c.heads, part = rest % parts, item = rest / parts;
     uint32_t b, tile;
     if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kManyRows - 1) / kManyRows; }, b, tile)) return;
@@ -156,6 +161,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     for (int i = 0; i < NS; ++i) o[i] = f32x16{};
     float base = -1e38f, l = 0.0f, vref = 0.0f;
     u32x4 piece[kUnits];
+    float kscale[SB], vscale[SB];
     const auto fetch = [&](uint32_t blk) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
@@ -163,8 +169,78 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             if (blk + sb < w.end)
                 piece[i] = *reinterpret_cast<const u32x4 *>((kv ? v : k) + (size_t)(blk + sb) * (32 * D) + 1024 * j + 16 * lane);
         }
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+            const uint32_t at = min(blk + i, w.end - 1);
+            kscale[i] = ks[at];
+            vscale[i] = vs[at];
+        }
     };
-    fetch(w.first);
+    // One block: its operands in LDS, its first slot p0.  kEdge: a row sees it in part, or it stands for NaN; then the
+    // scores are masked one by one.
+    const auto block = [&](auto edge, const u32x4 (*kl)[64], const u32x4 (*vl)[64], float kscale, float vscale, uint32_t p0) {
+        constexpr bool kEdge = decltype(edge)::value;
+        f32x16 p = {};
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j)
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kl[j][lane]), q.f[j], p, 0, 0, 0);
+        float c = q.c * kscale;
+        const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
+        if constexpr (kEdge) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
+            c = 1.0f;
+        }
+        float top = fmaxf(fmaxf(p[0], p[1]), p[2]);
+#pragma unroll
+        for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
+        top = fmaxf(top, p[15]) * c;
+        top = fmaxf(top, xchg32(top, lane));
+        // The base of the exponents follows the maximum only when it is passed by 2^8: the probabilities stay within fp16, and
+        // O is scaled down a few times in all.  The values' scale relative to the largest so far joins the exponent: what
+        // enters the second product stays in range, and l takes it out again.
+        const bool finite = vscale < INFINITY;
+        if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
+            const float base1 = fmaxf(base, top);
+            float down = __builtin_amdgcn_exp2f(base - base1);
+            base = base1;
+            l *= down;
+            if (finite && vscale > vref) {
+                down *= vref / vscale;
+                vref = vscale;
+            }
+#pragma unroll
+            for (int d = 0; d < NS; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= down;
+        }
+        // a block of zeros (scale 0) has no values to keep in range; below 2^-30 of the largest the scale is held there
+        const float shift = finite && vscale > 0.0f ? fmaxf(__log2f(vscale / vref), -30.0f) : 0.0f;
+        const float from = base - shift;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
+            sum += p[i];
+        }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+        if constexpr (kEdge) {
+            if (!finite) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i >> 2) + 4 * h + (i & 3) < room) p[i] = __builtin_nanf("");
+            }
+        }
+        f16x8_t pf[2];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)p[i];
+#pragma unroll
+        for (int d = 0; d < NS; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vl[2 * d][lane]), pf[0], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vl[2 * d + 1][lane]), pf[1], o[d], 0, 0, 0);
+        }
+    };
+    if (w.first < w.end) fetch(w.first);
     for (uint32_t blk = w.first; blk < w.end; blk += SB) {
         __syncthreads();  // the tile before has been read
 #pragma unroll
@@ -173,72 +249,22 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             lds[sb][kv][2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].x, piece[i].y));
             lds[sb][kv][2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].z, piece[i].w));
         }
+        float kc[SB], vc[SB];
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+            kc[i] = uniform(kscale[i]);
+            vc[i] = uniform(vscale[i]);
+        }
         __syncthreads();
         if (blk + SB < w.end) fetch(blk + SB);
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) {
             const uint32_t p0 = (blk + sb) * 32;
             if (blk + sb >= w.end || p0 >= wave_most) break;
-            f32x16 p = {};
-#pragma unroll
-            for (int j = 0; j < 2 * NS; ++j)
-                p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][0][j][lane]), q.f[j], p, 0, 0, 0);
-            float c = q.c * ks[blk + sb];
-            const float vscale = vs[blk + sb];
-            const bool finite = vscale < INFINITY;
-            // blocks that some row sees in part, or that stand for NaN: the scores masked one by one
-            const bool edge = p0 + 32 > wave_least || !finite;
-            const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
-                c = 1.0f;
-            }
-            float top = fmaxf(fmaxf(p[0], p[1]), p[2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
-            top = fmaxf(top, p[15]) * c;
-            top = fmaxf(top, xchg32(top, lane));
-            // The base of the exponents follows the maximum only when it is passed by 2^8: the probabilities stay within fp16, and
-            // O is scaled down a few times in all.  The values' scale relative to the largest so far joins the exponent: what
-            // enters the second product stays in range, and l takes it out again.
-            if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
-                const float base1 = fmaxf(base, top);
-                float down = __builtin_amdgcn_exp2f(base - base1);
-                base = base1;
-                l *= down;
-                if (finite && vscale > vref) {
-                    down *= vref / vscale;
-                    vref = vscale;
-                }
-#pragma unroll
-                for (int d = 0; d < NS; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= down;
-            }
-            // a block of zeros (scale 0) has no values to keep in range; below 2^-30 of the largest the scale is held there
-            const float shift = finite && vscale > 0.0f ? fmaxf(__log2f(vscale / vref), -30.0f) : 0.0f;
-            const float from = base - shift;
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
-                sum += p[i];
-            }
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
-            if (edge && !finite) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (8 * (i >> 2) + 4 * h + (i & 3) < room) p[i] = __builtin_nanf("");
-            }
-            f16x8_t pf[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)p[i];
-#pragma unroll
-            for (int d = 0; d < NS; ++d) {
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][1][2 * d][lane]), pf[0], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, lds[sb][1][2 * d + 1][lane]), pf[1], o[d], 0, 0, 0);
-            }
+            if (p0 + 32 > wave_least || !(vc[sb] < INFINITY))
+                block(std::true_type{}, lds[sb][0], lds[sb][1], kc[sb], vc[sb], p0);
+            else
+                block(std::false_type{}, lds[sb][0], lds[sb][1], kc[sb], vc[sb], p0);
         }
     }
     if (!live) return;

@@ -134,10 +134,14 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
  * weight f32 [batch, kv_heads, max_ctx]: for every slot p < lengths[b] of every kv head
  *   weight[p] = decay * (p < n - m ? weight[p] : 0) + sum over the m new tokens and the heads of the group of e^(scale q . K_p - lse)
  * with the lse that kr_kv8_attention gave for the same q (slots of the new tokens start at zero: no initial contents are
- * needed; slots from lengths[b] on are left as they were).  Sums in f32, in a fixed order.  tokens == 0 does nothing. */
+ * needed; slots from lengths[b] on are left as they were).  Sums in f32, in a fixed order.  tokens == 0 does nothing.
+ * workspace: kr_kv8_weight_workspace_bytes(cache, q_heads, tokens) bytes (none for few rows, else about the size of weight), 16-byte
+ * aligned, no initial contents; calls sharing it must not overlap in time. */
+size_t kr_kv8_weight_workspace_bytes(const kr_kv8_cache *cache, uint32_t q_heads, uint32_t tokens);
 int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stride, uint32_t q_heads,
                              uint32_t tokens, const uint32_t *starts, const uint32_t *lengths, float scale,
-                             const float *lse, float decay, float *weight, void *stream);
+                             const float *lse, float decay, float *weight, void *workspace, size_t workspace_bytes,
+                             void *stream);
 
 /* Copies each sequence into `to`, cut to `budget` tokens where it is longer: every kv head keeps its first `sink` and
  * last `recent` tokens and, of those between, the budget - sink - recent of largest weight (ties to the lowest slot;

@@ -222,9 +222,16 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
     return hip_status(launch_kv8_attention(a, (hipStream_t)stream), "kr_kv8_attention");
 }
 
+size_t kr_kv8_weight_workspace_bytes(const kr_kv8_cache *cache, uint32_t q_heads, uint32_t tokens) {
+    if (!cache || cache->kv_heads == 0 || q_heads == 0 || q_heads % cache->kv_heads || tokens == 0 || cache->batch == 0) return 0;
+    const size_t n = kv8_weight_workspace_bytes(cache->batch, cache->kv_heads, q_heads / cache->kv_heads, tokens, cache->max_ctx);
+    return (n + 255) / 256 * 256;
+}
+
 int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stride, uint32_t q_heads,
                              uint32_t tokens, const uint32_t *starts, const uint32_t *lengths, float scale,
-                             const float *lse, float decay, float *weight, void *stream) {
+                             const float *lse, float decay, float *weight, void *workspace, size_t workspace_bytes,
+                             void *stream) {
     if (int rc = check_cache(cache, "cache")) return rc;
     if (int rc = check_queries(cache, q, q_stride, q_heads, tokens)) return rc;
     if (!(fabsf(scale) < INFINITY) || !(fabsf(decay) < INFINITY)) return fail(KR_E_INVALID, "scale and decay must be finite");
@@ -232,6 +239,10 @@ int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_
     if (int rc = check_step(cache, tokens, starts, lengths)) return rc;
     if (!lse || !weight) return fail(KR_E_INVALID, "lse and weight must not be NULL");
     if (!on(lse, 4) || !on(weight, 4)) return fail(KR_E_ALIGN, "lse and weight must be 4-byte aligned");
+    const size_t need = kr_kv8_weight_workspace_bytes(cache, q_heads, tokens);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(KR_E_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
+    if (!on(workspace, 16)) return fail(KR_E_ALIGN, "workspace must be 16-byte aligned");
     Kv8AttnArgs a{};
     a.c = to_kv8(cache);
     a.step = Kv8Step{starts, lengths, cache->batch, tokens};
@@ -243,6 +254,7 @@ int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_
     a.lse = const_cast<float *>(lse);
     a.decay = decay;
     a.weight = weight;
+    a.part = (float *)workspace;
     return hip_status(launch_kv8_weight(a, (hipStream_t)stream), "kr_kv8_accumulate_weight");
 }
 

@@ -87,23 +87,95 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
     return min(s.n - s.m + i + 1, max_ctx);
 }
 
-// A part of a context that is split over workgroups: its blocks, and the parts in use.
-struct Part {
-    uint32_t first, end, parts;
+// ---- the work of a launch
+//
+// Tiles of kRows query rows; the context of a tile is split into parts of `per` blocks, so that the workgroups have about the
+// same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
+// A sequence's tiles all have as many parts as its longest: workgroup sum_{b' < b} tiles parts + part tiles + tile, and
+// those past a shorter tile's end have nothing to do.  (The tile varies first: workgroups go round the XCDs in turn, and
+// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads took 201 us so, and x now.)
+struct Split {
+    uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
+    uint32_t rows;    // of a tile
+    uint32_t unit;    // `per` is a multiple of it
+    int causal;       // tiles see half of the new tokens on average: count that (then up to 2 target + tiles workgroups)
 };
-// All parts in use but the last have the same number of blocks, a multiple of `unit`.
-__device__ __forceinline__ Part part_of(uint32_t blocks, uint32_t most, uint32_t part, uint32_t unit) {
-    const uint32_t per = max(((blocks + most - 1) / most + unit - 1) / unit * unit, unit);
-    return Part{min(part * per, blocks), min((part + 1) * per, blocks), (blocks + per - 1) / per};
+__device__ __forceinline__ uint32_t tiles_of(const Kv8AttnArgs &a, const Split &w, const Kv8Span &s) {
+    return (s.m * a.group + w.rows - 1) / w.rows;
 }
-
-// Where a part's normalised O of a query row lies in the workspace, in rows; its m and l in pairs behind all of them.
-__device__ __forceinline__ size_t part_at(uint32_t item, uint32_t heads, uint32_t head, uint32_t parts, uint32_t part,
-                                          uint32_t tile_rows, uint32_t row) {
-    return (((size_t)item * heads + head) * parts + part) * tile_rows + row;
+__device__ __forceinline__ uint32_t blocks_of(const Kv8AttnArgs &a, const Kv8Span &s) {
+    return (min(s.n, a.c.max_ctx) + 31) / 32;
 }
+// Blocks of a part.  Every wave computes it alike.
+__device__ __forceinline__ uint32_t split_per(const Kv8AttnArgs &a, const Split &w) {
+    if (w.target == 0) return 1u << 26;  // more than a cache has
+    unsigned long long total = 0;
+    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+        const Kv8Span s = kv8_span(a.step, b);
+        const uint32_t n = min(s.n, a.c.max_ctx), past = n > s.m ? n - s.m : 0u;
+        const uint32_t seen = w.causal ? past + (min(s.m, n) + 1) / 2 : n;  // never below half of n
+        total += (unsigned long long)tiles_of(a, w, s) * ((seen + 31) / 32);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o /= 2) total += __shfl_xor(total, o);
+    const unsigned long long per = total >> 31 ? (total + w.target - 1) / w.target
+                                               : ((uint32_t)total + w.target - 1) / w.target;
+    return max((uint32_t)((per + w.unit - 1) / w.unit) * w.unit, w.unit);
+}
+__device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t per) { return max((blocks + per - 1) / per, 1u); }
 
-constexpr uint32_t kMostParts = 512;
+// What workgroup `idx` of a head does.
+struct Work {
+    Kv8Span s;
+    uint32_t b, tile, part, parts, per;  // parts: of this tile, at least 1
+    uint32_t rows, most;                 // query rows of the sequence; slots that the tile's last row sees
+};
+__device__ __forceinline__ void fill_work(const Kv8AttnArgs &a, const Split &w, Work &o) {
+    o.rows = o.s.m * a.group;
+    o.most = row_limit(o.s, min(w.rows * (o.tile + 1), o.rows) - 1, a.group, a.c.max_ctx);
+    o.parts = parts_of((o.most + 31) / 32, o.per);
+}
+__device__ __forceinline__ bool find_work(const Kv8AttnArgs &a, const Split &w, uint32_t idx, Work &o) {
+    o.per = split_per(a, w);
+    uint32_t item;
+    const auto count = [&](uint32_t i) {
+        const Kv8Span s = kv8_span(a.step, i);
+        return tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
+    };
+    if (!kv8_find(idx, a.c.batch, count, o.b, item)) return false;
+    o.s = kv8_span(a.step, o.b);
+    const uint32_t tiles = tiles_of(a, w, o.s);
+    o.tile = item % tiles;
+    o.part = item / tiles;
+    if (w.causal) o.tile = tiles - 1 - o.tile;  // the tiles that see the most first
+    fill_work(a, w, o);
+    return o.part < o.parts;
+}
+// The same for the tile-th tile of all, and its parts' workgroups: idx, idx + step, ...
+__device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, uint32_t tile, Work &o, uint32_t &idx,
+                                          uint32_t &step) {
+    o.per = split_per(a, w);
+    if (!kv8_find(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, kv8_span(a.step, i)); }, o.b, o.tile)) return false;
+    o.part = 0;
+    o.s = kv8_span(a.step, o.b);
+    fill_work(a, w, o);
+    uint32_t before = 0;
+    for (uint32_t i = __lane_id(); i < o.b; i += 64) {
+        const Kv8Span s = kv8_span(a.step, i);
+        before += tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
+    }
+#pragma unroll
+    for (int x = 32; x > 0; x /= 2) before += __shfl_xor(before, x);
+    step = tiles_of(a, w, o.s);
+    idx = __builtin_amdgcn_readfirstlane(before) + (w.causal ? step - 1 - o.tile : o.tile);
+    return true;
+}
+// parts of a tile: at most twice `target` and one (half of a tile's blocks may not be counted), and target is at most 1024
+constexpr uint32_t kMostParts = 2112;
+// Where a part's normalised O of a row lies in the workspace, in rows; m and l of all rows lie behind them, in pairs.
+__device__ __forceinline__ size_t part_at(const Kv8AttnArgs &a, const Split &w, uint32_t idx, uint32_t head, uint32_t row) {
+    return ((size_t)idx * a.c.heads + head) * w.rows + row;
+}
 
 // A value that every lane holds, in a scalar register.
 __device__ __forceinline__ float uniform(float v) {
@@ -125,32 +197,26 @@ template <int NS>
 constexpr int kTileBlocks = NS <= 2 ? 4 : (NS <= 4 ? 2 : 1);
 
 template <int NS, int E4M3>
-__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts) {
+__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, Split split, uint32_t grid) {
     constexpr uint32_t D = 32 * NS;
     constexpr int SB = kTileBlocks<NS>, kUnits = SB * 2 * NS / 4;  // 1 KB pieces of a tile that a wave takes
     static_assert(SB * 2 * NS % 4 == 0, "whole pieces a wave");
-    __shared__ u32x4 lds[SB][2][2 * NS][64];
+    __shared__ u32x4 lds[2][SB][2][2 * NS][64];
     const uint32_t lane = __lane_id(), h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // Work order: heads side by side (with eight of them each XCD's L2 keeps one), a sequence's last tiles, which see the most,
-    // first; every second round of 256 workgroups reversed, so that a compute unit's workgroups add up to about the same.
-    uint32_t idx = blockIdx.x;
-    const uint32_t round = idx / 256;
-    if (round & 1) idx = round * 256 + min(gridDim.x - round * 256, 256u) - 1 - idx % 256;
-    const uint32_t head = idx % a.c.heads, rest = idx / a.c.heads, part = rest % parts, item = rest / parts;
-    uint32_t b, tile;
-    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kManyRows - 1) / kManyRows; }, b, tile)) return;
-    const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t rows = s.m * a.group, tiles = (rows + kManyRows - 1) / kManyRows;
-    const uint32_t tile_in_work = tile;
-    tile = tiles - 1 - tile_in_work;
-    const uint32_t r0 = kManyRows * tile, r = r0 + 32 * wave + (lane & 31);
-    const bool live = r < rows;
+    // heads side by side: with eight of them each XCD's L2 keeps the bytes of one
+    // every second round of 256 workgroups mirrored: a compute unit's add up to about the same
+    uint32_t at = blockIdx.x;
+    if (at / 256 & 1) at = at / 256 * 256 + min(gridDim.x - at / 256 * 256, 256u) - 1 - at % 256;
+    const uint32_t head = at % a.c.heads, idx = at / a.c.heads;
+    Work w;
+    if (!find_work(a, split, idx, w)) return;
+    const Kv8Span &s = w.s;
+    const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + (lane & 31);
+    const bool live = r < w.rows;
     const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-    const uint32_t most = row_limit(s, min(r0 + kManyRows, rows) - 1, a.group, a.c.max_ctx);
     const uint32_t wave_most = wave_max_uniform(limit), wave_least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);
-    const Part w = part_of((most + 31) / 32, parts, part, SB);
-    if (part > 0 && part >= w.parts) return;
-    const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
+    const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32);
+    const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     QueryRow<NS> q;
     load_query<NS>(q, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
     const size_t bh = (size_t)b * a.c.heads + head;
@@ -166,12 +232,12 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
-            if (blk + sb < w.end)
+            if (blk + sb < end)
                 piece[i] = *reinterpret_cast<const u32x4 *>((kv ? v : k) + (size_t)(blk + sb) * (32 * D) + 1024 * j + 16 * lane);
         }
 #pragma unroll
         for (int i = 0; i < SB; ++i) {
-            const uint32_t at = min(blk + i, w.end - 1);
+            const uint32_t at = min(blk + i, end - 1);
             kscale[i] = ks[at];
             vscale[i] = vs[at];
         }
@@ -180,10 +246,17 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     // scores are masked one by one.
     const auto block = [&](auto edge, const u32x4 (*kl)[64], const u32x4 (*vl)[64], float kscale, float vscale, uint32_t p0) {
         constexpr bool kEdge = decltype(edge)::value;
+        u32x4 kf[2 * NS], vf[2 * NS];
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) kf[j] = kl[j][lane];
         f32x16 p = {};
 #pragma unroll
         for (int j = 0; j < 2 * NS; ++j)
-            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kl[j][lane]), q.f[j], p, 0, 0, 0);
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kf[j]), q.f[j], p, 0, 0, 0);
+        // the values' operands on their way while the softmax is taken
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) vf[j] = vl[j][lane];
+        __builtin_amdgcn_sched_barrier(0);
         float c = q.c * kscale;
         const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
         if constexpr (kEdge) {
@@ -236,41 +309,47 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
         for (int i = 0; i < 16; ++i) pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)p[i];
 #pragma unroll
         for (int d = 0; d < NS; ++d) {
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vl[2 * d][lane]), pf[0], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vl[2 * d + 1][lane]), pf[1], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d]), pf[0], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d + 1]), pf[1], o[d], 0, 0, 0);
         }
     };
-    if (w.first < w.end) fetch(w.first);
-    for (uint32_t blk = w.first; blk < w.end; blk += SB) {
-        __syncthreads();  // the tile before has been read
+    const auto stage = [&](uint32_t side) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
             const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
-            lds[sb][kv][2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].x, piece[i].y));
-            lds[sb][kv][2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].z, piece[i].w));
+            lds[side][sb][kv][2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].x, piece[i].y));
+            lds[side][sb][kv][2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].z, piece[i].w));
         }
+    };
+    if (first < end) {
+        fetch(first);
+        stage(0);
+    }
+    uint32_t side = 0;
+    for (uint32_t blk = first; blk < end; blk += SB, side ^= 1) {
         float kc[SB], vc[SB];
 #pragma unroll
         for (int i = 0; i < SB; ++i) {
             kc[i] = uniform(kscale[i]);
             vc[i] = uniform(vscale[i]);
         }
-        __syncthreads();
-        if (blk + SB < w.end) fetch(blk + SB);
+        __syncthreads();  // this tile is written; the tile before, in the other half, has been read
+        if (blk + SB < end) fetch(blk + SB);
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) {
             const uint32_t p0 = (blk + sb) * 32;
-            if (blk + sb >= w.end || p0 >= wave_most) break;
+            if (blk + sb >= end || p0 >= wave_most) break;
             if (p0 + 32 > wave_least || !(vc[sb] < INFINITY))
-                block(std::true_type{}, lds[sb][0], lds[sb][1], kc[sb], vc[sb], p0);
+                block(std::true_type{}, lds[side][sb][0], lds[side][sb][1], kc[sb], vc[sb], p0);
             else
-                block(std::false_type{}, lds[sb][0], lds[sb][1], kc[sb], vc[sb], p0);
+                block(std::false_type{}, lds[side][sb][0], lds[side][sb][1], kc[sb], vc[sb], p0);
         }
+        if (blk + SB < end) stage(side ^ 1);
     }
     if (!live) return;
     l += xchg32(l, lane);
     const float norm = l == 0.0f ? 0.0f : vref / l;
-    if (parts == 1) {
+    if (w.parts == 1) {
         const size_t at = (size_t)t * a.q_heads + qh;
         if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
         uint16_t *out = a.out + at * D;
@@ -283,8 +362,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
             }
     } else {
-        // the workspace is in the order of the tiles, not of the work
-        const size_t at = part_at(item - tile_in_work + tile, a.c.heads, head, parts, part, kManyRows, r - r0);
+        const size_t at = part_at(a, split, idx, head, r - r0);
 #pragma unroll
         for (int d = 0; d < NS; ++d)
 #pragma unroll
@@ -292,7 +370,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
                     f32x4{o[d][4 * i] * norm, o[d][4 * i + 1] * norm, o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm};
         if (h == 0) {
-            float *ml = a.part + (size_t)items * parts * a.c.heads * kManyRows * D + 2 * at;
+            float *ml = a.part + (size_t)grid * a.c.heads * kManyRows * D + 2 * at;
             ml[0] = base;
             ml[1] = l;
         }
@@ -308,6 +386,10 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 // On v_mfma_f32_16x16x32_f16: lane (column l & 15, g = l >> 4) holds slots 16 t + 4 g + j after the first product, and
 // needs of dim d the slots 16 s + 4 g + j for the second, eight bytes of v's order (h = g & 1, a = g >> 1).
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
+template <int NS>
+constexpr uint32_t kFewAhead = NS <= 4 ? 2 : 1;
+template <int NS>
+constexpr int kFewGroups = NS <= 2 ? 4 : (NS <= 3 ? 3 : (NS <= 6 ? 2 : 1));  // workgroups a compute unit
 
 template <int NS>
 __device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, const uint16_t *row, bool live, float scale_log2) {
@@ -368,22 +450,20 @@ __device__ __forceinline__ void load_few(FewBlock<NS> &f, const uint8_t *k, cons
 }
 
 template <int NS, int E4M3>
-__global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t parts) {
+__global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArgs a, Split split) {
     constexpr uint32_t D = 32 * NS;
     __shared__ float sm[kFewWaves][kFewRows], sl[kFewWaves][kFewRows];
     __shared__ float so[kFewWaves][kFewRows][D + 4];
     const uint32_t lane = __lane_id(), r16 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-    const uint32_t head = blockIdx.y, item = blockIdx.x / parts, part = blockIdx.x % parts;
-    uint32_t b, tile;
-    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + kFewRows - 1) / kFewRows; }, b, tile)) return;
-    const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t rows = s.m * a.group, r = kFewRows * tile + r16;
-    const bool live = r < rows;
+    const uint32_t head = blockIdx.y, idx = blockIdx.x;
+    Work w;
+    if (!find_work(a, split, idx, w)) return;
+    const Kv8Span &s = w.s;
+    const uint32_t r0 = kFewRows * w.tile, r = r0 + r16;
+    const bool live = r < w.rows;
     const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-    const uint32_t most = row_limit(s, min(kFewRows * tile + kFewRows, rows) - 1, a.group, a.c.max_ctx);
-    const uint32_t least = row_limit(s, kFewRows * tile, a.group, a.c.max_ctx);
-    const Part w = part_of((most + 31) / 32, parts, part, kFewWaves);
-    if (part > 0 && part >= w.parts) return;
+    const uint32_t least = row_limit(s, r0, a.group, a.c.max_ctx);
+    const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32), b = w.b;
     const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     f16x8_t q[NS];
     float qc;
@@ -394,11 +474,10 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
     f32x4 o[2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f, vref = 0.0f;
-    uint32_t blk = w.first + wave;
-    FewBlock<NS> f;
-    if (blk < w.end) load_few<NS>(f, k, v, ks, vs, blk);
-    for (; blk < w.end; blk += kFewWaves) {
+    float m = -1e38f, l = 0.0f, vref = 0.0f;
+    uint32_t blk = first + wave;
+    const auto step = [&](auto masked, const FewBlock<NS> &f, uint32_t blk) {
+        constexpr bool kEdge = decltype(masked)::value;
         f32x4 p[2] = {};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -410,47 +489,61 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
             if constexpr (NS & 1)
                 p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.ke[h].x, f.ke[h].y), q[NS - 1], p[h], 0, 0, 0);
         }
-        f16x8_t vf[2 * NS];
-#pragma unroll
-        for (int d = 0; d < 2 * NS; ++d) vf[d] = kv8_operand<E4M3>(f.v[d].x, f.v[d].y);
         const float c = qc * f.ks, vscale = f.vs;
-        if (blk + kFewWaves < w.end) load_few<NS>(f, k, v, ks, vs, blk + kFewWaves);
-        const bool edge = blk * 32 + 32 > least;
         const uint32_t room = limit > blk * 32 ? limit - blk * 32 : 0u;
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             float x = p[i >> 2][i & 3] * c;
-            if (edge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = -INFINITY;
+            if (kEdge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = -INFINITY;
             p[i >> 2][i & 3] = x;
             top = fmaxf(top, x);
         }
         top = fmaxf(top, xchg32(top, lane));
         top = fmaxf(top, xchg16(top, lane));
-        const float m1 = fmaxf(m, top);
-        const float base = m1 == -INFINITY ? 0.0f : m1;
-        float down = __builtin_amdgcn_exp2f(m - base);
-        m = m1;
-        l *= down;
-        if (vscale > vref && vscale < INFINITY) {
-            down *= vref / vscale;
-            vref = vscale;
+        // as in the kernel above: the base follows the maximum when it is passed by 2^8
+        if (__any(top > m + 8.0f) || (vscale > vref && vscale < INFINITY)) {
+            const float m1 = fmaxf(m, top);
+            float down = __builtin_amdgcn_exp2f(m - m1);
+            m = m1;
+            l *= down;
+            if (vscale > vref && vscale < INFINITY) {
+                down *= vref / vscale;
+                vref = vscale;
+            }
+#pragma unroll
+            for (int d = 0; d < 2 * NS; ++d) o[d] *= down;
         }
         const float vrel = vref > 0.0f ? vscale / vref : (vscale == 0.0f ? 0.0f : vscale);
         f16x8_t pf;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(p[i >> 2][i & 3] - base);
+            const float e = __builtin_amdgcn_exp2f(p[i >> 2][i & 3] - m);
             l += e;
             float x = e * vrel;
-            if (edge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = 0.0f;
+            if (kEdge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = 0.0f;
             pf[i] = (_Float16)x;
         }
 #pragma unroll
-        for (int d = 0; d < 2 * NS; ++d) {
+        for (int d = 0; d < 2 * NS; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.v[d].x, f.v[d].y), pf, o[d], 0, 0, 0);
+    };
+    // kFewAhead<NS> blocks of a wave on their way: with the waves that the registers allow about 100 KB a compute unit
+    constexpr uint32_t kAhead = kFewAhead<NS>;
+    FewBlock<NS> f[kAhead];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] *= down;
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[d], pf, o[d], 0, 0, 0);
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (blk + i * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, blk + i * kFewWaves);
+    for (; blk < end; blk += kAhead * kFewWaves) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t at = blk + i * kFewWaves;
+            if (at >= end) break;
+            f[i].ks = uniform(f[i].ks);
+            f[i].vs = uniform(f[i].vs);
+            if (at * 32 + 32 > least || !(f[i].vs < INFINITY)) step(std::true_type{}, f[i], at);
+            else step(std::false_type{}, f[i], at);
+            if (at + kAhead * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, at + kAhead * kFewWaves);
         }
     }
     l += xchg32(l, lane);
@@ -466,8 +559,8 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
     __syncthreads();
     // four dims of a row a thread
     for (uint32_t i = threadIdx.x; i < kFewRows * (D / 4); i += 256) {
-        const uint32_t row = i / (D / 4), d = i % (D / 4) * 4, rr = kFewRows * tile + row;
-        if (rr >= rows) continue;
+        const uint32_t row = i / (D / 4), d = i % (D / 4) * 4, rr = r0 + row;
+        if (rr >= w.rows) continue;
         float M = sm[0][row], L = 0.0f;
 #pragma unroll
         for (uint32_t x = 1; x < kFewWaves; ++x) M = fmaxf(M, sm[x][row]);
@@ -486,14 +579,14 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
         if (nan) L = __builtin_nanf("");
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
         acc *= inv;
-        if (parts == 1) {
+        if (w.parts == 1) {
             const uint32_t tt = s.t0 + rr / a.group, hh = head * a.group + rr % a.group;
             const size_t at = (size_t)tt * a.q_heads + hh;
             const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
             *reinterpret_cast<u32x2 *>(a.out + at * D + d) = y;
             if (a.lse && d == 0) a.lse[at] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
         } else {
-            const size_t at = part_at(item, a.c.heads, head, parts, part, kFewRows, row);
+            const size_t at = part_at(a, split, idx, head, row);
             *reinterpret_cast<f32x4 *>(a.part + at * D + d) = acc;
             if (d == 0) {
                 float *ml = a.part + (size_t)gridDim.x * a.c.heads * kFewRows * D + 2 * at;
@@ -504,135 +597,304 @@ __global__ __launch_bounds__(256) void kv8_few_kernel(Kv8AttnArgs a, uint32_t pa
     }
 }
 
-// A workgroup per query row: thread (i, j) adds up parts i, i + n, ... of four dims, then the n sums are joined.
-template <int NS>
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, uint32_t items, uint32_t parts, uint32_t tile_rows,
-                                                       uint32_t unit) {
-    constexpr uint32_t D = 32 * NS, kQuads = D / 4, kWays = 256 / kQuads;
-    __shared__ float red[4], wl[kMostParts];
-    __shared__ f32x4 so[kWays][kQuads];
-    const uint32_t head = blockIdx.y, item = blockIdx.x / tile_rows, row = blockIdx.x % tile_rows;
-    uint32_t b, tile;
-    if (!kv8_find(item, a.c.batch, [&](uint32_t i) { return (kv8_span(a.step, i).m * a.group + tile_rows - 1) / tile_rows; }, b, tile)) return;
-    const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t rows = s.m * a.group, r = tile_rows * tile + row;
-    if (r >= rows) return;
-    const uint32_t most = row_limit(s, min(tile_rows * tile + tile_rows, rows) - 1, a.group, a.c.max_ctx);
-    const uint32_t used = max(part_of((most + 31) / 32, parts, 0, unit).parts, 1u);
-    const size_t at = part_at(item, a.c.heads, head, parts, 0, tile_rows, row);  // part p: at + p tile_rows
-    const float *ml = a.part + (size_t)items * parts * a.c.heads * tile_rows * D;
-    // weights of the parts, relative to the largest m
-    const uint32_t tid = threadIdx.x;
-    float mx = -INFINITY;
-    for (uint32_t p = tid; p < used; p += 256) mx = fmaxf(mx, ml[2 * (at + (size_t)p * tile_rows)]);
-    mx = wave_max(mx);
-    if ((tid & 63) == 0) red[tid >> 6] = mx;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    for (uint32_t p = tid; p < used; p += 256) {
-        const float *x = ml + 2 * (at + (size_t)p * tile_rows);
-        const float lx = x[1];
-        wl[p] = lx == 0.0f ? 0.0f : lx * __builtin_amdgcn_exp2f(x[0] - M);  // NaN stays
-    }
-    __syncthreads();
-    float L = 0.0f;
-    for (uint32_t p = 0; p < used; ++p) L += wl[p];
-    const uint32_t way = tid / kQuads, quad = tid % kQuads;
-    if (way < kWays) {
+// Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
+// of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile.
+constexpr uint32_t kJoinThreads = 1024;
+template <int NS, bool kWide>
+__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t grid, uint32_t per_group) {
+    constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
+    __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
+    __shared__ float ws[kWide ? kMostParts : kJoinThreads], red[2][kJoinThreads / 64];
+    const uint32_t lane = __lane_id(), head = blockIdx.y, wave = threadIdx.x >> 6, tid = kWide ? threadIdx.x : lane;
+    const uint32_t groups = split.rows / per_group;
+    Work w;
+    uint32_t idx, tiles;
+    if (!find_tile(a, split, blockIdx.x / groups, w, idx, tiles)) return;
+    if (w.parts == 1) return;
+    const size_t step = (size_t)tiles * a.c.heads * split.rows;  // between parts, in rows
+    const float *all_ml = a.part + (size_t)grid * a.c.heads * split.rows * D;
+    const uint32_t way = tid / kQuads, quad = tid % kQuads, row0 = blockIdx.x % groups * per_group;
+    for (uint32_t row = row0 + (kWide ? 0 : wave); row < row0 + per_group; row += kWide ? 1 : kJoinThreads / 64) {
+        const uint32_t r = split.rows * w.tile + row;
+        if (r >= w.rows) return;
+        const size_t at = part_at(a, split, idx, head, row);
+        const float2 *ml = reinterpret_cast<const float2 *>(all_ml) + at;
         f32x4 acc = {0, 0, 0, 0};
-#pragma unroll 4
-        for (uint32_t p = way; p < used; p += kWays)
-            acc += wl[p] * *reinterpret_cast<const f32x4 *>(a.part + (at + (size_t)p * tile_rows) * D + 4 * quad);
-        so[way][quad] = acc;
-    }
-    __syncthreads();
-    if (tid < kQuads) {
-        f32x4 acc = so[0][tid];
+        float M = -INFINITY, L = 0.0f;
+        for (uint32_t p = tid; p < w.parts; p += kThreads) M = fmaxf(M, ml[p * step].x);
+        M = wave_max(M);
+        if constexpr (kWide) {
+            if (lane == 0) red[0][wave] = M;
+            __syncthreads();
 #pragma unroll
-        for (uint32_t i = 1; i < kWays; ++i) acc += so[i][tid];
-        acc *= L == 0.0f ? 0.0f : 1.0f / L;
-        const size_t to = (size_t)(s.t0 + r / a.group) * a.q_heads + head * a.group + r % a.group;
-        const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
-        *reinterpret_cast<u32x2 *>(a.out + to * D + 4 * tid) = y;
-        if (a.lse && tid == 0) a.lse[to] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
+            for (uint32_t i = 0; i < kJoinThreads / 64; ++i) M = fmaxf(M, red[0][i]);
+        }
+        const float *o = a.part + at * D + 4 * quad;
+        for (uint32_t p0 = 0; p0 < w.parts; p0 += kWide ? kMostParts : 64) {  // (kWide: once)
+            const uint32_t n = min(w.parts - p0, kWide ? kMostParts : 64u);
+            float *wl = kWide ? ws : ws + 64 * wave, sum = 0.0f;
+            for (uint32_t p = tid; p < n; p += kThreads) {
+                const float2 x = ml[(p0 + p) * step];
+                const float f = x.y == 0.0f ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - M);  // NaN stays
+                wl[p] = f;
+                sum += f;
+            }
+            L += wave_sum(sum);
+            if constexpr (kWide) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (way < kWays) {
+#pragma unroll 8
+                for (uint32_t p = way; p < n; p += kWays)
+                    acc += wl[p] * *reinterpret_cast<const f32x4 *>(o + (p0 + p) * step * D);
+            }
+            if constexpr (!kWide) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        if constexpr (kWide) {
+            if (way < kWays) so[way][quad] = acc;
+            if (lane == 0) red[1][wave] = L;
+            __syncthreads();
+            if (tid >= kQuads) return;
+            acc = so[0][tid];
+#pragma unroll
+            for (uint32_t i = 1; i < kWays; ++i) acc += so[i][tid];
+            L = red[1][0];
+#pragma unroll
+            for (uint32_t i = 1; i < kJoinThreads / 64; ++i) L += red[1][i];
+        } else {
+#pragma unroll
+            for (uint32_t i = 1; i < kWays; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float other = __shfl(acc[x], (lane + i * kQuads) & 63);
+                    acc[x] += lane < kQuads ? other : 0.0f;
+                }
+        }
+        if (tid < kQuads) {
+            acc *= L == 0.0f ? 0.0f : 1.0f / L;
+            const size_t to = (size_t)(w.s.t0 + r / a.group) * a.q_heads + head * a.group + r % a.group;
+            const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
+            *reinterpret_cast<u32x2 *>(a.out + to * D + 4 * tid) = y;
+            if (a.lse && tid == 0) a.lse[to] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
+        }
     }
 }
 
-// A wave per block of 32 slots of one sequence and kv head: its keys stay in registers, the query rows that see it
-// pass by in tiles of 32, and lane (column, h) adds up its own rows' probabilities of slots 8 i + 4 h + j; the 32
-// columns are summed at the end.
-template <int NS, int E4M3>
-__global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a) {
-    constexpr uint32_t D = 32 * NS;
-    const uint32_t lane = __lane_id(), h = lane >> 5;
-    const uint32_t head = blockIdx.y, b = blockIdx.z, blk = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const Kv8Span s = kv8_span(a.step, b);
-    const uint32_t n = min(s.n, a.c.max_ctx), p0 = blk * 32;
-    if (p0 >= n) return;
-    const size_t bh = (size_t)b * a.c.heads + head;
-    u32x4 kw[NS];
-    load_units<NS>(kw, a.c.k + (bh * a.c.blocks + blk) * (size_t)(32 * D));
-    const float kscale = a.c.ks[bh * a.c.blocks + blk];
-    const uint32_t old = s.n > s.m ? s.n - s.m : 0u;  // tokens before the new ones
-    float acc[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-    // token i sees slots up to n - m + i: the first that sees this block
-    const uint32_t i0 = p0 + s.m >= s.n ? p0 + s.m - s.n : 0u;
-    const uint32_t rows = s.m * a.group;
-    for (uint32_t r0 = i0 * a.group / 32 * 32; r0 < rows; r0 += 32) {
-        const uint32_t r = r0 + (lane & 31);
-        const bool live = r < rows;
-        const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
-        QueryRow<NS> q;
-        load_query<NS>(q, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
-        const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-        const uint32_t room = limit > p0 ? limit - p0 : 0u;
-        const float lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
-        const f32x16 p = key_product<NS, E4M3>(kw, q);
-        const float c = q.c * kscale;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(p[i], c, -lse));
-            if (8 * (i >> 2) + 4 * h + (i & 3) < room) acc[i] += e;
-        }
+// ---- attention weights of the slots
+//
+// Column sums of the attention matrix, from K and the rows' lse alone: weight_p += sum_r 2^(c_r s_rp - lse_r).  The products are taken as
+// S = Q K^T here: a lane holds one slot (column l & 31), the rows are summed in its registers, and c_r and lse_r come from LDS.
+// A workgroup takes 128 slots, 32 a wave, whose keys stay in registers as fp16 operands, and walks the query rows that see
+// them in tiles of 32 that it turns to fp16 in LDS together.  Where there are many rows they are split into parts whose sums
+// kv8_weight_join_kernel adds in order.  The workgroups loop over the work that the lengths turn out to be.
+constexpr uint32_t kWeightSlots = 128, kWeightRows = 32, kWeightTarget = 1536;
+
+struct WeightSpan {
+    Kv8Span s;
+    uint32_t n, chunks, rows, tiles;  // slots in the cache, chunks of 128 of them; query rows, tiles of 32 of them
+};
+__device__ __forceinline__ WeightSpan weight_span(const Kv8AttnArgs &a, uint32_t b) {
+    WeightSpan w;
+    w.s = kv8_span(a.step, b);
+    w.n = min(w.s.n, a.c.max_ctx);
+    w.chunks = (w.n + kWeightSlots - 1) / kWeightSlots;
+    w.rows = w.s.m * a.group;
+    w.tiles = (w.rows + kWeightRows - 1) / kWeightRows;
+    return w;
+}
+// Row tiles of a part: the launch's (chunk, tile) pairs over the workgroups wanted, at least 4 (their start costs as much as one).
+__device__ __forceinline__ uint32_t weight_per(const Kv8AttnArgs &a, uint32_t target) {
+    unsigned long long total = 0;
+    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+        const WeightSpan w = weight_span(a, b);
+        total += (unsigned long long)w.chunks * w.tiles;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int o = 32; o > 0; o /= 2) total += __shfl_xor(total, o);
+    const unsigned long long per = total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
+    return max((uint32_t)per, 4u);
+}
+__device__ __forceinline__ uint32_t weight_parts(uint32_t tiles, uint32_t per) { return max((tiles + per - 1) / per, 1u); }
+// The first row tile that sees a chunk: token i sees slots up to n - m + i.
+__device__ __forceinline__ uint32_t weight_first(const Kv8AttnArgs &a, const WeightSpan &w, uint32_t chunk) {
+    const uint32_t p0 = chunk * kWeightSlots, i0 = p0 + w.s.m > w.s.n ? p0 + w.s.m - w.s.n : 0u;
+    return min(i0 * a.group / kWeightRows, w.tiles);
+}
+
+template <int NS, int E4M3>
+__global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t target) {
+    constexpr uint32_t D = 32 * NS;
+    __shared__ u32x4 ql[2][2 * NS][64];
+    __shared__ __align__(16) float2 cl[2][kWeightRows];  // c_r, -lse_r
+    __shared__ uint32_t lim[2][kWeightRows];
+    const uint32_t lane = __lane_id(), h = lane >> 5, wave = threadIdx.x >> 6, head = blockIdx.y;
+    const uint32_t per = weight_per(a, target);
+    const auto count = [&](uint32_t i) {
+        const WeightSpan w = weight_span(a, i);
+        return w.chunks * weight_parts(w.tiles, per);
+    };
+    for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {
+        uint32_t b, item;
+        if (!kv8_find(idx, a.c.batch, count, b, item)) return;
+        const WeightSpan w = weight_span(a, b);
+        const uint32_t chunk = item % w.chunks, part = item / w.chunks;
+        const bool split = weight_parts(w.tiles, per) > 1;
+        const uint32_t t0 = weight_first(a, w, chunk) + part * per, t1 = min(t0 + per, w.tiles);
+        if (part > 0 && t0 >= w.tiles) continue;  // part 0 writes also where no row sees the chunk
+        const uint32_t p0 = chunk * kWeightSlots + 32 * wave, p = p0 + (lane & 31);
+        const size_t bh = (size_t)b * a.c.heads + head;
+        const uint32_t old = w.s.n > w.s.m ? w.s.n - w.s.m : 0u;  // slots before the new tokens
+        float *to = a.weight + bh * a.c.max_ctx + p;
+        const float had = !split && p < min(old, w.n) ? a.decay * *to : 0.0f;
+        const uint32_t blk = min(p0 / 32, a.c.blocks - 1);
+        u32x4 kw[NS];
+        load_units<NS>(kw, a.c.k + (bh * a.c.blocks + blk) * (size_t)(32 * D));
+        const float kscale = a.c.ks[bh * a.c.blocks + blk];
+        f16x8_t kf[2 * NS];
 #pragma unroll
-        for (int x = 1; x < 32; x *= 2) acc[i] += __shfl_xor(acc[i], x);
-    float *w = a.weight + bh * a.c.max_ctx;
+        for (int j = 0; j < NS; ++j) {
+            kf[2 * j] = kv8_operand<E4M3>(kw[j].x, kw[j].y);
+            kf[2 * j + 1] = kv8_operand<E4M3>(kw[j].z, kw[j].w);
+        }
+        // eight threads a row, NS / 2 (or one more) of its 8-dim units each
+        constexpr int kUnits = (D / 8 + 7) / 8;
+        const uint32_t mine = threadIdx.x / 8, part8 = threadIdx.x % 8;
+        u32x4 raw[kUnits];
+        float lse = 0.0f;
+        uint32_t limit = 0;
+        const auto fetch = [&](uint32_t tile) {
+            const uint32_t r = kWeightRows * tile + mine;
+            const bool live = r < w.rows;
+            const uint32_t t = w.s.t0 + r / a.group, qh = head * a.group + r % a.group;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t p = p0 + 8 * (i >> 2) + 4 * h + (i & 3);
-        if ((lane & 31) == i && p < n) w[p] = (p < old ? a.decay * w[p] : 0.0f) + acc[i];
+            for (int x = 0; x < kUnits; ++x) {
+                raw[x] = u32x4{0, 0, 0, 0};
+                if (live && part8 + 8 * x < D / 8)
+                    raw[x] = *reinterpret_cast<const u32x4 *>(a.q + t * a.q_stride + (size_t)qh * D + 8 * (part8 + 8 * x));
+            }
+            lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
+            limit = live ? row_limit(w.s, r, a.group, a.c.max_ctx) : 0u;
+        };
+        const auto stage = [&](uint32_t side) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int x = 0; x < kUnits; ++x) top = max(top, bf16_unit_max_bits(raw[x]));
+            top = row16_max_u32<true>(top);
+            const int e = row_stage_exp(top, 14, 14, 14);
+            const float up = exp2_int(e);
+#pragma unroll
+            for (int x = 0; x < kUnits; ++x) {
+                const uint32_t u = part8 + 8 * x, W[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+                f16x8_t f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    f[2 * y] = (_Float16)(__uint_as_float(W[y] << 16) * up);
+                    f[2 * y + 1] = (_Float16)(__uint_as_float(W[y] & 0xFFFF0000u) * up);
+                }
+                // unit 4 j + 2 h + s is step 2 j + s of lane (row, h)
+                if (u < D / 8) ql[side][2 * (u >> 2) + (u & 1)][mine + 32 * ((u >> 1) & 1)] = __builtin_bit_cast(u32x4, f);
+            }
+            if (part8 == 0) {
+                cl[side][mine] = make_float2(a.scale_log2 * exp2_int(-e), -lse);
+                lim[side][mine] = limit;
+            }
+        };
+        float sum = 0.0f;
+        if (t0 < t1) {
+            fetch(t0);
+            stage(0);
+        }
+        uint32_t side = 0;
+        for (uint32_t tile = t0; tile < t1; ++tile, side ^= 1) {
+            __syncthreads();  // this tile is written, the one before has been read
+            if (tile + 1 < t1) fetch(tile + 1);
+            f32x16 s = {};
+#pragma unroll
+            for (int j = 0; j < 2 * NS; ++j)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, ql[side][j][lane]), kf[j], s, 0, 0, 0);
+            // the tile's first row sees the least; its last one may lie behind the sequence's rows
+            const bool edge = lim[side][0] < p0 + 32 || kWeightRows * (tile + 1) > w.rows;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const uint32_t r = 8 * (i >> 2) + 4 * h + (i & 3);
+                const f32x4 c = *reinterpret_cast<const f32x4 *>(&cl[side][r]);
+                float x = __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c.z * kscale, c.w));
+                if (edge) {
+                    if (p >= lim[side][r]) x = 0.0f;
+                    if (p >= lim[side][r + 1]) y = 0.0f;
+                }
+                sum += x;
+                sum += y;
+            }
+            if (tile + 1 < t1) stage(side ^ 1);
+        }
+        sum += xchg32(sum, lane);
+        if (lane < 32) {
+            if (split)
+                a.part[((size_t)idx * a.c.heads + head) * kWeightSlots + p - chunk * kWeightSlots] = sum;
+            else if (p < w.n)
+                *to = had + sum;
+        }
+        __syncthreads();  // LDS is free for the next work
+    }
+}
+
+// Adds the parts of a chunk in order to what its slots had.
+__global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnArgs a, uint32_t target) {
+    const uint32_t head = blockIdx.y, per = weight_per(a, target);
+    for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {  // chunks
+        uint32_t b, chunk, before = 0;
+        if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return weight_span(a, i).chunks; }, b, chunk)) return;
+        const WeightSpan w = weight_span(a, b);
+        const uint32_t parts = weight_parts(w.tiles, per), p = chunk * kWeightSlots + threadIdx.x;
+        if (parts == 1 || p >= w.n) continue;
+        for (uint32_t i = 0; i < b; ++i) {
+            const WeightSpan o = weight_span(a, i);
+            before += o.chunks * weight_parts(o.tiles, per);
+        }
+        const uint32_t seen = w.tiles - weight_first(a, w, chunk), used = weight_parts(seen, per);
+        const uint32_t old = w.s.n > w.s.m ? w.s.n - w.s.m : 0u;
+        float *to = a.weight + ((size_t)b * a.c.heads + head) * a.c.max_ctx + p;
+        float sum = p < old ? a.decay * *to : 0.0f;
+        for (uint32_t i = 0; i < used; ++i)
+            sum += a.part[((size_t)(before + i * w.chunks + chunk) * a.c.heads + head) * kWeightSlots + threadIdx.x];
+        *to = sum;
     }
 }
 
 namespace {
 
 // How a step is launched: tiles of 16 rows where the sequences have few query rows (one or two tokens of a group of
-// heads), else of 128; and the parts that a context is split into, so that there are workgroups for the whole card.
+// heads), else of 128.
 struct AttnPlan {
     bool few;
-    uint32_t rows, items, parts;
+    Split split;
+    uint32_t tiles, grid;  // at most, a head
 };
-AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens) {
-    AttnPlan p;
+AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
+    AttnPlan p{};
     p.few = (uint64_t)tokens * group <= 32ull * batch;
-    p.rows = p.few ? kFewRows : kManyRows;
+    p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
-    p.items = (uint32_t)((uint64_t)tokens * group / p.rows) + std::min(batch, tokens);
-    const uint64_t tiles = (uint64_t)p.items * kv_heads, want = p.few ? 1024 : 512;
-    p.parts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kMostParts, want / tiles));
+    p.tiles = (uint32_t)((uint64_t)tokens * group / p.split.rows) + std::min(batch, tokens);
+    const uint64_t all = (uint64_t)p.tiles * kv_heads;
+    if (p.few) {
+        p.split.unit = kFewWaves;
+        p.split.target = std::max((D <= 64 ? 1024 : (D <= 96 ? 768 : (D <= 192 ? 512 : 256))) / kv_heads, std::min(p.tiles, 1024u));
+        p.grid = p.split.target + p.tiles;
+    } else {
+        p.split.unit = D <= 64 ? kTileBlocks<2> : (D <= 128 ? kTileBlocks<4> : 1);
+        p.split.causal = 1;
+        p.split.target = all < 256 ? std::max(512 / kv_heads, 1u) : 0;
+        p.grid = 2 * p.split.target + p.tiles;
+    }
     return p;
 }
 
 }  // namespace
 
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
-    const AttnPlan p = plan_of(batch, kv_heads, group, tokens);
-    return p.parts == 1 ? 0 : (size_t)p.items * kv_heads * p.parts * p.rows * (D + 2) * sizeof(float);
+    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
+    return p.split.target == 0 ? 0 : (size_t)p.grid * kv_heads * p.split.rows * (D + 2) * sizeof(float);
 }
 
 namespace {
@@ -654,25 +916,46 @@ hipError_t by_shape(const Kv8 &c, F &&f) {
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
-    const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.step.tokens);
+    const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.c.D, a.step.tokens);
     return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
         constexpr int NS = decltype(ns)::value, E4M3 = decltype(e4m3)::value;
         if (p.few)
-            kv8_few_kernel<NS, E4M3><<<dim3(p.items * p.parts, a.c.heads), 256, 0, s>>>(a, p.parts);
+            kv8_few_kernel<NS, E4M3><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
         else
-            kv8_many_kernel<NS, E4M3><<<dim3(p.items * p.parts * a.c.heads), 256, 0, s>>>(a, p.items, p.parts);
+            kv8_many_kernel<NS, E4M3><<<dim3(p.grid * a.c.heads), 256, 0, s>>>(a, p.split, p.grid);
         if (hipError_t e = hipGetLastError()) return e;
-        if (p.parts == 1) return hipSuccess;
-        kv8_join_kernel<NS><<<dim3(p.items * p.rows, a.c.heads), 256, 0, s>>>(a, p.items, p.parts, p.rows,
-                                                                             p.few ? kFewWaves : kTileBlocks<NS>);
+        if (p.split.target == 0) return hipSuccess;
+        if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 512) {
+            kv8_join_kernel<NS, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.grid, 1);
+        } else {
+            uint32_t per_group = kJoinThreads / 64;
+            while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 1024) per_group *= 2;
+            kv8_join_kernel<NS, false><<<dim3(p.tiles * (p.split.rows / per_group), a.c.heads), kJoinThreads, 0, s>>>(
+                a, p.split, p.grid, per_group);
+        }
         return hipGetLastError();
     });
 }
 
+// Workgroups wanted a head, and whether rows may be split: one new token each is a tile or two.
+static uint32_t weight_target(uint32_t kv_heads) { return std::max(kWeightTarget / kv_heads, 1u); }
+
+size_t kv8_weight_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens, uint32_t max_ctx) {
+    if ((uint64_t)tokens * group <= 4 * kWeightRows) return 0;  // never more than one part
+    const size_t chunks = (size_t)batch * ((max_ctx + kWeightSlots - 1) / kWeightSlots);
+    return (weight_target(kv_heads) + chunks) * kv_heads * kWeightSlots * sizeof(float);
+}
+
 hipError_t launch_kv8_weight(const Kv8AttnArgs &a, hipStream_t s) {
-    return by_shape(a.c, [&](auto ns, auto e4m3) {
-        kv8_weight_kernel<decltype(ns)::value, decltype(e4m3)::value>
-            <<<dim3((a.c.blocks + 3) / 4, a.c.heads, a.c.batch), 256, 0, s>>>(a);
+    const uint32_t target = weight_target(a.c.heads);
+    const uint64_t chunks = (uint64_t)a.c.batch * ((a.c.max_ctx + kWeightSlots - 1) / kWeightSlots);
+    return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
+        const dim3 grid((uint32_t)std::min<uint64_t>(chunks + target, std::max(2048 / a.c.heads, 1u)), a.c.heads);
+        kv8_weight_kernel<decltype(ns)::value, decltype(e4m3)::value><<<grid, 256, 0, s>>>(a, target);
+        if (hipError_t e = hipGetLastError()) return e;
+        if ((uint64_t)a.step.tokens * a.group <= 4 * kWeightRows) return hipSuccess;
+        const dim3 join((uint32_t)std::min<uint64_t>(chunks, std::max(2048 / a.c.heads, 1u)), a.c.heads);
+        kv8_weight_join_kernel<<<join, kWeightSlots, 0, s>>>(a, target);
         return hipGetLastError();
     });
 }

@@ -120,7 +120,9 @@ def lib():
             "kr_kv8_dequant": (i32, [vp, vp, vp, u32, vp, vp, i32, vp]),
             "kr_kv8_attention_workspace_bytes": (sz, [vp, u32, u32]),
             "kr_kv8_attention": (i32, [vp, vp, sz, u32, u32, vp, vp, ctypes.c_float, vp, vp, vp, sz, vp]),
-            "kr_kv8_accumulate_weight": (i32, [vp, vp, sz, u32, u32, vp, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp]),
+            "kr_kv8_weight_workspace_bytes": (sz, [vp, u32, u32]),
+            "kr_kv8_accumulate_weight": (i32, [vp, vp, sz, u32, u32, vp, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp,
+                                               sz, vp]),
             "kr_kv8_evict": (i32, [vp, vp, vp, u32, u32, u32, vp, vp, vp, vp, vp]),
             "kr_rope_attention_q4_out": (i32, [vp, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp, u32, M, vp, i32, vp, sz,
                                                vp]),

@@ -170,9 +170,15 @@ def attention(cache: Kv8Cache, q: torch.Tensor, lengths: torch.Tensor, starts: O
     return out, lse
 
 
+def weight_workspace(cache: Kv8Cache, q_heads: int, tokens: int) -> torch.Tensor:
+    """Device workspace of accumulate_weight (sums of parts of many query rows)."""
+    n = int(lib().kr_kv8_weight_workspace_bytes(cache.desc, q_heads, tokens))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+
+
 def accumulate_weight(cache: Kv8Cache, q: torch.Tensor, lse: torch.Tensor, lengths: torch.Tensor, weight: torch.Tensor,
                       starts: Optional[torch.Tensor] = None, scale: Optional[float] = None, decay: float = 1.0,
-                      stream=None) -> torch.Tensor:
+                      workspace: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """weight f32 [batch, kv_heads, max_ctx], in place: decay times what it holds, plus the attention weights that the
     tokens of q give each slot (kr_kv8_accumulate_weight); lse as attention returned it for this q."""
     qs = _queries(cache, q)
@@ -180,10 +186,14 @@ def accumulate_weight(cache: Kv8Cache, q: torch.Tensor, lse: torch.Tensor, lengt
     s, n = _step(cache, tokens, starts, lengths)
     checked("lse", lse, torch.float32, (tokens, heads), cache.k)
     checked("weight", weight, torch.float32, (cache.batch, cache.kv_heads, cache.max_ctx), cache.k)
+    if workspace is None:
+        workspace = weight_workspace(cache, heads, tokens)
+    checked("workspace", workspace, torch.uint8, None, cache.k)
     with at(cache.k):
         _check(lib().kr_kv8_accumulate_weight(cache.desc, q.data_ptr(), qs, heads, tokens, s, n,
                                               1.0 / math.sqrt(d) if scale is None else scale, lse.data_ptr(), decay,
-                                              weight.data_ptr(), stream_of(cache.k, stream)))
+                                              weight.data_ptr(), workspace.data_ptr(), workspace.numel(),
+                                              stream_of(cache.k, stream)))
     return weight
 
 

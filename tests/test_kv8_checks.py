@@ -41,7 +41,7 @@ def test_every_entry_point_refuses_a_bad_cache(kq, change, code):
     assert L.kr_kv8_append(bad, None, x, x, 128, None, None, 0, 0, 2, None, n, None) == code
     assert L.kr_kv8_dequant(bad, n, None, 10, x, x, 0, None) == code
     assert L.kr_kv8_attention(bad, x, 256, 4, 2, None, n, 0.125, x, None, x, 1 << 30, None) == code
-    assert L.kr_kv8_accumulate_weight(bad, x, 256, 4, 2, None, n, 0.125, x, 1.0, x, None) == code
+    assert L.kr_kv8_accumulate_weight(bad, x, 256, 4, 2, None, n, 0.125, x, 1.0, x, x, 1 << 30, None) == code
     assert L.kr_kv8_evict(bad, n, x, 10, 1, 1, good, x + 64, x, None, None) == code
     assert L.kr_kv8_evict(good, n, x, 10, 1, 1, bad, x + 64, x, None, None) == code
     assert L.kr_kv8_append(None, None, x, x, 128, None, None, 0, 0, 2, None, n, None) == kq.KR_E_INVALID
@@ -84,8 +84,8 @@ def test_attention_and_weight_refusals(kq):
     def att(q=q, qs=256, qh=4, t=2, st=None, n=n, sc=0.125, out=0xA0000, lse=0xB0000, ws=0xC0000, wb=big):
         return L.kr_kv8_attention(cr, q, qs, qh, t, st, n, sc, out, lse, ws, wb, None)
 
-    def wei(q=q, qs=256, qh=4, t=2, st=None, n=n, sc=0.125, lse=0xB0000, de=1.0, w=0xD0000):
-        return L.kr_kv8_accumulate_weight(cr, q, qs, qh, t, st, n, sc, lse, de, w, None)
+    def wei(q=q, qs=256, qh=4, t=2, st=None, n=n, sc=0.125, lse=0xB0000, de=1.0, w=0xD0000, ws=0xE0000, wb=big):
+        return L.kr_kv8_accumulate_weight(cr, q, qs, qh, t, st, n, sc, lse, de, w, ws, wb, None)
     for f in (att, wei):
         assert f(q=None) == kq.KR_E_INVALID and f(q=q + 8) == kq.KR_E_ALIGN
         assert f(qh=3) == kq.KR_E_SHAPE and f(qh=0) == kq.KR_E_SHAPE
@@ -99,7 +99,11 @@ def test_attention_and_weight_refusals(kq):
     if need:
         assert att(ws=None) == kq.KR_E_WORKSPACE and att(wb=need - 1) == kq.KR_E_WORKSPACE
     assert wei(lse=None) == kq.KR_E_INVALID and wei(w=None) == kq.KR_E_INVALID and wei(w=0xD0001) == kq.KR_E_ALIGN
-    assert wei(de=math.inf) == kq.KR_E_INVALID
+    assert wei(de=math.inf) == kq.KR_E_INVALID and wei(ws=0xE0008) == kq.KR_E_ALIGN
+    assert L.kr_kv8_weight_workspace_bytes(cr, 4, 2) == 0
+    need = L.kr_kv8_weight_workspace_bytes(cr, 4, 1000)
+    assert need >= 2 * 2 * 100 * 4 and need % 256 == 0
+    assert wei(t=1000, st=n, ws=None) == kq.KR_E_WORKSPACE and wei(t=1000, st=n, wb=need - 1) == kq.KR_E_WORKSPACE
 
 
 def test_attention_workspace_grows_with_the_step_and_is_bounded(kq):

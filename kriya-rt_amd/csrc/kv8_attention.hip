@@ -684,61 +684,71 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
 // Column sums of the attention matrix, from K and the rows' lse alone: weight_p += sum_r 2^(c_r s_rp - lse_r).  The products are taken as
 // S = Q K^T here: a lane holds one slot (column l & 31), the rows are summed in its registers, and c_r and lse_r come from LDS.
 // A workgroup takes 128 slots, 32 a wave, whose keys stay in registers as fp16 operands, and walks the query rows that see
-// them in tiles of 32 that it turns to fp16 in LDS together.  Where there are many rows they are split into parts whose sums
+// them in tiles of 64 that it turns to fp16 in LDS together, two tiles on their way.  Where there are many rows they are split into parts whose sums
 // kv8_weight_join_kernel adds in order.  The workgroups loop over the work that the lengths turn out to be.
-constexpr uint32_t kWeightSlots = 128, kWeightRows = 32, kWeightTarget = 1536;
+// Few rows a sequence (one or two tokens): tiles of 32, nothing on its way (21 -> 15 us for 16 decoded tokens over up to 8000
+// slots: more workgroups a compute unit), and no parts.
+constexpr uint32_t kWeightSlots = 128, kWeightTarget = 768;
+constexpr uint32_t weight_rows(bool few) { return few ? 32 : 64; }
 
+template <bool kFew>
 struct WeightSpan {
     Kv8Span s;
-    uint32_t n, chunks, rows, tiles;  // slots in the cache, chunks of 128 of them; query rows, tiles of 32 of them
+    uint32_t n, chunks, rows, tiles;  // slots in the cache, chunks of 128 of them; query rows, tiles of them
 };
-__device__ __forceinline__ WeightSpan weight_span(const Kv8AttnArgs &a, uint32_t b) {
-    WeightSpan w;
+template <bool kFew>
+__device__ __forceinline__ WeightSpan<kFew> weight_span(const Kv8AttnArgs &a, uint32_t b) {
+    constexpr uint32_t kRows = weight_rows(kFew);
+    WeightSpan<kFew> w;
     w.s = kv8_span(a.step, b);
     w.n = min(w.s.n, a.c.max_ctx);
     w.chunks = (w.n + kWeightSlots - 1) / kWeightSlots;
     w.rows = w.s.m * a.group;
-    w.tiles = (w.rows + kWeightRows - 1) / kWeightRows;
+    w.tiles = (w.rows + kRows - 1) / kRows;
     return w;
 }
-// Row tiles of a part: the launch's (chunk, tile) pairs over the workgroups wanted, at least 4 (their start costs as much as one).
+// Row tiles of a part: the launch's (chunk, tile) pairs over the workgroups wanted, at least 2 (their start costs as much).
+template <bool kFew>
 __device__ __forceinline__ uint32_t weight_per(const Kv8AttnArgs &a, uint32_t target) {
+    if (kFew) return 1u << 27;  // more than there are
     unsigned long long total = 0;
     for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
-        const WeightSpan w = weight_span(a, b);
+        const auto w = weight_span<kFew>(a, b);
         total += (unsigned long long)w.chunks * w.tiles;
     }
 #pragma unroll
     for (int o = 32; o > 0; o /= 2) total += __shfl_xor(total, o);
     const unsigned long long per = total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
-    return max((uint32_t)per, 4u);
+    return max((uint32_t)per, 2u);
 }
 __device__ __forceinline__ uint32_t weight_parts(uint32_t tiles, uint32_t per) { return max((tiles + per - 1) / per, 1u); }
 // The first row tile that sees a chunk: token i sees slots up to n - m + i.
-__device__ __forceinline__ uint32_t weight_first(const Kv8AttnArgs &a, const WeightSpan &w, uint32_t chunk) {
+template <bool kFew>
+__device__ __forceinline__ uint32_t weight_first(const Kv8AttnArgs &a, const WeightSpan<kFew> &w, uint32_t chunk) {
     const uint32_t p0 = chunk * kWeightSlots, i0 = p0 + w.s.m > w.s.n ? p0 + w.s.m - w.s.n : 0u;
-    return min(i0 * a.group / kWeightRows, w.tiles);
+    return min(i0 * a.group / weight_rows(kFew), w.tiles);
 }
 
-template <int NS, int E4M3>
+template <int NS, int E4M3, bool kFew>
 __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t target) {
-    constexpr uint32_t D = 32 * NS;
-    __shared__ u32x4 ql[2][2 * NS][64];
-    __shared__ __align__(16) float2 cl[2][kWeightRows];  // c_r, -lse_r
-    __shared__ uint32_t lim[2][kWeightRows];
+    constexpr uint32_t D = 32 * NS, kRows = weight_rows(kFew), kHalves = kRows / 32, kSides = kFew ? 1 : 2;
+    __shared__ u32x4 ql[kSides][kHalves][2 * NS][64];         // [side][half of the rows][step][lane]
+    __shared__ __align__(16) float2 cl[kSides][kRows];  // c_r, -lse_r
+    __shared__ uint32_t lim[kSides][kRows];
     const uint32_t lane = __lane_id(), h = lane >> 5, wave = threadIdx.x >> 6, head = blockIdx.y;
-    const uint32_t per = weight_per(a, target);
+    const uint32_t per = weight_per<kFew>(a, target);
     const auto count = [&](uint32_t i) {
-        const WeightSpan w = weight_span(a, i);
+        const auto w = weight_span<kFew>(a, i);
         return w.chunks * weight_parts(w.tiles, per);
     };
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {
         uint32_t b, item;
         if (!kv8_find(idx, a.c.batch, count, b, item)) return;
-        const WeightSpan w = weight_span(a, b);
-        const uint32_t chunk = item % w.chunks, part = item / w.chunks;
+        const auto w = weight_span<kFew>(a, b);
+        // the chunks of every other part in reverse: late ones see fewer rows, and workgroups go round the XCDs in turn
+        const uint32_t part = item / w.chunks, chunk = part & 1 ? w.chunks - 1 - item % w.chunks : item % w.chunks;
         const bool split = weight_parts(w.tiles, per) > 1;
-        const uint32_t t0 = weight_first(a, w, chunk) + part * per, t1 = min(t0 + per, w.tiles);
+        const uint32_t t0 = weight_first<kFew>(a, w, chunk) + part * per, t1 = min(t0 + per, w.tiles);
         if (part > 0 && t0 >= w.tiles) continue;  // part 0 writes also where no row sees the chunk
         const uint32_t p0 = chunk * kWeightSlots + 32 * wave, p = p0 + (lane & 31);
         const size_t bh = (size_t)b * a.c.heads + head;
@@ -755,35 +765,51 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
             kf[2 * j] = kv8_operand<E4M3>(kw[j].x, kw[j].y);
             kf[2 * j + 1] = kv8_operand<E4M3>(kw[j].z, kw[j].w);
         }
-        // eight threads a row, NS / 2 (or one more) of its 8-dim units each
-        constexpr int kUnits = (D / 8 + 7) / 8;
-        const uint32_t mine = threadIdx.x / 8, part8 = threadIdx.x % 8;
-        u32x4 raw[kUnits];
-        float lse = 0.0f;
-        uint32_t limit = 0;
-        const auto fetch = [&](uint32_t tile) {
-            const uint32_t r = kWeightRows * tile + mine;
-            const bool live = r < w.rows;
-            const uint32_t t = w.s.t0 + r / a.group, qh = head * a.group + r % a.group;
+        // the threads of a row take its 8-dim units in turn
+        constexpr uint32_t kOfRow = 256 / kRows;
+        constexpr int kUnits = (D / 8 + kOfRow - 1) / kOfRow;
+        const uint32_t mine = threadIdx.x / kOfRow, first_u = threadIdx.x % kOfRow;
+        struct Rows {
+            u32x4 raw[kUnits];
+            float lse;
+            uint32_t limit;
+        } rows[2];
+        // the row that is fetched next: token ti, head tg of the group
+        uint32_t ti = (kRows * t0 + mine) / a.group, tg = (kRows * t0 + mine) % a.group;
+        const uint32_t step_i = kRows / a.group, step_g = kRows % a.group;
+        const auto fetch = [&](Rows &x) {
+            const bool live = ti < w.s.m;
+            const uint32_t t = w.s.t0 + ti, qh = head * a.group + tg;
 #pragma unroll
-            for (int x = 0; x < kUnits; ++x) {
-                raw[x] = u32x4{0, 0, 0, 0};
-                if (live && part8 + 8 * x < D / 8)
-                    raw[x] = *reinterpret_cast<const u32x4 *>(a.q + t * a.q_stride + (size_t)qh * D + 8 * (part8 + 8 * x));
+            for (int i = 0; i < kUnits; ++i) {
+                x.raw[i] = u32x4{0, 0, 0, 0};
+                const uint32_t u = first_u + kOfRow * i;
+                if (live && u < D / 8) x.raw[i] = *reinterpret_cast<const u32x4 *>(a.q + t * a.q_stride + (size_t)qh * D + 8 * u);
             }
-            lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
-            limit = live ? row_limit(w.s, r, a.group, a.c.max_ctx) : 0u;
+            x.lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
+            x.limit = live && w.s.n + ti + 1 > w.s.m ? min(w.s.n - w.s.m + ti + 1, a.c.max_ctx) : 0u;
+            ti += step_i;
+            tg += step_g;
+            if (tg >= a.group) {
+                tg -= a.group;
+                ++ti;
+            }
         };
-        const auto stage = [&](uint32_t side) {
+        const auto stage = [&](const Rows &x, uint32_t side) {
             uint32_t top = 0;
 #pragma unroll
-            for (int x = 0; x < kUnits; ++x) top = max(top, bf16_unit_max_bits(raw[x]));
-            top = row16_max_u32<true>(top);
+            for (int i = 0; i < kUnits; ++i) top = max(top, bf16_unit_max_bits(x.raw[i]));
+            if constexpr (kFew) {
+                top = row16_max_u32<true>(top);  // groups of 8
+            } else {
+                top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xF, 0xF, false));
+                top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xF, 0xF, false));
+            }
             const int e = row_stage_exp(top, 14, 14, 14);
             const float up = exp2_int(e);
 #pragma unroll
-            for (int x = 0; x < kUnits; ++x) {
-                const uint32_t u = part8 + 8 * x, W[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+            for (int i = 0; i < kUnits; ++i) {
+                const uint32_t W[4] = {x.raw[i].x, x.raw[i].y, x.raw[i].z, x.raw[i].w};
                 f16x8_t f;
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
@@ -791,41 +817,68 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
                     f[2 * y + 1] = (_Float16)(__uint_as_float(W[y] & 0xFFFF0000u) * up);
                 }
                 // unit 4 j + 2 h + s is step 2 j + s of lane (row, h)
-                if (u < D / 8) ql[side][2 * (u >> 2) + (u & 1)][mine + 32 * ((u >> 1) & 1)] = __builtin_bit_cast(u32x4, f);
+                const uint32_t u = first_u + kOfRow * i;
+                if (u < D / 8) ql[side][mine >> 5][2 * (u >> 2) + (u & 1)][(mine & 31) + 32 * ((u >> 1) & 1)] = __builtin_bit_cast(u32x4, f);
             }
-            if (part8 == 0) {
-                cl[side][mine] = make_float2(a.scale_log2 * exp2_int(-e), -lse);
-                lim[side][mine] = limit;
+            if (first_u == 0) {
+                cl[side][mine] = make_float2(a.scale_log2 * exp2_int(-e), -x.lse);
+                lim[side][mine] = x.limit;
             }
         };
         float sum = 0.0f;
-        if (t0 < t1) {
-            fetch(t0);
-            stage(0);
-        }
-        uint32_t side = 0;
-        for (uint32_t tile = t0; tile < t1; ++tile, side ^= 1) {
-            __syncthreads();  // this tile is written, the one before has been read
-            if (tile + 1 < t1) fetch(tile + 1);
-            f32x16 s = {};
+        const auto tile_sum = [&](uint32_t side, uint32_t tile) {
+            // the tile's first row sees the least; its last ones may lie behind the sequence's rows
+            const bool edge = __builtin_amdgcn_readfirstlane(lim[side][0]) < p0 + 32 || kRows * (tile + 1) > w.rows;
 #pragma unroll
-            for (int j = 0; j < 2 * NS; ++j)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, ql[side][j][lane]), kf[j], s, 0, 0, 0);
-            // the tile's first row sees the least; its last one may lie behind the sequence's rows
-            const bool edge = lim[side][0] < p0 + 32 || kWeightRows * (tile + 1) > w.rows;
+            for (uint32_t x = 0; x < kHalves; ++x) {
+                if (kRows * tile + 32 * x >= w.rows) break;
+                f32x16 s = {};
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const uint32_t r = 8 * (i >> 2) + 4 * h + (i & 3);
-                const f32x4 c = *reinterpret_cast<const f32x4 *>(&cl[side][r]);
-                float x = __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y)), y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], c.z * kscale, c.w));
+                for (int j = 0; j < 2 * NS; ++j)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, ql[side][x][j][lane]), kf[j], s, 0, 0, 0);
                 if (edge) {
-                    if (p >= lim[side][r]) x = 0.0f;
-                    if (p >= lim[side][r + 1]) y = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t r = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
+                        const float2 c = cl[side][r];
+                        const float y = __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y));
+                        sum += p < lim[side][r] ? y : 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const f32x4 c = *reinterpret_cast<const f32x4 *>(&cl[side][32 * x + 8 * (i >> 2) + 4 * h + (i & 3)]);
+                        sum += __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y));
+                        sum += __builtin_amdgcn_exp2f(fmaf(s[i + 1], c.z * kscale, c.w));
+                    }
                 }
-                sum += x;
-                sum += y;
             }
-            if (tile + 1 < t1) stage(side ^ 1);
+        };
+        if constexpr (kFew) {
+            for (uint32_t tile = t0; tile < t1; ++tile) {
+                fetch(rows[0]);
+                stage(rows[0], 0);
+                __syncthreads();
+                tile_sum(0, tile);
+                if (tile + 1 < t1) __syncthreads();
+            }
+        } else {
+            if (t0 < t1) {
+                fetch(rows[0]);
+                fetch(rows[1]);
+                stage(rows[0], 0);
+            }
+            for (uint32_t tile = t0; tile < t1; tile += 2) {
+                fetch(rows[0]);  // (rows past the end are not read)
+                __syncthreads();  // this tile is written, the one before has been read
+                tile_sum(0, tile);
+                if (tile + 1 >= t1) break;
+                stage(rows[1], 1);
+                fetch(rows[1]);
+                __syncthreads();
+                tile_sum(1, tile + 1);
+                if (tile + 2 < t1) stage(rows[0], 0);
+            }
         }
         sum += xchg32(sum, lane);
         if (lane < 32) {
@@ -840,23 +893,24 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
 
 // Adds the parts of a chunk in order to what its slots had.
 __global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnArgs a, uint32_t target) {
-    const uint32_t head = blockIdx.y, per = weight_per(a, target);
+    const uint32_t head = blockIdx.y, per = weight_per<false>(a, target);
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {  // chunks
         uint32_t b, chunk, before = 0;
-        if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return weight_span(a, i).chunks; }, b, chunk)) return;
-        const WeightSpan w = weight_span(a, b);
+        if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return weight_span<false>(a, i).chunks; }, b, chunk)) return;
+        const auto w = weight_span<false>(a, b);
         const uint32_t parts = weight_parts(w.tiles, per), p = chunk * kWeightSlots + threadIdx.x;
         if (parts == 1 || p >= w.n) continue;
         for (uint32_t i = 0; i < b; ++i) {
-            const WeightSpan o = weight_span(a, i);
+            const auto o = weight_span<false>(a, i);
             before += o.chunks * weight_parts(o.tiles, per);
         }
-        const uint32_t seen = w.tiles - weight_first(a, w, chunk), used = weight_parts(seen, per);
+        const uint32_t seen = w.tiles - weight_first<false>(a, w, chunk), used = weight_parts(seen, per);
         const uint32_t old = w.s.n > w.s.m ? w.s.n - w.s.m : 0u;
         float *to = a.weight + ((size_t)b * a.c.heads + head) * a.c.max_ctx + p;
         float sum = p < old ? a.decay * *to : 0.0f;
+#pragma unroll 16
         for (uint32_t i = 0; i < used; ++i)
-            sum += a.part[((size_t)(before + i * w.chunks + chunk) * a.c.heads + head) * kWeightSlots + threadIdx.x];
+            sum += a.part[((size_t)(before + i * w.chunks + (i & 1 ? w.chunks - 1 - chunk : chunk)) * a.c.heads + head) * kWeightSlots + threadIdx.x];
         *to = sum;
     }
 }
@@ -870,9 +924,10 @@ struct AttnPlan {
     Split split;
     uint32_t tiles, grid;  // at most, a head
 };
+bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
 AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
     AttnPlan p{};
-    p.few = (uint64_t)tokens * group <= 32ull * batch;
+    p.few = few_rows(batch, group, tokens);
     p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)((uint64_t)tokens * group / p.split.rows) + std::min(batch, tokens);
@@ -937,11 +992,11 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
     });
 }
 
-// Workgroups wanted a head, and whether rows may be split: one new token each is a tile or two.
+// Workgroups wanted a head.
 static uint32_t weight_target(uint32_t kv_heads) { return std::max(kWeightTarget / kv_heads, 1u); }
 
 size_t kv8_weight_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens, uint32_t max_ctx) {
-    if ((uint64_t)tokens * group <= 4 * kWeightRows) return 0;  // never more than one part
+    if (few_rows(batch, group, tokens)) return 0;
     const size_t chunks = (size_t)batch * ((max_ctx + kWeightSlots - 1) / kWeightSlots);
     return (weight_target(kv_heads) + chunks) * kv_heads * kWeightSlots * sizeof(float);
 }
@@ -951,9 +1006,13 @@ hipError_t launch_kv8_weight(const Kv8AttnArgs &a, hipStream_t s) {
     const uint64_t chunks = (uint64_t)a.c.batch * ((a.c.max_ctx + kWeightSlots - 1) / kWeightSlots);
     return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
         const dim3 grid((uint32_t)std::min<uint64_t>(chunks + target, std::max(2048 / a.c.heads, 1u)), a.c.heads);
-        kv8_weight_kernel<decltype(ns)::value, decltype(e4m3)::value><<<grid, 256, 0, s>>>(a, target);
+        constexpr int NS = decltype(ns)::value, E4M3 = decltype(e4m3)::value;
+        if (few_rows(a.c.batch, a.group, a.step.tokens)) {
+            kv8_weight_kernel<NS, E4M3, true><<<grid, 256, 0, s>>>(a, target);
+            return hipGetLastError();
+        }
+        kv8_weight_kernel<NS, E4M3, false><<<grid, 256, 0, s>>>(a, target);
         if (hipError_t e = hipGetLastError()) return e;
-        if ((uint64_t)a.step.tokens * a.group <= 4 * kWeightRows) return hipSuccess;
         const dim3 join((uint32_t)std::min<uint64_t>(chunks, std::max(2048 / a.c.heads, 1u)), a.c.heads);
         kv8_weight_join_kernel<<<join, kWeightSlots, 0, s>>>(a, target);
         return hipGetLastError();

@@ -182,26 +182,24 @@ __device__ __forceinline__ float uniform(float v) {
     return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
 }
 
-__device__ __forceinline__ uint32_t wave_max_uniform(uint32_t v) { return wave_max_u32(v); }
 __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_max_u32(~v); }
 
 }  // namespace
 
 // ---- many rows: prompts and chunks
 //
-// A workgroup of four waves takes 128 query rows, 32 a wave, and walks the blocks that they see, kTileBlocks<NS> at a time:
-// every wave turns its share of the bytes into fp16 operands in LDS once for all four (a wave unpacking for itself would
-// spend more vector cycles on it than the matrix cores take), each as the 16 bytes a lane that an operand load takes.
+// A workgroup of four waves takes 128 query rows, 32 a wave, and walks the blocks that they see.  The waves turn a block's bytes
+// into fp16 operands in LDS together (a wave unpacking for itself would spend more vector cycles on it than the matrix
+// cores take), each as the 16 bytes a lane that an operand load takes.  Body n of the loop takes block n's softmax and second
+// product and block n + 1's first; it reads keys n + 1 and values n, and writes keys n + 2 and values n + 1 into the other
+// halves, so that one barrier a block is enough.
 constexpr uint32_t kManyRows = 128;
-template <int NS>
-constexpr int kTileBlocks = NS <= 2 ? 4 : (NS <= 4 ? 2 : 1);
 
 template <int NS, int E4M3>
 __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, Split split, uint32_t grid) {
     constexpr uint32_t D = 32 * NS;
-    constexpr int SB = kTileBlocks<NS>, kUnits = SB * 2 * NS / 4;  // 1 KB pieces of a tile that a wave takes
-    static_assert(SB * 2 * NS % 4 == 0, "whole pieces a wave");
-    __shared__ u32x4 lds[2][SB][2][2 * NS][64];
+    constexpr int kUnits = (2 * NS + 3) / 4;   // 1 KB pieces of a block's keys and values that a wave takes
+    __shared__ u32x4 lds[2][2][2 * NS][64];    // [keys, values][block & 1][step][lane]
     const uint32_t lane = __lane_id(), h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // heads side by side: with eight of them each XCD's L2 keeps the bytes of one
     // every second round of 256 workgroups mirrored: a compute unit's add up to about the same
@@ -214,7 +212,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + (lane & 31);
     const bool live = r < w.rows;
     const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-    const uint32_t wave_most = wave_max_uniform(limit), wave_least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);
+    const uint32_t least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);  // the slots that all rows of the wave see
     const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32);
     const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     QueryRow<NS> q;
@@ -225,130 +223,161 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     f32x16 o[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) o[i] = f32x16{};
-    float base = -1e38f, l = 0.0f, vref = 0.0f;
+    float base = -1e38f, l = 0.0f, vref = 0.0f, vinv = 0.0f;  // vref: the largest scale of values so far, vinv its reciprocal
+    float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
+    // what body n writes: this wave's pieces of keys n + 2 and values n + 1
     u32x4 piece[kUnits];
-    float kscale[SB], vscale[SB];
-    const auto fetch = [&](uint32_t blk) {
+    const auto fetch = [&](uint32_t n) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
-            if (blk + sb < end)
-                piece[i] = *reinterpret_cast<const u32x4 *>((kv ? v : k) + (size_t)(blk + sb) * (32 * D) + 1024 * j + 16 * lane);
-        }
-#pragma unroll
-        for (int i = 0; i < SB; ++i) {
-            const uint32_t at = min(blk + i, end - 1);
-            kscale[i] = ks[at];
-            vscale[i] = vs[at];
+            // (past the end: the last block once more, which nothing reads)
+            const uint32_t u = min(wave + 4 * i, 2u * NS - 1), at = min(u < NS ? n + 2 : n + 1, end - 1), j = u < NS ? u : u - NS;
+            piece[i] = *reinterpret_cast<const u32x4 *>((u < NS ? k : v) + (size_t)at * (32 * D) + 1024 * j + 16 * lane);
         }
     };
-    // One block: its operands in LDS, its first slot p0.  kEdge: a row sees it in part, or it stands for NaN; then the
-    // scores are masked one by one.
-    const auto block = [&](auto edge, const u32x4 (*kl)[64], const u32x4 (*vl)[64], float kscale, float vscale, uint32_t p0) {
-        constexpr bool kEdge = decltype(edge)::value;
-        u32x4 kf[2 * NS], vf[2 * NS];
+    const auto put = [&](u32x4 (*to)[64], uint32_t j, const u32x4 &w) {
+        to[2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.x, w.y));
+        to[2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.z, w.w));
+    };
+    const auto stage = [&](uint32_t n) {
 #pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) kf[j] = kl[j][lane];
-        f32x16 p = {};
+        for (int i = 0; i < kUnits; ++i) {
+            const uint32_t u = min(wave + 4 * i, 2u * NS - 1);  // (the same piece twice where they do not divide)
+            put(u < NS ? lds[0][n & 1] : lds[1][(n + 1) & 1], u < NS ? u : u - NS, piece[i]);
+        }
+    };
+    float ks1 = 0.0f, vs1 = 0.0f;  // scales of block n + 1, on their way
+    const auto fetch_scales = [&](uint32_t n) {
+        const uint32_t at = min(n + 1, end - 1);
+        ks1 = ks[at];
+        vs1 = vs[at];
+    };
+    // The scores of the block in work, times c the exponents; its row maximum has been taken into `base`.
+    f32x16 p;
+    float c;
+    const auto key_steps = [&](f32x16 &s, const u32x4 (&kf)[2 * NS]) {
 #pragma unroll
         for (int j = 0; j < 2 * NS; ++j)
-            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kf[j]), q.f[j], p, 0, 0, 0);
-        // the values' operands on their way while the softmax is taken
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kf[j]), q.f[j], s, 0, 0, 0);
+    };
+    const auto row_top = [&](const f32x16 &s) {
+        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
 #pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) vf[j] = vl[j][lane];
-        __builtin_amdgcn_sched_barrier(0);
-        float c = q.c * kscale;
-        const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
-        if constexpr (kEdge) {
+        for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+        return fmaxf(top, s[15]);
+    };
+    // What a new block's scores change: slots that a row does not see get -infinity; the base of the exponents follows the
+    // maximum only when it is passed by 2^8 (the probabilities stay within fp16, and O is scaled down a few times in all); the
+    // largest scale of values so far grows.
+    const auto enter = [&](float top, float vscale, uint32_t p0) {
+        const bool finite = vscale < INFINITY;
+        if (p0 + 32 > least || !finite) {
+            const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
 #pragma unroll
             for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
             c = 1.0f;
+            top = row_top(p);
+            top = fmaxf(top, xchg32(top, lane));
+            if (!finite && room) poison = __builtin_nanf("");
         }
-        float top = fmaxf(fmaxf(p[0], p[1]), p[2]);
-#pragma unroll
-        for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
-        top = fmaxf(top, p[15]) * c;
-        top = fmaxf(top, xchg32(top, lane));
-        // The base of the exponents follows the maximum only when it is passed by 2^8: the probabilities stay within fp16, and
-        // O is scaled down a few times in all.  The values' scale relative to the largest so far joins the exponent: what
-        // enters the second product stays in range, and l takes it out again.
-        const bool finite = vscale < INFINITY;
         if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
             const float base1 = fmaxf(base, top);
             float down = __builtin_amdgcn_exp2f(base - base1);
             base = base1;
             l *= down;
             if (finite && vscale > vref) {
-                down *= vref / vscale;
-                vref = vscale;
+                const float to = fmaxf(vscale, 0x1p-126f);  // whose reciprocal is finite
+                vinv = 1.0f / to;
+                down *= vref * vinv;
+                vref = to;
             }
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= down;
         }
-        // a block of zeros (scale 0) has no values to keep in range; below 2^-30 of the largest the scale is held there
-        const float shift = finite && vscale > 0.0f ? fmaxf(__log2f(vscale / vref), -30.0f) : 0.0f;
+    };
+    // Body n.  One run of instructions, so that the vector unit takes the exponentials while the matrix cores multiply the
+    // next keys, and the next row maximum while they multiply values.
+    const auto body = [&](auto more, uint32_t n, float vscale) {
+        constexpr bool kMore = decltype(more)::value;
+        u32x4 kf[2 * NS], vf[2 * NS];
+        if constexpr (kMore) {
+#pragma unroll
+            for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][(n + 1) & 1][j][lane];
+            stage(n);
+            fetch(n + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j][lane];
+        // The values' scale relative to the largest so far joins the exponent: what enters the second product stays in range, and
+        // l takes it out again. A block of zeros (scale 0) has none to keep; below 2^-30 of the largest it is held there.
+        const float shift = vscale > 0.0f && vscale < INFINITY ? fmaxf(__log2f(vscale * vinv), -30.0f) : 0.0f;
         const float from = base - shift;
         float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
-            sum += p[i];
-        }
-        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
-        if constexpr (kEdge) {
-            if (!finite) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (8 * (i >> 2) + 4 * h + (i & 3) < room) p[i] = __builtin_nanf("");
-            }
-        }
         f16x8_t pf[2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)p[i];
+        for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
+            sum += e;
+            pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)e;
+        }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+        if constexpr (kMore) {
+            p = f32x16{};
+            key_steps(p, kf);
+        }
 #pragma unroll
         for (int d = 0; d < NS; ++d) {
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d]), pf[0], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d + 1]), pf[1], o[d], 0, 0, 0);
         }
-    };
-    const auto stage = [&](uint32_t side) {
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const uint32_t u = wave + 4 * i, sb = u / (2 * NS), kv = u / NS % 2, j = u % NS;
-            lds[side][sb][kv][2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].x, piece[i].y));
-            lds[side][sb][kv][2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(piece[i].z, piece[i].w));
+        if constexpr (kMore) {
+            c = q.c * uniform(ks1);
+            const float vnext = uniform(vs1);
+            fetch_scales(n + 1);
+            float top = row_top(p) * c;
+            top = fmaxf(top, xchg32(top, lane));
+            enter(top, vnext, (n + 1) * 32);
+            return vnext;
         }
+        return 0.0f;
     };
     if (first < end) {
+        // keys first and first + 1, values first
+        for (uint32_t u = wave; u < 3 * NS; u += 4) {
+            const uint32_t j = u % NS, at = u / NS == 1 ? first + 1 : first;
+            if (at >= end) continue;
+            const uint8_t *from = (u / NS == 2 ? v : k) + (size_t)at * (32 * D) + 1024 * j + 16 * lane;
+            put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
+        }
+        float vnow = uniform(vs[first]);
+        c = q.c * uniform(ks[first]);
         fetch(first);
-        stage(0);
-    }
-    uint32_t side = 0;
-    for (uint32_t blk = first; blk < end; blk += SB, side ^= 1) {
-        float kc[SB], vc[SB];
+        fetch_scales(first);
+        __syncthreads();
+        u32x4 kf[2 * NS];
 #pragma unroll
-        for (int i = 0; i < SB; ++i) {
-            kc[i] = uniform(kscale[i]);
-            vc[i] = uniform(vscale[i]);
+        for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][first & 1][j][lane];
+        p = f32x16{};
+        key_steps(p, kf);
+        float top = row_top(p) * c;
+        top = fmaxf(top, xchg32(top, lane));
+        enter(top, vnow, first * 32);
+        for (uint32_t n = first; n + 1 < end; ++n) {
+            // a wave in its body goes before one that is still at the barrier's end: 593 -> 570 us for 2048 tokens over 14000
+            // (32/4 heads, D 128); with one wave a SIMD there is none to go before
+            if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(0);
+            __syncthreads();
+            if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(1);
+            vnow = body(std::true_type{}, n, vnow);
         }
-        __syncthreads();  // this tile is written; the tile before, in the other half, has been read
-        if (blk + SB < end) fetch(blk + SB);
-#pragma unroll
-        for (int sb = 0; sb < SB; ++sb) {
-            const uint32_t p0 = (blk + sb) * 32;
-            if (blk + sb >= end || p0 >= wave_most) break;
-            if (p0 + 32 > wave_least || !(vc[sb] < INFINITY))
-                block(std::true_type{}, lds[side][sb][0], lds[side][sb][1], kc[sb], vc[sb], p0);
-            else
-                block(std::false_type{}, lds[side][sb][0], lds[side][sb][1], kc[sb], vc[sb], p0);
-        }
-        if (blk + SB < end) stage(side ^ 1);
+        __syncthreads();
+        body(std::false_type{}, end - 1, vnow);
     }
     if (!live) return;
     l += xchg32(l, lane);
-    const float norm = l == 0.0f ? 0.0f : vref / l;
+    const float norm = (l == 0.0f ? 0.0f : vref / l) + poison;
     if (w.parts == 1) {
         const size_t at = (size_t)t * a.q_heads + qh;
         if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
@@ -937,7 +966,7 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
         p.split.target = std::max((D <= 64 ? 1024 : (D <= 96 ? 768 : (D <= 192 ? 512 : 256))) / kv_heads, std::min(p.tiles, 1024u));
         p.grid = p.split.target + p.tiles;
     } else {
-        p.split.unit = D <= 64 ? kTileBlocks<2> : (D <= 128 ? kTileBlocks<4> : 1);
+        p.split.unit = 1;
         p.split.causal = 1;
         p.split.target = all < 256 ? std::max(512 / kv_heads, 1u) : 0;
         p.grid = 2 * p.split.target + p.tiles;

@@ -263,6 +263,26 @@ def test_attention_range_of_values(kv8, gain):
     cache = kv8.Kv8Cache(1, 1, d, n)
     kv8.append(cache, k.cuda(), v.cuda(), _i32([n]), starts=_starts([n]))
     _check_attention(kv8, cache, q, _starts([3]), _i32([n]))
+    q = (_rand(g, 40, 2, d).float() / gain).to(BF)  # as a chunk of many rows
+    _check_attention(kv8, cache, q, _starts([40]), _i32([n]))
+
+
+@pytest.mark.parametrize("m", [1, 60])
+def test_attention_over_values_near_the_smallest(kv8, m):
+    """Values whose scales are subnormal floats, blocks of zeros among them: within the codes' own steps of the exact result."""
+    g = torch.Generator().manual_seed(14)
+    n, d = 130, 64
+    k, v = _rand(g, n, 1, d), (_rand(g, n, 1, d).float() * 2.0 ** -122).to(BF)
+    v[32:64] = 0.0
+    cache = kv8.Kv8Cache(1, 1, d, n)
+    kv8.append(cache, k.cuda(), v.cuda(), _i32([n]), starts=_starts([n]))
+    q = _rand(g, m, 2, d)
+    out, _ = kv8.attention(cache, q.cuda(), _i32([n]), starts=_starts([m]))
+    _, vv = ref.read(cache, n)
+    want, _, mass, _, _ = ref.attention(q, *ref.read(cache, n), torch.tensor([0, m]), [n], 1 / 8, n)
+    # P and V relative to 2^-126 in fp16 (P's steps below 2^-14 are 2^-24, times codes up to 127), outputs in bf16 (subnormal step 2^-133)
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -10 * mass + n * 127 * 2.0 ** -25 * 2.0 ** -126 + 2.0 ** -133
+    assert (((out.cpu().double() - want).abs() - tol) <= 0).all() and float(want.abs().max()) > 0
 
 
 def test_attention_strided_queries_peaked_and_infinite_rows(kv8):

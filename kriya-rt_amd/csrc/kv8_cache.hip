@@ -11,9 +11,9 @@ namespace kr {
 
 namespace {
 
-// Codes a block from 32 x D values held as groups of 4 slots x 8 dims: group i of 128 threads is slots 4 (i / (D/8)) ..
-// + 3, dims 8 (i % (D/8)) .. + 7.  D <= 256: at most two groups a thread.
-constexpr uint32_t kGroups = 2;
+// A block is coded by two sides of 64 or 128 threads, keys and values.  A thread holds groups of 4 slots x 8 dims: group i is
+// slots 4 (i / (D / 8)) .. + 3, dims 8 (i % (D / 8)) .. + 7; D > 128 makes two groups a thread.
+__host__ __device__ constexpr uint32_t side_threads(uint32_t D) { return D <= 64 ? 64 : 128; }
 
 struct GroupAt {
     uint32_t g, u;  // 4 g: first slot; 8 u: first dim
@@ -22,34 +22,31 @@ __device__ __forceinline__ GroupAt group_at(uint32_t i, uint32_t units) { return
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// max |x| of the block over the 128 threads of a side (0 keys, 1 values), as bits: magnitudes order as integers, and
-// an infinity or NaN comes out on top.  All 256 threads call it.
-__device__ __forceinline__ float side_amax(uint32_t bits, uint32_t (&red)[4]) {
+// max |x| of the block over the waves of a side, as bits: magnitudes order as integers, and an infinity or NaN comes out on
+// top.  All threads of the workgroup call it.
+__device__ __forceinline__ float side_amax(uint32_t bits, uint32_t (&red)[4], uint32_t per_side) {
     bits = wave_max_u32(bits);
     const uint32_t w = threadIdx.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[w] = bits;
     __syncthreads();
-    return __uint_as_float(max(red[w & 2], red[(w & 2) + 1]));
+    return __uint_as_float(per_side == 64 ? red[w] : max(red[w & 2], red[(w & 2) + 1]));
 }
 
-__device__ __forceinline__ void store_codes(uint8_t *blk, bool values, GroupAt at, const float (&x)[4][8], float scale,
-                                            int e4m3) {
-    uint32_t code[4][8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) code[j][e] = kv8_code(x[j][e], scale, e4m3);
+// The codes of a group into the block's bytes in LDS, in the cache's order (straight to memory the values' words would be
+// spread 16 bytes apart: 64 lines an instruction).
+template <int E4M3>
+__device__ __forceinline__ void put_codes(uint8_t *blk, bool values, GroupAt at, const float (&x)[4][8], const Kv8Coder &c) {
     if (values) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<uint32_t *>(blk + kv8_value_at(at.g, 8 * at.u + e)) =
-                code[0][e] | code[1][e] << 8 | code[2][e] << 16 | code[3][e] << 24;
+                kv8_codes<E4M3>(c, x[0][e], x[1][e], x[2][e], x[3][e]);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const u32x2 w = {code[j][0] | code[j][1] << 8 | code[j][2] << 16 | code[j][3] << 24,
-                             code[j][4] | code[j][5] << 8 | code[j][6] << 16 | code[j][7] << 24};
+            const u32x2 w = {kv8_codes<E4M3>(c, x[j][0], x[j][1], x[j][2], x[j][3]),
+                             kv8_codes<E4M3>(c, x[j][4], x[j][5], x[j][6], x[j][7])};
             *reinterpret_cast<u32x2 *>(blk + kv8_key_at(4 * at.g + j, 8 * at.u)) = w;
         }
     }
@@ -77,29 +74,30 @@ __device__ __forceinline__ AppendSpan append_span(const Kv8AppendArgs &a, uint32
 
 }  // namespace
 
-// Workgroups 0 .. items * heads - 1: one block each (keys by threads 0 .. 127, values by the others), then one for
+// Workgroups 0 .. items * heads - 1: one block each (keys by the first side of threads, values by the second), then one for
 // every token's q.  A block that already holds tokens is coded again from its raw rows (at most 32 rows; all of a
 // decoded token's traffic is 24 KB a head, well under a microsecond of HBM), so its codes are those of the whole
-// block coded at once.  Bound by latency at one token a sequence: one round of loads, one reduction, one of stores.
+// block coded at once.  Bound by latency at one token a sequence: all rows are loaded in one round (from clamped addresses, what
+// does not count is zeroed after), with rotation after a round for positions and one for the table.
+// kRope: 0 none, 1 in 8-dim units, 2 any rotary_dim.
+template <int E4M3, int kGroups, int kRope>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32_t items) {
     __shared__ uint32_t red[4];
-    const uint32_t D = a.c.D, units = D / 8;
+    __shared__ __align__(16) uint8_t codes[2][kKv8Block * 128 * kGroups];
+    const uint32_t D = a.c.D, units = D / 8, per_side = blockDim.x / 2;
     if (blockIdx.x >= items * a.c.heads) {
-        const uint32_t t = blockIdx.x - items * a.c.heads;
-        const uint16_t *src = a.q + t * a.q_stride;
-        uint16_t *dst = a.q_out + t * a.q_stride;
-        if (a.rope_units)
-            rope_token<uint16_t, true>(a.rope, t, src, dst, a.q_heads, D);
-        else
-            rope_token<uint16_t, false>(a.rope, t, src, dst, a.q_heads, D);
+        if constexpr (kRope != 0) {
+            const uint32_t t = blockIdx.x - items * a.c.heads;
+            rope_token<uint16_t, kRope == 1>(a.rope, t, a.q + t * a.q_stride, a.q_out + t * a.q_stride, a.q_heads, D);
+        }
         return;
     }
     const uint32_t head = blockIdx.x % a.c.heads;
     uint32_t b, item;
     if (!kv8_find(blockIdx.x / a.c.heads, a.c.batch, [&](uint32_t i) { return append_span(a, i).items; }, b, item)) return;
     const AppendSpan s = append_span(a, b);
-    const bool values = threadIdx.x >= 128;
-    const uint32_t tid = threadIdx.x & 127;
+    const bool values = threadIdx.x >= per_side;
+    const uint32_t tid = values ? threadIdx.x - per_side : threadIdx.x;
     const size_t bh = (size_t)b * a.c.heads + head;
     uint16_t *open = (values ? a.c.vo : a.c.ko) + bh * kKv8Block * D;
     const uint16_t *fresh = (values ? a.v : a.k) + (size_t)head * D;
@@ -108,40 +106,78 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
         uint32_t top = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; ++i) {
-            if (tid + 128 * i >= D) continue;
-            const GroupAt at = group_at(tid + 128 * i, units);
+            const GroupAt at = group_at(min(tid + per_side * i, D - 1), units);  // (threads past D repeat the last group)
+            const uint16_t *row[4];
+            const float *cs[4];
+            bool turn[4];
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t slot = blk * kKv8Block + 4 * at.g + j;
+                const uint32_t slot = min(blk * kKv8Block + 4 * at.g + j, s.end - 1);
+                const uint32_t t = s.s.t0 + (max(slot, s.n0) + s.s.m - s.s.n);
+                row[j] = slot < s.n0 ? open + (slot % kKv8Block) * D : fresh + t * a.kv_stride;
+                if constexpr (kRope != 0) {
+                    const uint32_t pos = a.rope.positions[t];
+                    turn[j] = !values && slot >= s.n0 && pos < a.rope.rows && 8 * at.u < a.rope.rotary_dim;
+                    cs[j] = a.rope.cos_sin + (size_t)(turn[j] ? pos : 0u) * a.rope.rotary_dim;
+                }
+            }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][j][e] = 0.0f;
-                if (slot >= s.end) continue;
-                if (slot < s.n0) {
-                    load8(open + (4 * at.g + j) * D + 8 * at.u, x[i][j]);
+            for (uint32_t j = 0; j < 4; ++j) load8(row[j] + 8 * at.u, x[i][j]);
+            if constexpr (kRope == 1) {
+                const uint32_t half = a.rope.rotary_dim / 2;
+                const bool low = 8 * at.u < half;
+                const uint32_t turned = 8 * at.u < a.rope.rotary_dim ? at.u : 0u;  // a unit whose pairs are in the table
+                if (a.rope.interleaved) {
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        float c[8];
+                        load8(cs[j] + 8 * turned, c);
+                        if (turn[j]) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) rope_pair(x[i][j][e], x[i][j][e + 1], c[e], c[e + 1], x[i][j][e], x[i][j][e + 1]);
+                        }
+                    }
                 } else {
-                    const uint32_t t = s.s.t0 + (slot + s.s.m - s.s.n);
-                    const uint16_t *row = fresh + t * a.kv_stride;
-                    const uint32_t pos = values || !a.rope.cos_sin ? 0xFFFFFFFFu : a.rope.positions[t];
-                    if (!values && a.rope.cos_sin && pos < a.rope.rows) {
-                        rope_unit(row, at.u, a.rope.cos_sin + (size_t)pos * a.rope.rotary_dim, a.rope.rotary_dim,
-                                  a.rope.interleaved, x[i][j]);
+                    const uint32_t other = turned == 0 || low ? turned + half / 8 : turned - half / 8;
+                    const uint32_t pair = turned < half / 8 ? turned : turned - half / 8;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[i][j][e] = bf16_to_f32(pack_bf16_rne(x[i][j][e], 0.0f) & 0xFFFFu);
-                    } else {
-                        load8(row + 8 * at.u, x[i][j]);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        float o[8], c[16];
+                        load8(row[j] + 8 * other, o);
+                        load8(cs[j] + 16 * pair, *reinterpret_cast<float(*)[8]>(&c[0]));
+                        load8(cs[j] + 16 * pair + 8, *reinterpret_cast<float(*)[8]>(&c[8]));
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            float y0, y1;
+                            rope_pair(low ? x[i][j][e] : o[e], low ? o[e] : x[i][j][e], c[2 * e], c[2 * e + 1], y0, y1);
+                            if (turn[j]) x[i][j][e] = low ? y0 : y1;
+                        }
                     }
                 }
+            }
+            if constexpr (kRope == 2) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[i][j][e]));
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (turn[j]) rope_unit(row[j], at.u, cs[j], a.rope.rotary_dim, a.rope.interleaved, x[i][j]);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const bool there = blk * kKv8Block + 4 * at.g + j < s.end;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if constexpr (kRope != 0) x[i][j][e] = bf16_to_f32(pack_bf16_rne(x[i][j][e], 0.0f) & 0xFFFFu);
+                    x[i][j][e] = there ? x[i][j][e] : 0.0f;
+                    top = max(top, abs_bits(x[i][j][e]));
+                }
             }
         }
-        const float scale = side_amax(top, red) / kv8_largest(a.c.e4m3);
-        uint8_t *bytes = (values ? a.c.v : a.c.k) + (bh * a.c.blocks + blk) * (size_t)(kKv8Block * D);
+        const float scale = side_amax(top, red, per_side) / kv8_largest(E4M3);
+        const Kv8Coder coder = kv8_coder(scale);
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; ++i) {
-            if (tid + 128 * i >= D) continue;
-            const GroupAt at = group_at(tid + 128 * i, units);
-            store_codes(bytes, values, at, x[i], scale, a.c.e4m3);
+            if (tid + per_side * i >= D) continue;
+            const GroupAt at = group_at(tid + per_side * i, units);
+            put_codes<E4M3>(codes[values], values, at, x[i], coder);
             if (blk != s.last) continue;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
@@ -150,22 +186,40 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
             }
         }
         if (tid == 0) (values ? a.c.vs : a.c.ks)[bh * a.c.blocks + blk] = scale;
+        __syncthreads();
+        u32x4 *bytes = reinterpret_cast<u32x4 *>((values ? a.c.v : a.c.k) + (bh * a.c.blocks + blk) * (size_t)(kKv8Block * D));
+        for (uint32_t i = tid; i < kKv8Block * D / 16; i += per_side) bytes[i] = reinterpret_cast<const u32x4 *>(codes[values])[i];
         if (item != 0 || blk == s.last) return;
+        __syncthreads();
     }
 }
 
 hipError_t launch_kv8_append(const Kv8AppendArgs &a, hipStream_t s) {
     // at most one block a token, and 31 others a full block: the sequences' blocks are counted on the device
     const uint64_t items = a.step.starts ? a.step.tokens / kKv8Block + std::min(a.c.batch, a.step.tokens) : a.c.batch;
-    const uint32_t q_blocks = a.q ? a.step.tokens : 0;
-    kv8_append_kernel<<<dim3((uint32_t)(items * a.c.heads) + q_blocks), 256, 0, s>>>(a, (uint32_t)items);
+    const dim3 grid((uint32_t)(items * a.c.heads) + (a.q ? a.step.tokens : 0));
+    const uint32_t threads = 2 * side_threads(a.c.D);
+    const auto go = [&](auto rope) {
+        constexpr int kRope = decltype(rope)::value;
+        const uint32_t n = (uint32_t)items;
+        if (a.c.D <= 128) {
+            if (a.c.e4m3) kv8_append_kernel<1, 1, kRope><<<grid, threads, 0, s>>>(a, n);
+            else kv8_append_kernel<0, 1, kRope><<<grid, threads, 0, s>>>(a, n);
+        } else {
+            if (a.c.e4m3) kv8_append_kernel<1, 2, kRope><<<grid, threads, 0, s>>>(a, n);
+            else kv8_append_kernel<0, 2, kRope><<<grid, threads, 0, s>>>(a, n);
+        }
+    };
+    if (!a.rope.cos_sin) go(std::integral_constant<int, 0>{});
+    else if (a.rope_units) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 2>{});
     return hipGetLastError();
 }
 
 // ---- reading back
 
 // A thread takes 4 slots (aligned to the cache's groups of 4) x 8 dims of one head.
-template <class T>
+template <int E4M3, class T>
 __global__ __launch_bounds__(256) void kv8_dequant_kernel(Kv8 c, const uint32_t *lengths, const uint32_t *first,
                                                           uint32_t count, uint32_t groups, T *k_out, T *v_out) {
     const uint32_t units = c.D / 8, b = blockIdx.z;
@@ -192,15 +246,19 @@ __global__ __launch_bounds__(256) void kv8_dequant_kernel(Kv8 c, const uint32_t 
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const uint32_t v = *reinterpret_cast<const uint32_t *>(bytes + kv8_value_at(g, 8 * u + e));
+                float y[4];
+                kv8_values<E4M3>(v, y);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j][e] = kv8_value(v, j, c.e4m3) * scale;
+                for (int j = 0; j < 4; ++j) x[j][e] = y[j] * scale;
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const u32x2 v = *reinterpret_cast<const u32x2 *>(bytes + kv8_key_at(4 * g + j, 8 * u));
+                kv8_values<E4M3>(v.x, x[j]);
+                kv8_values<E4M3>(v.y, x[j] + 4);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[j][e] = kv8_value(e < 4 ? v.x : v.y, e & 3, c.e4m3) * scale;
+                for (int e = 0; e < 8; ++e) x[j][e] *= scale;
             }
         }
     }
@@ -221,11 +279,15 @@ hipError_t launch_kv8_dequant(const Kv8 &c, const uint32_t *lengths, const uint3
     const uint32_t groups = (count + 3) / 4 + (first ? 1 : 0);
     const uint64_t threads = (uint64_t)groups * c.heads * (c.D / 8);
     const dim3 grid((uint32_t)((threads + 255) / 256), 2, c.batch);
-    if (f32)
-        kv8_dequant_kernel<float><<<grid, 256, 0, s>>>(c, lengths, first, count, groups, (float *)k_out, (float *)v_out);
-    else
-        kv8_dequant_kernel<uint16_t><<<grid, 256, 0, s>>>(c, lengths, first, count, groups, (uint16_t *)k_out,
-                                                          (uint16_t *)v_out);
+    const auto go = [&](auto e4m3, auto *k, auto *v) {
+        kv8_dequant_kernel<decltype(e4m3)::value><<<grid, 256, 0, s>>>(c, lengths, first, count, groups, k, v);
+    };
+    const auto of = [&](auto *k, auto *v) {
+        if (c.e4m3) go(std::integral_constant<int, 1>{}, k, v);
+        else go(std::integral_constant<int, 0>{}, k, v);
+    };
+    if (f32) of((float *)k_out, (float *)v_out);
+    else of((uint16_t *)k_out, (uint16_t *)v_out);
     return hipGetLastError();
 }
 
@@ -355,20 +417,23 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs
     }
 }
 
-// A workgroup per new block: keys by threads 0 .. 127, values by the others, as in the append.  The slots behind the
-// new length are given code 0.
+// A workgroup per new block: keys by the first side of threads (4 slots x 8 dims each, as in the append), values by the second, a
+// dim each with all 32 slots: its bytes lie 16 apart in the old blocks, so a wave's loads of one slot cover whole
+// lines, and its new bytes are two 16-byte units.  The slots behind the new length are given code 0.
+template <int E4M3, int kGroups>
 __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
     __shared__ uint32_t red[4];
     __shared__ uint32_t from[kKv8Block];
-    const uint32_t blk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.from.D, units = D / 8;
+    __shared__ __align__(16) uint8_t codes[kKv8Block * 128 * kGroups];
+    const uint32_t blk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.from.D, units = D / 8, per_side = blockDim.x / 2;
     const uint32_t n = min(a.lengths[b], a.from.max_ctx), left = min(n, a.budget);
     const uint32_t base = blk * kKv8Block;
     if (base >= left) return;
     const size_t bh = (size_t)b * a.from.heads + head;
     const uint32_t mine = min(left - base, kKv8Block), last = (left - 1) / kKv8Block, old_last = (n - 1) / kKv8Block;
-    const bool values = threadIdx.x >= 128, fits = n <= a.budget;
-    const uint32_t tid = threadIdx.x & 127;
-    if (threadIdx.x < kKv8Block) from[threadIdx.x] = threadIdx.x < mine ? a.kept[bh * a.budget + base + threadIdx.x] : 0u;
+    const bool values = threadIdx.x >= per_side, fits = n <= a.budget;
+    const uint32_t tid = values ? threadIdx.x - per_side : threadIdx.x;
+    if (threadIdx.x < kKv8Block) from[threadIdx.x] = a.kept[bh * a.budget + base + min(threadIdx.x, mine - 1)];
     __syncthreads();
     const size_t block_bytes = (size_t)kKv8Block * D;
     const uint8_t *src = (values ? a.from.v : a.from.k) + bh * a.from.blocks * block_bytes;
@@ -378,65 +443,103 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
     const uint16_t *open = (values ? a.from.vo : a.from.ko) + bh * block_bytes;
     uint16_t *to_open = (values ? a.to.vo : a.to.ko) + bh * block_bytes;
     if (fits || (blk != last && from[kKv8Block - 1] == base + kKv8Block - 1)) {  // in their places: slots only move down
-        for (uint32_t i = tid; i < block_bytes / 16; i += 128)
+        for (uint32_t i = tid; i < block_bytes / 16; i += per_side)
             reinterpret_cast<u32x4 *>(dst)[i] = reinterpret_cast<const u32x4 *>(src + blk * block_bytes)[i];
         if (blk == last)
-            for (uint32_t i = tid; i < block_bytes / 8; i += 128)
+            for (uint32_t i = tid; i < block_bytes / 8; i += per_side)
                 reinterpret_cast<u32x4 *>(to_open)[i] = reinterpret_cast<const u32x4 *>(open)[i];
         if (tid == 0) *ds = ss[blk];
         return;
     }
-    float x[kGroups][4][8];
+    // 32 elements a thread and group: x[i][4 j' + j] is slot 4 j' + j of dim tid (values), x[i][8 j + e] slot 4 g + j of
+    // dim 8 u + e (keys)
+    float x[kGroups][32];
     uint32_t top = 0;
+    const bool raw_rows = from[mine - 1] / kKv8Block == old_last;  // the block takes some of the old last block's
 #pragma unroll
     for (uint32_t i = 0; i < kGroups; ++i) {
-        if (tid + 128 * i >= D) continue;
-        const GroupAt at = group_at(tid + 128 * i, units);
+        const uint32_t d = min(tid + per_side * i, D - 1);  // (threads past D repeat the last)
+        const GroupAt at = group_at(d, units);
+        if (values) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t r = 4 * at.g + j;
+            for (uint32_t r = 0; r < kKv8Block; ++r) {
+                const uint32_t p = from[r], pb = p / kKv8Block, pr = p % kKv8Block;
+                x[i][r] = kv8_value<E4M3>(src[pb * block_bytes + kv8_value_at(pr / 4, d) + pr % 4]) * ss[pb];
+            }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][j][e] = 0.0f;
-            if (r >= mine) continue;
-            const uint32_t p = from[r], pb = p / kKv8Block, pr = p % kKv8Block;
-            if (pb == old_last) {
-                load8(open + pr * D + 8 * at.u, x[i][j]);
-            } else {
-                const uint8_t *bytes = src + pb * block_bytes;
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t p = from[4 * at.g + j], pb = p / kKv8Block;
+                const u32x2 v = *reinterpret_cast<const u32x2 *>(src + pb * block_bytes + kv8_key_at(p % kKv8Block, 8 * at.u));
                 const float scale = ss[pb];
-                if (values) {
+                kv8_values<E4M3>(v.x, &x[i][8 * j]);
+                kv8_values<E4M3>(v.y, &x[i][8 * j + 4]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        x[i][j][e] = kv8_value(bytes[kv8_value_at(pr / 4, 8 * at.u + e) + pr % 4], 0, a.from.e4m3) * scale;
-                } else {
-                    const u32x2 v = *reinterpret_cast<const u32x2 *>(bytes + kv8_key_at(pr, 8 * at.u));
+                for (int e = 0; e < 8; ++e) x[i][8 * j + e] *= scale;
+            }
+        }
+        if (raw_rows || blk == last) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[i][j][e] = kv8_value(e < 4 ? v.x : v.y, e & 3, a.from.e4m3) * scale;
+            for (uint32_t y = 0; y < 32; ++y) {
+                const uint32_t r = values ? y : 4 * at.g + y / 8, dim = values ? d : 8 * at.u + y % 8, p = from[r];
+                if (p / kKv8Block == old_last) x[i][y] = bf16_to_f32(open[(p % kKv8Block) * D + dim]);
+                if (blk == last) {
+                    const uint32_t bits = pack_bf16_rne(x[i][y], 0.0f) & 0xFFFFu;
+                    x[i][y] = bf16_to_f32(bits);
+                    if (r < mine && tid + per_side * i < D) to_open[r * D + dim] = (uint16_t)bits;
                 }
             }
-            if (blk == last) {
+        }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][j][e] = bf16_to_f32(pack_bf16_rne(x[i][j][e], 0.0f) & 0xFFFFu);
-                store8(to_open + r * D + 8 * at.u, x[i][j]);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[i][j][e]));
+        for (uint32_t y = 0; y < 32; ++y) {
+            x[i][y] = (values ? y : 4 * at.g + y / 8) < mine ? x[i][y] : 0.0f;
+            top = max(top, abs_bits(x[i][y]));
         }
     }
-    const float scale = side_amax(top, red) / kv8_largest(a.from.e4m3);
+    const float scale = side_amax(top, red, per_side) / kv8_largest(E4M3);
+    const Kv8Coder coder = kv8_coder(scale);
 #pragma unroll
     for (uint32_t i = 0; i < kGroups; ++i) {
-        if (tid + 128 * i >= D) continue;
-        store_codes(dst, values, group_at(tid + 128 * i, units), x[i], scale, a.from.e4m3);
+        const uint32_t d = tid + per_side * i;
+        if (d >= D) continue;
+        if (values) {
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                u32x4 w;
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y) {  // slots 16 s + 8 a + 4 h + j, y = 2 a + s
+                    const uint32_t r = 16 * (y & 1) + 8 * (y >> 1) + 4 * h;
+                    w[y] = kv8_codes<E4M3>(coder, x[i][r], x[i][r + 1], x[i][r + 2], x[i][r + 3]);
+                }
+                *reinterpret_cast<u32x4 *>(dst + kv8_value_at(h, d)) = w;
+            }
+        } else {
+            float y[4][8];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e / 8][e % 8] = x[i][e];
+            put_codes<E4M3>(codes, false, group_at(d, units), y, coder);
+        }
     }
     if (tid == 0) *ds = scale;
+    __syncthreads();
+    if (!values)
+        for (uint32_t i = tid; i < block_bytes / 16; i += per_side)
+            reinterpret_cast<u32x4 *>(dst)[i] = reinterpret_cast<const u32x4 *>(codes)[i];
 }
 
 hipError_t launch_kv8_evict(const Kv8EvictArgs &a, hipStream_t s) {
     kv8_select_kernel<<<dim3(a.from.heads, a.from.batch), kSelectThreads, 0, s>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
     const uint32_t blocks = (a.budget + kKv8Block - 1) / kKv8Block;
-    kv8_gather_kernel<<<dim3(blocks, a.from.heads, a.from.batch), 256, 0, s>>>(a);
+    const dim3 grid(blocks, a.from.heads, a.from.batch);
+    const uint32_t threads = 2 * side_threads(a.from.D);
+    if (a.from.D <= 128) {
+        if (a.from.e4m3) kv8_gather_kernel<1, 1><<<grid, threads, 0, s>>>(a);
+        else kv8_gather_kernel<0, 1><<<grid, threads, 0, s>>>(a);
+    } else {
+        if (a.from.e4m3) kv8_gather_kernel<1, 2><<<grid, threads, 0, s>>>(a);
+        else kv8_gather_kernel<0, 2><<<grid, threads, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 

@@ -303,46 +303,59 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr uint32_t kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
+constexpr uint32_t kSelectHeld = 16;    // weights a thread holds in registers: contexts up to 16384
+constexpr uint32_t kSelectCopies = 8;   // of the histogram: the lanes of a wave share a few exponents, and take turns at a word
 
-}  // namespace
+// The slots of a wave: run consecutive ones, 64 an index.
+struct SelectRun {
+    const float *w;
+    uint32_t p0, run, n;
+};
 
-// A workgroup per (sequence, head): the kept slots in order.  Of the middle (slots sink .. n - recent - 1) the `want`
-// largest keys: the smallest of them is found eight bits a pass by histograms, ties are taken from the lowest
-// slot.  Then every wave counts its run of slots, and writes the kept ones behind those of the waves before it.
-__global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t found[2];                          // the digit, and how many keys of larger digits
-    __shared__ uint32_t kept_of[kSelectWaves], ties_of[kSelectWaves];
-    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const size_t bh = (size_t)b * a.from.heads + head;
-    const float *w = a.weight + bh * a.from.max_ctx;
-    float *to_w = a.to_weight + bh * a.to.max_ctx;
-    uint32_t *kept = a.kept + bh * a.budget;
-    const uint32_t n = min(a.lengths[b], a.from.max_ctx);
-    if (a.to_lengths && head == 0 && tid == 0) a.to_lengths[b] = min(n, a.budget);
-    if (n <= a.budget) {
-        for (uint32_t p = tid; p < n; p += kSelectThreads) {
-            kept[p] = p;
-            to_w[p] = w[p];
+// kHeld: run <= 64 kSelectHeld, the weights read once; else from memory (the caches) each time.
+template <bool kHeld>
+__device__ void select_slots(const Kv8EvictArgs &a, const SelectRun &s, float *to_w, uint32_t *kept,
+                             uint32_t (&hist)[256][kSelectCopies + 1], uint32_t (&found)[2], uint32_t (&kept_of)[kSelectWaves],
+                             uint32_t (&ties_of)[kSelectWaves]) {
+    const uint32_t tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    float held[kSelectHeld];
+    const auto slot = [&](uint32_t i) { return s.p0 + 64 * i + lane; };
+    const auto hold = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t i = 0; i < kSelectHeld; ++i) held[i] = s.w[min(slot(first + i), s.n - 1)];
+    };
+    if constexpr (kHeld) hold(0);
+    // f(slot, weight) for the wave's slots, 64 at a time, all lanes together
+    const auto each = [&](auto &&f) {
+        for (uint32_t first = 0; first < (kHeld ? 1 : s.run / 64); first += kSelectHeld) {
+            if constexpr (!kHeld) hold(first);
+#pragma unroll
+            for (uint32_t i = 0; i < kSelectHeld; ++i)
+                if (64 * (first + i) < s.run) f(slot(first + i), held[i]);
         }
-        return;
-    }
-    const uint32_t lo = a.sink, hi = n - a.recent;  // sink + recent <= budget < n
+    };
+    const uint32_t lo = a.sink, hi = s.n - a.recent;  // sink + recent <= budget < n
     uint32_t want = a.budget - a.sink - a.recent;
     uint32_t prefix = 0, mask = 0;
-    if (want) {
+    const bool any = want > 0;
+    if (any) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            for (uint32_t i = tid; i < 256 * (kSelectCopies + 1); i += kSelectThreads) (&hist[0][0])[i] = 0;
             __syncthreads();
-            for (uint32_t p = lo + tid; p < hi; p += kSelectThreads) {
-                const uint32_t key = weight_key(w[p]);
-                if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-            }
+            each([&](uint32_t p, float w) {
+                const uint32_t key = weight_key(w);
+                if (p >= lo && p < hi && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u][lane % kSelectCopies], 1u);
+            });
             __syncthreads();
             if (wave == 0) {  // the digit in which the want-th largest falls: lane l holds digits 4 l .. 4 l + 3
                 uint32_t c[4], sum = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum += c[i] = hist[4 * lane + i];
+                for (int i = 0; i < 4; ++i) {
+                    c[i] = 0;
+#pragma unroll
+                    for (uint32_t x = 0; x < kSelectCopies; ++x) c[i] += hist[4 * lane + i][x];
+                    sum += c[i];
+                }
                 uint32_t above = sum;  // keys in this lane's digits and those of the lanes above
 #pragma unroll
                 for (uint32_t o = 1; o < 64; o *= 2) {
@@ -365,27 +378,19 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs
             want -= found[1];
             prefix |= found[0] << shift;
             mask |= 255u << shift;
-            __syncthreads();
         }
     }
     // keys above `prefix` stay, and the first `want` that equal it
-    const bool any = a.budget > a.sink + a.recent;
-    const uint32_t run = (n + kSelectThreads - 1) / kSelectThreads * 64;  // slots of a wave
-    const uint32_t p0 = wave * run, p1 = min(p0 + run, n);
-    uint32_t sure = 0, ties = 0;
-    for (uint32_t p = p0 + lane; p < p0 + run; p += 64) {
-        bool s = false, t = false;
-        if (p < p1) {
-            const uint32_t key = any ? weight_key(w[p]) : 0u;
-            const bool middle = p >= lo && p < hi;
-            s = !middle || (any && key > prefix);
-            t = middle && any && key == prefix;
-        }
-        sure += (uint32_t)__builtin_popcountll(__ballot(s));
-        ties += (uint32_t)__builtin_popcountll(__ballot(t));
-    }
+    const auto sure = [&](uint32_t p, uint32_t key) { return p < s.n && (p < lo || p >= hi || (any && key > prefix)); };
+    const auto tie = [&](uint32_t p, uint32_t key) { return p >= lo && p < hi && any && key == prefix; };
+    uint32_t sures = 0, ties = 0;
+    each([&](uint32_t p, float w) {
+        const uint32_t key = weight_key(w);
+        sures += (uint32_t)__builtin_popcountll(__ballot(sure(p, key)));
+        ties += (uint32_t)__builtin_popcountll(__ballot(tie(p, key)));
+    });
     if (lane == 0) {
-        kept_of[wave] = sure;
+        kept_of[wave] = sures;
         ties_of[wave] = ties;
     }
     __syncthreads();
@@ -394,27 +399,48 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs
         at += kept_of[i] + min(ties_of[i], want - min(tied, want));
         tied += ties_of[i];
     }
-    for (uint32_t p = p0 + lane; p < p0 + run; p += 64) {
-        bool s = false, t = false;
-        float wp = 0.0f;
-        if (p < p1) {
-            wp = w[p];
-            const uint32_t key = any ? weight_key(wp) : 0u;
-            const bool middle = p >= lo && p < hi;
-            s = !middle || (any && key > prefix);
-            t = middle && any && key == prefix;
-        }
-        const uint64_t tm = __ballot(t), below = (1ull << lane) - 1;
-        t = t && tied + (uint32_t)__builtin_popcountll(tm & below) < want;
+    each([&](uint32_t p, float w) {
+        const uint32_t key = weight_key(w);
+        const uint64_t below = (1ull << lane) - 1, tm = __ballot(tie(p, key));
+        const bool keep = sure(p, key) || (tie(p, key) && tied + (uint32_t)__builtin_popcountll(tm & below) < want);
         tied += (uint32_t)__builtin_popcountll(tm);
-        const uint64_t km = __ballot(s || t);
-        if (s || t) {
+        const uint64_t km = __ballot(keep);
+        if (keep) {
             const uint32_t i = at + (uint32_t)__builtin_popcountll(km & below);
             kept[i] = p;
-            to_w[i] = wp;
+            to_w[i] = w;
         }
         at += (uint32_t)__builtin_popcountll(km);
+    });
+}
+
+}  // namespace
+
+// A workgroup per (sequence, head): the kept slots in order.  Of the middle (slots sink .. n - recent - 1) the `want`
+// largest keys: the smallest of them is found eight bits a pass by histograms, ties are taken from the lowest
+// slot.  Then every wave counts its run of slots, and writes the kept ones behind those of the waves before it.
+__global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs a) {
+    __shared__ uint32_t hist[256][kSelectCopies + 1];  // (one word more: the digits' first words in different banks)
+    __shared__ uint32_t found[2];                      // the digit, and how many keys of larger digits
+    __shared__ uint32_t kept_of[kSelectWaves], ties_of[kSelectWaves];
+    const uint32_t head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const size_t bh = (size_t)b * a.from.heads + head;
+    const float *w = a.weight + bh * a.from.max_ctx;
+    float *to_w = a.to_weight + bh * a.to.max_ctx;
+    uint32_t *kept = a.kept + bh * a.budget;
+    const uint32_t n = min(a.lengths[b], a.from.max_ctx);
+    if (a.to_lengths && head == 0 && tid == 0) a.to_lengths[b] = min(n, a.budget);
+    if (n <= a.budget) {
+        for (uint32_t p = tid; p < n; p += kSelectThreads) {
+            kept[p] = p;
+            to_w[p] = w[p];
+        }
+        return;
     }
+    const uint32_t run = (n + kSelectThreads - 1) / kSelectThreads * 64;
+    const SelectRun s{w, (tid >> 6) * run, run, n};
+    if (run <= 64 * kSelectHeld) select_slots<true>(a, s, to_w, kept, hist, found, kept_of, ties_of);
+    else select_slots<false>(a, s, to_w, kept, hist, found, kept_of, ties_of);
 }
 
 // A workgroup per new block: keys by the first side of threads (4 slots x 8 dims each, as in the append), values by the second, a

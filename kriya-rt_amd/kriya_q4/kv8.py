@@ -23,6 +23,7 @@ from ._device import at, checked, stream_of
 
 INT8, E4M3 = 0, 1
 BLOCK = 32
+_BF16 = (torch.bfloat16,)
 
 
 class kr_kv8_cache(ctypes.Structure):
@@ -85,8 +86,14 @@ def _step(cache: Kv8Cache, tokens: int, starts, lengths) -> Tuple[Optional[int],
     return starts.data_ptr(), lengths.data_ptr()
 
 
+def _same(t: torch.Tensor, like: torch.Tensor) -> bool:
+    """Whether t has the type, shape, strides and device of a tensor that has been checked."""
+    return (t is like or (t.dtype is like.dtype and t.shape == like.shape and t.stride() == like.stride()
+                          and t.get_device() == like.get_device()))
+
+
 def _queries(cache: Kv8Cache, q: torch.Tensor) -> int:
-    stride = _rope.rows_of("q", q, (torch.bfloat16,), cache.k)
+    stride = _rope.rows_of("q", q, _BF16, cache.k)
     if q.shape[2] != cache.head_dim:
         raise ValueError(f"q has head_dim {q.shape[2]}, the cache {cache.head_dim}")
     return stride
@@ -98,11 +105,11 @@ def append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Ten
            positions: Optional[torch.Tensor] = None, layout: int = _rope.HALF, stream=None) -> None:
     """Codes k, v (bf16 [tokens, kv_heads, head_dim]) into the last slots of their sequences; with cos_sin and positions,
     k is rotated first and q into q_out (q where None), all in one launch (kr_kv8_append)."""
-    tokens = k.shape[0] if k.dim() == 3 else -1
-    stride = _rope.rows_of("k", k, (torch.bfloat16,), cache.k)
-    if _rope.rows_of("v", v, (torch.bfloat16,), cache.k) != stride or v.shape != k.shape:
-        raise ValueError("k and v must have the same shape and strides")
-    if tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
+    stride = _rope.rows_of("k", k, _BF16, cache.k)
+    if not _same(v, k) and (v.dtype is not k.dtype or v.shape != k.shape or _rope.rows_of("v", v, _BF16, cache.k) != stride):
+        raise ValueError("k and v must have the same type, shape and strides")
+    tokens, heads, d = k.shape
+    if heads != cache.kv_heads or d != cache.head_dim:
         raise ValueError(f"k must be [tokens, {cache.kv_heads}, {cache.head_dim}], not {tuple(k.shape)}")
     s, n = _step(cache, tokens, starts, lengths)
     r, qp, op, qs, heads = None, None, None, 0, 0
@@ -113,7 +120,7 @@ def append(cache: Kv8Cache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Ten
     if q is not None:
         q_out = q if q_out is None else q_out
         qs, heads = _queries(cache, q), q.shape[1]
-        if q.shape[0] != tokens or q_out.shape != q.shape or _queries(cache, q_out) != qs:
+        if q.shape[0] != tokens or not (_same(q_out, q) or (q_out.shape == q.shape and _queries(cache, q_out) == qs)):
             raise ValueError("q and q_out must have the tokens of k, and the same shape and strides")
         qp, op = q.data_ptr(), q_out.data_ptr()
     with at(cache.k):
@@ -127,11 +134,13 @@ def dequant(cache: Kv8Cache, lengths: torch.Tensor, count: int, first: Optional[
     lengths[b] on (kr_kv8_dequant)."""
     shape = (cache.batch, count, cache.kv_heads, cache.head_dim)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
+        device = cache.k.device
+        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    else:
+        checked("out[0]", out[0], out[0].dtype, shape, cache.k)
+        checked("out[1]", out[1], out[0].dtype, shape, cache.k)
     if out[0].dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dequant to {out[0].dtype}")
-    for t in out:
-        checked("out", t, out[0].dtype, shape, cache.k)
     _, n = _step(cache, 0, None, lengths)
     f = checked("first", first, torch.int32, (cache.batch,), cache.k).data_ptr() if first is not None else None
     with at(cache.k):

@@ -73,12 +73,13 @@ def rows_of(name: str, t: torch.Tensor, dtypes, like: Optional[torch.Tensor] = N
     """The token stride of t [tokens, heads, head_dim], whose heads lie side by side."""
     if t.dim() != 3 or t.dtype not in dtypes:
         raise ValueError(f"{name} must be [tokens, heads, head_dim] of {dtypes}, not {tuple(t.shape)} of {t.dtype}")
-    if not t.is_cuda or (like is not None and t.device != like.device):
+    if not t.is_cuda or (like is not None and t.get_device() != like.get_device()):
         raise ValueError(f"{name} must be on the same GPU as the other tensors")
     tokens, heads, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != d):
+    s0, s1, s2 = t.stride()
+    if (d > 1 and s2 != 1) or (heads > 1 and s1 != d):
         raise ValueError(f"{name}: the heads of a token must be contiguous, strides are {t.stride()}")
-    stride = t.stride(0) if tokens > 1 else max(heads * d, 1)
+    stride = s0 if tokens > 1 else max(heads * d, 1)
     if tokens > 1 and stride < heads * d:
         raise KrError(KR_E_SHAPE, f"{name}: tokens overlap, strides are {t.stride()}")
     return stride

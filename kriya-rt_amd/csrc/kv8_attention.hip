@@ -116,8 +116,7 @@ __device__ __forceinline__ uint32_t split_per(const Kv8AttnArgs &a, const Split 
         const uint32_t seen = w.causal ? past + (min(s.m, n) + 1) / 2 : n;  // never below half of n
         total += (unsigned long long)tiles_of(a, w, s) * ((seen + 31) / 32);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) total += __shfl_xor(total, o);
+    total = wave_sum_u64(total);
     const unsigned long long per = total >> 31 ? (total + w.target - 1) / w.target
                                                : ((uint32_t)total + w.target - 1) / w.target;
     return max((uint32_t)((per + w.unit - 1) / w.unit) * w.unit, w.unit);
@@ -164,10 +163,9 @@ __device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, 
         const Kv8Span s = kv8_span(a.step, i);
         before += tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
     }
-#pragma unroll
-    for (int x = 32; x > 0; x /= 2) before += __shfl_xor(before, x);
+    before = wave_sum_u32(before);
     step = tiles_of(a, w, o.s);
-    idx = __builtin_amdgcn_readfirstlane(before) + (w.causal ? step - 1 - o.tile : o.tile);
+    idx = before + (w.causal ? step - 1 - o.tile : o.tile);
     return true;
 }
 // parts of a tile: at most twice `target` and one (half of a tile's blocks may not be counted), and target is at most 1024
@@ -494,17 +492,23 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
     const uint32_t least = row_limit(s, r0, a.group, a.c.max_ctx);
     const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32), b = w.b;
     const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
-    f16x8_t q[NS];
-    float qc;
-    load_query16<NS>(q, qc, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
     const size_t bh = (size_t)b * a.c.heads + head;
     const uint8_t *k = a.c.k + bh * a.c.blocks * (size_t)(32 * D), *v = a.c.v + bh * a.c.blocks * (size_t)(32 * D);
     const float *ks = a.c.ks + bh * a.c.blocks, *vs = a.c.vs + bh * a.c.blocks;
+    uint32_t blk = first + wave;
+    // kFewAhead<NS> blocks of a wave on their way: with the waves that the registers allow about 100 KB a compute unit
+    constexpr uint32_t kAhead = kFewAhead<NS>;
+    FewBlock<NS> f[kAhead];
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i)
+        if (blk + i * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, blk + i * kFewWaves);
+    f16x8_t q[NS];
+    float qc;
+    load_query16<NS>(q, qc, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
     f32x4 o[2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -1e38f, l = 0.0f, vref = 0.0f;
-    uint32_t blk = first + wave;
     const auto step = [&](auto masked, const FewBlock<NS> &f, uint32_t blk) {
         constexpr bool kEdge = decltype(masked)::value;
         f32x4 p[2] = {};
@@ -557,12 +561,6 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
         for (int d = 0; d < 2 * NS; ++d)
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.v[d].x, f.v[d].y), pf, o[d], 0, 0, 0);
     };
-    // kFewAhead<NS> blocks of a wave on their way: with the waves that the registers allow about 100 KB a compute unit
-    constexpr uint32_t kAhead = kFewAhead<NS>;
-    FewBlock<NS> f[kAhead];
-#pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i)
-        if (blk + i * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, blk + i * kFewWaves);
     for (; blk < end; blk += kAhead * kFewWaves) {
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
@@ -745,8 +743,7 @@ __device__ __forceinline__ uint32_t weight_per(const Kv8AttnArgs &a, uint32_t ta
         const auto w = weight_span<kFew>(a, b);
         total += (unsigned long long)w.chunks * w.tiles;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o /= 2) total += __shfl_xor(total, o);
+    total = wave_sum_u64(total);
     const unsigned long long per = total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
     return max((uint32_t)per, 2u);
 }

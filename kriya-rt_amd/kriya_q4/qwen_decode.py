@@ -114,7 +114,7 @@ class QwenQ4Decoder:
         kv = c.kv_heads * c.head_dim
         self.layers: List[Layer] = []
         for _ in range(c.layers):
-            self.layers.append(Layer(
+            self.layers.append(self._placed(Layer(
                 ln1=_bf16(1.0 + 0.1 * torch.randn(c.hidden, device=device, generator=gen)),
                 ln2=_bf16(1.0 + 0.1 * torch.randn(c.hidden, device=device, generator=gen)),
                 q=_random_q4(c.q_heads * c.head_dim, c.hidden, gen, device),
@@ -131,7 +131,7 @@ class QwenQ4Decoder:
                                           generator=gen)),
                 v_cache=_bf16(torch.randn((batch, self.max_ctx, c.kv_heads, c.head_dim), device=device,
                                           generator=gen)),
-            ))
+            )))
         self.embed = _random_q4(c.vocab, c.hidden, gen, device)
         self.ln_f = _bf16(1.0 + 0.1 * torch.randn(c.hidden, device=device, generator=gen))
         self.cos_sin = rope_table(self.max_ctx, c.head_dim, c.rope_theta).to(device)
@@ -148,6 +148,10 @@ class QwenQ4Decoder:
         self.argmax_ws = argmax_workspace(batch, c.vocab, device=device)
         self.ws = rmsnorm_mlp_workspace(batch, c.hidden, c.inter, device=device)
         self.attn_ws = attention_q4_out_workspace(batch, c.q_heads, c.head_dim, self.max_ctx, device=device)
+
+    def _placed(self, layer: Layer) -> Layer:
+        """A new layer as the decoder keeps it."""
+        return layer
 
     def load_weights(self, archive) -> None:
         """Replaces the random weights with a checkpoint's (a kriya_q4.loader.Archive in the Hugging Face /

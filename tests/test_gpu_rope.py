@@ -35,7 +35,7 @@ def _freq(r, theta, kind, factor, ctx, slow, fast):
                                                  (256, (1 << 32) - 9, 9, 5e5)])
 def test_table(rope, kind, r, first, count, theta):
     if kind == "ntk" and r == 2:
-        pytest.skip("no such scaling of a single pair")
+        r = 4  # a single pair has no such scaling
     z = rope.Scaling(kind, 8.0, 4096, 1.0, 32.0, 1.25)
     got = rope.table(r, count, theta, first=first, scaling=z).cpu().double()
     pos = torch.arange(first, first + count, dtype=torch.float64)

@@ -106,22 +106,52 @@ __device__ __forceinline__ uint32_t tiles_of(const Kv8AttnArgs &a, const Split &
 __device__ __forceinline__ uint32_t blocks_of(const Kv8AttnArgs &a, const Kv8Span &s) {
     return (min(s.n, a.c.max_ctx) + 31) / 32;
 }
-// Blocks of a part.  Every wave computes it alike.
+__device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t per) { return max((blocks + per - 1) / per, 1u); }
+
+// Blocks of a part.  Every wave computes it alike.  Where the workgroups wanted are those that the card holds at once, a
+// few more would take a round of their own: `per` grows until the parts fit (300 tokens over 30000, 8/1 heads, D 256: 161 -> 120 us).
 __device__ __forceinline__ uint32_t split_per(const Kv8AttnArgs &a, const Split &w) {
     if (w.target == 0) return 1u << 26;  // more than a cache has
-    unsigned long long total = 0;
-    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+    uint32_t tiles = 0, seen = 0;        // of this lane's sequence: tiles, and the blocks that one of them sees
+    const auto look = [&](uint32_t b) {
+        tiles = seen = 0;
+        if (b >= a.c.batch) return;
         const Kv8Span s = kv8_span(a.step, b);
         const uint32_t n = min(s.n, a.c.max_ctx), past = n > s.m ? n - s.m : 0u;
-        const uint32_t seen = w.causal ? past + (min(s.m, n) + 1) / 2 : n;  // never below half of n
-        total += (unsigned long long)tiles_of(a, w, s) * ((seen + 31) / 32);
+        tiles = tiles_of(a, w, s);
+        seen = ((w.causal ? past + (min(s.m, n) + 1) / 2 : n) + 31) / 32;  // never below half of n
+    };
+    unsigned long long total = 0;
+    uint32_t all = 0;
+    for (uint32_t b = __lane_id(); b < (a.c.batch + 63) / 64 * 64; b += 64) {
+        look(b);
+        total += (unsigned long long)tiles * seen;
+        all += tiles;
     }
     total = wave_sum_u64(total);
-    const unsigned long long per = total >> 31 ? (total + w.target - 1) / w.target
-                                               : ((uint32_t)total + w.target - 1) / w.target;
-    return max((uint32_t)((per + w.unit - 1) / w.unit) * w.unit, w.unit);
+    all = wave_sum_u32(all);
+    const unsigned long long fair = total >> 31 ? (total + w.target - 1) / w.target
+                                                : ((uint32_t)total + w.target - 1) / w.target;
+    uint32_t per = max((uint32_t)((fair + w.unit - 1) / w.unit) * w.unit, w.unit);
+    // (few rows: their parts take a few microseconds, and this takes one)
+    if (!w.causal || 2 * (unsigned long long)all > w.target || total == 0) return per;  // else whole tiles are too many to fit them in
+    for (int i = 0; i < 6; ++i) {
+        uint32_t count = 0;
+        if (a.c.batch <= 64) {
+            count = tiles * parts_of(seen, per);
+        } else {
+            for (uint32_t b = __lane_id(); b < (a.c.batch + 63) / 64 * 64; b += 64) {
+                look(b);
+                count += tiles * parts_of(seen, per);
+            }
+        }
+        count = wave_sum_u32(count);
+        if (count <= w.target) break;
+        const uint32_t grown = (uint32_t)((unsigned long long)per * count / w.target);
+        per = max((grown + w.unit - 1) / w.unit * w.unit, per + w.unit);
+    }
+    return per;
 }
-__device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t per) { return max((blocks + per - 1) / per, 1u); }
 
 // What workgroup `idx` of a head does.
 struct Work {
@@ -965,7 +995,7 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
     } else {
         p.split.unit = 1;
         p.split.causal = 1;
-        p.split.target = all < 256 ? std::max(512 / kv_heads, 1u) : 0;
+        p.split.target = all < 256 ? std::max(256u * (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) / kv_heads, 1u) : 0;
         p.grid = 2 * p.split.target + p.tiles;
     }
     return p;

@@ -489,8 +489,10 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
         if (values) {
 #pragma unroll
             for (uint32_t r = 0; r < kKv8Block; ++r) {
-                const uint32_t p = from[r], pb = p / kKv8Block, pr = p % kKv8Block;
-                x[i][r] = kv8_value<E4M3>(src[pb * block_bytes + kv8_value_at(pr / 4, d) + pr % 4]) * ss[pb];
+                // the slot is the whole wave's: its part of the address in scalar registers
+                const uint32_t p = (uint32_t)__builtin_amdgcn_readfirstlane((int)from[r]), pb = p / kKv8Block, pr = p % kKv8Block;
+                const uint8_t *slot = src + (pb * block_bytes + kv8_value_at(pr / 4, 0) + pr % 4);
+                x[i][r] = kv8_value<E4M3>(slot[kv8_value_at(0, d)]) * ss[pb];
             }
         } else {
 #pragma unroll

@@ -309,6 +309,29 @@ def test_attention_takes_back_tokens_of_the_last_block(kv8):
     _check_attention(kv8, cache, _rand(g, 1, 2, 64), None, _i32([51]))
 
 
+@pytest.mark.parametrize("batch", [63, 64, 65, 130])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_many_sequences(kv8, batch, ragged):
+    """Batches around and past a wave's lanes, with empty sequences in them: appended, attended, weighted."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 60, (batch,), generator=g).tolist()
+    counts = [min(n, c) for n, c in zip(lens, torch.randint(0, 9, (batch,), generator=g).tolist())]
+    lens[-1], counts[-1] = 300, 200 if ragged else 1
+    if ragged:
+        lens[0] = counts[0] = 0
+    else:
+        counts = [1] * batch
+    cache = _fill(kv8, g, lens, 1, 64, 0, 310)
+    starts = _starts(counts) if ragged else None
+    q = _rand(g, sum(counts), 3, 64)
+    out, lse, want, off = _check_attention(kv8, cache, q, starts, _i32(lens))
+    w = torch.zeros(batch, 1, 310, device="cuda")
+    kv8.accumulate_weight(cache, q.cuda(), lse, _i32(lens), w, starts=starts)
+    want = want.clone()
+    tol = (4 * float(off.max()) + 900 * 2.0 ** -24 + 2.0 ** -20) * want + 1e-30
+    assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
 def test_attention_across_more_than_4_gib(kv8):
     """Offsets past 32 bits: the last sequence of a cache whose keys alone are more than 4 GiB."""
     g = torch.Generator().manual_seed(2)

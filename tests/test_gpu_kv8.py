@@ -332,6 +332,45 @@ def test_many_sequences(kv8, batch, ragged):
     assert ((w.cpu().double() - want).abs() <= tol).all()
 
 
+def test_calls_that_share_a_workspace_and_replays(kv8):
+    """One workspace under calls of many shapes back to back (decoding in parts, chunks in parts, whole prompts), eager and
+    captured, gives each call's own bits; 24 rounds."""
+    g = torch.Generator().manual_seed(33)
+    calls = []
+    for lens, counts, kv, group, d in (([3000] * 3 + [1, 2500], None, 2, 4, 64), ([4000], None, 1, 3, 64), ([2000, 3000], [40, 3], 1, 8, 64),
+                                       ([700] * 9, None, 8, 1, 64), ([6000], None, 1, 16, 128), ([500, 900] * 20, None, 2, 2, 96)):
+        cache = _fill(kv8, g, lens, kv, d, 0, max(lens))
+        starts = None if counts is None else _starts(counts)
+        q = _rand(g, len(lens) if counts is None else sum(counts), kv * group, d).cuda()
+        calls.append((cache, q, _i32(lens), starts))
+    own = [kv8.attention(*c[:3], starts=c[3]) for c in calls]
+    ws = max((kv8.attention_workspace(c[0], c[1].shape[1], c[1].shape[0]) for c in calls), key=lambda t: t.numel()).fill_(255)
+    outs = [(torch.empty_like(o), torch.empty_like(l)) for o, l in own]
+
+    def all_calls():
+        for (cache, q, n, st), (o, l) in zip(calls, outs):
+            kv8.attention(cache, q, n, starts=st, out=o, lse=l, workspace=ws)
+    all_calls()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            all_calls()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(24):
+        for o, l in outs:
+            o.zero_()
+            l.zero_()
+        if i % 2:
+            graph.replay()
+        else:
+            all_calls()
+        if i % 5 == 0:
+            torch.cuda.synchronize()
+        for (o, l), (wo, wl) in zip(outs, own):
+            assert torch.equal(o, wo) and torch.equal(l, wl), i
+
+
 def test_attention_across_more_than_4_gib(kv8):
     """Offsets past 32 bits: the last sequence of a cache whose keys alone are more than 4 GiB."""
     g = torch.Generator().manual_seed(2)

@@ -771,7 +771,9 @@ __device__ __forceinline__ uint32_t weight_per(const Kv8AttnArgs &a, uint32_t ta
     unsigned long long total = 0;
     for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
         const auto w = weight_span<kFew>(a, b);
-        total += (unsigned long long)w.chunks * w.tiles;
+        // chunks of new tokens are seen by half of the rows on average: never below half of all pairs
+        const uint32_t past = w.n > w.s.m ? w.n - w.s.m : 0u;
+        total += ((unsigned long long)w.chunks * w.tiles + (unsigned long long)(past / kWeightSlots) * w.tiles + 1) / 2;
     }
     total = wave_sum_u64(total);
     const unsigned long long per = total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
@@ -816,11 +818,6 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
         load_units<NS>(kw, a.c.k + (bh * a.c.blocks + blk) * (size_t)(32 * D));
         const float kscale = a.c.ks[bh * a.c.blocks + blk];
         f16x8_t kf[2 * NS];
-#pragma unroll
-        for (int j = 0; j < NS; ++j) {
-            kf[2 * j] = kv8_operand<E4M3>(kw[j].x, kw[j].y);
-            kf[2 * j + 1] = kv8_operand<E4M3>(kw[j].z, kw[j].w);
-        }
         // the threads of a row take its 8-dim units in turn
         constexpr uint32_t kOfRow = 256 / kRows;
         constexpr int kUnits = (D / 8 + kOfRow - 1) / kOfRow;
@@ -881,6 +878,14 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
                 lim[side][mine] = x.limit;
             }
         };
+        // the keys' operands, once the first rows are on their way too
+        const auto keys = [&] {
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                kf[2 * j] = kv8_operand<E4M3>(kw[j].x, kw[j].y);
+                kf[2 * j + 1] = kv8_operand<E4M3>(kw[j].z, kw[j].w);
+            }
+        };
         float sum = 0.0f;
         const auto tile_sum = [&](uint32_t side, uint32_t tile) {
             // the tile's first row sees the least; its last ones may lie behind the sequence's rows
@@ -913,6 +918,7 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
         if constexpr (kFew) {
             for (uint32_t tile = t0; tile < t1; ++tile) {
                 fetch(rows[0]);
+                if (tile == t0) keys();
                 stage(rows[0], 0);
                 __syncthreads();
                 tile_sum(0, tile);
@@ -922,6 +928,7 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
             if (t0 < t1) {
                 fetch(rows[0]);
                 fetch(rows[1]);
+                keys();
                 stage(rows[0], 0);
             }
             for (uint32_t tile = t0; tile < t1; tile += 2) {
@@ -1054,14 +1061,15 @@ static uint32_t weight_target(uint32_t kv_heads) { return std::max(kWeightTarget
 size_t kv8_weight_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens, uint32_t max_ctx) {
     if (few_rows(batch, group, tokens)) return 0;
     const size_t chunks = (size_t)batch * ((max_ctx + kWeightSlots - 1) / kWeightSlots);
-    return (weight_target(kv_heads) + chunks) * kv_heads * kWeightSlots * sizeof(float);
+    // at most 2 target + chunks parts a head: half of the pairs may not be counted
+    return (2 * weight_target(kv_heads) + chunks) * kv_heads * kWeightSlots * sizeof(float);
 }
 
 hipError_t launch_kv8_weight(const Kv8AttnArgs &a, hipStream_t s) {
     const uint32_t target = weight_target(a.c.heads);
     const uint64_t chunks = (uint64_t)a.c.batch * ((a.c.max_ctx + kWeightSlots - 1) / kWeightSlots);
     return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
-        const dim3 grid((uint32_t)std::min<uint64_t>(chunks + target, std::max(2048 / a.c.heads, 1u)), a.c.heads);
+        const dim3 grid((uint32_t)std::min<uint64_t>(chunks + 2 * target, std::max(2048 / a.c.heads, 1u)), a.c.heads);
         constexpr int NS = decltype(ns)::value, E4M3 = decltype(e4m3)::value;
         if (few_rows(a.c.batch, a.group, a.step.tokens)) {
             kv8_weight_kernel<NS, E4M3, true><<<grid, 256, 0, s>>>(a, target);

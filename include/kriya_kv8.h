@@ -121,7 +121,8 @@ int kr_kv8_dequant(const kr_kv8_cache *cache, const uint32_t *lengths, const uin
  * sums, maxima and the softmax are f32.  A row that sees no slot gives zeros and lse = -infinity.  A row whose q
  * is infinite or NaN, or that sees a block that stands for NaN, gives NaN.
  *   q, out: bf16 [tokens, q_heads, head_dim], q tokens q_stride elements apart (a multiple of 8), out contiguous; both 16-byte
- *   aligned; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads.
+ *   aligned and apart from each other; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
+ *   be negative or 0).
  * From one token per sequence to whole prompts; the launch is chosen from tokens, heads and batch alone.
  * workspace: kr_kv8_attention_workspace_bytes(cache, q_heads, tokens) bytes, 16-byte aligned, no initial contents; calls
  * sharing it must not overlap in time.  Results are the same bits from run to run. */

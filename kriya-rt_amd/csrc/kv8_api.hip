@@ -64,6 +64,8 @@ int check_queries(const kr_kv8_cache *c, const uint16_t *q, size_t q_stride, uin
     return KR_OK;
 }
 
+constexpr float kMaxScale = 0x1p100f;  // times log2(e) and a row's power of two it is a float
+
 bool finite_positive(double v) { return v > 0.0 && v < INFINITY; }
 
 }  // namespace
@@ -199,7 +201,7 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
                      void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = check_cache(cache, "cache")) return rc;
     if (int rc = check_queries(cache, q, q_stride, q_heads, tokens)) return rc;
-    if (!(fabsf(scale) < INFINITY)) return fail(KR_E_INVALID, "scale must be finite");
+    if (!(fabsf(scale) < kMaxScale)) return fail(KR_E_INVALID, "scale must be below 2^100 in size");
     if (tokens == 0 || cache->batch == 0) return ok();
     if (int rc = check_step(cache, tokens, starts, lengths)) return rc;
     if (!out) return fail(KR_E_INVALID, "out is NULL");
@@ -234,7 +236,8 @@ int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_
                              void *stream) {
     if (int rc = check_cache(cache, "cache")) return rc;
     if (int rc = check_queries(cache, q, q_stride, q_heads, tokens)) return rc;
-    if (!(fabsf(scale) < INFINITY) || !(fabsf(decay) < INFINITY)) return fail(KR_E_INVALID, "scale and decay must be finite");
+    if (!(fabsf(scale) < kMaxScale) || !(fabsf(decay) < INFINITY))
+        return fail(KR_E_INVALID, "scale must be below 2^100 in size, decay finite");
     if (tokens == 0 || cache->batch == 0) return ok();
     if (int rc = check_step(cache, tokens, starts, lengths)) return rc;
     if (!lse || !weight) return fail(KR_E_INVALID, "lse and weight must not be NULL");

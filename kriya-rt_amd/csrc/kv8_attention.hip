@@ -27,7 +27,7 @@ constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 template <int NS>
 struct QueryRow {
     f16x8_t f[2 * NS];
-    float c;  // scale log2(e) 2^-e
+    float c;  // |scale| log2(e) 2^-e (the sign goes into the row: a maximum stays one under c)
 };
 
 // The row in fp16 times a power of two that brings its largest value to [2^14, 2^15): bf16 holds 8 bits of significand
@@ -46,8 +46,8 @@ __device__ __forceinline__ void load_query(QueryRow<NS> &q, const uint16_t *row,
     }
     top = max(top, (uint32_t)__float_as_uint(xchg32(__uint_as_float(top), __lane_id())));
     const int e = row_stage_exp(top, 14, 14, 14);
-    const float up = exp2_int(e);
-    q.c = scale_log2 * exp2_int(-e);
+    const float up = copysignf(exp2_int(e), scale_log2);
+    q.c = fabsf(scale_log2) * exp2_int(-e);
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) {
         const uint32_t W[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
 // same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
 // A sequence's tiles all have as many parts as its longest: workgroup sum_{b' < b} tiles parts + part tiles + tile, and
 // those past a shorter tile's end have nothing to do.  (The tile varies first: workgroups go round the XCDs in turn, and
-// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads took 201 us so, and x now.)
+// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads, split, took 201 us so and 122 with the tile first.)
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
     uint32_t rows;    // of a tile
@@ -958,15 +958,18 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
 __global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnArgs a, uint32_t target) {
     const uint32_t head = blockIdx.y, per = weight_per<false>(a, target);
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {  // chunks
-        uint32_t b, chunk, before = 0;
+        uint32_t b, chunk;
         if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return weight_span<false>(a, i).chunks; }, b, chunk)) return;
         const auto w = weight_span<false>(a, b);
         const uint32_t parts = weight_parts(w.tiles, per), p = chunk * kWeightSlots + threadIdx.x;
-        if (parts == 1 || p >= w.n) continue;
-        for (uint32_t i = 0; i < b; ++i) {
+        if (parts == 1) continue;
+        uint32_t before = 0;
+        for (uint32_t i = __lane_id(); i < b; i += 64) {
             const auto o = weight_span<false>(a, i);
             before += o.chunks * weight_parts(o.tiles, per);
         }
+        before = wave_sum_u32(before);
+        if (p >= w.n) continue;
         const uint32_t seen = w.tiles - weight_first<false>(a, w, chunk), used = weight_parts(seen, per);
         const uint32_t old = w.s.n > w.s.m ? w.s.n - w.s.m : 0u;
         float *to = a.weight + ((size_t)b * a.c.heads + head) * a.c.max_ctx + p;

@@ -24,6 +24,14 @@ def stream_of(t: torch.Tensor, stream):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
+def held(t: torch.Tensor, stream) -> torch.Tensor:
+    """t, a tensor that a call allocates for itself on the current stream, kept from reuse until the call's own stream is done."""
+    if stream is not None:
+        t.record_stream(stream if isinstance(stream, torch.cuda.Stream) else
+                        torch.cuda.ExternalStream(stream_of(t, stream), device=t.device))
+    return t
+
+
 def checked(name: str, t: torch.Tensor, dtype, shape=None, like=None) -> torch.Tensor:
     """t, after a check of its type, its shape (where one is given), its contiguity and its device."""
     if t.dtype is not dtype:

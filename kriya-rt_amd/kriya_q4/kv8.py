@@ -19,7 +19,7 @@ import torch
 
 from . import DTYPE_BF16, DTYPE_F32, _check, lib
 from . import rope as _rope
-from ._device import at, checked, stream_of
+from ._device import at, checked, held, stream_of
 
 INT8, E4M3 = 0, 1
 BLOCK = 32
@@ -170,7 +170,7 @@ def attention(cache: Kv8Cache, q: torch.Tensor, lengths: torch.Tensor, starts: O
     checked("out", out, torch.bfloat16, (tokens, heads, d), cache.k)
     checked("lse", lse, torch.float32, (tokens, heads), cache.k)
     if workspace is None:
-        workspace = attention_workspace(cache, heads, tokens)
+        workspace = held(attention_workspace(cache, heads, tokens), stream)
     checked("workspace", workspace, torch.uint8, None, cache.k)
     with at(cache.k):
         _check(lib().kr_kv8_attention(cache.desc, q.data_ptr(), qs, heads, tokens, s, n,
@@ -196,7 +196,7 @@ def accumulate_weight(cache: Kv8Cache, q: torch.Tensor, lse: torch.Tensor, lengt
     checked("lse", lse, torch.float32, (tokens, heads), cache.k)
     checked("weight", weight, torch.float32, (cache.batch, cache.kv_heads, cache.max_ctx), cache.k)
     if workspace is None:
-        workspace = weight_workspace(cache, heads, tokens)
+        workspace = held(weight_workspace(cache, heads, tokens), stream)
     checked("workspace", workspace, torch.uint8, None, cache.k)
     with at(cache.k):
         _check(lib().kr_kv8_accumulate_weight(cache.desc, q.data_ptr(), qs, heads, tokens, s, n,

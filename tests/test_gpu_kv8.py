@@ -299,6 +299,43 @@ def test_attention_strided_queries_peaked_and_infinite_rows(kv8):
     assert torch.equal(o2[0, 1:], out[0, 1:]) and torch.equal(o2[1], out[1]) and torch.equal(l2[1], lse[1])
 
 
+@pytest.mark.parametrize("scale", [-0.25, 0.0, 1.5])
+@pytest.mark.parametrize("m", [1, 50])
+def test_attention_and_weights_at_any_scale(kv8, scale, m):
+    g = torch.Generator().manual_seed(19)
+    n, d = 200, 64
+    cache = _fill(kv8, g, [n], 2, d, 0, n)
+    q, starts, lens = _rand(g, m, 4, d), _starts([m]), _i32([n])
+    out, lse, want, off = _check_attention(kv8, cache, q, starts, lens, scale=scale)
+    w = kv8.accumulate_weight(cache, q.cuda(), lse, lens, torch.zeros(1, 2, n, device="cuda"), starts=starts, scale=scale)
+    tol = (4 * float(off.max()) + (n + 2 * m) * 2.0 ** -24 + 2.0 ** -20) * want + 1e-30
+    assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
+def test_calls_on_another_stream_with_workspaces_of_their_own(kv8):
+    """Calls on a side stream whose workspaces are freed as soon as they return, while the current stream allocates and fills."""
+    g = torch.Generator().manual_seed(23)
+    cache = _fill(kv8, g, [3000, 2000], 2, 64, 0, 3000)
+    q, lens = _rand(g, 400, 8, 64).cuda(), _i32([3000, 2000])
+    starts = _starts([300, 100])
+    own, lse = kv8.attention(cache, q, lens, starts=starts)
+    weight = kv8.accumulate_weight(cache, q, lse, lens, torch.zeros(2, 2, 3000, device="cuda"), starts=starts)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for stream in (side, side.cuda_stream):
+        got = []
+        for _ in range(4):
+            w = torch.zeros(2, 2, 3000, device="cuda")
+            side.wait_stream(torch.cuda.current_stream())
+            a = kv8.attention(cache, q, lens, starts=starts, stream=stream)
+            kv8.accumulate_weight(cache, q, lse, lens, w, starts=starts, stream=stream)
+            torch.full((8 << 20,), 255, dtype=torch.uint8, device="cuda")
+            got.append((a, w))
+        side.synchronize()
+        for (o, l), w in got:
+            assert torch.equal(o, own) and torch.equal(l, lse) and torch.equal(w, weight)
+
+
 def test_attention_takes_back_tokens_of_the_last_block(kv8):
     g = torch.Generator().manual_seed(6)
     cache = _fill(kv8, g, [60], 1, 64, 0, 64)

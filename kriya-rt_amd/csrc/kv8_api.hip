@@ -7,6 +7,9 @@
 namespace kr {
 namespace {
 
+// A launch has fewer than 2^32 threads in a dimension: this many workgroups of 256.
+constexpr uint64_t kMostGroups = 0xFFFFFFFFull / 256;
+
 bool on(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 
 int check_cache(const kr_kv8_cache *c, const char *name) {
@@ -42,6 +45,7 @@ int check_rope(const kr_rope *r, uint32_t head_dim) {
     if (!r->cos_sin || !r->positions) return fail(KR_E_INVALID, "rope: NULL pointer");
     if (r->layout != KR_ROPE_HALF && r->layout != KR_ROPE_INTERLEAVED) return fail(KR_E_INVALID, "rope: layout %d", r->layout);
     if (r->inverse != 0 && r->inverse != 1) return fail(KR_E_INVALID, "rope: inverse must be 0 or 1");
+    if (r->rows == 0) return fail(KR_E_SHAPE, "rope: the table has no rows");
     if (r->rotary_dim == 0 || r->rotary_dim % 2 || r->rotary_dim > head_dim)
         return fail(KR_E_SHAPE, "rope: rotary_dim=%u is not even, 2 .. head_dim=%u", r->rotary_dim, head_dim);
     if (!on(r->cos_sin, 8) || !on(r->positions, 4)) return fail(KR_E_ALIGN, "rope: cos_sin must be 8-byte aligned");
@@ -89,12 +93,12 @@ int kr_rope_table(float *cos_sin, uint32_t first, uint32_t count, uint32_t rotar
         return fail(KR_E_SHAPE, "NTK scaling needs rotary_dim > 2");
     if (z.kind == KR_ROPE_SCALE_PARTS && (!finite_positive(z.original_ctx) || !(z.slow < z.fast)))
         return fail(KR_E_INVALID, "scaling by parts needs original_ctx > 0 and slow < fast");
-    if (!(fabs(z.gain) < INFINITY)) return fail(KR_E_INVALID, "scaling gain must be finite");
+    if (!(fabsf((float)z.gain) < INFINITY)) return fail(KR_E_INVALID, "scaling gain must be finite in 32 bits");
     if ((uint64_t)first + count > (1ull << 32)) return fail(KR_E_SHAPE, "first + count exceeds 2^32");
     if (count == 0) return ok();
     if (!cos_sin) return fail(KR_E_INVALID, "cos_sin is NULL");
     if (!on(cos_sin, 8)) return fail(KR_E_ALIGN, "cos_sin must be 8-byte aligned");
-    if ((uint64_t)count * (rotary_dim / 2) > (1ull << 38)) return fail(KR_E_SHAPE, "table too large");
+    if ((uint64_t)count * (rotary_dim / 2) > kMostGroups * 256) return fail(KR_E_SHAPE, "count=%u is too large for one launch", count);
     RopeTurns f{};
     const double pi2 = 6.283185307179586476925, half = rotary_dim / 2;
     if (z.kind == KR_ROPE_SCALE_NTK) theta *= pow(z.factor, half / (half - 1.0));
@@ -124,7 +128,7 @@ int kr_rope_apply(const kr_rope *rope, const void *x, size_t x_stride, void *y, 
     if (x_stride < (size_t)heads * head_dim || y_stride < (size_t)heads * head_dim)
         return fail(KR_E_SHAPE, "strides below heads * head_dim");
     if (x == y && x_stride != y_stride) return fail(KR_E_SHAPE, "in place with different strides");
-    if (tokens > 0x7FFFFFFFu) return fail(KR_E_SHAPE, "tokens=%u exceeds 2^31 - 1", tokens);
+    if (tokens > kMostGroups) return fail(KR_E_SHAPE, "tokens=%u is too many for one launch", tokens);
     const size_t es = dtype == KR_DTYPE_F32 ? 4 : 2;
     if (!on(x, es) || !on(y, es)) return fail(KR_E_ALIGN, "x and y must be aligned to their elements");
     return hip_status(launch_rope_apply(to_rope(rope), x, x_stride, y, y_stride, dtype == KR_DTYPE_F32, tokens, heads,
@@ -154,7 +158,7 @@ int kr_kv8_append(const kr_kv8_cache *cache, const kr_rope *rope, const uint16_t
             return fail(KR_E_SHAPE, "q_stride=%zu is not a multiple of 8, at least q_heads * head_dim", q_stride);
         if (!on(q, 16) || !on(q_out, 16)) return fail(KR_E_ALIGN, "q and q_out must be 16-byte aligned");
     }
-    if (((uint64_t)tokens / kKv8Block + cache->batch) * cache->kv_heads + tokens > 0x7FFFFFFFull)
+    if (((uint64_t)tokens / kKv8Block + cache->batch) * cache->kv_heads + tokens > kMostGroups)
         return fail(KR_E_SHAPE, "too many tokens for one launch");
     Kv8AppendArgs a{};
     a.c = to_kv8(cache);
@@ -206,6 +210,8 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
     if (int rc = check_step(cache, tokens, starts, lengths)) return rc;
     if (!out) return fail(KR_E_INVALID, "out is NULL");
     if (!on(out, 16) || !on(lse, 4)) return fail(KR_E_ALIGN, "out must be 16-byte aligned, lse 4-byte");
+    if (kv8_attention_groups(cache->batch, cache->kv_heads, q_heads / cache->kv_heads, cache->head_dim, tokens) > kMostGroups)
+        return fail(KR_E_SHAPE, "tokens=%u of %u sequences and %u heads are too many for one launch", tokens, cache->batch, q_heads);
     const size_t need = kr_kv8_attention_workspace_bytes(cache, q_heads, tokens);
     if (need && (!workspace || workspace_bytes < need))
         return fail(KR_E_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
@@ -269,6 +275,7 @@ int kr_kv8_evict(const kr_kv8_cache *cache, const uint32_t *lengths, const float
     if (to->batch != cache->batch || to->kv_heads != cache->kv_heads || to->head_dim != cache->head_dim || to->format != cache->format)
         return fail(KR_E_SHAPE, "`to` must have the cache's batch, kv_heads, head_dim and format");
     if (budget == 0 || budget > to->max_ctx) return fail(KR_E_SHAPE, "budget=%u is not 1 .. to->max_ctx=%u", budget, to->max_ctx);
+    if ((budget + kKv8Block - 1) / kKv8Block > kMostGroups) return fail(KR_E_SHAPE, "budget=%u is too large for one launch", budget);
     if ((uint64_t)sink + recent > budget) return fail(KR_E_SHAPE, "sink=%u + recent=%u exceeds budget=%u", sink, recent, budget);
     if (cache->batch == 0) return ok();
     if (!lengths || !weight || !to_weight || !kept) return fail(KR_E_INVALID, "NULL pointer");

@@ -1013,6 +1013,11 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
 
 }  // namespace
 
+uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
+    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
+    return (uint64_t)p.grid * (p.few ? 1 : kv_heads);  // (few: heads are another dimension)
+}
+
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
     const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
     return p.split.target == 0 ? 0 : (size_t)p.grid * kv_heads * p.split.rows * (D + 2) * sizeof(float);

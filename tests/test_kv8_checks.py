@@ -170,6 +170,27 @@ def test_rope_refusals(kq):
     assert L.kr_rope_apply(None, 1, 1, 1, 1, 0, 1, 1, 2, None) == kq.KR_E_INVALID
 
 
+def test_calls_too_large_for_a_launch_and_tables_without_rows(kq):
+    from kriya_q4.rope import kr_rope, kr_rope_scaling
+
+    L, n, x, big = kq.lib(), 0x80000, 0x70000, 1 << 62
+    wide = _cache(batch=65535, kv_heads=65535)
+    empty = kr_rope(0x20000, 0x30000, 0, 64, 0, 0)
+    full = kr_rope(0x20000, 0x30000, 10, 64, 0, 0)
+    assert L.kr_rope_apply(ctypes.byref(empty), x, 256, x, 256, 0, 3, 2, 128, None) == kq.KR_E_SHAPE
+    assert L.kr_kv8_append(ctypes.byref(_cache()), ctypes.byref(empty), x, x, 128, None, None, 0, 0, 2, None, n, None) == kq.KR_E_SHAPE
+    assert L.kr_rope_apply(ctypes.byref(full), x, 256, x, 256, 0, 1 << 24, 2, 128, None) == kq.KR_E_SHAPE
+    assert L.kr_rope_table(x, 0, 1 << 26, 128, 1e4, None, None) == kq.KR_E_SHAPE
+    assert L.kr_rope_table(x, 0, 8, 128, 1e4, ctypes.byref(kr_rope_scaling(0, 1.0, 0.0, 0.0, 0.0, 1e39)), None) == kq.KR_E_INVALID
+    assert L.kr_kv8_append(ctypes.byref(wide), None, x, x, 65535 * 64, None, None, 0, 0, 65535, None, n, None) == kq.KR_E_SHAPE
+    assert L.kr_kv8_append(ctypes.byref(_cache()), None, x, x, 128, None, None, 0, 0, 1 << 25, n, n, None) == kq.KR_E_SHAPE
+    many = _cache(batch=60000, kv_heads=300)  # 33 rows a sequence and head, a workgroup each at least
+    assert L.kr_kv8_attention(ctypes.byref(many), x, 33 * 300 * 64, 33 * 300, 60000, n, n, 0.125, x, x, x, big, None) == kq.KR_E_SHAPE
+    long = dict(max_ctx=1 << 30)
+    to = _cache(k=0x110000, v=0x120000, k_scale=0x130000, v_scale=0x140000, k_open=0x150000, v_open=0x160000, **long)
+    assert L.kr_kv8_evict(ctypes.byref(_cache(**long)), n, x, 1 << 30, 0, 0, ctypes.byref(to), x + 64, x, None, None) == kq.KR_E_SHAPE
+
+
 def test_python_checks_name_the_tensor(kq):
     from kriya_q4 import kv8, rope
 

@@ -61,18 +61,6 @@ __device__ __forceinline__ void load_query(QueryRow<NS> &q, const uint16_t *row,
     }
 }
 
-// S^T of one block: 32 slots (rows) x 32 query rows (columns), without the scales.
-template <int NS, int E4M3>
-__device__ __forceinline__ f32x16 key_product(const u32x4 (&kw)[NS], const QueryRow<NS> &q) {
-    f32x16 s = {};
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kv8_operand<E4M3>(kw[j].x, kw[j].y), q.f[2 * j], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kv8_operand<E4M3>(kw[j].z, kw[j].w), q.f[2 * j + 1], s, 0, 0, 0);
-    }
-    return s;
-}
-
 // A lane's 16-byte units of a block's keys (or values): unit j of lane l at 1024 j + 16 l.
 template <int NS>
 __device__ __forceinline__ void load_units(u32x4 (&w)[NS], const uint8_t *blk) {
@@ -83,7 +71,7 @@ __device__ __forceinline__ void load_units(u32x4 (&w)[NS], const uint8_t *blk) {
 // Row r of sequence span s: the slots that it sees, 0 for a row past the end.
 __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint32_t group, uint32_t max_ctx) {
     const uint32_t i = r / group;
-    if (i >= s.m || s.n + i + 1 <= s.m) return 0u;
+    if (i >= s.m || s.n < s.m - i) return 0u;
     return min(s.n - s.m + i + 1, max_ctx);
 }
 
@@ -93,7 +81,8 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
 // same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
 // A sequence's tiles all have as many parts as its longest: workgroup sum_{b' < b} tiles parts + part tiles + tile, and
 // those past a shorter tile's end have nothing to do.  (The tile varies first: workgroups go round the XCDs in turn, and
-// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads, split, took 201 us so and 122 with the tile first.)
+// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads, split, took 201 us so, 122 with the
+// tile first.)
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
     uint32_t rows;    // of a tile
@@ -667,7 +656,9 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
     Work w;
     uint32_t idx, tiles;
     if (!find_tile(a, split, blockIdx.x / groups, w, idx, tiles)) return;
-    if (w.parts == 1) return;
+    // (starts that decrease can make more parts than the launch has: none behind its last)
+    if (idx < grid) w.parts = min(w.parts, (grid - idx + tiles - 1) / tiles);
+    if (w.parts == 1 || idx >= grid) return;
     const size_t step = (size_t)tiles * a.c.heads * split.rows;  // between parts, in rows
     const float *all_ml = a.part + (size_t)grid * a.c.heads * split.rows * D;
     const uint32_t way = tid / kQuads, quad = tid % kQuads, row0 = blockIdx.x % groups * per_group;
@@ -840,7 +831,7 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
                 if (live && u < D / 8) x.raw[i] = *reinterpret_cast<const u32x4 *>(a.q + t * a.q_stride + (size_t)qh * D + 8 * u);
             }
             x.lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
-            x.limit = live && w.s.n + ti + 1 > w.s.m ? min(w.s.n - w.s.m + ti + 1, a.c.max_ctx) : 0u;
+            x.limit = live && w.s.n >= w.s.m - ti ? min(w.s.n - w.s.m + ti + 1, a.c.max_ctx) : 0u;
             ti += step_i;
             tg += step_g;
             if (tg >= a.group) {

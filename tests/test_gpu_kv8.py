@@ -249,6 +249,30 @@ def test_attention_rows_that_see_nothing_and_cut_lengths(kv8):
     assert torch.equal(a[0], b[0]) and torch.equal(a[3:], b[3:]) and torch.equal(la[1], lb[1])
 
 
+def test_lengths_of_any_size_see_the_whole_cache_and_no_more(kv8):
+    """Lengths up to 2^32 - 1, the largest (-1 as int32): every slot there is, as for a length of max_ctx and all its tokens old."""
+    g = torch.Generator().manual_seed(29)
+    cache = _fill(kv8, g, [100, 100], 2, 64, 0, 100)
+    for counts in ([1, 1], [70, 3]):
+        starts, m = _starts(counts), sum(counts)
+        q = _rand(g, m, 4, 64).cuda()
+        lens = _i32([-1, 100 + counts[1]])
+        out, lse = kv8.attention(cache, q, lens, starts=starts)
+        each, each_lse = [], []
+        for t in range(m):  # each row by itself, at a length that sees all
+            b = int(t >= counts[0])
+            c = kv8.Kv8Cache.wrap(*(x[b:b + 1] for x in (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_open, cache.v_open)), 100)
+            o, l = kv8.attention(c, q[t:t + 1], _i32([100]))
+            each.append(o)
+            each_lse.append(l)
+        # fp16 probabilities in another grouping: 2^-11 of values below 6, and bf16's half step twice
+        assert (out.float() - torch.cat(each).float()).abs().max() <= 2 * (2.0 ** -11 + 2.0 ** -8) * 6
+        assert (lse - torch.cat(each_lse)).abs().max() <= 1e-5
+        w = kv8.accumulate_weight(cache, q, lse, lens, torch.zeros(2, 2, 100, device="cuda"), starts=starts)
+        got = w.sum(-1)  # every row's weights add up to one
+        assert (got - torch.tensor(counts, device="cuda")[:, None] * 2.0).abs().max() <= 1e-4 * max(counts)
+
+
 @pytest.mark.parametrize("gain", [1e-30, 1e-6, 1e3, 1e30])
 def test_attention_range_of_values(kv8, gain):
     """bf16 range: q and k of any size whose scores stay in f32, values of any size, blocks of values far apart."""

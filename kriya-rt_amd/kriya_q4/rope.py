@@ -97,8 +97,6 @@ def apply(x: torch.Tensor, cos_sin: torch.Tensor, positions: torch.Tensor, layou
         raise ValueError(f"out is {tuple(out.shape)}, x {tuple(x.shape)}")
     tokens, heads, d = x.shape
     r = descriptor(cos_sin, positions, tokens, layout, inverse, x)
-    if out.data_ptr() == x.data_ptr():
-        ys = xs
     with at(x):
         _check(lib().kr_rope_apply(ctypes.byref(r), x.data_ptr(), xs, out.data_ptr(), ys,
                                    DTYPE_F32 if x.dtype == torch.float32 else DTYPE_BF16, tokens, heads, d,

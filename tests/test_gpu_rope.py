@@ -129,3 +129,6 @@ def test_binding_refuses(rope):
         rope.apply(x, torch.zeros(4, 33, 2, device="cuda"), pos)
     with pytest.raises(RuntimeError, match="overlap"):
         rope.apply(torch.zeros(128, device="cuda").as_strided((2, 1, 64), (32, 64, 1)), cs, pos)
+    with pytest.raises(RuntimeError, match="different strides"):  # the same memory with tokens elsewhere
+        buf = torch.zeros(256, device="cuda")
+        rope.apply(buf.view(4, 1, 64)[:2], cs, pos, out=buf.view(2, 1, 128)[..., :64])

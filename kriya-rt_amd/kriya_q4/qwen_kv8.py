@@ -37,7 +37,8 @@ class QwenKv8Decoder(QwenQ4Decoder):
         super().__init__(cfg, batch, ctx, seed, device)
         positions = self._capacity if max_positions is None else max_positions
         self.cos_sin = rope.table(cfg.head_dim, positions, cfg.rope_theta, scaling=scaling, device=device)
-        self._used = ctx  # tokens of the longest sequence, as far as the calls made here tell
+        # tokens in the caches and next positions of the sequences, as far as the calls made here tell
+        self._used, self._next = [ctx] * batch, [ctx] * batch
         self._spare = None
         self.attn = torch.empty((batch, cfg.q_heads, cfg.head_dim), dtype=torch.bfloat16, device=device)
         self.lse = torch.empty((batch, cfg.q_heads), dtype=torch.float32, device=device)
@@ -78,18 +79,21 @@ class QwenKv8Decoder(QwenQ4Decoder):
             q4_linear(L.o, attn, y=h, accumulate=True, workspace=o_ws, stream=stream)
             rmsnorm_mlp(L.gate, L.up, L.down, h, L.ln2, c.eps, activation=ACT_SWIGLU, workspace=mlp_ws, stream=stream)
 
-    def _grow(self, tokens: int) -> None:
-        if self._used + tokens > self._capacity:
-            raise ValueError(f"{self._used} + {tokens} tokens exceed max_ctx={self._capacity}: evict first")
-        self._used += tokens
+    def _grow(self, counts) -> None:
+        used, after = ([a + n for a, n in zip(to, counts)] for to in (self._used, self._next))
+        if max(used) > self._capacity:
+            raise ValueError(f"a sequence of {max(used)} tokens exceeds max_ctx={self._capacity}: evict first")
+        if max(after) > self.cos_sin.shape[0]:
+            raise ValueError(f"position {max(after) - 1} has no row in the rotary table: max_positions={self.cos_sin.shape[0]}")
+        self._used, self._next = used, after
 
     def step(self, stream=None) -> torch.Tensor:
         """One greedy decode step of every sequence: `tokens` are appended at `positions`, both move on; returns the
         next-token buffer.  stream: a torch.cuda.Stream.  Nothing returns to the host, so a step can be captured and replayed
-        (as long as the caches hold: what does not fit is cut off)."""
+        (as long as caches and rotary table hold: keys that do not fit are cut off, positions past the table not turned)."""
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
             if not torch.cuda.is_current_stream_capturing():
-                self._grow(1)
+                self._grow([1] * self.batch)
             self.lengths.add_(1)
             embedding(self.embed, self.tokens, out=self.h, stream=stream)
             self._layers(self.h, self.x, (self.q, self.k, self.v), self.attn, self.lse, self.positions, None,
@@ -109,7 +113,7 @@ class QwenKv8Decoder(QwenQ4Decoder):
             raise ValueError(f"counts={counts} do not split {m} tokens over {self.batch} sequences")
         if m == 0:
             return self.next
-        self._grow(max(counts))
+        self._grow(counts)
         n = torch.tensor(counts, dtype=torch.int32, device=device)
         starts = torch.zeros(self.batch + 1, dtype=torch.int32, device=device)
         torch.cumsum(n, 0, dtype=torch.int32, out=starts[1:])
@@ -154,5 +158,5 @@ class QwenKv8Decoder(QwenQ4Decoder):
             self._spare = L.cache, L.weight
             L.cache, L.weight = cache, weight
         self.lengths.copy_(left)
-        self._used = min(self._used, budget)
+        self._used = [min(n, budget) for n in self._used]
 

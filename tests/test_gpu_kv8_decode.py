@@ -168,6 +168,26 @@ def test_evict_and_go_on(make):
     assert_rms_close(m.logits.cpu().numpy()[[1]], want[[19]], rel=BAR, what="prompt after the eviction")
 
 
+def test_sequences_grow_for_themselves_and_positions_end(make):
+    """Prompts of one sequence each that only fit one by one are taken; positions past the rotary table are refused, before
+    anything has changed."""
+    m = make(max_ctx=64, max_positions=66, track_weights=True)
+    ids = torch.zeros(24, dtype=torch.int32, device="cuda")
+    for b in range(BATCH):
+        m.prefill(ids, [24 * (i == b) for i in range(BATCH)])
+    assert m.lengths.tolist() == [64] * BATCH
+    with pytest.raises(ValueError, match="evict first"):
+        m.step()
+    m.evict(20, sink=2, recent=10)
+    m.step()
+    m.step()
+    with pytest.raises(ValueError, match="max_positions"):
+        m.step()
+    with pytest.raises(ValueError, match="max_positions"):
+        m.prefill(ids[:1], [0, 1, 0])
+    assert m.lengths.tolist() == [22] * BATCH and m.positions.tolist() == [66] * BATCH
+
+
 def test_refusals(make):
     m = make(max_ctx=42)
     m.step()

@@ -136,6 +136,7 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
  *   weight[p] = decay * (p < n - m ? weight[p] : 0) + sum over the m new tokens and the heads of the group of e^(scale q . K_p - lse)
  * with the lse that kr_kv8_attention gave for the same q (slots of the new tokens start at zero: no initial contents are
  * needed; slots from lengths[b] on are left as they were).  Sums in f32, in a fixed order.  tokens == 0 does nothing.
+ * The codes enter the matrix cores as bf16 (exact), as q does; the scores are f32.
  * workspace: kr_kv8_weight_workspace_bytes(cache, q_heads, tokens) bytes (none for few rows, else about the size of weight), 16-byte
  * aligned, no initial contents; calls sharing it must not overlap in time. */
 size_t kr_kv8_weight_workspace_bytes(const kr_kv8_cache *cache, uint32_t q_heads, uint32_t tokens);

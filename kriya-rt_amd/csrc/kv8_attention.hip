@@ -729,13 +729,16 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
 
 // ---- attention weights of the slots
 //
-// Column sums of the attention matrix, from K and the rows' lse alone: weight_p += sum_r 2^(c_r s_rp - lse_r).  The products are taken as
-// S = Q K^T here: a lane holds one slot (column l & 31), the rows are summed in its registers, and c_r and lse_r come from LDS.
-// A workgroup takes 128 slots, 32 a wave, whose keys stay in registers as fp16 operands, and walks the query rows that see
-// them in tiles of 64 that it turns to fp16 in LDS together, two tiles on their way.  Where there are many rows they are split into parts whose sums
-// kv8_weight_join_kernel adds in order.  The workgroups loop over the work that the lengths turn out to be.
-// Few rows a sequence (one or two tokens): tiles of 32, nothing on its way (21 -> 15 us for 16 decoded tokens over up to 8000
-// slots: more workgroups a compute unit), and no parts.
+// Column sums of the attention matrix, from K and the rows' lse alone: weight_p += sum_r 2^(c s_rp - lse_r).  The products are taken
+// as S = Q K^T here: a lane holds one slot (column l & 31), the rows are summed in its registers, and their lse come from LDS.
+// A workgroup takes 128 slots, 32 a wave, whose keys stay in registers, and walks the query rows that see them in tiles of 64:
+// one in LDS that is multiplied, the next one on its way.  Both operands are bf16, so that a query row enters as it is and only
+// the keys are converted, once a workgroup (with rows brought to fp16 as in the kernels above that took half of the vector
+// instructions: 2000 tokens of 16/2 heads, D 128, 46 -> 31 us; 1000 over 8000 in two sequences 95 -> 61 us, 550 TF/s).
+// Where there are many rows they are split into parts whose sums kv8_weight_join_kernel adds in order.  The workgroups loop over
+// the work that the lengths turn out to be.  Short calls are bound by latency: of the 31 us about 10 are instructions.
+// Few rows a sequence (one or two tokens): tiles of 32, nothing on its way, and no parts (16 decoded tokens over up to 8000 slots:
+// 21 us with tiles of 64, 13.5 so: more workgroups a compute unit).
 constexpr uint32_t kWeightSlots = 128, kWeightTarget = 768;
 constexpr uint32_t weight_rows(bool few) { return few ? 32 : 64; }
 
@@ -778,13 +781,26 @@ __device__ __forceinline__ uint32_t weight_first(const Kv8AttnArgs &a, const Wei
     return min(i0 * a.group / weight_rows(kFew), w.tiles);
 }
 
+// Eight codes as bf16, exact, times 2^-17: a sum of 256 of their products with bf16 values stays within f32.
+template <int E4M3>
+__device__ __forceinline__ bf16x8_t weight_key(uint32_t lo, uint32_t hi) {
+    float y[8];
+    kv8_values<E4M3>(lo, y);
+    kv8_values<E4M3>(hi, y + 4);
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(y[2 * i + 1] * 0x1p-17f), __float_as_uint(y[2 * i] * 0x1p-17f), 0x07060302u);
+    return __builtin_bit_cast(bf16x8_t, w);
+}
+
 template <int NS, int E4M3, bool kFew>
-__global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t target) {
+__global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t target) {
     constexpr uint32_t D = 32 * NS, kRows = weight_rows(kFew), kHalves = kRows / 32, kSides = kFew ? 1 : 2;
     __shared__ u32x4 ql[kSides][kHalves][2 * NS][64];         // [side][half of the rows][step][lane]
-    __shared__ __align__(16) float2 cl[kSides][kRows];  // c_r, -lse_r
-    __shared__ uint32_t lim[kSides][kRows];
-    const uint32_t lane = __lane_id(), h = lane >> 5, wave = threadIdx.x >> 6, head = blockIdx.y;
+    __shared__ __align__(16) float cl[kSides][kRows];         // -lse_r in powers of two
+    const uint32_t lane = __lane_id(), h = lane >> 5, head = blockIdx.y;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per = weight_per<kFew>(a, target);
     const auto count = [&](uint32_t i) {
         const auto w = weight_span<kFew>(a, i);
@@ -808,131 +824,93 @@ __global__ __launch_bounds__(256) void kv8_weight_kernel(Kv8AttnArgs a, uint32_t
         u32x4 kw[NS];
         load_units<NS>(kw, a.c.k + (bh * a.c.blocks + blk) * (size_t)(32 * D));
         const float kscale = a.c.ks[bh * a.c.blocks + blk];
-        f16x8_t kf[2 * NS];
-        // the threads of a row take its 8-dim units in turn
-        constexpr uint32_t kOfRow = 256 / kRows;
-        constexpr int kUnits = (D / 8 + kOfRow - 1) / kOfRow;
+        bf16x8_t kf[2 * NS];
+        const float ck = a.scale_log2 * (kscale * 0x1p17f);
+        // The query rows that see slot p are first_row .. w.rows - 1; the wave's slots are all seen from tile `clear` on.
+        const auto first_row = [&](uint32_t p) { return (p + w.s.m > w.s.n ? p + w.s.m - w.s.n : 0u) * a.group; };
+        const uint32_t row0 = p < w.n ? first_row(p) : w.rows, seen = w.rows - row0;
+        const uint32_t clear = p0 + 32 <= w.n ? (first_row(p0 + 31) + kRows - 1) / kRows : 0xFFFFFFFFu;
+        // kOfRow threads take a row's 16-byte units in turn.  Unit u = 4 j + 2 h + s goes to step 2 j + s of lane (row, h), its place
+        // turned by the unit: the rows and units that are written together, and the rows read together, lie in all banks.
+        constexpr uint32_t kOfRow = 256 / kRows, kUnits = (D / 8 + kOfRow - 1) / kOfRow;
         const uint32_t mine = threadIdx.x / kOfRow, first_u = threadIdx.x % kOfRow;
-        struct Rows {
-            u32x4 raw[kUnits];
-            float lse;
-            uint32_t limit;
-        } rows[2];
-        // the row that is fetched next: token ti, head tg of the group
-        uint32_t ti = (kRows * t0 + mine) / a.group, tg = (kRows * t0 + mine) % a.group;
-        const uint32_t step_i = kRows / a.group, step_g = kRows % a.group;
-        const auto fetch = [&](Rows &x) {
-            const bool live = ti < w.s.m;
-            const uint32_t t = w.s.t0 + ti, qh = head * a.group + tg;
+        const auto place = [](uint32_t lane, uint32_t u) { return lane ^ (16 / kOfRow * (u % kOfRow)); };
+        u32x4 raw[kUnits];
+        float lse = 0.0f;
+        uint32_t row = kRows * t0 + mine, tg = row % a.group;  // what is fetched next
+        const uint16_t *at = a.q + (w.s.t0 + row / a.group) * a.q_stride + (size_t)(head * a.group + tg) * D + 8 * first_u;
+        const float *lse_at = a.lse + (size_t)(w.s.t0 + row / a.group) * a.q_heads + head * a.group + tg;
+        const size_t next_token = a.q_stride - (size_t)a.group * D, next_tile = kRows / a.group * a.q_stride + (size_t)(kRows % a.group) * D;
+        const auto fetch = [&] {
+            const bool live = row < w.rows;
+            const uint16_t *from = live ? at : a.q;  // (what lies past the rows is not counted)
 #pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                x.raw[i] = u32x4{0, 0, 0, 0};
-                const uint32_t u = first_u + kOfRow * i;
-                if (live && u < D / 8) x.raw[i] = *reinterpret_cast<const u32x4 *>(a.q + t * a.q_stride + (size_t)qh * D + 8 * u);
-            }
-            x.lse = live ? a.lse[(size_t)t * a.q_heads + qh] * kLog2e : 0.0f;
-            x.limit = live && w.s.n >= w.s.m - ti ? min(w.s.n - w.s.m + ti + 1, a.c.max_ctx) : 0u;
-            ti += step_i;
-            tg += step_g;
+            for (uint32_t i = 0; i < kUnits; ++i)
+                if (D / 8 % kOfRow == 0 || first_u + kOfRow * i < D / 8) raw[i] = *reinterpret_cast<const u32x4 *>(from + 8 * kOfRow * i);
+            lse = *(live ? lse_at : a.lse);
+            row += kRows;
+            at += next_tile;
+            lse_at += kRows / a.group * a.q_heads + kRows % a.group;
+            tg += kRows % a.group;
             if (tg >= a.group) {
                 tg -= a.group;
-                ++ti;
+                at += next_token;
+                lse_at += a.q_heads - a.group;
             }
         };
-        const auto stage = [&](const Rows &x, uint32_t side) {
-            uint32_t top = 0;
+        const auto stage = [&](uint32_t side) {
 #pragma unroll
-            for (int i = 0; i < kUnits; ++i) top = max(top, bf16_unit_max_bits(x.raw[i]));
-            if constexpr (kFew) {
-                top = row16_max_u32<true>(top);  // groups of 8
-            } else {
-                top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0xB1, 0xF, 0xF, false));
-                top = max(top, (uint32_t)__builtin_amdgcn_update_dpp((int)top, (int)top, 0x4E, 0xF, 0xF, false));
-            }
-            const int e = row_stage_exp(top, 14, 14, 14);
-            const float up = exp2_int(e);
-#pragma unroll
-            for (int i = 0; i < kUnits; ++i) {
-                const uint32_t W[4] = {x.raw[i].x, x.raw[i].y, x.raw[i].z, x.raw[i].w};
-                f16x8_t f;
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    f[2 * y] = (_Float16)(__uint_as_float(W[y] << 16) * up);
-                    f[2 * y + 1] = (_Float16)(__uint_as_float(W[y] & 0xFFFF0000u) * up);
-                }
-                // unit 4 j + 2 h + s is step 2 j + s of lane (row, h)
+            for (uint32_t i = 0; i < kUnits; ++i) {
                 const uint32_t u = first_u + kOfRow * i;
-                if (u < D / 8) ql[side][mine >> 5][2 * (u >> 2) + (u & 1)][(mine & 31) + 32 * ((u >> 1) & 1)] = __builtin_bit_cast(u32x4, f);
+                if (D / 8 % kOfRow == 0 || u < D / 8)
+                    ql[side][mine >> 5][2 * (u >> 2) + (u & 1)][place((mine & 31) + 32 * ((u >> 1) & 1), u)] = raw[i];
             }
-            if (first_u == 0) {
-                cl[side][mine] = make_float2(a.scale_log2 * exp2_int(-e), -x.lse);
-                lim[side][mine] = x.limit;
-            }
-        };
-        // the keys' operands, once the first rows are on their way too
-        const auto keys = [&] {
-#pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                kf[2 * j] = kv8_operand<E4M3>(kw[j].x, kw[j].y);
-                kf[2 * j + 1] = kv8_operand<E4M3>(kw[j].z, kw[j].w);
-            }
+            if (first_u == 0) cl[side][mine] = -lse * kLog2e;
         };
         float sum = 0.0f;
         const auto tile_sum = [&](uint32_t side, uint32_t tile) {
-            // the tile's first row sees the least; its last ones may lie behind the sequence's rows
-            const bool edge = __builtin_amdgcn_readfirstlane(lim[side][0]) < p0 + 32 || kRows * (tile + 1) > w.rows;
+            const bool edge = tile < clear || kRows * (tile + 1) > w.rows;
 #pragma unroll
             for (uint32_t x = 0; x < kHalves; ++x) {
-                if (kRows * tile + 32 * x >= w.rows) break;
                 f32x16 s = {};
 #pragma unroll
                 for (int j = 0; j < 2 * NS; ++j)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, ql[side][x][j][lane]), kf[j], s, 0, 0, 0);
-                if (edge) {
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, ql[side][x][j][place(lane, 4 * (j >> 1) + 2 * h + (j & 1))]), kf[j], s, 0, 0, 0);
+                const auto rows = [&](auto all) {
+                    const uint32_t r = kRows * tile + 32 * x + 4 * h - row0;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const uint32_t r = 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
-                        const float2 c = cl[side][r];
-                        const float y = __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y));
-                        sum += p < lim[side][r] ? y : 0.0f;
-                    }
-                } else {
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x4 c = *reinterpret_cast<const f32x4 *>(&cl[side][32 * x + 2 * i + 4 * h]);
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const f32x4 c = *reinterpret_cast<const f32x4 *>(&cl[side][32 * x + 8 * (i >> 2) + 4 * h + (i & 3)]);
-                        sum += __builtin_amdgcn_exp2f(fmaf(s[i], c.x * kscale, c.y));
-                        sum += __builtin_amdgcn_exp2f(fmaf(s[i + 1], c.z * kscale, c.w));
+                        for (int y = 0; y < 4; ++y) {
+                            const float e = __builtin_amdgcn_exp2f(fmaf(s[i + y], ck, c[y]));
+                            sum += decltype(all)::value || r + 2 * i + y < seen ? e : 0.0f;
+                        }
                     }
-                }
+                };
+                if (edge) rows(std::false_type{});
+                else rows(std::true_type{});
             }
         };
-        if constexpr (kFew) {
-            for (uint32_t tile = t0; tile < t1; ++tile) {
-                fetch(rows[0]);
-                if (tile == t0) keys();
-                stage(rows[0], 0);
-                __syncthreads();
-                tile_sum(0, tile);
-                if (tile + 1 < t1) __syncthreads();
+        if (t0 < t1) {
+            fetch();
+            // the keys' operands, once the first rows are on their way too
+#pragma unroll
+            for (int j = 0; j < NS; ++j) {
+                kf[2 * j] = weight_key<E4M3>(kw[j].x, kw[j].y);
+                kf[2 * j + 1] = weight_key<E4M3>(kw[j].z, kw[j].w);
             }
-        } else {
-            if (t0 < t1) {
-                fetch(rows[0]);
-                fetch(rows[1]);
-                keys();
-                stage(rows[0], 0);
-            }
-            for (uint32_t tile = t0; tile < t1; tile += 2) {
-                fetch(rows[0]);  // (rows past the end are not read)
-                __syncthreads();  // this tile is written, the one before has been read
-                tile_sum(0, tile);
-                if (tile + 1 >= t1) break;
-                stage(rows[1], 1);
-                fetch(rows[1]);
-                __syncthreads();
-                tile_sum(1, tile + 1);
-                if (tile + 2 < t1) stage(rows[0], 0);
-            }
+            stage(0);
+            if (t0 + 1 < t1) fetch();
+        }
+        for (uint32_t tile = t0; tile < t1; ++tile) {
+            const uint32_t side = kFew ? 0 : (tile - t0) & 1;
+            __syncthreads();  // this tile is written, the one before has been read
+            tile_sum(side, tile);
+            if (tile + 1 >= t1) break;
+            if constexpr (kFew) __syncthreads();
+            stage(kFew ? 0 : side ^ 1);
+            if (tile + 2 < t1) fetch();
         }
         sum += xchg32(sum, lane);
         if (lane < 32) {

@@ -336,6 +336,20 @@ def test_attention_and_weights_at_any_scale(kv8, scale, m):
     assert ((w.cpu().double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("gain", [1e-30, 1e30])
+@pytest.mark.parametrize("m", [1, 50])
+def test_accumulated_weights_range_of_values(kv8, gain, m):
+    """Keys near the ends of f32 against queries near the other: scores of ordinary size."""
+    g = torch.Generator().manual_seed(31)
+    n, d = 300, 96
+    cache = _fill(kv8, g, [n], 2, d, 0, n, gain=gain)
+    q, starts, lens = (_rand(g, m, 4, d).float() / gain).to(BF), _starts([m]), _i32([n])
+    out, lse, want, off = _check_attention(kv8, cache, q, starts, lens)
+    w = kv8.accumulate_weight(cache, q.cuda(), lse, lens, torch.zeros(1, 2, n, device="cuda"), starts=starts)
+    tol = (4 * float(off.max()) + (n + 2 * m) * 2.0 ** -24 + 2.0 ** -20) * want + 1e-30
+    assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
 def test_calls_on_another_stream_with_workspaces_of_their_own(kv8):
     """Calls on a side stream whose workspaces are freed as soon as they return, while the current stream allocates and fills."""
     g = torch.Generator().manual_seed(23)

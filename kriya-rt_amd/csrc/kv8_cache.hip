@@ -446,8 +446,11 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs
 // A workgroup per new block: keys by the first side of threads (4 slots x 8 dims each, as in the append), values by the second, a
 // dim each with all 32 slots: its bytes lie 16 apart in the old blocks, so a wave's loads of one slot cover whole
 // lines, and its new bytes are two 16-byte units.  The slots behind the new length are given code 0.
+// Bound by the latency of three dependent loads (kept slots, scales and bytes, stores) and by half of the vector instructions'
+// time; registers for four workgroups a compute unit (54 -> 52 us for the three launches of 8 sequences of 8100 cut to 4000, 2 heads,
+// D 128, read back; with five it took 56).
 template <int E4M3, int kGroups>
-__global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
+__global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(Kv8EvictArgs a) {
     __shared__ uint32_t red[4];
     __shared__ uint32_t from[kKv8Block];
     __shared__ __align__(16) uint8_t codes[kKv8Block * 128 * kGroups];
@@ -518,11 +521,12 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
                 }
             }
         }
+        if (mine < kKv8Block) {
 #pragma unroll
-        for (uint32_t y = 0; y < 32; ++y) {
-            x[i][y] = (values ? y : 4 * at.g + y / 8) < mine ? x[i][y] : 0.0f;
-            top = max(top, abs_bits(x[i][y]));
+            for (uint32_t y = 0; y < 32; ++y) x[i][y] = (values ? y : 4 * at.g + y / 8) < mine ? x[i][y] : 0.0f;
         }
+#pragma unroll
+        for (uint32_t y = 0; y < 32; ++y) top = max(top, abs_bits(x[i][y]));
     }
     const float scale = side_amax(top, red, per_side) / kv8_largest(E4M3);
     const Kv8Coder coder = kv8_coder(scale);

@@ -78,17 +78,18 @@ __device__ __forceinline__ float kv8_value(uint8_t b) {
 // outside 2^-70 .. 2^100 (a block of zeros, one that stands for NaN) take the division.
 struct Kv8Coder {
     float scale, inv;
-    bool plain;
+    bool plain;  // in a scalar register (else the compiler takes both ways and selects: 500 instructions more for 32 codes)
 };
+// scale: the same in all lanes
 __device__ __forceinline__ Kv8Coder kv8_coder(float scale) {
-    return Kv8Coder{scale, 1.0f / scale, scale >= 0x1p-70f && scale <= 0x1p100f};
+    return Kv8Coder{scale, 1.0f / scale, __builtin_amdgcn_readfirstlane(scale >= 0x1p-70f && scale <= 0x1p100f) != 0};
 }
 // Four codes in a word.  The quotients are at most M up to rounding, NaN only where the scale is infinite or NaN, which
 // is stored as code 0 (times that scale: NaN).
-template <int E4M3>
+template <int E4M3, bool kPlain>
 __device__ __forceinline__ uint32_t kv8_codes(const Kv8Coder &c, float x0, float x1, float x2, float x3) {
     float x[4] = {x0, x1, x2, x3};
-    if (c.plain) {
+    if constexpr (kPlain) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float q = x[j] * c.inv;

@@ -35,18 +35,18 @@ __device__ __forceinline__ float side_amax(uint32_t bits, uint32_t (&red)[4], ui
 
 // The codes of a group into the block's bytes in LDS, in the cache's order (straight to memory the values' words would be
 // spread 16 bytes apart: 64 lines an instruction).
-template <int E4M3>
+template <int E4M3, bool kPlain>
 __device__ __forceinline__ void put_codes(uint8_t *blk, bool values, GroupAt at, const float (&x)[4][8], const Kv8Coder &c) {
     if (values) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             *reinterpret_cast<uint32_t *>(blk + kv8_value_at(at.g, 8 * at.u + e)) =
-                kv8_codes<E4M3>(c, x[0][e], x[1][e], x[2][e], x[3][e]);
+                kv8_codes<E4M3, kPlain>(c, x[0][e], x[1][e], x[2][e], x[3][e]);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const u32x2 w = {kv8_codes<E4M3>(c, x[j][0], x[j][1], x[j][2], x[j][3]),
-                             kv8_codes<E4M3>(c, x[j][4], x[j][5], x[j][6], x[j][7])};
+            const u32x2 w = {kv8_codes<E4M3, kPlain>(c, x[j][0], x[j][1], x[j][2], x[j][3]),
+                             kv8_codes<E4M3, kPlain>(c, x[j][4], x[j][5], x[j][6], x[j][7])};
             *reinterpret_cast<u32x2 *>(blk + kv8_key_at(4 * at.g + j, 8 * at.u)) = w;
         }
     }
@@ -162,13 +162,16 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
             }
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-                const bool there = blk * kKv8Block + 4 * at.g + j < s.end;
+                if constexpr (kRope != 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if constexpr (kRope != 0) x[i][j][e] = bf16_to_f32(pack_bf16_rne(x[i][j][e], 0.0f) & 0xFFFFu);
-                    x[i][j][e] = there ? x[i][j][e] : 0.0f;
-                    top = max(top, abs_bits(x[i][j][e]));
+                    for (int e = 0; e < 8; ++e) x[i][j][e] = bf16_to_f32(pack_bf16_rne(x[i][j][e], 0.0f) & 0xFFFFu);
                 }
+                if (blk * kKv8Block + 4 * at.g + j >= s.end) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[i][j][e] = 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max(top, abs_bits(x[i][j][e]));
             }
         }
         const float scale = side_amax(top, red, per_side) / kv8_largest(E4M3);
@@ -177,7 +180,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
         for (uint32_t i = 0; i < kGroups; ++i) {
             if (tid + per_side * i >= D) continue;
             const GroupAt at = group_at(tid + per_side * i, units);
-            put_codes<E4M3>(codes[values], values, at, x[i], coder);
+            if (coder.plain) put_codes<E4M3, true>(codes[values], values, at, x[i], coder);
+            else put_codes<E4M3, false>(codes[values], values, at, x[i], coder);
             if (blk != s.last) continue;
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
@@ -530,28 +534,32 @@ __global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(K
     }
     const float scale = side_amax(top, red, per_side) / kv8_largest(E4M3);
     const Kv8Coder coder = kv8_coder(scale);
+    const auto put = [&](auto plain) {
 #pragma unroll
-    for (uint32_t i = 0; i < kGroups; ++i) {
-        const uint32_t d = tid + per_side * i;
-        if (d >= D) continue;
-        if (values) {
+        for (uint32_t i = 0; i < kGroups; ++i) {
+            const uint32_t d = tid + per_side * i;
+            if (d >= D) continue;
+            if (values) {
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-                u32x4 w;
+                for (uint32_t h = 0; h < 2; ++h) {
+                    u32x4 w;
 #pragma unroll
-                for (uint32_t y = 0; y < 4; ++y) {  // slots 16 s + 8 a + 4 h + j, y = 2 a + s
-                    const uint32_t r = 16 * (y & 1) + 8 * (y >> 1) + 4 * h;
-                    w[y] = kv8_codes<E4M3>(coder, x[i][r], x[i][r + 1], x[i][r + 2], x[i][r + 3]);
+                    for (uint32_t y = 0; y < 4; ++y) {  // slots 16 s + 8 a + 4 h + j, y = 2 a + s
+                        const uint32_t r = 16 * (y & 1) + 8 * (y >> 1) + 4 * h;
+                        w[y] = kv8_codes<E4M3, decltype(plain)::value>(coder, x[i][r], x[i][r + 1], x[i][r + 2], x[i][r + 3]);
+                    }
+                    *reinterpret_cast<u32x4 *>(dst + kv8_value_at(h, d)) = w;
                 }
-                *reinterpret_cast<u32x4 *>(dst + kv8_value_at(h, d)) = w;
-            }
-        } else {
-            float y[4][8];
+            } else {
+                float y[4][8];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e / 8][e % 8] = x[i][e];
-            put_codes<E4M3>(codes, false, group_at(d, units), y, coder);
+                for (int e = 0; e < 32; ++e) y[e / 8][e % 8] = x[i][e];
+                put_codes<E4M3, decltype(plain)::value>(codes, false, group_at(d, units), y, coder);
+            }
         }
-    }
+    };
+    if (coder.plain) put(std::true_type{});
+    else put(std::false_type{});
     if (tid == 0) *ds = scale;
     __syncthreads();
     if (!values)

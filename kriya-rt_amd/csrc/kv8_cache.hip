@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
     uint32_t b, item;
     if (!kv8_find(blockIdx.x / a.c.heads, a.c.batch, [&](uint32_t i) { return append_span(a, i).items; }, b, item)) return;
     const AppendSpan s = append_span(a, b);
-    const bool values = threadIdx.x >= per_side;
+    const bool values = __builtin_amdgcn_readfirstlane(threadIdx.x >= per_side);
     const uint32_t tid = values ? threadIdx.x - per_side : threadIdx.x;
     const size_t bh = (size_t)b * a.c.heads + head;
     uint16_t *open = (values ? a.c.vo : a.c.ko) + bh * kKv8Block * D;
@@ -360,13 +360,8 @@ __device__ void select_slots(const Kv8EvictArgs &a, const SelectRun &s, float *t
                     for (uint32_t x = 0; x < kSelectCopies; ++x) c[i] += hist[4 * lane + i][x];
                     sum += c[i];
                 }
-                uint32_t above = sum;  // keys in this lane's digits and those of the lanes above
-#pragma unroll
-                for (uint32_t o = 1; o < 64; o *= 2) {
-                    const uint32_t down = __shfl_down(above, o);
-                    if (lane + o < 64) above += down;
-                }
-                above -= sum;
+                const uint32_t upto = wave_scan_u32(sum);
+                uint32_t above = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63) - upto;  // keys in the digits of the lanes above
                 if (above < want && above + sum >= want) {
 #pragma unroll
                     for (int i = 3; i >= 0; --i) {
@@ -447,24 +442,26 @@ __global__ __launch_bounds__(kSelectThreads) void kv8_select_kernel(Kv8EvictArgs
     else select_slots<false>(a, s, to_w, kept, hist, found, kept_of, ties_of);
 }
 
-// A workgroup per new block: keys by the first side of threads (4 slots x 8 dims each, as in the append), values by the second, a
-// dim each with all 32 slots: its bytes lie 16 apart in the old blocks, so a wave's loads of one slot cover whole
-// lines, and its new bytes are two 16-byte units.  The slots behind the new length are given code 0.
-// Bound by the latency of three dependent loads (kept slots, scales and bytes, stores) and by half of the vector instructions'
-// time; registers for four workgroups a compute unit (54 -> 52 us for the three launches of 8 sequences of 8100 cut to 4000, 2 heads,
-// D 128, read back; with five it took 56).
+// A workgroup per new block: keys by the first side of threads, 16 dims of a slot each (the kept slots of 32 lanes lie side by side
+// but for the gaps), values by the second, a dim each with all 32 slots: its bytes lie 16 apart in the old blocks, so a wave's loads
+// of one slot cover whole lines.  Both sides' new bytes are 16-byte units.  The slots behind the new length are given code 0.
+// Where the kept slots come from a few old blocks (four: every other token kept needs two or three), a thread loads its dim's
+// bytes of those whole, 16 a load, and picks from them in LDS; else byte by byte.  8 sequences of 8100 cut to 4000, 2 heads, D 128:
+// 25 -> 22 us, of which the bytes (every old line holds some that stay: 50 MB) take 10 at a copy's rate.
+constexpr uint32_t kGatherSpan = 4;  // old blocks that go through LDS (16 or 32 KB)
 template <int E4M3, int kGroups>
-__global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(Kv8EvictArgs a) {
+__global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8EvictArgs a) {
     __shared__ uint32_t red[4];
     __shared__ uint32_t from[kKv8Block];
-    __shared__ __align__(16) uint8_t codes[kKv8Block * 128 * kGroups];
-    const uint32_t blk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.from.D, units = D / 8, per_side = blockDim.x / 2;
+    constexpr uint32_t kDims = 128 * kGroups;
+    __shared__ u32x4 units[kGatherSpan][2][kDims];  // [old block][h][dim]
+    const uint32_t blk = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.from.D, per_side = blockDim.x / 2;
     const uint32_t n = min(a.lengths[b], a.from.max_ctx), left = min(n, a.budget);
     const uint32_t base = blk * kKv8Block;
     if (base >= left) return;
     const size_t bh = (size_t)b * a.from.heads + head;
     const uint32_t mine = min(left - base, kKv8Block), last = (left - 1) / kKv8Block, old_last = (n - 1) / kKv8Block;
-    const bool values = threadIdx.x >= per_side, fits = n <= a.budget;
+    const bool values = __builtin_amdgcn_readfirstlane(threadIdx.x >= per_side), fits = n <= a.budget;
     const uint32_t tid = values ? threadIdx.x - per_side : threadIdx.x;
     if (threadIdx.x < kKv8Block) from[threadIdx.x] = a.kept[bh * a.budget + base + min(threadIdx.x, mine - 1)];
     __syncthreads();
@@ -484,50 +481,74 @@ __global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(K
         if (tid == 0) *ds = ss[blk];
         return;
     }
-    // 32 elements a thread and group: x[i][4 j' + j] is slot 4 j' + j of dim tid (values), x[i][8 j + e] slot 4 g + j of
-    // dim 8 u + e (keys)
+    // 32 elements a thread and group: x[i][r] is slot r of dim tid (values), x[i][16 j + e] slot tid % 32 of dim 16 c + e (keys)
+    const uint32_t mine_r = tid % kKv8Block, mine_p = from[mine_r], mine_b = mine_p / kKv8Block;  // lane r: slot r comes from here
+    const float mine_scale = ss[mine_b];
+    const uint32_t first_b = __builtin_amdgcn_readfirstlane(from[0] / kKv8Block), last_b = __builtin_amdgcn_readfirstlane(from[mine - 1] / kKv8Block);
+    const auto chunk_at = [&](uint32_t i, uint32_t j) { return tid / kKv8Block + per_side / kKv8Block * (2 * i + j); };  // c
     float x[kGroups][32];
     uint32_t top = 0;
     const bool raw_rows = from[mine - 1] / kKv8Block == old_last;  // the block takes some of the old last block's
 #pragma unroll
     for (uint32_t i = 0; i < kGroups; ++i) {
         const uint32_t d = min(tid + per_side * i, D - 1);  // (threads past D repeat the last)
-        const GroupAt at = group_at(d, units);
-        if (values) {
+        if (values && last_b - first_b < kGatherSpan) {
+            // the dim's bytes of the old blocks, and those of the kept slots out of LDS (each thread reads what it wrote)
+            u32x4 w[kGatherSpan][2];
+#pragma unroll
+            for (uint32_t q = 0; q < kGatherSpan; ++q)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+                    w[q][h] = *reinterpret_cast<const u32x4 *>(src + min(first_b + q, last_b) * block_bytes + kv8_value_at(h, d));
+#pragma unroll
+            for (uint32_t q = 0; q < kGatherSpan; ++q)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) units[q][h][tid + per_side * i] = w[q][h];
+            const uint32_t g = mine_p % kKv8Block / 4;
+            const uint32_t at = ((mine_b - first_b) * 2 + (g & 1)) * (kDims * 16) + kv8_value_at(g & ~1u, 0) + mine_p % 4;
+            const uint8_t *bytes = reinterpret_cast<const uint8_t *>(&units[0][0][tid + per_side * i]);
 #pragma unroll
             for (uint32_t r = 0; r < kKv8Block; ++r) {
-                // the slot is the whole wave's: its part of the address in scalar registers
-                const uint32_t p = (uint32_t)__builtin_amdgcn_readfirstlane((int)from[r]), pb = p / kKv8Block, pr = p % kKv8Block;
-                const uint8_t *slot = src + (pb * block_bytes + kv8_value_at(pr / 4, 0) + pr % 4);
-                x[i][r] = kv8_value<E4M3>(slot[kv8_value_at(0, d)]) * ss[pb];
+                const float scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_scale), r));
+                x[i][r] = kv8_value<E4M3>(bytes[__builtin_amdgcn_readlane(at, r)]) * scale;
+            }
+        } else if (values) {
+            const uint64_t at = mine_b * block_bytes + kv8_value_at(mine_p % kKv8Block / 4, 0) + mine_p % 4;
+#pragma unroll
+            for (uint32_t r = 0; r < kKv8Block; ++r) {
+                // the slot is the whole wave's: its part of the address and its scale go through scalar registers
+                const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)at, r), hi = __builtin_amdgcn_readlane((uint32_t)(at >> 32), r);
+                const uint8_t *slot = src + ((uint64_t)hi << 32 | lo);
+                const float scale = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine_scale), r));
+                x[i][r] = kv8_value<E4M3>(slot[kv8_value_at(0, d)]) * scale;
             }
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t p = from[4 * at.g + j], pb = p / kKv8Block;
-                const u32x2 v = *reinterpret_cast<const u32x2 *>(src + pb * block_bytes + kv8_key_at(p % kKv8Block, 8 * at.u));
-                const float scale = ss[pb];
-                kv8_values<E4M3>(v.x, &x[i][8 * j]);
-                kv8_values<E4M3>(v.y, &x[i][8 * j + 4]);
+            for (uint32_t j = 0; j < 2; ++j) {
+                const uint32_t c = min(chunk_at(i, j), D / 16 - 1);
+                const u32x4 v = *reinterpret_cast<const u32x4 *>(src + mine_b * block_bytes + kv8_key_at(mine_p % kKv8Block, 16 * c));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][8 * j + e] *= scale;
+                for (uint32_t y = 0; y < 4; ++y) kv8_values<E4M3>(v[y], &x[i][16 * j + 4 * y]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[i][16 * j + e] *= mine_scale;
             }
         }
         if (raw_rows || blk == last) {
 #pragma unroll
             for (uint32_t y = 0; y < 32; ++y) {
-                const uint32_t r = values ? y : 4 * at.g + y / 8, dim = values ? d : 8 * at.u + y % 8, p = from[r];
+                const uint32_t r = values ? y : mine_r, c = chunk_at(i, y / 16), p = from[r];
+                const uint32_t dim = values ? d : 16 * min(c, D / 16 - 1) + y % 16;
                 if (p / kKv8Block == old_last) x[i][y] = bf16_to_f32(open[(p % kKv8Block) * D + dim]);
                 if (blk == last) {
                     const uint32_t bits = pack_bf16_rne(x[i][y], 0.0f) & 0xFFFFu;
                     x[i][y] = bf16_to_f32(bits);
-                    if (r < mine && tid + per_side * i < D) to_open[r * D + dim] = (uint16_t)bits;
+                    if (r < mine && (values ? tid + per_side * i < D : c < D / 16)) to_open[r * D + dim] = (uint16_t)bits;
                 }
             }
         }
         if (mine < kKv8Block) {
 #pragma unroll
-            for (uint32_t y = 0; y < 32; ++y) x[i][y] = (values ? y : 4 * at.g + y / 8) < mine ? x[i][y] : 0.0f;
+            for (uint32_t y = 0; y < 32; ++y) x[i][y] = (values ? y : mine_r) < mine ? x[i][y] : 0.0f;
         }
 #pragma unroll
         for (uint32_t y = 0; y < 32; ++y) top = max(top, abs_bits(x[i][y]));
@@ -538,8 +559,8 @@ __global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(K
 #pragma unroll
         for (uint32_t i = 0; i < kGroups; ++i) {
             const uint32_t d = tid + per_side * i;
-            if (d >= D) continue;
             if (values) {
+                if (d >= D) continue;
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
                     u32x4 w;
@@ -551,20 +572,24 @@ __global__ __launch_bounds__(256, kGroups == 1 ? 4 : 3) void kv8_gather_kernel(K
                     *reinterpret_cast<u32x4 *>(dst + kv8_value_at(h, d)) = w;
                 }
             } else {
-                float y[4][8];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) y[e / 8][e % 8] = x[i][e];
-                put_codes<E4M3, decltype(plain)::value>(codes, false, group_at(d, units), y, coder);
+                for (uint32_t j = 0; j < 2; ++j) {
+                    const uint32_t c = chunk_at(i, j);
+                    if (c >= D / 16) continue;
+                    u32x4 w;
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) {
+                        const float *v = &x[i][16 * j + 4 * y];
+                        w[y] = kv8_codes<E4M3, decltype(plain)::value>(coder, v[0], v[1], v[2], v[3]);
+                    }
+                    *reinterpret_cast<u32x4 *>(dst + kv8_key_at(mine_r, 16 * c)) = w;
+                }
             }
         }
     };
     if (coder.plain) put(std::true_type{});
     else put(std::false_type{});
     if (tid == 0) *ds = scale;
-    __syncthreads();
-    if (!values)
-        for (uint32_t i = tid; i < block_bytes / 16; i += per_side)
-            reinterpret_cast<u32x4 *>(dst)[i] = reinterpret_cast<const u32x4 *>(codes)[i];
 }
 
 hipError_t launch_kv8_evict(const Kv8EvictArgs &a, hipStream_t s) {

@@ -77,17 +77,15 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
 
 // ---- the work of a launch
 //
-// Tiles of kRows query rows; the context of a tile is split into parts of `per` blocks, so that the workgroups have about the
-// same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
+// Few rows: tiles of `rows` query rows; the context of a tile is split into parts of `per` blocks, so that the workgroups have
+// about the same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
 // A sequence's tiles all have as many parts as its longest: workgroup sum_{b' < b} tiles parts + part tiles + tile, and
 // those past a shorter tile's end have nothing to do.  (The tile varies first: workgroups go round the XCDs in turn, and
-// with the part first one XCD would get all the empty ones: 3907 tokens of 16/2 heads, split, took 201 us so, 122 with the
-// tile first.)
+// with the part first one XCD would get all the empty ones.)
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
     uint32_t rows;    // of a tile
     uint32_t unit;    // `per` is a multiple of it
-    int causal;       // tiles see half of the new tokens on average: count that (then up to 2 target + tiles workgroups)
 };
 __device__ __forceinline__ uint32_t tiles_of(const Kv8AttnArgs &a, const Split &w, const Kv8Span &s) {
     return (s.m * a.group + w.rows - 1) / w.rows;
@@ -97,49 +95,20 @@ __device__ __forceinline__ uint32_t blocks_of(const Kv8AttnArgs &a, const Kv8Spa
 }
 __device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t per) { return max((blocks + per - 1) / per, 1u); }
 
-// Blocks of a part.  Every wave computes it alike.  Where the workgroups wanted are those that the card holds at once, a
-// few more would take a round of their own: `per` grows until the parts fit (300 tokens over 30000, 8/1 heads, D 256: 161 -> 120 us).
+// total / target, rounded up
+__device__ __forceinline__ unsigned long long fair_share(unsigned long long total, uint32_t target) {
+    return total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
+}
+
+// Blocks of a part.  Every wave computes it alike.
 __device__ __forceinline__ uint32_t split_per(const Kv8AttnArgs &a, const Split &w) {
-    if (w.target == 0) return 1u << 26;  // more than a cache has
-    uint32_t tiles = 0, seen = 0;        // of this lane's sequence: tiles, and the blocks that one of them sees
-    const auto look = [&](uint32_t b) {
-        tiles = seen = 0;
-        if (b >= a.c.batch) return;
-        const Kv8Span s = kv8_span(a.step, b);
-        const uint32_t n = min(s.n, a.c.max_ctx), past = n > s.m ? n - s.m : 0u;
-        tiles = tiles_of(a, w, s);
-        seen = ((w.causal ? past + (min(s.m, n) + 1) / 2 : n) + 31) / 32;  // never below half of n
-    };
     unsigned long long total = 0;
-    uint32_t all = 0;
-    for (uint32_t b = __lane_id(); b < (a.c.batch + 63) / 64 * 64; b += 64) {
-        look(b);
-        total += (unsigned long long)tiles * seen;
-        all += tiles;
+    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+        const Kv8Span s = kv8_span(a.step, b);
+        total += (unsigned long long)tiles_of(a, w, s) * blocks_of(a, s);
     }
-    total = wave_sum_u64(total);
-    all = wave_sum_u32(all);
-    const unsigned long long fair = total >> 31 ? (total + w.target - 1) / w.target
-                                                : ((uint32_t)total + w.target - 1) / w.target;
-    uint32_t per = max((uint32_t)((fair + w.unit - 1) / w.unit) * w.unit, w.unit);
-    // (few rows: their parts take a few microseconds, and this takes one)
-    if (!w.causal || 2 * (unsigned long long)all > w.target || total == 0) return per;  // else whole tiles are too many to fit them in
-    for (int i = 0; i < 6; ++i) {
-        uint32_t count = 0;
-        if (a.c.batch <= 64) {
-            count = tiles * parts_of(seen, per);
-        } else {
-            for (uint32_t b = __lane_id(); b < (a.c.batch + 63) / 64 * 64; b += 64) {
-                look(b);
-                count += tiles * parts_of(seen, per);
-            }
-        }
-        count = wave_sum_u32(count);
-        if (count <= w.target) break;
-        const uint32_t grown = (uint32_t)((unsigned long long)per * count / w.target);
-        per = max((grown + w.unit - 1) / w.unit * w.unit, per + w.unit);
-    }
-    return per;
+    const unsigned long long fair = fair_share(wave_sum_u64(total), w.target);
+    return max((uint32_t)((fair + w.unit - 1) / w.unit) * w.unit, w.unit);
 }
 
 // What workgroup `idx` of a head does.
@@ -149,9 +118,9 @@ struct Work {
     uint32_t rows, most;                 // query rows of the sequence; slots that the tile's last row sees
 };
 __device__ __forceinline__ void fill_work(const Kv8AttnArgs &a, const Split &w, Work &o) {
+    o.s = kv8_span(a.step, o.b);
     o.rows = o.s.m * a.group;
     o.most = row_limit(o.s, min(w.rows * (o.tile + 1), o.rows) - 1, a.group, a.c.max_ctx);
-    o.parts = parts_of((o.most + 31) / 32, o.per);
 }
 __device__ __forceinline__ bool find_work(const Kv8AttnArgs &a, const Split &w, uint32_t idx, Work &o) {
     o.per = split_per(a, w);
@@ -161,34 +130,87 @@ __device__ __forceinline__ bool find_work(const Kv8AttnArgs &a, const Split &w, 
         return tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
     };
     if (!kv8_find(idx, a.c.batch, count, o.b, item)) return false;
-    o.s = kv8_span(a.step, o.b);
-    const uint32_t tiles = tiles_of(a, w, o.s);
+    const uint32_t tiles = tiles_of(a, w, kv8_span(a.step, o.b));
     o.tile = item % tiles;
     o.part = item / tiles;
-    if (w.causal) o.tile = tiles - 1 - o.tile;  // the tiles that see the most first
     fill_work(a, w, o);
+    o.parts = parts_of((o.most + 31) / 32, o.per);
     return o.part < o.parts;
 }
-// The same for the tile-th tile of all, and its parts' workgroups: idx, idx + step, ...
-__device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, uint32_t tile, Work &o, uint32_t &idx,
-                                          uint32_t &step) {
-    o.per = split_per(a, w);
-    if (!kv8_find(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, kv8_span(a.step, i)); }, o.b, o.tile)) return false;
-    o.part = 0;
-    o.s = kv8_span(a.step, o.b);
+
+// Many rows: where there are fewer tiles than compute units, the tiles' blocks stand in one line, tile after tile, and a workgroup
+// takes an equal share of it: the end of a tile, whole ones, the beginning of the next.  (Parts of equal length, of which a whole
+// number fits a tile, leave the longest workgroup a quarter more than the mean: 600 tokens over up to 12000 in four sequences,
+// 10/2 heads, D 256: 124 -> 113 us.)  A tile's blocks are those that its sequence's last row sees.
+struct Share {
+    uint32_t units, shift;  // a workgroup's, in units of 2^shift blocks; 0: a workgroup takes a tile
+};
+__device__ __forceinline__ uint32_t tile_units(const Kv8AttnArgs &a, const Kv8Span &s, uint32_t shift) {
+    return max((blocks_of(a, s) + (1u << shift) - 1) >> shift, 1u);  // (a tile that sees nothing is written too)
+}
+__device__ __forceinline__ Share share_of(const Kv8AttnArgs &a, const Split &w) {
+    Share r{0, 0};
+    if (w.target == 0) return r;
+    for (;; r.shift = 6) {  // (contexts so long that the line's blocks pass 2^30 are shared in units of 64)
+        unsigned long long total = 0;
+        for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+            const Kv8Span s = kv8_span(a.step, b);
+            total += (unsigned long long)tiles_of(a, w, s) * tile_units(a, s, r.shift);
+        }
+        total = wave_sum_u64(total);
+        r.units = max((uint32_t)fair_share(total, w.target), 1u);
+        if (total >> 30 == 0 || r.shift) return r;
+    }
+}
+// The tile in which place `at` of the line falls, and where in it.
+__device__ __forceinline__ bool find_place(const Kv8AttnArgs &a, const Split &w, uint32_t shift, uint32_t at, Work &o, uint32_t &unit,
+                                           uint32_t &units) {
+    uint32_t item;
+    const auto count = [&](uint32_t i) {
+        const Kv8Span s = kv8_span(a.step, i);
+        return tiles_of(a, w, s) * tile_units(a, s, shift);
+    };
+    if (!kv8_find(at, a.c.batch, count, o.b, item)) return false;
+    units = tile_units(a, kv8_span(a.step, o.b), shift);
+    o.tile = item / units;
+    unit = item % units;
     fill_work(a, w, o);
+    return true;
+}
+
+// For the joins: the tile-th tile of all, and where its parts lie in the workspace: slot `slot` + (part 0: `odd`) + part * `step`.
+template <bool kMany>
+__device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, uint32_t tile, Work &o, uint32_t &slot,
+                                          uint32_t &odd, uint32_t &step) {
+    if (!kv8_find(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, kv8_span(a.step, i)); }, o.b, o.tile)) return false;
+    fill_work(a, w, o);
+    Share share{};
+    if constexpr (kMany) share = share_of(a, w);
+    else o.per = split_per(a, w);
     uint32_t before = 0;
     for (uint32_t i = __lane_id(); i < o.b; i += 64) {
         const Kv8Span s = kv8_span(a.step, i);
-        before += tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
+        before += tiles_of(a, w, s) * (kMany ? tile_units(a, s, share.shift) : parts_of(blocks_of(a, s), o.per));
     }
     before = wave_sum_u32(before);
-    step = tiles_of(a, w, o.s);
-    idx = before + (w.causal ? step - 1 - o.tile : o.tile);
+    if constexpr (kMany) {
+        const uint32_t from = before + o.tile * tile_units(a, o.s, share.shift);
+        const uint32_t seen = max(((o.most + 31) / 32 + (1u << share.shift) - 1) >> share.shift, 1u);
+        const uint32_t first = from / share.units, last = (from + seen - 1) / share.units;
+        o.parts = last - first + 1;
+        slot = 2 * first;  // a workgroup's first piece in the even slot, its last one in the odd
+        odd = first * share.units < from;
+        step = 2;
+    } else {
+        o.parts = parts_of((o.most + 31) / 32, o.per);
+        slot = before + o.tile;
+        odd = 0;
+        step = tiles_of(a, w, o.s);
+    }
     return true;
 }
-// parts of a tile: at most twice `target` and one (half of a tile's blocks may not be counted), and target is at most 1024
-constexpr uint32_t kMostParts = 2112;
+// parts of a tile of few rows: at most `target` and one, and target is at most 1024
+constexpr uint32_t kMostParts = 1056;
 // Where a part's normalised O of a row lies in the workspace, in rows; m and l of all rows lie behind them, in pairs.
 __device__ __forceinline__ size_t part_at(const Kv8AttnArgs &a, const Split &w, uint32_t idx, uint32_t head, uint32_t row) {
     return ((size_t)idx * a.c.heads + head) * w.rows + row;
@@ -213,7 +235,7 @@ __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_
 constexpr uint32_t kManyRows = 128;
 
 template <int NS, int E4M3>
-__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, Split split, uint32_t grid) {
+__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnArgs a, Split split, uint32_t slots) {
     constexpr uint32_t D = 32 * NS;
     constexpr int kUnits = (2 * NS + 3) / 4;   // 1 KB pieces of a block's keys and values that a wave takes
     __shared__ u32x4 lds[2][2][2 * NS][64];    // [keys, values][block & 1][step][lane]
@@ -223,202 +245,223 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     uint32_t at = blockIdx.x;
     if (at / 256 & 1) at = at / 256 * 256 + min(gridDim.x - at / 256 * 256, 256u) - 1 - at % 256;
     const uint32_t head = at % a.c.heads, idx = at / a.c.heads;
-    Work w;
-    if (!find_work(a, split, idx, w)) return;
-    const Kv8Span &s = w.s;
-    const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + (lane & 31);
-    const bool live = r < w.rows;
-    const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
-    const uint32_t least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);  // the slots that all rows of the wave see
-    const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32);
-    const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
-    QueryRow<NS> q;
-    load_query<NS>(q, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
-    const size_t bh = (size_t)b * a.c.heads + head;
-    const uint8_t *k = a.c.k + bh * a.c.blocks * (size_t)(32 * D), *v = a.c.v + bh * a.c.blocks * (size_t)(32 * D);
-    const float *ks = a.c.ks + bh * a.c.blocks, *vs = a.c.vs + bh * a.c.blocks;
-    f32x16 o[NS];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) o[i] = f32x16{};
-    float base = -1e38f, l = 0.0f, vref = 0.0f, vinv = 0.0f;  // vref: the largest scale of values so far, vinv its reciprocal
-    float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
-    // what body n writes: this wave's pieces of keys n + 2 and values n + 1
-    u32x4 piece[kUnits];
-    const auto fetch = [&](uint32_t n) {
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            // (past the end: the last block once more, which nothing reads)
-            const uint32_t u = min(wave + 4 * i, 2u * NS - 1), at = min(u < NS ? n + 2 : n + 1, end - 1), j = u < NS ? u : u - NS;
-            piece[i] = *reinterpret_cast<const u32x4 *>((u < NS ? k : v) + (size_t)at * (32 * D) + 1024 * j + 16 * lane);
+    const Share share = share_of(a, split);
+    uint32_t place = idx * share.units, left = share.units;
+    for (uint32_t odd = 0;; odd = 1) {  // the pieces of this workgroup's share
+        Work w;
+        uint32_t first = 0, end;
+        bool whole = true;
+        if (share.units) {
+            uint32_t unit, units;
+            if (left == 0 || !find_place(a, split, share.shift, place, w, unit, units)) return;
+            const uint32_t take = min(left, units - unit), seen = (w.most + 31) / 32;
+            left -= take;
+            place += take;
+            first = unit << share.shift;
+            end = min((unit + take) << share.shift, seen);
+            whole = unit == 0 && end == seen;
+            if (unit && first >= seen) continue;
+            if (odd) __syncthreads();  // the last piece's bytes have been read
+        } else {
+            if (odd || !kv8_find(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, kv8_span(a.step, i)); }, w.b, w.tile)) return;
+            w.tile = tiles_of(a, split, kv8_span(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
+            fill_work(a, split, w);
+            end = (w.most + 31) / 32;
         }
-    };
-    const auto put = [&](u32x4 (*to)[64], uint32_t j, const u32x4 &w) {
-        to[2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.x, w.y));
-        to[2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.z, w.w));
-    };
-    const auto stage = [&](uint32_t n) {
+        const Kv8Span &s = w.s;
+        const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + (lane & 31);
+        const bool live = r < w.rows;
+        const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
+        const uint32_t least = wave_min_uniform(live ? limit : 0xFFFFFFFFu);  // the slots that all rows of the wave see
+        const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
+        QueryRow<NS> q;
+        load_query<NS>(q, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
+        const size_t bh = (size_t)b * a.c.heads + head;
+        const uint8_t *k = a.c.k + bh * a.c.blocks * (size_t)(32 * D), *v = a.c.v + bh * a.c.blocks * (size_t)(32 * D);
+        const float *ks = a.c.ks + bh * a.c.blocks, *vs = a.c.vs + bh * a.c.blocks;
+        f32x16 o[NS];
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const uint32_t u = min(wave + 4 * i, 2u * NS - 1);  // (the same piece twice where they do not divide)
-            put(u < NS ? lds[0][n & 1] : lds[1][(n + 1) & 1], u < NS ? u : u - NS, piece[i]);
-        }
-    };
-    float ks1 = 0.0f, vs1 = 0.0f;  // scales of block n + 1, on their way
-    const auto fetch_scales = [&](uint32_t n) {
-        const uint32_t at = min(n + 1, end - 1);
-        ks1 = ks[at];
-        vs1 = vs[at];
-    };
-    // The scores of the block in work, times c the exponents; its row maximum has been taken into `base`.
-    f32x16 p;
-    float c;
-    const auto key_steps = [&](f32x16 &s, const u32x4 (&kf)[2 * NS]) {
+        for (int i = 0; i < NS; ++i) o[i] = f32x16{};
+        float base = -1e38f, l = 0.0f, vref = 0.0f, vinv = 0.0f;  // vref: the largest scale of values so far, vinv its reciprocal
+        float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
+        // what body n writes: this wave's pieces of keys n + 2 and values n + 1
+        u32x4 piece[kUnits];
+        const auto fetch = [&](uint32_t n) {
 #pragma unroll
-        for (int j = 0; j < 2 * NS; ++j)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kf[j]), q.f[j], s, 0, 0, 0);
-    };
-    const auto row_top = [&](const f32x16 &s) {
-        float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
-#pragma unroll
-        for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
-        return fmaxf(top, s[15]);
-    };
-    // What a new block's scores change: slots that a row does not see get -infinity; the base of the exponents follows the
-    // maximum only when it is passed by 2^8 (the probabilities stay within fp16, and O is scaled down a few times in all); the
-    // largest scale of values so far grows.
-    const auto enter = [&](float top, float vscale, uint32_t p0) {
-        const bool finite = vscale < INFINITY;
-        if (p0 + 32 > least || !finite) {
-            const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
-#pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
-            c = 1.0f;
-            top = row_top(p);
-            top = fmaxf(top, xchg32(top, lane));
-            if (!finite && room) poison = __builtin_nanf("");
-        }
-        if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
-            const float base1 = fmaxf(base, top);
-            float down = __builtin_amdgcn_exp2f(base - base1);
-            base = base1;
-            l *= down;
-            if (finite && vscale > vref) {
-                const float to = fmaxf(vscale, 0x1p-126f);  // whose reciprocal is finite
-                vinv = 1.0f / to;
-                down *= vref * vinv;
-                vref = to;
+            for (int i = 0; i < kUnits; ++i) {
+                // (past the end: the last block once more, which nothing reads)
+                const uint32_t u = min(wave + 4 * i, 2u * NS - 1), at = min(u < NS ? n + 2 : n + 1, end - 1), j = u < NS ? u : u - NS;
+                piece[i] = *reinterpret_cast<const u32x4 *>((u < NS ? k : v) + (size_t)at * (32 * D) + 1024 * j + 16 * lane);
             }
+        };
+        const auto put = [&](u32x4 (*to)[64], uint32_t j, const u32x4 &w) {
+            to[2 * j][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.x, w.y));
+            to[2 * j + 1][lane] = __builtin_bit_cast(u32x4, kv8_operand<E4M3>(w.z, w.w));
+        };
+        const auto stage = [&](uint32_t n) {
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i) {
+                const uint32_t u = min(wave + 4 * i, 2u * NS - 1);  // (the same piece twice where they do not divide)
+                put(u < NS ? lds[0][n & 1] : lds[1][(n + 1) & 1], u < NS ? u : u - NS, piece[i]);
+            }
+        };
+        float ks1 = 0.0f, vs1 = 0.0f;  // scales of block n + 1, on their way
+        const auto fetch_scales = [&](uint32_t n) {
+            const uint32_t at = min(n + 1, end - 1);
+            ks1 = ks[at];
+            vs1 = vs[at];
+        };
+        // The scores of the block in work, times c the exponents; its row maximum has been taken into `base`.
+        f32x16 p;
+        float c;
+        const auto key_steps = [&](f32x16 &s, const u32x4 (&kf)[2 * NS]) {
+#pragma unroll
+            for (int j = 0; j < 2 * NS; ++j)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, kf[j]), q.f[j], s, 0, 0, 0);
+        };
+        const auto row_top = [&](const f32x16 &s) {
+            float top = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
+            return fmaxf(top, s[15]);
+        };
+        // What a new block's scores change: slots that a row does not see get -infinity; the base of the exponents follows the
+        // maximum only when it is passed by 2^8 (the probabilities stay within fp16, and O is scaled down a few times in all); the
+        // largest scale of values so far grows.
+        const auto enter = [&](float top, float vscale, uint32_t p0) {
+            const bool finite = vscale < INFINITY;
+            if (p0 + 32 > least || !finite) {
+                const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
+                c = 1.0f;
+                top = row_top(p);
+                top = fmaxf(top, xchg32(top, lane));
+                if (!finite && room) poison = __builtin_nanf("");
+            }
+            if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
+                const float base1 = fmaxf(base, top);
+                float down = __builtin_amdgcn_exp2f(base - base1);
+                base = base1;
+                l *= down;
+                if (finite && vscale > vref) {
+                    const float to = fmaxf(vscale, 0x1p-126f);  // whose reciprocal is finite
+                    vinv = 1.0f / to;
+                    down *= vref * vinv;
+                    vref = to;
+                }
+#pragma unroll
+                for (int d = 0; d < NS; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= down;
+            }
+        };
+        // Body n.  One run of instructions, so that the vector unit takes the exponentials while the matrix cores multiply the
+        // next keys, and the next row maximum while they multiply values.
+        const auto body = [&](auto more, uint32_t n, float vscale) {
+            constexpr bool kMore = decltype(more)::value;
+            u32x4 kf[2 * NS], vf[2 * NS];
+            if constexpr (kMore) {
+#pragma unroll
+                for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][(n + 1) & 1][j][lane];
+                stage(n);
+                fetch(n + 1);
+            }
+#pragma unroll
+            for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j][lane];
+            // The values' scale relative to the largest so far joins the exponent: what enters the second product stays in range, and
+            // l takes it out again. A block of zeros (scale 0) has none to keep; below 2^-30 of the largest it is held there.
+            const float shift = vscale > 0.0f && vscale < INFINITY ? fmaxf(__log2f(vscale * vinv), -30.0f) : 0.0f;
+            const float from = base - shift;
+            float sum = 0.0f;
+            f16x8_t pf[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
+                sum += e;
+                pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)e;
+            }
+            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+            if constexpr (kMore) {
+                p = f32x16{};
+                key_steps(p, kf);
+            }
+#pragma unroll
+            for (int d = 0; d < NS; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d]), pf[0], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d + 1]), pf[1], o[d], 0, 0, 0);
+            }
+            if constexpr (kMore) {
+                c = q.c * uniform(ks1);
+                const float vnext = uniform(vs1);
+                fetch_scales(n + 1);
+                float top = row_top(p) * c;
+                top = fmaxf(top, xchg32(top, lane));
+                enter(top, vnext, (n + 1) * 32);
+                return vnext;
+            }
+            return 0.0f;
+        };
+        if (first < end) {
+            // keys first and first + 1, values first
+            for (uint32_t u = wave; u < 3 * NS; u += 4) {
+                const uint32_t j = u % NS, at = u / NS == 1 ? first + 1 : first;
+                if (at >= end) continue;
+                const uint8_t *from = (u / NS == 2 ? v : k) + (size_t)at * (32 * D) + 1024 * j + 16 * lane;
+                put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
+            }
+            float vnow = uniform(vs[first]);
+            c = q.c * uniform(ks[first]);
+            fetch(first);
+            fetch_scales(first);
+            __syncthreads();
+            u32x4 kf[2 * NS];
+#pragma unroll
+            for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][first & 1][j][lane];
+            p = f32x16{};
+            key_steps(p, kf);
+            float top = row_top(p) * c;
+            top = fmaxf(top, xchg32(top, lane));
+            enter(top, vnow, first * 32);
+            for (uint32_t n = first; n + 1 < end; ++n) {
+                // a wave in its body goes before one that is still at the barrier's end: 593 -> 570 us for 2048 tokens over 14000
+                // (32/4 heads, D 128); with one wave a SIMD there is none to go before
+                if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(0);
+                __syncthreads();
+                if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(1);
+                vnow = body(std::true_type{}, n, vnow);
+            }
+            __syncthreads();
+            body(std::false_type{}, end - 1, vnow);
+        }
+        l += xchg32(l, lane);
+        const float norm = (l == 0.0f ? 0.0f : vref / l) + poison;
+        if (!live) {  // (a row past the sequence's)
+        } else if (whole) {
+            const size_t at = (size_t)t * a.q_heads + qh;
+            if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
+            uint16_t *out = a.out + at * D;
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= down;
-        }
-    };
-    // Body n.  One run of instructions, so that the vector unit takes the exponentials while the matrix cores multiply the
-    // next keys, and the next row maximum while they multiply values.
-    const auto body = [&](auto more, uint32_t n, float vscale) {
-        constexpr bool kMore = decltype(more)::value;
-        u32x4 kf[2 * NS], vf[2 * NS];
-        if constexpr (kMore) {
+                for (int i = 0; i < 4; ++i) {
+                    const u32x2 y = {pack_bf16_rne(o[d][4 * i] * norm, o[d][4 * i + 1] * norm),
+                                     pack_bf16_rne(o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm)};
+                    *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
+                }
+        } else {
+            const size_t at = part_at(a, split, 2 * idx + odd, head, r - r0);
 #pragma unroll
-            for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][(n + 1) & 1][j][lane];
-            stage(n);
-            fetch(n + 1);
-        }
+            for (int d = 0; d < NS; ++d)
 #pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j][lane];
-        // The values' scale relative to the largest so far joins the exponent: what enters the second product stays in range, and
-        // l takes it out again. A block of zeros (scale 0) has none to keep; below 2^-30 of the largest it is held there.
-        const float shift = vscale > 0.0f && vscale < INFINITY ? fmaxf(__log2f(vscale * vinv), -30.0f) : 0.0f;
-        const float from = base - shift;
-        float sum = 0.0f;
-        f16x8_t pf[2];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(fmaf(p[i], c, -from));
-            sum += e;
-            pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)e;
-        }
-        l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
-        if constexpr (kMore) {
-            p = f32x16{};
-            key_steps(p, kf);
-        }
-#pragma unroll
-        for (int d = 0; d < NS; ++d) {
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d]), pf[0], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d + 1]), pf[1], o[d], 0, 0, 0);
-        }
-        if constexpr (kMore) {
-            c = q.c * uniform(ks1);
-            const float vnext = uniform(vs1);
-            fetch_scales(n + 1);
-            float top = row_top(p) * c;
-            top = fmaxf(top, xchg32(top, lane));
-            enter(top, vnext, (n + 1) * 32);
-            return vnext;
-        }
-        return 0.0f;
-    };
-    if (first < end) {
-        // keys first and first + 1, values first
-        for (uint32_t u = wave; u < 3 * NS; u += 4) {
-            const uint32_t j = u % NS, at = u / NS == 1 ? first + 1 : first;
-            if (at >= end) continue;
-            const uint8_t *from = (u / NS == 2 ? v : k) + (size_t)at * (32 * D) + 1024 * j + 16 * lane;
-            put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
-        }
-        float vnow = uniform(vs[first]);
-        c = q.c * uniform(ks[first]);
-        fetch(first);
-        fetch_scales(first);
-        __syncthreads();
-        u32x4 kf[2 * NS];
-#pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) kf[j] = lds[0][first & 1][j][lane];
-        p = f32x16{};
-        key_steps(p, kf);
-        float top = row_top(p) * c;
-        top = fmaxf(top, xchg32(top, lane));
-        enter(top, vnow, first * 32);
-        for (uint32_t n = first; n + 1 < end; ++n) {
-            // a wave in its body goes before one that is still at the barrier's end: 593 -> 570 us for 2048 tokens over 14000
-            // (32/4 heads, D 128); with one wave a SIMD there is none to go before
-            if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(0);
-            __syncthreads();
-            if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(1);
-            vnow = body(std::true_type{}, n, vnow);
-        }
-        __syncthreads();
-        body(std::false_type{}, end - 1, vnow);
-    }
-    if (!live) return;
-    l += xchg32(l, lane);
-    const float norm = (l == 0.0f ? 0.0f : vref / l) + poison;
-    if (w.parts == 1) {
-        const size_t at = (size_t)t * a.q_heads + qh;
-        if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
-        uint16_t *out = a.out + at * D;
-#pragma unroll
-        for (int d = 0; d < NS; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const u32x2 y = {pack_bf16_rne(o[d][4 * i] * norm, o[d][4 * i + 1] * norm),
-                                 pack_bf16_rne(o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm)};
-                *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
+                        f32x4{o[d][4 * i] * norm, o[d][4 * i + 1] * norm, o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm};
+            if (h == 0) {
+                float *ml = a.part + (size_t)slots * a.c.heads * kManyRows * D + 2 * at;
+                ml[0] = base;
+                ml[1] = l;
             }
-    } else {
-        const size_t at = part_at(a, split, idx, head, r - r0);
-#pragma unroll
-        for (int d = 0; d < NS; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
-                    f32x4{o[d][4 * i] * norm, o[d][4 * i + 1] * norm, o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm};
-        if (h == 0) {
-            float *ml = a.part + (size_t)grid * a.c.heads * kManyRows * D + 2 * at;
-            ml[0] = base;
-            ml[1] = l;
         }
     }
 }
@@ -646,30 +689,31 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
 // Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
 // of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile.
 constexpr uint32_t kJoinThreads = 1024;
-template <int NS, bool kWide>
-__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t grid, uint32_t per_group) {
+template <int NS, bool kMany, bool kWide>
+__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t slots, uint32_t per_group) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
     __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
     __shared__ float ws[kWide ? kMostParts : kJoinThreads], red[2][kJoinThreads / 64];
     const uint32_t lane = __lane_id(), head = blockIdx.y, wave = threadIdx.x >> 6, tid = kWide ? threadIdx.x : lane;
     const uint32_t groups = split.rows / per_group;
     Work w;
-    uint32_t idx, tiles;
-    if (!find_tile(a, split, blockIdx.x / groups, w, idx, tiles)) return;
+    uint32_t slot, odd, slot_step;
+    if (!find_tile<kMany>(a, split, blockIdx.x / groups, w, slot, odd, slot_step)) return;
     // (starts that decrease can make more parts than the launch has: none behind its last)
-    if (idx < grid) w.parts = min(w.parts, (grid - idx + tiles - 1) / tiles);
-    if (w.parts == 1 || idx >= grid) return;
-    const size_t step = (size_t)tiles * a.c.heads * split.rows;  // between parts, in rows
-    const float *all_ml = a.part + (size_t)grid * a.c.heads * split.rows * D;
+    if (slot < slots) w.parts = min(w.parts, (slots - slot + slot_step - 1) / slot_step);
+    if (w.parts == 1 || slot >= slots) return;
+    const size_t slot_rows = (size_t)a.c.heads * split.rows, step = slot_step * slot_rows;  // between parts, in rows
+    const auto part_row = [&](uint32_t p) { return p * step + (p == 0 ? odd * slot_rows : 0); };
+    const float *all_ml = a.part + slots * slot_rows * D;
     const uint32_t way = tid / kQuads, quad = tid % kQuads, row0 = blockIdx.x % groups * per_group;
     for (uint32_t row = row0 + (kWide ? 0 : wave); row < row0 + per_group; row += kWide ? 1 : kJoinThreads / 64) {
         const uint32_t r = split.rows * w.tile + row;
         if (r >= w.rows) return;
-        const size_t at = part_at(a, split, idx, head, row);
+        const size_t at = part_at(a, split, slot, head, row);
         const float2 *ml = reinterpret_cast<const float2 *>(all_ml) + at;
         f32x4 acc = {0, 0, 0, 0};
         float M = -INFINITY, L = 0.0f;
-        for (uint32_t p = tid; p < w.parts; p += kThreads) M = fmaxf(M, ml[p * step].x);
+        for (uint32_t p = tid; p < w.parts; p += kThreads) M = fmaxf(M, ml[part_row(p)].x);
         M = wave_max(M);
         if constexpr (kWide) {
             if (lane == 0) red[0][wave] = M;
@@ -682,7 +726,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
             const uint32_t n = min(w.parts - p0, kWide ? kMostParts : 64u);
             float *wl = kWide ? ws : ws + 64 * wave, sum = 0.0f;
             for (uint32_t p = tid; p < n; p += kThreads) {
-                const float2 x = ml[(p0 + p) * step];
+                const float2 x = ml[part_row(p0 + p)];
                 const float f = x.y == 0.0f ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - M);  // NaN stays
                 wl[p] = f;
                 sum += f;
@@ -693,7 +737,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
             if (way < kWays) {
 #pragma unroll 8
                 for (uint32_t p = way; p < n; p += kWays)
-                    acc += wl[p] * *reinterpret_cast<const f32x4 *>(o + (p0 + p) * step * D);
+                    acc += wl[p] * *reinterpret_cast<const f32x4 *>(o + part_row(p0 + p) * D);
             }
             if constexpr (!kWide) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -957,7 +1001,7 @@ namespace {
 struct AttnPlan {
     bool few;
     Split split;
-    uint32_t tiles, grid;  // at most, a head
+    uint32_t tiles, grid, slots;  // at most, a head; slots: of parts in the workspace
 };
 bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
 AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
@@ -966,16 +1010,15 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
     p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)((uint64_t)tokens * group / p.split.rows) + std::min(batch, tokens);
-    const uint64_t all = (uint64_t)p.tiles * kv_heads;
     if (p.few) {
         p.split.unit = kFewWaves;
         p.split.target = std::max((D <= 64 ? 1024 : (D <= 96 ? 768 : (D <= 192 ? 512 : 256))) / kv_heads, std::min(p.tiles, 1024u));
-        p.grid = p.split.target + p.tiles;
+        p.slots = p.grid = p.split.target + p.tiles;
     } else {
-        p.split.unit = 1;
-        p.split.causal = 1;
-        p.split.target = all < 256 ? std::max(256u * (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) / kv_heads, 1u) : 0;
-        p.grid = 2 * p.split.target + p.tiles;
+        // as many workgroups as the card holds at once
+        p.split.target = (uint64_t)p.tiles * kv_heads < 256 ? std::max(256u * (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) / kv_heads, 1u) : 0;
+        p.grid = p.split.target ? p.split.target : p.tiles;
+        p.slots = 2 * p.split.target;
     }
     return p;
 }
@@ -989,7 +1032,7 @@ uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group,
 
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
     const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
-    return p.split.target == 0 ? 0 : (size_t)p.grid * kv_heads * p.split.rows * (D + 2) * sizeof(float);
+    return (size_t)p.slots * kv_heads * p.split.rows * (D + 2) * sizeof(float);
 }
 
 namespace {
@@ -1017,16 +1060,17 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
         if (p.few)
             kv8_few_kernel<NS, E4M3><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
         else
-            kv8_many_kernel<NS, E4M3><<<dim3(p.grid * a.c.heads), 256, 0, s>>>(a, p.split, p.grid);
+            kv8_many_kernel<NS, E4M3><<<dim3(p.grid * a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 512) {
-            kv8_join_kernel<NS, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.grid, 1);
+            kv8_join_kernel<NS, false, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
         } else {
             uint32_t per_group = kJoinThreads / 64;
             while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 1024) per_group *= 2;
-            kv8_join_kernel<NS, false><<<dim3(p.tiles * (p.split.rows / per_group), a.c.heads), kJoinThreads, 0, s>>>(
-                a, p.split, p.grid, per_group);
+            const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
+            if (p.few) kv8_join_kernel<NS, false, false><<<grid, kJoinThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            else kv8_join_kernel<NS, true, false><<<grid, kJoinThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     });

@@ -687,13 +687,14 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
 }
 
 // Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
-// of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile.
-constexpr uint32_t kJoinThreads = 1024;
+// of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile (four waves: with 16, which
+// find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).
+constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;
 template <int NS, bool kMany, bool kWide>
-__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t slots, uint32_t per_group) {
+__global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t slots, uint32_t per_group) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
     __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
-    __shared__ float ws[kWide ? kMostParts : kJoinThreads], red[2][kJoinThreads / 64];
+    __shared__ float ws[kWide ? kMostParts : kJoinRowThreads], red[2][kJoinThreads / 64];
     const uint32_t lane = __lane_id(), head = blockIdx.y, wave = threadIdx.x >> 6, tid = kWide ? threadIdx.x : lane;
     const uint32_t groups = split.rows / per_group;
     Work w;
@@ -706,7 +707,7 @@ __global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnArgs a, S
     const auto part_row = [&](uint32_t p) { return p * step + (p == 0 ? odd * slot_rows : 0); };
     const float *all_ml = a.part + slots * slot_rows * D;
     const uint32_t way = tid / kQuads, quad = tid % kQuads, row0 = blockIdx.x % groups * per_group;
-    for (uint32_t row = row0 + (kWide ? 0 : wave); row < row0 + per_group; row += kWide ? 1 : kJoinThreads / 64) {
+    for (uint32_t row = row0 + (kWide ? 0 : wave); row < row0 + per_group; row += kWide ? 1 : kJoinRowThreads / 64) {
         const uint32_t r = split.rows * w.tile + row;
         if (r >= w.rows) return;
         const size_t at = part_at(a, split, slot, head, row);
@@ -1066,11 +1067,11 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 512) {
             kv8_join_kernel<NS, false, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
         } else {
-            uint32_t per_group = kJoinThreads / 64;
-            while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 1024) per_group *= 2;
+            uint32_t per_group = kJoinRowThreads / 64;
+            while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 2048) per_group *= 2;
             const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
-            if (p.few) kv8_join_kernel<NS, false, false><<<grid, kJoinThreads, 0, s>>>(a, p.split, p.slots, per_group);
-            else kv8_join_kernel<NS, true, false><<<grid, kJoinThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            if (p.few) kv8_join_kernel<NS, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            else kv8_join_kernel<NS, true, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     });

@@ -378,8 +378,8 @@ struct Kv8AttnArgs {
     float *part;             // workspace
     float decay, *weight;    // weights
 };
-uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens);  // workgroups
-size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens);
+uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);  // workgroups
+size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s);
 size_t kv8_weight_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t tokens, uint32_t max_ctx);
 hipError_t launch_kv8_weight(const Kv8AttnArgs &a, hipStream_t s);

@@ -196,7 +196,7 @@ int kr_kv8_dequant(const kr_kv8_cache *cache, const uint32_t *lengths, const uin
 size_t kr_kv8_attention_workspace_bytes(const kr_kv8_cache *cache, uint32_t q_heads, uint32_t tokens) {
     if (!cache || cache->kv_heads == 0 || q_heads == 0 || q_heads % cache->kv_heads || tokens == 0 || cache->batch == 0) return 0;
     const size_t n = kv8_attention_workspace_bytes(cache->batch, cache->kv_heads, q_heads / cache->kv_heads,
-                                                   cache->head_dim, tokens);
+                                                   cache->head_dim, tokens, cache->max_ctx);
     return (n + 255) / 256 * 256;
 }
 
@@ -210,7 +210,7 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
     if (int rc = check_step(cache, tokens, starts, lengths)) return rc;
     if (!out) return fail(KR_E_INVALID, "out is NULL");
     if (!on(out, 16) || !on(lse, 4)) return fail(KR_E_ALIGN, "out must be 16-byte aligned, lse 4-byte");
-    if (kv8_attention_groups(cache->batch, cache->kv_heads, q_heads / cache->kv_heads, cache->head_dim, tokens) > kMostGroups)
+    if (kv8_attention_groups(cache->batch, cache->kv_heads, q_heads / cache->kv_heads, cache->head_dim, tokens, cache->max_ctx) > kMostGroups)
         return fail(KR_E_SHAPE, "tokens=%u of %u sequences and %u heads are too many for one launch", tokens, cache->batch, q_heads);
     const size_t need = kr_kv8_attention_workspace_bytes(cache, q_heads, tokens);
     if (need && (!workspace || workspace_bytes < need))

@@ -85,7 +85,7 @@ __device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
     uint32_t rows;    // of a tile
-    uint32_t unit;    // `per` is a multiple of it
+    uint32_t unit;    // few rows: `per` is a multiple of it; many: workgroups that a compute unit holds
 };
 __device__ __forceinline__ uint32_t tiles_of(const Kv8AttnArgs &a, const Split &w, const Kv8Span &s) {
     return (s.m * a.group + w.rows - 1) / w.rows;
@@ -142,38 +142,37 @@ __device__ __forceinline__ bool find_work(const Kv8AttnArgs &a, const Split &w, 
 // takes an equal share of it: the end of a tile, whole ones, the beginning of the next.  (Parts of equal length, of which a whole
 // number fits a tile, leave the longest workgroup a quarter more than the mean: 600 tokens over up to 12000 in four sequences,
 // 10/2 heads, D 256: 124 -> 113 us.)  A tile's blocks are those that its sequence's last row sees.
-struct Share {
-    uint32_t units, shift;  // a workgroup's, in units of 2^shift blocks; 0: a workgroup takes a tile
-};
-__device__ __forceinline__ uint32_t tile_units(const Kv8AttnArgs &a, const Kv8Span &s, uint32_t shift) {
-    return max((blocks_of(a, s) + (1u << shift) - 1) >> shift, 1u);  // (a tile that sees nothing is written too)
+// Parts cost about 14 blocks' time (O through memory, and the join), and a tile alone on a compute unit is faster than one of
+// several: where the longest tile has no more blocks than 14 and the shares that a compute unit would hold, tiles stay whole
+// (16/2 heads, split and whole, us.  D 128: 500 tokens 26 and 23, 1000 31 and 34, 2000 58 and 58, 200 over 1000 25 and 38;
+// D 256: 1000 tokens 47 and 55; D 64: 31 and 26).
+__device__ __forceinline__ uint32_t tile_blocks(const Kv8AttnArgs &a, const Kv8Span &s) {
+    return max(blocks_of(a, s), 1u);  // (a tile that sees nothing is written too)
 }
-__device__ __forceinline__ Share share_of(const Kv8AttnArgs &a, const Split &w) {
-    Share r{0, 0};
-    if (w.target == 0) return r;
-    for (;; r.shift = 6) {  // (contexts so long that the line's blocks pass 2^30 are shared in units of 64)
-        unsigned long long total = 0;
-        for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
-            const Kv8Span s = kv8_span(a.step, b);
-            total += (unsigned long long)tiles_of(a, w, s) * tile_units(a, s, r.shift);
-        }
-        total = wave_sum_u64(total);
-        r.units = max((uint32_t)fair_share(total, w.target), 1u);
-        if (total >> 30 == 0 || r.shift) return r;
+// A workgroup's share, in blocks; 0: a workgroup takes a tile.
+__device__ __forceinline__ uint32_t share_of(const Kv8AttnArgs &a, const Split &w) {
+    if (w.target == 0) return 0;
+    uint32_t total = 0, most = 0;  // (the host splits no launch whose blocks pass 2^31)
+    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
+        const Kv8Span s = kv8_span(a.step, b);
+        const uint32_t tiles = tiles_of(a, w, s), blocks = tile_blocks(a, s);
+        total += tiles * blocks;
+        if (tiles) most = max(most, blocks);
     }
+    const uint32_t share = max((wave_sum_u32(total) + w.target - 1) / w.target, 1u);
+    return wave_max_u32(most) <= 14 + w.unit * share ? 0 : share;
 }
 // The tile in which place `at` of the line falls, and where in it.
-__device__ __forceinline__ bool find_place(const Kv8AttnArgs &a, const Split &w, uint32_t shift, uint32_t at, Work &o, uint32_t &unit,
-                                           uint32_t &units) {
+__device__ __forceinline__ bool find_place(const Kv8AttnArgs &a, const Split &w, uint32_t at, Work &o, uint32_t &block, uint32_t &blocks) {
     uint32_t item;
     const auto count = [&](uint32_t i) {
         const Kv8Span s = kv8_span(a.step, i);
-        return tiles_of(a, w, s) * tile_units(a, s, shift);
+        return tiles_of(a, w, s) * tile_blocks(a, s);
     };
     if (!kv8_find(at, a.c.batch, count, o.b, item)) return false;
-    units = tile_units(a, kv8_span(a.step, o.b), shift);
-    o.tile = item / units;
-    unit = item % units;
+    blocks = tile_blocks(a, kv8_span(a.step, o.b));
+    o.tile = item / blocks;
+    block = item % blocks;
     fill_work(a, w, o);
     return true;
 }
@@ -184,22 +183,28 @@ __device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, 
                                           uint32_t &odd, uint32_t &step) {
     if (!kv8_find(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, kv8_span(a.step, i)); }, o.b, o.tile)) return false;
     fill_work(a, w, o);
-    Share share{};
-    if constexpr (kMany) share = share_of(a, w);
-    else o.per = split_per(a, w);
+    uint32_t share = 0;
+    if constexpr (kMany) {
+        share = share_of(a, w);
+        if (share == 0) {
+            o.parts = 1;
+            return true;
+        }
+    } else {
+        o.per = split_per(a, w);
+    }
     uint32_t before = 0;
     for (uint32_t i = __lane_id(); i < o.b; i += 64) {
         const Kv8Span s = kv8_span(a.step, i);
-        before += tiles_of(a, w, s) * (kMany ? tile_units(a, s, share.shift) : parts_of(blocks_of(a, s), o.per));
+        before += tiles_of(a, w, s) * (kMany ? tile_blocks(a, s) : parts_of(blocks_of(a, s), o.per));
     }
     before = wave_sum_u32(before);
     if constexpr (kMany) {
-        const uint32_t from = before + o.tile * tile_units(a, o.s, share.shift);
-        const uint32_t seen = max(((o.most + 31) / 32 + (1u << share.shift) - 1) >> share.shift, 1u);
-        const uint32_t first = from / share.units, last = (from + seen - 1) / share.units;
+        const uint32_t from = before + o.tile * tile_blocks(a, o.s), seen = max((o.most + 31) / 32, 1u);
+        const uint32_t first = from / share, last = (from + seen - 1) / share;
         o.parts = last - first + 1;
         slot = 2 * first;  // a workgroup's first piece in the even slot, its last one in the odd
-        odd = first * share.units < from;
+        odd = first * share < from;
         step = 2;
     } else {
         o.parts = parts_of((o.most + 31) / 32, o.per);
@@ -245,22 +250,21 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
     uint32_t at = blockIdx.x;
     if (at / 256 & 1) at = at / 256 * 256 + min(gridDim.x - at / 256 * 256, 256u) - 1 - at % 256;
     const uint32_t head = at % a.c.heads, idx = at / a.c.heads;
-    const Share share = share_of(a, split);
-    uint32_t place = idx * share.units, left = share.units;
+    const uint32_t share = share_of(a, split);
+    uint32_t place = idx * share, left = share;
     for (uint32_t odd = 0;; odd = 1) {  // the pieces of this workgroup's share
         Work w;
         uint32_t first = 0, end;
         bool whole = true;
-        if (share.units) {
-            uint32_t unit, units;
-            if (left == 0 || !find_place(a, split, share.shift, place, w, unit, units)) return;
-            const uint32_t take = min(left, units - unit), seen = (w.most + 31) / 32;
+        if (share) {
+            uint32_t blocks;
+            if (left == 0 || !find_place(a, split, place, w, first, blocks)) return;
+            const uint32_t take = min(left, blocks - first), seen = (w.most + 31) / 32;
             left -= take;
             place += take;
-            first = unit << share.shift;
-            end = min((unit + take) << share.shift, seen);
-            whole = unit == 0 && end == seen;
-            if (unit && first >= seen) continue;
+            end = min(first + take, seen);
+            whole = first == 0 && end == seen;
+            if (first && first >= seen) continue;
             if (odd) __syncthreads();  // the last piece's bytes have been read
         } else {
             if (odd || !kv8_find(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, kv8_span(a.step, i)); }, w.b, w.tile)) return;
@@ -1005,7 +1009,7 @@ struct AttnPlan {
     uint32_t tiles, grid, slots;  // at most, a head; slots: of parts in the workspace
 };
 bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
-AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
+AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     AttnPlan p{};
     p.few = few_rows(batch, group, tokens);
     p.split.rows = p.few ? kFewRows : kManyRows;
@@ -1017,7 +1021,9 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
         p.slots = p.grid = p.split.target + p.tiles;
     } else {
         // as many workgroups as the card holds at once
-        p.split.target = (uint64_t)p.tiles * kv_heads < 256 ? std::max(256u * (D <= 64 ? 3 : (D <= 128 ? 2 : 1)) / kv_heads, 1u) : 0;
+        p.split.unit = D <= 64 ? 3 : (D <= 128 ? 2 : 1);
+        const bool split = (uint64_t)p.tiles * kv_heads < 256 && (uint64_t)p.tiles * ((max_ctx + 31) / 32) < 1ull << 31;
+        p.split.target = split ? 256 * p.split.unit / kv_heads : 0;  // at least `tiles`
         p.grid = p.split.target ? p.split.target : p.tiles;
         p.slots = 2 * p.split.target;
     }
@@ -1026,13 +1032,13 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
 
 }  // namespace
 
-uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
-    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
+uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
+    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens, max_ctx);
     return (uint64_t)p.grid * (p.few ? 1 : kv_heads);  // (few: heads are another dimension)
 }
 
-size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens) {
-    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens);
+size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
+    const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens, max_ctx);
     return (size_t)p.slots * kv_heads * p.split.rows * (D + 2) * sizeof(float);
 }
 
@@ -1055,7 +1061,7 @@ hipError_t by_shape(const Kv8 &c, F &&f) {
 }  // namespace
 
 hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
-    const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.c.D, a.step.tokens);
+    const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.c.D, a.step.tokens, a.c.max_ctx);
     return by_shape(a.c, [&](auto ns, auto e4m3) -> hipError_t {
         constexpr int NS = decltype(ns)::value, E4M3 = decltype(e4m3)::value;
         if (p.few)

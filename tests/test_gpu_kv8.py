@@ -235,6 +235,17 @@ def test_attention_ragged_chunks(kv8, d, kv, group, counts, lens, e4m3):
     _check_attention(kv8, cache, _rand(g, sum(counts), kv * group, d), _starts(counts), _i32(lens))
 
 
+@pytest.mark.parametrize("d,kv,group,counts,lens", [
+    (64, 2, 4, [40, 0, 9, 1], [3000, 7, 40, 1500]), (128, 1, 3, [60, 100], [1800, 130]), (256, 2, 5, [55, 13, 26], [1999, 1300, 26]),
+    (96, 3, 2, [33, 64, 64], [2500, 64, 1025]), (192, 1, 8, [1, 1, 140], [1, 2, 2222]), (128, 8, 1, [200, 3], [900, 2900])])
+def test_attention_chunks_whose_tiles_are_shared_out(kv8, d, kv, group, counts, lens):
+    """Long contexts under few tiles: workgroups take ends, whole ones and beginnings of tiles, short sequences between long ones."""
+    g = torch.Generator().manual_seed(d + group + kv)
+    cache = _fill(kv8, g, lens, kv, d, 1 if d == 96 else 0, max(lens) + 3)
+    q, lengths = _rand(g, sum(counts), kv * group, d), _i32(lens)
+    _check_attention(kv8, cache, q, _starts(counts), lengths)
+
+
 def test_attention_rows_that_see_nothing_and_cut_lengths(kv8):
     g = torch.Generator().manual_seed(21)
     lens = [40, 3, 0, 33]

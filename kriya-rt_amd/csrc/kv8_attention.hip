@@ -1001,17 +1001,17 @@ __global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnAr
 
 namespace {
 
-// How a step is launched: tiles of 16 rows where the sequences have few query rows (one or two tokens of a group of
-// heads), else of 128.
+// How a step is launched: tiles of 16 rows where the sequences have few query rows (a few tokens of a group of heads), else of
+// 128.  With 40 rows a sequence, D 128, three tiles of 16 take 43 and 25 us (one sequence of 131072, eight of 8000), one of 128 48 and
+// 29; with 64 they are even; at D 256, where the small tiles' operands leave one workgroup a compute unit, 64 rows take 68 and 48.
 struct AttnPlan {
     bool few;
     Split split;
     uint32_t tiles, grid, slots;  // at most, a head; slots: of parts in the workspace
 };
-bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
 AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     AttnPlan p{};
-    p.few = few_rows(batch, group, tokens);
+    p.few = (uint64_t)tokens * group <= (D <= 128 ? 48ull : 32ull) * batch;
     p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)((uint64_t)tokens * group / p.split.rows) + std::min(batch, tokens);
@@ -1082,6 +1082,9 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
         return hipGetLastError();
     });
 }
+
+// Where a sequence's rows are one tile of 32, a workgroup takes them all.
+static bool few_rows(uint32_t batch, uint32_t group, uint32_t tokens) { return (uint64_t)tokens * group <= 32ull * batch; }
 
 // Workgroups wanted a head.
 static uint32_t weight_target(uint32_t kv_heads) { return std::max(kWeightTarget / kv_heads, 1u); }

@@ -385,6 +385,37 @@ def test_calls_on_another_stream_with_workspaces_of_their_own(kv8):
             assert torch.equal(o, own) and torch.equal(l, lse) and torch.equal(w, weight)
 
 
+@pytest.mark.parametrize("counts,lens", [([1, 1], [900, 40]), ([1, 0], [40, 9]), ([90, 30], [70, 2600]), ([60, 50], [200, 300])])
+def test_rows_behind_the_last_sequence_and_no_lse(kv8, kq, counts, lens):
+    """Seven rows more than the sequences have: their results stay as they were.  Without lse: the same output."""
+    g = torch.Generator().manual_seed(37)
+    cache = _fill(kv8, g, lens, 2, 64, 0, max(lens))
+    n, starts, lengths = sum(counts), _starts(counts), _i32(lens)
+    q = _rand(g, n + 7, 8, 64).cuda()
+    out, lse = torch.full_like(q, 3.0), torch.full((n + 7, 8), 5.0, device="cuda")
+    kv8.attention(cache, q, lengths, starts=starts, out=out, lse=lse)
+    assert (out[n:] == 3.0).all() and (lse[n:] == 5.0).all()
+    want, want_lse = kv8.attention(cache, q[:n], lengths, starts=starts)
+    sees = want_lse > -math.inf  # (a row of a sequence with more new tokens than tokens may see none)
+    assert (out[:n].float() - want.float()).abs().max() <= 2 * (2.0 ** -11 + 2.0 ** -8) * 6
+    assert torch.equal(lse[:n] > -math.inf, sees) and (lse[:n] - want_lse)[sees].abs().max() <= 1e-5
+    bare, ws = torch.full_like(q, 3.0), kv8.attention_workspace(cache, 8, n + 7)
+    kq._check(kq.lib().kr_kv8_attention(cache.desc, q.data_ptr(), 512, 8, n + 7, starts.data_ptr(), lengths.data_ptr(), 0.125,
+                                        bare.data_ptr(), None, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(bare, out)
+    weight = kv8.accumulate_weight(cache, q, lse, lengths, torch.zeros(2, 2, max(lens), device="cuda"), starts=starts)
+    live = torch.tensor([min(c, k) for c, k in zip(counts, lens)], device="cuda")
+    assert (weight.sum(-1) - live[:, None] * 4.0).abs().max() <= 1e-4 * max(counts) * 4
+    rows = torch.full((n + 7, 2, 64), float("nan"), dtype=BF, device="cuda")
+    rows[:n] = 1.0
+    before = cache.k.clone(), cache.v_scale.clone(), cache.k_open.clone()
+    two = kv8.Kv8Cache.wrap(before[0], cache.v.clone(), cache.k_scale.clone(), before[1], before[2], cache.v_open.clone(), max(lens))
+    kv8.append(cache, rows, rows, lengths, starts=starts)
+    kv8.append(two, rows[:n].contiguous(), rows[:n].contiguous(), lengths, starts=starts)
+    for x, y in zip(ref.read(cache, max(lens)), ref.read(two, max(lens))):  # (slots behind the lengths hold what they held)
+        assert all(torch.equal(x[b, :, :k], y[b, :, :k]) for b, k in enumerate(lens))
+
+
 def test_attention_takes_back_tokens_of_the_last_block(kv8):
     g = torch.Generator().manual_seed(6)
     cache = _fill(kv8, g, [60], 1, 64, 0, 64)

@@ -125,7 +125,7 @@ int kr_kv8_dequant(const kr_kv8_cache *cache, const uint32_t *lengths, const uin
  *   q, out: bf16 [tokens, q_heads, head_dim], q tokens q_stride elements apart (a multiple of 8), out contiguous; both 16-byte
  *   aligned and apart from each other; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
  *   be negative or 0).
- * From one token per sequence to whole prompts; the launch is chosen from tokens, heads and batch alone.
+ * From one token per sequence to whole prompts; the launch is chosen from the cache's sizes, tokens and heads, the shares on the device.
  * workspace: kr_kv8_attention_workspace_bytes(cache, q_heads, tokens) bytes, 16-byte aligned, no initial contents; calls
  * sharing it must not overlap in time.  Results are the same bits from run to run. */
 size_t kr_kv8_attention_workspace_bytes(const kr_kv8_cache *cache, uint32_t q_heads, uint32_t tokens);

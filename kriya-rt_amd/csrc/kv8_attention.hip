@@ -236,7 +236,9 @@ __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_
 // into fp16 operands in LDS together (a wave unpacking for itself would spend more vector cycles on it than the matrix
 // cores take), each as the 16 bytes a lane that an operand load takes.  Body n of the loop takes block n's softmax and second
 // product and block n + 1's first; it reads keys n + 1 and values n, and writes keys n + 2 and values n + 1 into the other
-// halves, so that one barrier a block is enough.
+// halves, so that one barrier a block is enough.  Bound by what the matrix cores and the vector unit cannot overlap: 2048 tokens
+// over 14000, 32/4 heads, int8: D 128 870 TFLOP/s, D 256 865, D 64 680; a prompt of 3907 of 16/2 heads of 128 102 us (610: the
+// diagonal's tiles are of unequal length).
 constexpr uint32_t kManyRows = 128;
 
 template <int NS, int E4M3>
@@ -478,6 +480,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 //   out = sum_s 2^(m_s - M) l_s O_s / L,   L = sum_s 2^(m_s - M) l_s
 // On v_mfma_f32_16x16x32_f16: lane (column l & 15, g = l >> 4) holds slots 16 t + 4 g + j after the first product, and
 // needs of dim d the slots 16 s + 4 g + j for the second, eight bytes of v's order (h = g & 1, a = g >> 1).
+// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64: 298 MB in 53 us (5.6 TB/s); 131072 slots of 2 heads of 128 16.8 us
+// (4 TB/s, the start of all workgroups included).
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
 template <int NS>
 constexpr uint32_t kFewAhead = NS <= 4 ? 2 : 1;
@@ -692,10 +696,12 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
 
 // Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
 // of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile (four waves: with 16, which
-// find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).
+// find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).  Bound by latency (work count,
+// maxima, parts): 16 rows in 512 parts 6.5 us, 1536 rows in a few 8.4, 6000 rows of 256 10.3 for 34 MB.
 constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;
 template <int NS, bool kMany, bool kWide>
-__global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split, uint32_t slots, uint32_t per_group) {
+__global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split,
+                                                                                          uint32_t slots, uint32_t per_group) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
     __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
     __shared__ float ws[kWide ? kMostParts : kJoinRowThreads], red[2][kJoinThreads / 64];
@@ -924,7 +930,8 @@ __global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint3
                 f32x16 s = {};
 #pragma unroll
                 for (int j = 0; j < 2 * NS; ++j)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, ql[side][x][j][place(lane, 4 * (j >> 1) + 2 * h + (j & 1))]), kf[j], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(bf16x8_t, ql[side][x][j][place(lane, 4 * (j >> 1) + 2 * h + (j & 1))]), kf[j], s, 0, 0, 0);
                 const auto rows = [&](auto all) {
                     const uint32_t r = kRows * tile + 32 * x + 4 * h - row0;
 #pragma unroll
@@ -972,7 +979,7 @@ __global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint3
     }
 }
 
-// Adds the parts of a chunk in order to what its slots had.
+// Adds the parts of a chunk in order to what its slots had.  Bound by latency: 2000 slots of 2 heads 6 us.
 __global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnArgs a, uint32_t target) {
     const uint32_t head = blockIdx.y, per = weight_per<false>(a, target);
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {  // chunks

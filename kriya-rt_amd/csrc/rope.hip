@@ -12,7 +12,7 @@ namespace kr {
 
 // The angle of position p at f turns a position is p f turns, of which only the fraction counts.  p f is taken in 64
 // bits (an error of 2^-53 p f turns: 1e-11 at a million), the fraction by rint, and only the fraction's sine and
-// cosine in 32.
+// cosine in 32.  Bound by its launch: 3907 rows of 16 pairs 1.7 us.
 __global__ __launch_bounds__(256) void rope_table_kernel(RopeTurns f, uint32_t half, uint32_t first, uint32_t count,
                                                          float gain, float *cos_sin) {
     const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
@@ -32,6 +32,8 @@ hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, 
     return hipGetLastError();
 }
 
+// A workgroup a token: its table row is loaded once for all heads.  Bound by bytes where there are many: 3907 tokens of 16 heads of
+// 128 in f32, a quarter turned, 64 MB in 13.6 us (4.7 TB/s); 16 tokens of 18 heads 3 us, a launch and two dependent loads.
 template <class T, bool kUnits>
 __global__ __launch_bounds__(256) void rope_apply_kernel(RopeArgs a, const T *x, size_t xs, T *y, size_t ys,
                                                          uint32_t heads, uint32_t D) {

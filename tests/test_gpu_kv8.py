@@ -389,7 +389,8 @@ def test_calls_on_another_stream_with_workspaces_of_their_own(kv8):
 def test_rows_behind_the_last_sequence_and_no_lse(kv8, kq, counts, lens):
     """Seven rows more than the sequences have: their results stay as they were.  Without lse: the same output."""
     g = torch.Generator().manual_seed(37)
-    cache = _fill(kv8, g, lens, 2, 64, 0, max(lens))
+    ctx = max(lens) + max(counts)
+    cache = _fill(kv8, g, lens, 2, 64, 0, ctx)
     n, starts, lengths = sum(counts), _starts(counts), _i32(lens)
     q = _rand(g, n + 7, 8, 64).cuda()
     out, lse = torch.full_like(q, 3.0), torch.full((n + 7, 8), 5.0, device="cuda")
@@ -403,17 +404,18 @@ def test_rows_behind_the_last_sequence_and_no_lse(kv8, kq, counts, lens):
     kq._check(kq.lib().kr_kv8_attention(cache.desc, q.data_ptr(), 512, 8, n + 7, starts.data_ptr(), lengths.data_ptr(), 0.125,
                                         bare.data_ptr(), None, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream))
     assert torch.equal(bare, out)
-    weight = kv8.accumulate_weight(cache, q, lse, lengths, torch.zeros(2, 2, max(lens), device="cuda"), starts=starts)
+    weight = kv8.accumulate_weight(cache, q, lse, lengths, torch.zeros(2, 2, ctx, device="cuda"), starts=starts)
     live = torch.tensor([min(c, k) for c, k in zip(counts, lens)], device="cuda")
     assert (weight.sum(-1) - live[:, None] * 4.0).abs().max() <= 1e-4 * max(counts) * 4
     rows = torch.full((n + 7, 2, 64), float("nan"), dtype=BF, device="cuda")
     rows[:n] = 1.0
     before = cache.k.clone(), cache.v_scale.clone(), cache.k_open.clone()
-    two = kv8.Kv8Cache.wrap(before[0], cache.v.clone(), cache.k_scale.clone(), before[1], before[2], cache.v_open.clone(), max(lens))
-    kv8.append(cache, rows, rows, lengths, starts=starts)
-    kv8.append(two, rows[:n].contiguous(), rows[:n].contiguous(), lengths, starts=starts)
-    for x, y in zip(ref.read(cache, max(lens)), ref.read(two, max(lens))):  # (slots behind the lengths hold what they held)
-        assert all(torch.equal(x[b, :, :k], y[b, :, :k]) for b, k in enumerate(lens))
+    two = kv8.Kv8Cache.wrap(before[0], cache.v.clone(), cache.k_scale.clone(), before[1], before[2], cache.v_open.clone(), ctx)
+    longer = [a + b for a, b in zip(lens, counts)]
+    kv8.append(cache, rows, rows, _i32(longer), starts=starts)
+    kv8.append(two, rows[:n].contiguous(), rows[:n].contiguous(), _i32(longer), starts=starts)
+    for x, y in zip(ref.read(cache, ctx), ref.read(two, ctx)):  # (slots behind the lengths hold what they held)
+        assert all(torch.equal(x[b, :, :k], y[b, :, :k]) for b, k in enumerate(longer))
 
 
 def test_attention_takes_back_tokens_of_the_last_block(kv8):

@@ -184,8 +184,8 @@ def test_calls_too_large_for_a_launch_and_tables_without_rows(kq):
     assert L.kr_rope_table(x, 0, 8, 128, 1e4, ctypes.byref(kr_rope_scaling(0, 1.0, 0.0, 0.0, 0.0, 1e39)), None) == kq.KR_E_INVALID
     assert L.kr_kv8_append(ctypes.byref(wide), None, x, x, 65535 * 64, None, None, 0, 0, 65535, None, n, None) == kq.KR_E_SHAPE
     assert L.kr_kv8_append(ctypes.byref(_cache()), None, x, x, 128, None, None, 0, 0, 1 << 25, n, n, None) == kq.KR_E_SHAPE
-    many = _cache(batch=60000, kv_heads=300)  # 33 rows a sequence and head, a workgroup each at least
-    assert L.kr_kv8_attention(ctypes.byref(many), x, 33 * 300 * 64, 33 * 300, 60000, n, n, 0.125, x, x, x, big, None) == kq.KR_E_SHAPE
+    many = _cache(batch=60000, kv_heads=300)  # 65 rows a sequence and head, a workgroup each at least
+    assert L.kr_kv8_attention(ctypes.byref(many), x, 65 * 300 * 64, 65 * 300, 60000, n, n, 0.125, x, x, x, big, None) == kq.KR_E_SHAPE
     long = dict(max_ctx=1 << 30)
     to = _cache(k=0x110000, v=0x120000, k_scale=0x130000, v_scale=0x140000, k_open=0x150000, v_open=0x160000, **long)
     assert L.kr_kv8_evict(ctypes.byref(_cache(**long)), n, x, 1 << 30, 0, 0, ctypes.byref(to), x + 64, x, None, None) == kq.KR_E_SHAPE

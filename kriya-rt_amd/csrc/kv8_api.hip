@@ -68,7 +68,7 @@ int check_queries(const kr_kv8_cache *c, const uint16_t *q, size_t q_stride, uin
     return KR_OK;
 }
 
-constexpr float kMaxScale = 0x1p100f;  // times log2(e) and a row's power of two it is a float
+constexpr float kMaxScale = 0x1p100f;  // times log2(e) a float
 
 bool finite_positive(double v) { return v > 0.0 && v < INFINITY; }
 

@@ -22,13 +22,22 @@ namespace {
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
+// The power of two that brings a row to [2^14, 2^15), from the bf16 bits of its largest |q|; 2^126 at most, which is exact too: rows
+// below 2^-112 are multiples of 2^-133 and become multiples of 2^-7.  From -114 (rows with an infinity or NaN, which keep them).
+__device__ __forceinline__ int query_exp(uint32_t top) { return min(141 - (int)(top >> 7), 126); }
+
 // Query row r of a tile, held as the operands of D / 16 steps: lane (column l & 31, h = l >> 5) holds for step 2 j + s
 // dims 32 j + 16 h + 8 s .. + 7, the dims that a lane's 16 key bytes cover.
 template <int NS>
 struct QueryRow {
     f16x8_t f[2 * NS];
-    float c;  // |scale| log2(e) 2^-e (the sign goes into the row: a maximum stays one under c)
+    float c;  // |scale| log2(e) 2^-e is c 2^x, c in [1/2, 1): times a block's scale it need be a float only
+    int x;    // (the sign of scale goes into the row: a maximum stays one under c)
 };
+// c 2^x times a block's scale of keys.
+__device__ __forceinline__ float score_scale(float c, int x, float ks) {
+    return ldexpf(c * __builtin_amdgcn_frexp_mantf(ks), x + __builtin_amdgcn_frexp_expf(ks));
+}
 
 // The row in fp16 times a power of two that brings its largest value to [2^14, 2^15): bf16 holds 8 bits of significand
 // and fp16 11, so every value down to 2^-28 of the largest is exact, and the rest are off by 2^-39 of it at
@@ -45,9 +54,10 @@ __device__ __forceinline__ void load_query(QueryRow<NS> &q, const uint16_t *row,
         top = max(top, bf16_unit_max_bits(raw[i]));
     }
     top = max(top, (uint32_t)__float_as_uint(xchg32(__uint_as_float(top), __lane_id())));
-    const int e = row_stage_exp(top, 14, 14, 14);
+    const int e = query_exp(top);
     const float up = copysignf(exp2_int(e), scale_log2);
-    q.c = fabsf(scale_log2) * exp2_int(-e);
+    q.c = __builtin_amdgcn_frexp_mantf(fabsf(scale_log2));
+    q.x = __builtin_amdgcn_frexp_expf(scale_log2) - e;
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) {
         const uint32_t W[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -398,7 +408,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[2 * d + 1]), pf[1], o[d], 0, 0, 0);
             }
             if constexpr (kMore) {
-                c = q.c * uniform(ks1);
+                c = score_scale(q.c, q.x, uniform(ks1));
                 const float vnext = uniform(vs1);
                 fetch_scales(n + 1);
                 float top = row_top(p) * c;
@@ -417,7 +427,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
             }
             float vnow = uniform(vs[first]);
-            c = q.c * uniform(ks[first]);
+            c = score_scale(q.c, q.x, uniform(ks[first]));
             fetch(first);
             fetch_scales(first);
             __syncthreads();
@@ -489,7 +499,7 @@ template <int NS>
 constexpr int kFewGroups = NS <= 2 ? 4 : (NS <= 3 ? 3 : (NS <= 6 ? 2 : 1));  // workgroups a compute unit
 
 template <int NS>
-__device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, const uint16_t *row, bool live, float scale_log2) {
+__device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, int &x, const uint16_t *row, bool live, float scale_log2) {
     const uint32_t lane = __lane_id(), g = lane >> 4;
     u32x4 raw[NS];
     uint32_t top = 0;
@@ -503,16 +513,17 @@ __device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, const u
     }
     top = max(top, (uint32_t)__float_as_uint(xchg32(__uint_as_float(top), lane)));
     top = max(top, (uint32_t)__float_as_uint(xchg16(__uint_as_float(top), lane)));
-    const int e = row_stage_exp(top, 14, 14, 14);
+    const int e = query_exp(top);
     const float up = exp2_int(e);
-    c = scale_log2 * exp2_int(-e);
+    c = __builtin_amdgcn_frexp_mantf(scale_log2);
+    x = __builtin_amdgcn_frexp_expf(scale_log2) - e;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
         const uint32_t W[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            f[i][2 * x] = (_Float16)(__uint_as_float(W[x] << 16) * up);
-            f[i][2 * x + 1] = (_Float16)(__uint_as_float(W[x] & 0xFFFF0000u) * up);
+        for (int y = 0; y < 4; ++y) {
+            f[i][2 * y] = (_Float16)(__uint_as_float(W[y] << 16) * up);
+            f[i][2 * y + 1] = (_Float16)(__uint_as_float(W[y] & 0xFFFF0000u) * up);
         }
     }
 }
@@ -574,7 +585,8 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
         if (blk + i * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, blk + i * kFewWaves);
     f16x8_t q[NS];
     float qc;
-    load_query16<NS>(q, qc, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
+    int qx;
+    load_query16<NS>(q, qc, qx, a.q + t * a.q_stride + (size_t)qh * D, live, a.scale_log2);
     f32x4 o[2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
@@ -592,7 +604,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
             if constexpr (NS & 1)
                 p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.ke[h].x, f.ke[h].y), q[NS - 1], p[h], 0, 0, 0);
         }
-        const float c = qc * f.ks, vscale = f.vs;
+        const float c = score_scale(qc, qx, f.ks), vscale = f.vs;
         const uint32_t room = limit > blk * 32 ? limit - blk * 32 : 0u;
         float top = -INFINITY;
 #pragma unroll

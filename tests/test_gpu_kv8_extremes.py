@@ -1,0 +1,27 @@
+"""GPU: attention over the 8-bit cache and its weights at the ends of the range, against 64 bits on the CPU: queries of any
+finite size, infinite ones, blocks of values far apart, keys and scales near the limits."""
+import math
+
+import pytest
+import torch
+
+import _kv8_ref as ref
+from test_gpu_kv8 import BF, _check_attention, _fill, _i32, _rand, _starts, kv8  # noqa: F401  (kv8: the fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("power", [-132, -112, -90, 112, 117, 126])
+@pytest.mark.parametrize("m", [1, 60])
+def test_queries_of_any_finite_size(kv8, power, m, e4m3):
+    """Rows whose largest |q| is near 2^power, subnormal ones among them, against keys near 2^-power: ordinary scores."""
+    g = torch.Generator().manual_seed(200 + power)
+    n, d, down = 150, 64, min(max(-power, -126), 125)
+    draw = lambda *s: torch.randn(*s, generator=g).clamp(-1.9, 1.9).double()  # noqa: E731
+    q, k = (draw(m, 4, d) * 2.0 ** power).to(BF), (draw(n, 2, d) * 2.0 ** down).to(BF)
+    assert q.isfinite().all() and k.isfinite().all() and float(q.abs().max()) > 0
+    cache = kv8.Kv8Cache(1, 2, d, n, format=e4m3)
+    kv8.append(cache, k.cuda(), _rand(g, n, 2, d).cuda(), _i32([n]), starts=_starts([n]))
+    _, _, _, off = _check_attention(kv8, cache, q, _starts([m]), _i32([n]), scale=2.0 ** (-power - down) / 8)
+    assert float(off.max()) < 2.0 ** -8  # (the scores are of ordinary size, so the tolerance means something)

@@ -23,8 +23,12 @@ namespace {
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // The power of two that brings a row to [2^14, 2^15), from the bf16 bits of its largest |q|; 2^126 at most, which is exact too: rows
-// below 2^-112 are multiples of 2^-133 and become multiples of 2^-7.  From -114 (rows with an infinity or NaN, which keep them).
+// below 2^-112 are multiples of 2^-133 and become multiples of 2^-7.
 __device__ __forceinline__ int query_exp(uint32_t top) { return min(141 - (int)(top >> 7), 126); }
+// The factor of a row's scores: NaN where it holds an infinity or NaN (scores that are all -infinity would look like no slot seen).
+__device__ __forceinline__ float query_factor(uint32_t top, float scale) {
+    return top >= 0x7F80u ? __builtin_nanf("") : __builtin_amdgcn_frexp_mantf(scale);
+}
 
 // Query row r of a tile, held as the operands of D / 16 steps: lane (column l & 31, h = l >> 5) holds for step 2 j + s
 // dims 32 j + 16 h + 8 s .. + 7, the dims that a lane's 16 key bytes cover.
@@ -41,7 +45,7 @@ __device__ __forceinline__ float score_scale(float c, int x, float ks) {
 
 // The row in fp16 times a power of two that brings its largest value to [2^14, 2^15): bf16 holds 8 bits of significand
 // and fp16 11, so every value down to 2^-28 of the largest is exact, and the rest are off by 2^-39 of it at
-// most.  Rows with an infinity or NaN keep them.
+// most.
 template <int NS>
 __device__ __forceinline__ void load_query(QueryRow<NS> &q, const uint16_t *row, bool live, float scale_log2) {
     const uint32_t h = __lane_id() >> 5;
@@ -56,7 +60,7 @@ __device__ __forceinline__ void load_query(QueryRow<NS> &q, const uint16_t *row,
     top = max(top, (uint32_t)__float_as_uint(xchg32(__uint_as_float(top), __lane_id())));
     const int e = query_exp(top);
     const float up = copysignf(exp2_int(e), scale_log2);
-    q.c = __builtin_amdgcn_frexp_mantf(fabsf(scale_log2));
+    q.c = query_factor(top, fabsf(scale_log2));
     q.x = __builtin_amdgcn_frexp_expf(scale_log2) - e;
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) {
@@ -515,7 +519,7 @@ __device__ __forceinline__ void load_query16(f16x8_t (&f)[NS], float &c, int &x,
     top = max(top, (uint32_t)__float_as_uint(xchg16(__uint_as_float(top), lane)));
     const int e = query_exp(top);
     const float up = exp2_int(e);
-    c = __builtin_amdgcn_frexp_mantf(scale_log2);
+    c = query_factor(top, scale_log2);
     x = __builtin_amdgcn_frexp_expf(scale_log2) - e;
 #pragma unroll
     for (int i = 0; i < NS; ++i) {

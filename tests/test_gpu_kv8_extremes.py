@@ -25,3 +25,32 @@ def test_queries_of_any_finite_size(kv8, power, m, e4m3):
     kv8.append(cache, k.cuda(), _rand(g, n, 2, d).cuda(), _i32([n]), starts=_starts([n]))
     _, _, _, off = _check_attention(kv8, cache, q, _starts([m]), _i32([n]), scale=2.0 ** (-power - down) / 8)
     assert float(off.max()) < 2.0 ** -8  # (the scores are of ordinary size, so the tolerance means something)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 40), (1, 5000), (60, 150), (60, 5000)])
+def test_infinite_queries_whose_scores_are_all_minus_infinity(kv8, m, n, sign):
+    """One infinite dim where every key has the other sign: NaN, not zeros; the other rows as without it.  A row that sees
+    nothing stays zero."""
+    g = torch.Generator().manual_seed(m + n)
+    d = 64
+    k = _rand(g, n, 2, d)
+    k[:, :, 3] = -1.0
+    cache = kv8.Kv8Cache(1, 2, d, n)
+    kv8.append(cache, k.cuda(), _rand(g, n, 2, d).cuda(), _i32([n]), starts=_starts([n]))
+    q, starts, lens, row = _rand(g, m, 4, d), _starts([m]), _i32([n]), m // 2
+    fine, fine_lse, _, _ = _check_attention(kv8, cache, q, starts, lens, scale=sign / 8)
+    bad = q.clone()
+    bad[row, 1, 3] = sign * math.inf
+    out, lse = kv8.attention(cache, bad.cuda(), lens, starts=starts, scale=sign / 8)
+    assert torch.isnan(out[row, 1]).all() and torch.isnan(lse[row, 1])
+    rest = torch.ones(m, 4, dtype=torch.bool)
+    rest[row, 1] = False
+    # another row's maximum may move a row's base: probabilities in fp16 of values below 6, outputs in bf16, twice
+    assert ((out - fine).float().abs()[rest] <= 2 * (2.0 ** -11 + 2.0 ** -8) * 6).all()
+    assert ((lse - fine_lse).abs()[rest] <= 1e-5).all()
+    weight = kv8.accumulate_weight(cache, bad.cuda(), lse, lens, torch.zeros(1, 2, n, device="cuda"), starts=starts, scale=sign / 8)
+    seen = n - m + row + 1
+    assert torch.isnan(weight[0, 0, :seen]).all() and torch.isfinite(weight[0, 0, seen:]).all() and torch.isfinite(weight[0, 1]).all()
+    none = kv8.attention(cache, bad.cuda(), _i32([0]), starts=starts, scale=sign / 8)
+    assert (none[0] == 0).all() and (none[1] == -math.inf).all()

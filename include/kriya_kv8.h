@@ -119,7 +119,8 @@ int kr_kv8_dequant(const kr_kv8_cache *cache, const uint32_t *lengths, const uin
  * For token i of the m new tokens of a sequence of n tokens, and query head g * kv head:
  *   out = sum_p softmax_p(scale q . K_p) V_p   over slots p <= n - m + i,   lse = ln sum_p e^(scale q . K_p)
  * with K_p, V_p the values that the cache's codes stand for.  The codes enter the matrix cores as fp16 (exact), q as
- * fp16 times a power of two of its row (exact down to 2^-29 of the row's largest), the probabilities as fp16;
+ * fp16 times a power of two of its row (exact down to 2^-29 of the row's largest), the probabilities times
+ * their block's scale of values as fp16 (half a step, and at most 2^-32 of the largest such product of the row);
  * sums, maxima and the softmax are f32, for which |scale| sum |q| |K_p| must stay below 2^126.  A row that sees no slot gives
  * zeros and lse = -infinity.  A row whose q is infinite or NaN, or that sees a block that stands for NaN, gives NaN.
  *   q, out: bf16 [tokens, q_heads, head_dim], q tokens q_stride elements apart (a multiple of 8), out contiguous; both 16-byte

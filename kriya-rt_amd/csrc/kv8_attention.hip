@@ -7,8 +7,10 @@
 // and value byte is used for the whole group.  In base 2, with c_r = scale log2(e) / 2^e_r, ks and vs the scales
 // of a block, q' = q 2^e_r in fp16:
 //   s_rp = (q'_r . k_p) (c_r ks),   m_r = max_p s_rp,   l_r = sum_p 2^(s_rp - m_r),
-//   out_r = sum_p 2^(s_rp - m_r) vs v_p / l_r
-// with k_p, v_p the codes.  One pass over the slots: m_r only grows, and sums made under an older m_r are scaled down.
+//   out_r = 2^d_r sum_p 2^(s_rp - m_r + log2 vs - d_r) v_p / l_r
+// with k_p, v_p the codes.  One pass over the slots: m_r only grows, and sums made under an older m_r are scaled down.  What enters
+// the second product is fp16, so its exponent has a reference of its own for each row: d_r follows the largest product of a
+// probability and its block's scale of values, so that a block of large values that a row hardly sees takes no bits from the others.
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_32x32x16_f16: a lane then holds one
 // query row (column l & 31) and the slots 8 i + 4 (l >> 5) + j of a block, its m_r and l_r are plain registers, and after
 // rounding to fp16 those probabilities are the second product's operand as they lie (see kv8.hpp for the order of v).
@@ -41,6 +43,37 @@ struct QueryRow {
 // c 2^x times a block's scale of keys.
 __device__ __forceinline__ float score_scale(float c, int x, float ks) {
     return ldexpf(c * __builtin_amdgcn_frexp_mantf(ks), x + __builtin_amdgcn_frexp_expf(ks));
+}
+
+// log2 of a block's scale of values: subnormal ones too; -infinity for a block of zeros, and for one that stands for NaN.
+__device__ __forceinline__ float value_scale_log2(float vs) {
+    return vs < INFINITY ? (float)__builtin_amdgcn_frexp_expf(vs) + __log2f(__builtin_amdgcn_frexp_mantf(vs)) : -INFINITY;
+}
+
+// A row's running sums: base m_r (lags the maximum by up to 2^8), l_r, and d_r.  The largest product is brought to 2^kTo and may grow
+// to 2^15 before d_r follows: fp16 then holds products down to 2^-21 of it in full, and half a step of the rest is 2^-32 of it.
+// kLeast keeps 2^d_r a normal float; products 2^-40 below 2^8 are none in fp16, so the exponent of a block that is further down (its
+// scale 2^-40 of what d_r stands for) is held there, where its probabilities still count in l_r.
+struct RowSums {
+    float base = -1e38f, l = 0.0f, d = 0.0f;
+};
+constexpr float kTo = 7.0f, kLeast = -126.0f, kFarDown = -40.0f;
+
+// A block's exponent beside its probabilities, log2 vs - d_r.
+__device__ __forceinline__ float value_shift(const RowSums &r, float vlog) { return fmaxf(vlog - r.d, kFarDown); }
+
+// Whether a block whose largest score of the row is `top` passes what the row's base or d allow (one comparison once top is known);
+// both following it, and the factor of O.
+__device__ __forceinline__ bool row_passed(const RowSums &r, float top, float vlog) {
+    return top > r.base + fminf(8.0f, 15.0f - (vlog - r.d));
+}
+__device__ __forceinline__ float row_follow(RowSums &r, float top, float vlog) {
+    const float base = fmaxf(r.base, top), down = r.base - base;
+    const float d = fmaxf(fmaxf(r.d + down, top + vlog - base - kTo), kLeast), od = down + (r.d - d);
+    r.base = base;
+    r.d = d;
+    r.l *= __builtin_amdgcn_exp2f(down);
+    return __builtin_amdgcn_exp2f(od);
 }
 
 // The row in fp16 times a power of two that brings its largest value to [2^14, 2^15): bf16 holds 8 bits of significand
@@ -302,7 +335,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
         f32x16 o[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) o[i] = f32x16{};
-        float base = -1e38f, l = 0.0f, vref = 0.0f, vinv = 0.0f;  // vref: the largest scale of values so far, vinv its reciprocal
+        RowSums sums;
         float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
         // what body n writes: this wave's pieces of keys n + 2 and values n + 1
         u32x4 piece[kUnits];
@@ -345,40 +378,34 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, s[i]), s[i + 1]);
             return fmaxf(top, s[15]);
         };
-        // What a new block's scores change: slots that a row does not see get -infinity; the base of the exponents follows the
-        // maximum only when it is passed by 2^8 (the probabilities stay within fp16, and O is scaled down a few times in all); the
-        // largest scale of values so far grows.
+        // What a new block's scores change: slots that a row does not see get -infinity; the row's base and reference follow only when
+        // they are passed (O is scaled down a few times in all).
+        // Returns the exponent beside the block's probabilities.
         const auto enter = [&](float top, float vscale, uint32_t p0) {
-            const bool finite = vscale < INFINITY;
-            if (p0 + 32 > least || !finite) {
+            float vlog = __log2f(vscale);
+            const bool normal = __builtin_amdgcn_classf(vscale, 0x100);  // (log2 takes subnormal numbers for 0)
+            if (p0 + 32 > least || !normal) {
                 const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
 #pragma unroll
                 for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
                 c = 1.0f;
                 top = row_top(p);
                 top = fmaxf(top, xchg32(top, lane));
-                if (!finite && room) poison = __builtin_nanf("");
+                if (!(vscale < INFINITY) && room) poison = __builtin_nanf("");
+                vlog = value_scale_log2(vscale);
             }
-            if (__any(top > base + 8.0f) || (finite && vscale > vref)) {
-                const float base1 = fmaxf(base, top);
-                float down = __builtin_amdgcn_exp2f(base - base1);
-                base = base1;
-                l *= down;
-                if (finite && vscale > vref) {
-                    const float to = fmaxf(vscale, 0x1p-126f);  // whose reciprocal is finite
-                    vinv = 1.0f / to;
-                    down *= vref * vinv;
-                    vref = to;
-                }
+            if (__any(row_passed(sums, top, vlog))) {
+                const float down = row_follow(sums, top, vlog);
 #pragma unroll
                 for (int d = 0; d < NS; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= down;
             }
+            return value_shift(sums, vlog);
         };
         // Body n.  One run of instructions, so that the vector unit takes the exponentials while the matrix cores multiply the
         // next keys, and the next row maximum while they multiply values.
-        const auto body = [&](auto more, uint32_t n, float vscale) {
+        const auto body = [&](auto more, uint32_t n, float shift) {
             constexpr bool kMore = decltype(more)::value;
             u32x4 kf[2 * NS], vf[2 * NS];
             if constexpr (kMore) {
@@ -389,10 +416,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             }
 #pragma unroll
             for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j][lane];
-            // The values' scale relative to the largest so far joins the exponent: what enters the second product stays in range, and
-            // l takes it out again. A block of zeros (scale 0) has none to keep; below 2^-30 of the largest it is held there.
-            const float shift = vscale > 0.0f && vscale < INFINITY ? fmaxf(__log2f(vscale * vinv), -30.0f) : 0.0f;
-            const float from = base - shift;
+            // the values' scale joins the exponent, and l takes it out again
+            const float from = sums.base - shift;
             float sum = 0.0f;
             f16x8_t pf[2];
 #pragma unroll
@@ -401,7 +426,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 sum += e;
                 pf[(i >> 2) & 1][(i >> 3) * 4 + (i & 3)] = (_Float16)e;
             }
-            l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), l);
+            sums.l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), sums.l);
             if constexpr (kMore) {
                 p = f32x16{};
                 key_steps(p, kf);
@@ -417,8 +442,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 fetch_scales(n + 1);
                 float top = row_top(p) * c;
                 top = fmaxf(top, xchg32(top, lane));
-                enter(top, vnext, (n + 1) * 32);
-                return vnext;
+                return enter(top, vnext, (n + 1) * 32);
             }
             return 0.0f;
         };
@@ -430,7 +454,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 const uint8_t *from = (u / NS == 2 ? v : k) + (size_t)at * (32 * D) + 1024 * j + 16 * lane;
                 put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
             }
-            float vnow = uniform(vs[first]);
+            const float vfirst = uniform(vs[first]);
             c = score_scale(q.c, q.x, uniform(ks[first]));
             fetch(first);
             fetch_scales(first);
@@ -442,31 +466,35 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             key_steps(p, kf);
             float top = row_top(p) * c;
             top = fmaxf(top, xchg32(top, lane));
-            enter(top, vnow, first * 32);
+            float shift = enter(top, vfirst, first * 32);
             for (uint32_t n = first; n + 1 < end; ++n) {
                 // a wave in its body goes before one that is still at the barrier's end: 593 -> 570 us for 2048 tokens over 14000
                 // (32/4 heads, D 128); with one wave a SIMD there is none to go before
                 if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(0);
                 __syncthreads();
                 if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(1);
-                vnow = body(std::true_type{}, n, vnow);
+                shift = body(std::true_type{}, n, shift);
             }
             __syncthreads();
-            body(std::false_type{}, end - 1, vnow);
+            body(std::false_type{}, end - 1, shift);
         }
-        l += xchg32(l, lane);
-        const float norm = (l == 0.0f ? 0.0f : vref / l) + poison;
+        const float l = sums.l + xchg32(sums.l, lane);
+        // (two factors: their product may be below the normal floats)
+        const float norm = (l == 0.0f ? 0.0f : 1.0f / l) + poison, up = __builtin_amdgcn_exp2f(sums.d);
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * norm * up;
         if (!live) {  // (a row past the sequence's)
         } else if (whole) {
             const size_t at = (size_t)t * a.q_heads + qh;
-            if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (base + __log2f(l)) * kLn2;
+            if (a.lse && h == 0) a.lse[at] = l == 0.0f ? -INFINITY : (sums.base + __log2f(l)) * kLn2;
             uint16_t *out = a.out + at * D;
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const u32x2 y = {pack_bf16_rne(o[d][4 * i] * norm, o[d][4 * i + 1] * norm),
-                                     pack_bf16_rne(o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm)};
+                    const u32x2 y = {pack_bf16_rne(o[d][4 * i], o[d][4 * i + 1]), pack_bf16_rne(o[d][4 * i + 2], o[d][4 * i + 3])};
                     *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = y;
                 }
         } else {
@@ -476,10 +504,10 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     *reinterpret_cast<f32x4 *>(a.part + at * D + 32 * d + 8 * i + 4 * h) =
-                        f32x4{o[d][4 * i] * norm, o[d][4 * i + 1] * norm, o[d][4 * i + 2] * norm, o[d][4 * i + 3] * norm};
+                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
             if (h == 0) {
                 float *ml = a.part + (size_t)slots * a.c.heads * kManyRows * D + 2 * at;
-                ml[0] = base;
+                ml[0] = sums.base;
                 ml[1] = l;
             }
         }
@@ -594,7 +622,8 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
     f32x4 o[2 * NS];
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
-    float m = -1e38f, l = 0.0f, vref = 0.0f;
+    RowSums sums;
+    float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
     const auto step = [&](auto masked, const FewBlock<NS> &f, uint32_t blk) {
         constexpr bool kEdge = decltype(masked)::value;
         f32x4 p[2] = {};
@@ -608,8 +637,9 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
             if constexpr (NS & 1)
                 p[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.ke[h].x, f.ke[h].y), q[NS - 1], p[h], 0, 0, 0);
         }
-        const float c = score_scale(qc, qx, f.ks), vscale = f.vs;
+        const float c = score_scale(qc, qx, f.ks), vlog = value_scale_log2(f.vs);
         const uint32_t room = limit > blk * 32 ? limit - blk * 32 : 0u;
+        if (kEdge && !(f.vs < INFINITY) && room) poison = __builtin_nanf("");
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -620,29 +650,21 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
         }
         top = fmaxf(top, xchg32(top, lane));
         top = fmaxf(top, xchg16(top, lane));
-        // as in the kernel above: the base follows the maximum when it is passed by 2^8
-        if (__any(top > m + 8.0f) || (vscale > vref && vscale < INFINITY)) {
-            const float m1 = fmaxf(m, top);
-            float down = __builtin_amdgcn_exp2f(m - m1);
-            m = m1;
-            l *= down;
-            if (vscale > vref && vscale < INFINITY) {
-                down *= vref / vscale;
-                vref = vscale;
-            }
+        if (__any(row_passed(sums, top, vlog))) {
+            const float down = row_follow(sums, top, vlog);
 #pragma unroll
             for (int d = 0; d < 2 * NS; ++d) o[d] *= down;
         }
-        const float vrel = vref > 0.0f ? vscale / vref : (vscale == 0.0f ? 0.0f : vscale);
+        const float shift = value_shift(sums, vlog), from = sums.base - shift;
+        float sum = 0.0f;
         f16x8_t pf;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(p[i >> 2][i & 3] - m);
-            l += e;
-            float x = e * vrel;
-            if (kEdge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = 0.0f;
-            pf[i] = (_Float16)x;
+            const float e = __builtin_amdgcn_exp2f(p[i >> 2][i & 3] - from);
+            sum += e;
+            pf[i] = (_Float16)e;
         }
+        sums.l = fmaf(sum, __builtin_amdgcn_exp2f(-shift), sums.l);
 #pragma unroll
         for (int d = 0; d < 2 * NS; ++d)
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv8_operand<E4M3>(f.v[d].x, f.v[d].y), pf, o[d], 0, 0, 0);
@@ -659,16 +681,16 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
             if (at + kAhead * kFewWaves < end) load_few<NS>(f[i], k, v, ks, vs, at + kAhead * kFewWaves);
         }
     }
-    l += xchg32(l, lane);
+    float l = sums.l + xchg32(sums.l, lane);
     l += xchg16(l, lane);
-    const float norm = l == 0.0f ? 0.0f : vref / l;
+    const float norm = (l == 0.0f ? 0.0f : 1.0f / l) + poison, up = __builtin_amdgcn_exp2f(sums.d);
     if (g == 0) {
-        sm[wave][r16] = m;
+        sm[wave][r16] = sums.base;
         sl[wave][r16] = l;
     }
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d)
-        *reinterpret_cast<f32x4 *>(&so[wave][r16][16 * d + 4 * g]) = o[d] * norm;
+        *reinterpret_cast<f32x4 *>(&so[wave][r16][16 * d + 4 * g]) = o[d] * norm * up;
     __syncthreads();
     // four dims of a row a thread
     for (uint32_t i = threadIdx.x; i < kFewRows * (D / 4); i += 256) {

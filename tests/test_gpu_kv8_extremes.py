@@ -54,3 +54,37 @@ def test_infinite_queries_whose_scores_are_all_minus_infinity(kv8, m, n, sign):
     assert torch.isnan(weight[0, 0, :seen]).all() and torch.isfinite(weight[0, 0, seen:]).all() and torch.isfinite(weight[0, 1]).all()
     none = kv8.attention(cache, bad.cuda(), _i32([0]), starts=starts, scale=sign / 8)
     assert (none[0] == 0).all() and (none[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("power", [16, 20, 26, 40, 60, 100])
+@pytest.mark.parametrize("batch,m,n", [(1, 1, 160), (130, 1, 700), (1, 60, 160), (16, 60, 1600)])
+def test_blocks_of_large_values_that_a_row_hardly_attends(kv8, batch, m, n, power, e4m3):
+    """Blocks of values 2^power times the others', which rows of one sign give weights of e^-40 (2^-58) and rows of the other
+    almost all: each row keeps the bits of what it attends."""
+    g = torch.Generator().manual_seed(300 + power + n)
+    d, t = 64, batch * m
+    k, v, q = _rand(g, batch, n, 1, d), _rand(g, batch, n, 1, d).double(), _rand(g, t, 2, d, gain=0.25)
+    large = (torch.arange(n) // 32 + torch.arange(batch)[:, None]) % 3 == 1
+    k[..., 0] = torch.where(large, -10.0, 0.0)[..., None]
+    v[large] *= 2.0 ** power
+    q[:, :, 0] = 4.0
+    q[::2, 1, 0] = q[1::2, 0, 0] = -4.0
+    cache = kv8.Kv8Cache(batch, 1, d, n, format=e4m3)
+    lens = [n] * batch
+    kv8.append(cache, k.flatten(0, 1).cuda(), v.to(BF).flatten(0, 1).cuda(), _i32(lens), starts=_starts(lens))
+    out, lse = kv8.attention(cache, q.cuda(), _i32(lens), starts=_starts([m] * batch), scale=1.0)
+    kk, vv = ref.read(cache, n)
+    want, wl, mass, terms, _ = ref.attention(q, kk, vv, _starts([m] * batch).cpu(), lens, 1.0, n)
+    # the largest product of a probability and its block's largest value
+    top = torch.nn.functional.pad(vv.abs().amax(-1), (0, -n % 32)).unflatten(-1, (-1, 32)).amax(-1).repeat_interleave(32, -1)[:, 0, :n]
+    x = (q.double().unflatten(0, (batch, m)).flatten(1, 2) @ kk[:, 0].mT).unflatten(1, (m, 2))
+    x = torch.where(torch.arange(n) < (torch.arange(m) + n - m + 1)[:, None, None], x, -math.inf)
+    most = (torch.softmax(x, -1) * top[:, None, None]).amax(-1).flatten(0, 1)
+    # as in _check_attention, but what fp16 loses below 2^-14 is half of 2^-24 of the row's own largest product; the exponents of
+    # two, up to 2^8 in size here, are rounded in f32 (2^-16 of a probability for score, scale and reference)
+    off = (d + 8) * 2.0 ** -24 * terms + 2.0 ** -22
+    p = 2.0 ** -11 + 2.0 ** -15 + 2 * off[..., None] + 2 * n * 2.0 ** -24
+    tol = 2.0 ** -8 * want.abs() + p * mass + n * 2.0 ** -25 * most[..., None]
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+    assert ((lse.cpu().double() - wl).abs() <= off + 2.0 ** -16 + n * 2.0 ** -24 + 2.0 ** -22 * (1 + wl.abs())).all()

@@ -874,16 +874,16 @@ __device__ __forceinline__ uint32_t weight_first(const Kv8AttnArgs &a, const Wei
     return min(i0 * a.group / weight_rows(kFew), w.tiles);
 }
 
-// Eight codes as bf16, exact, times 2^-17: a sum of 256 of their products with bf16 values stays within f32.
+// Eight codes as bf16, exact, times a power of two.
 template <int E4M3>
-__device__ __forceinline__ bf16x8_t weight_key(uint32_t lo, uint32_t hi) {
+__device__ __forceinline__ bf16x8_t weight_key(uint32_t lo, uint32_t hi, float up) {
     float y[8];
     kv8_values<E4M3>(lo, y);
     kv8_values<E4M3>(hi, y + 4);
     u32x4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        w[i] = __builtin_amdgcn_perm(__float_as_uint(y[2 * i + 1] * 0x1p-17f), __float_as_uint(y[2 * i] * 0x1p-17f), 0x07060302u);
+        w[i] = __builtin_amdgcn_perm(__float_as_uint(y[2 * i + 1] * up), __float_as_uint(y[2 * i] * up), 0x07060302u);
     return __builtin_bit_cast(bf16x8_t, w);
 }
 
@@ -918,7 +918,7 @@ __global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint3
         load_units<NS>(kw, a.c.k + (bh * a.c.blocks + blk) * (size_t)(32 * D));
         const float kscale = a.c.ks[bh * a.c.blocks + blk];
         bf16x8_t kf[2 * NS];
-        const float ck = a.scale_log2 * (kscale * 0x1p17f);
+        float ck = 0.0f;  // the scale of a score
         // The query rows that see slot p are first_row .. w.rows - 1; the wave's slots are all seen from tile `clear` on.
         const auto first_row = [&](uint32_t p) { return (p + w.s.m > w.s.n ? p + w.s.m - w.s.n : 0u) * a.group; };
         const uint32_t row0 = p < w.n ? first_row(p) : w.rows, seen = w.rows - row0;
@@ -988,11 +988,21 @@ __global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint3
         };
         if (t0 < t1) {
             fetch();
-            // the keys' operands, once the first rows are on their way too
+            // The keys' operands, once the first rows are on their way too.  The codes enter times 2^-17: a sum of 256 products with
+            // bf16 values stays within f32.  Scales so large that their product with 2^17 might not: they leave 2^43 of it here and
+            // take the rest into the codes (scores within f32 stay there).
+            ck = a.scale_log2 * (kscale * 0x1p17f);
+            float kup = 0x1p-17f;
+            if (!(fabsf(ck) < 0x1p60f)) {
+                const int es = __builtin_amdgcn_frexp_expf(a.scale_log2) + __builtin_amdgcn_frexp_expf(kscale);
+                const int kx = min(max(es - 43, -17), 100);
+                ck = ldexpf(__builtin_amdgcn_frexp_mantf(a.scale_log2) * __builtin_amdgcn_frexp_mantf(kscale), es - kx);
+                kup = exp2_int(kx);
+            }
 #pragma unroll
             for (int j = 0; j < NS; ++j) {
-                kf[2 * j] = weight_key<E4M3>(kw[j].x, kw[j].y);
-                kf[2 * j + 1] = weight_key<E4M3>(kw[j].z, kw[j].w);
+                kf[2 * j] = weight_key<E4M3>(kw[j].x, kw[j].y, kup);
+                kf[2 * j + 1] = weight_key<E4M3>(kw[j].z, kw[j].w, kup);
             }
             stage(0);
             if (t0 + 1 < t1) fetch();

@@ -88,3 +88,22 @@ def test_blocks_of_large_values_that_a_row_hardly_attends(kv8, batch, m, n, powe
     tol = 2.0 ** -8 * want.abs() + p * mass + n * 2.0 ** -25 * most[..., None]
     assert ((out.cpu().double() - want).abs() <= tol).all()
     assert ((lse.cpu().double() - wl).abs() <= off + 2.0 ** -16 + n * 2.0 ** -24 + 2.0 ** -22 * (1 + wl.abs())).all()
+
+
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("q_gain,k_gain,scale", [
+    (1e-36, 1e36, 0.125), (2.0 ** -49, 2.0 ** -50, 0.9 * 2.0 ** 96), (2.0 ** 20, 2.0 ** -119, -0.9 * 2.0 ** 96),
+    (2.0 ** -100, 1.0, 0.9 * 2.0 ** 97), (2.0 ** -120, 2.0 ** 20, 0.9 * 2.0 ** 97), (2.0 ** 50, 2.0 ** 50, 2.0 ** -103),
+    (2.0 ** 110, 2.0 ** -113, 1.0)])
+@pytest.mark.parametrize("m", [1, 50])
+def test_attention_and_weights_near_the_limits(kv8, m, q_gain, k_gain, scale, e4m3):
+    """Queries, keys and scale whose product is of ordinary size, each near an end of its range."""
+    g = torch.Generator().manual_seed(31)
+    n, d = 300, 96
+    cache = _fill(kv8, g, [n], 2, d, e4m3, n, gain=k_gain)
+    q, starts, lens = _rand(g, m, 4, d, gain=q_gain), _starts([m]), _i32([n])
+    out, lse, want, off = _check_attention(kv8, cache, q, starts, lens, scale=scale)
+    assert float(off.max()) < 2.0 ** -8  # (ordinary scores: the tolerance means something)
+    w = kv8.accumulate_weight(cache, q.cuda(), lse, lens, torch.zeros(1, 2, n, device="cuda"), starts=starts, scale=scale)
+    tol = (4 * float(off.max()) + (n + 2 * m) * 2.0 ** -24 + 2.0 ** -20) * want + 1e-30
+    assert ((w.cpu().double() - want).abs() <= tol).all()

@@ -86,7 +86,8 @@ int kr_rope_apply(const kr_rope *rope, const void *x, size_t x_stride, void *y, 
  * b are rows starts[b] .. starts[b + 1] - 1 of k, v, q (starts: device u32 [batch + 1], not decreasing; a
  * sequence may have none) and take its last slots.  starts == NULL: tokens == batch, one each.
  * Values beyond `tokens`, slots beyond max_ctx and lengths below the number of new tokens are cut off, never followed.
- * Rows behind the last sequence's are nobody's: nothing of them is appended, and their results are left as they were.
+ * Rows before the first sequence's and behind the last's are nobody's: nothing of them is appended, and their results (q_out
+ * among them) are left as they were.
  * A length may be lowered to take tokens back as long as one token of the sequence's last block stays: the raw rows are that
  * block's. */
 #define KR_KV8_INT8 0

@@ -89,6 +89,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
     if (blockIdx.x >= items * a.c.heads) {
         if constexpr (kRope != 0) {
             const uint32_t t = blockIdx.x - items * a.c.heads;
+            if (a.step.starts && (t < a.step.starts[0] || t >= a.step.starts[a.c.batch])) return;  // nobody's row
             rope_token<uint16_t, kRope == 1>(a.rope, t, a.q + t * a.q_stride, a.q_out + t * a.q_stride, a.q_heads, D);
         }
         return;

@@ -24,11 +24,18 @@ def stream_of(t: torch.Tensor, stream):
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
-def held(t: torch.Tensor, stream) -> torch.Tensor:
-    """t, a tensor that a call allocates for itself on the current stream, kept from reuse until the call's own stream is done."""
-    if stream is not None:
-        t.record_stream(stream if isinstance(stream, torch.cuda.Stream) else
-                        torch.cuda.ExternalStream(stream_of(t, stream), device=t.device))
+def new(shape, dtype, device: torch.device, stream=None) -> torch.Tensor:
+    """A tensor that a call on `stream` makes: of that stream's own memory, so that work still pending on the current stream never
+    meets it and it is not reused before the call is done, and kept for the current stream, on which the caller goes on."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    here = torch.cuda.current_stream(device)
+    raw = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+    if raw == here.cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(raw, device=here.device)):
+        t = torch.empty(shape, dtype=dtype, device=here.device)
+    t.record_stream(here)
     return t
 
 

@@ -19,7 +19,7 @@ import torch
 
 from . import DTYPE_BF16, DTYPE_F32, _check, lib
 from . import rope as _rope
-from ._device import at, checked, held, stream_of
+from ._device import at, checked, new, stream_of
 
 INT8, E4M3 = 0, 1
 BLOCK = 32
@@ -134,8 +134,7 @@ def dequant(cache: Kv8Cache, lengths: torch.Tensor, count: int, first: Optional[
     lengths[b] on (kr_kv8_dequant)."""
     shape = (cache.batch, count, cache.kv_heads, cache.head_dim)
     if out is None:
-        device = cache.k.device
-        out = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        out = new(shape, dtype, cache.k.device, stream), new(shape, dtype, cache.k.device, stream)
     else:
         checked("out[0]", out[0], out[0].dtype, shape, cache.k)
         checked("out[1]", out[1], out[0].dtype, shape, cache.k)
@@ -149,10 +148,11 @@ def dequant(cache: Kv8Cache, lengths: torch.Tensor, count: int, first: Optional[
     return out
 
 
-def attention_workspace(cache: Kv8Cache, q_heads: int, tokens: int) -> torch.Tensor:
-    """Device workspace of attention (partial sums of split contexts); one made for a step serves all its layers."""
+def attention_workspace(cache: Kv8Cache, q_heads: int, tokens: int, stream=None) -> torch.Tensor:
+    """Device workspace of attention (partial sums of split contexts) for calls on `stream` (the current one where None); one
+    made for a step serves all its layers."""
     n = int(lib().kr_kv8_attention_workspace_bytes(cache.desc, q_heads, tokens))
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+    return new((max(n, 16),), torch.uint8, cache.k.device, stream)
 
 
 def attention(cache: Kv8Cache, q: torch.Tensor, lengths: torch.Tensor, starts: Optional[torch.Tensor] = None,
@@ -164,13 +164,13 @@ def attention(cache: Kv8Cache, q: torch.Tensor, lengths: torch.Tensor, starts: O
     tokens, heads, d = q.shape
     s, n = _step(cache, tokens, starts, lengths)
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=torch.bfloat16, device=q.device)
+        out = new((tokens, heads, d), torch.bfloat16, q.device, stream)
     if lse is None:
-        lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device)
+        lse = new((tokens, heads), torch.float32, q.device, stream)
     checked("out", out, torch.bfloat16, (tokens, heads, d), cache.k)
     checked("lse", lse, torch.float32, (tokens, heads), cache.k)
     if workspace is None:
-        workspace = held(attention_workspace(cache, heads, tokens), stream)
+        workspace = attention_workspace(cache, heads, tokens, stream)
     checked("workspace", workspace, torch.uint8, None, cache.k)
     with at(cache.k):
         _check(lib().kr_kv8_attention(cache.desc, q.data_ptr(), qs, heads, tokens, s, n,
@@ -179,10 +179,10 @@ def attention(cache: Kv8Cache, q: torch.Tensor, lengths: torch.Tensor, starts: O
     return out, lse
 
 
-def weight_workspace(cache: Kv8Cache, q_heads: int, tokens: int) -> torch.Tensor:
-    """Device workspace of accumulate_weight (sums of parts of many query rows)."""
+def weight_workspace(cache: Kv8Cache, q_heads: int, tokens: int, stream=None) -> torch.Tensor:
+    """Device workspace of accumulate_weight (sums of parts of many query rows) for calls on `stream`."""
     n = int(lib().kr_kv8_weight_workspace_bytes(cache.desc, q_heads, tokens))
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=cache.k.device)
+    return new((max(n, 16),), torch.uint8, cache.k.device, stream)
 
 
 def accumulate_weight(cache: Kv8Cache, q: torch.Tensor, lse: torch.Tensor, lengths: torch.Tensor, weight: torch.Tensor,
@@ -196,7 +196,7 @@ def accumulate_weight(cache: Kv8Cache, q: torch.Tensor, lse: torch.Tensor, lengt
     checked("lse", lse, torch.float32, (tokens, heads), cache.k)
     checked("weight", weight, torch.float32, (cache.batch, cache.kv_heads, cache.max_ctx), cache.k)
     if workspace is None:
-        workspace = held(weight_workspace(cache, heads, tokens), stream)
+        workspace = weight_workspace(cache, heads, tokens, stream)
     checked("workspace", workspace, torch.uint8, None, cache.k)
     with at(cache.k):
         _check(lib().kr_kv8_accumulate_weight(cache.desc, q.data_ptr(), qs, heads, tokens, s, n,
@@ -214,9 +214,9 @@ def evict(cache: Kv8Cache, lengths: torch.Tensor, weight: torch.Tensor, budget: 
     int32 [batch])."""
     _, n = _step(cache, 0, None, lengths)
     if kept is None:
-        kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=cache.k.device)
+        kept = new((cache.batch, cache.kv_heads, budget), torch.int32, cache.k.device, stream)
     if to_lengths is None:
-        to_lengths = torch.empty_like(lengths)
+        to_lengths = new((cache.batch,), torch.int32, cache.k.device, stream)
     checked("to.k", to.k, torch.uint8, None, cache.k)
     checked("weight", weight, torch.float32, (cache.batch, cache.kv_heads, cache.max_ctx), cache.k)
     checked("to_weight", to_weight, torch.float32, (cache.batch, cache.kv_heads, to.max_ctx), cache.k)

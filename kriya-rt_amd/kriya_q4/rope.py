@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from . import DTYPE_BF16, DTYPE_F32, KrError, KR_E_SHAPE, _check, lib
-from ._device import at, checked, stream_of
+from ._device import at, checked, new, stream_of
 
 HALF, INTERLEAVED = 0, 1
 KINDS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
@@ -51,7 +51,7 @@ def table(rotary_dim: int, count: int, theta: float, first: int = 0, scaling: Op
           out: Optional[torch.Tensor] = None, device="cuda", stream=None) -> torch.Tensor:
     """cos and sin of positions first .. first + count - 1: f32 [count, rotary_dim / 2, 2] (kr_rope_table)."""
     if out is None:
-        out = torch.empty((count, rotary_dim // 2, 2), dtype=torch.float32, device=device)
+        out = new((count, rotary_dim // 2, 2), torch.float32, torch.device(device), stream)
     checked("out", out, torch.float32, (count, rotary_dim // 2, 2))
     z = ctypes.byref(scaling._c()) if scaling is not None else None
     with at(out):

@@ -37,8 +37,9 @@ class QwenKv8Decoder(QwenQ4Decoder):
         super().__init__(cfg, batch, ctx, seed, device)
         positions = self._capacity if max_positions is None else max_positions
         self.cos_sin = rope.table(cfg.head_dim, positions, cfg.rope_theta, scaling=scaling, device=device)
-        # tokens in the caches and next positions of the sequences, as far as the calls made here tell
-        self._used, self._next = [ctx] * batch, [ctx] * batch
+        # tokens in the caches and next positions of the sequences, as far as the calls made here tell: a captured step's replays
+        # move the device's alone
+        self._used, self._next, self._captured = [ctx] * batch, [ctx] * batch, False
         self._spare = None
         self.attn = torch.empty((batch, cfg.q_heads, cfg.head_dim), dtype=torch.bfloat16, device=device)
         self.lse = torch.empty((batch, cfg.q_heads), dtype=torch.float32, device=device)
@@ -79,6 +80,12 @@ class QwenKv8Decoder(QwenQ4Decoder):
             q4_linear(L.o, attn, y=h, accumulate=True, workspace=o_ws, stream=stream)
             rmsnorm_mlp(L.gate, L.up, L.down, h, L.ln2, c.eps, activation=ACT_SWIGLU, workspace=mlp_ws, stream=stream)
 
+    def _read_back(self, what: str) -> None:
+        """The host's counts from the device's (a synchronization)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} reads lengths back: it cannot be part of a capture")
+        self._used, self._next = torch.stack((self.lengths, self.positions)).tolist()
+
     def _grow(self, counts) -> None:
         used, after = ([a + n for a, n in zip(to, counts)] for to in (self._used, self._next))
         if max(used) > self._capacity:
@@ -90,9 +97,14 @@ class QwenKv8Decoder(QwenQ4Decoder):
     def step(self, stream=None) -> torch.Tensor:
         """One greedy decode step of every sequence: `tokens` are appended at `positions`, both move on; returns the
         next-token buffer.  stream: a torch.cuda.Stream.  Nothing returns to the host, so a step can be captured and replayed
-        (as long as caches and rotary table hold: keys that do not fit are cut off, positions past the table not turned)."""
+        (as long as caches and rotary table hold: in replays keys that do not fit are cut off, positions past the table not
+        turned).  Once a step has been captured, eager ones read the lengths back, to go by what replays have added."""
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
-            if not torch.cuda.is_current_stream_capturing():
+            if torch.cuda.is_current_stream_capturing():
+                self._captured = True
+            else:
+                if self._captured:
+                    self._read_back("an eager step")
                 self._grow([1] * self.batch)
             self.lengths.add_(1)
             embedding(self.embed, self.tokens, out=self.h, stream=stream)
@@ -106,13 +118,15 @@ class QwenKv8Decoder(QwenQ4Decoder):
 
     def prefill(self, tokens: torch.Tensor, counts) -> torch.Tensor:
         """Appends counts[b] tokens to each sequence b (tokens int32, sequence after sequence; a count may be 0) in one ragged
-        batch and sets `logits` and `tokens` of those that got any to what follows their last one; returns the next-token buffer."""
+        batch and sets `logits` and `tokens` of those that got any to what follows their last one; returns the next-token buffer.
+        Reads the lengths back, so it goes by what replays of a captured step have added too."""
         c, m, device = self.cfg, int(tokens.numel()), tokens.device
         counts = [int(n) for n in counts]
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != m:
             raise ValueError(f"counts={counts} do not split {m} tokens over {self.batch} sequences")
         if m == 0:
             return self.next
+        self._read_back("prefill")
         self._grow(counts)
         n = torch.tensor(counts, dtype=torch.int32, device=device)
         starts = torch.zeros(self.batch + 1, dtype=torch.int32, device=device)
@@ -143,10 +157,11 @@ class QwenKv8Decoder(QwenQ4Decoder):
 
     def evict(self, budget: int, sink: int = 4, recent: int = 64) -> None:
         """Cuts every sequence's cache to `budget` tokens (kv8.evict): the first `sink`, the last `recent` and those of most
-        attention weight since they were appended.  Needs track_weights.  The layers' caches change places with a spare one: a captured
-        step is to be captured again."""
+        attention weight since they were appended.  Needs track_weights.  Reads the lengths back; the layers' caches change places with a
+        spare one: a captured step is to be captured again."""
         if not self._track:
             raise ValueError("evict needs a decoder with track_weights=True")
+        self._read_back("evict")
         if self._spare is None:
             device = self.lengths.device
             self._spare = self._new_cache(device), self._new_weight(device)

@@ -42,8 +42,8 @@ typedef struct kr_rope_scaling {
     double gain;          /* multiplies cos and sin (1; YaRN's attention factor 0.1 ln s + 1) */
 } kr_rope_scaling;
 
-/* cos_sin[r] = the table row of position first + r, r < count.  Angles are reduced to a turn in 64 bits, so
- * far positions are as exact as near ones.  scaling: host pointer, NULL for none.  rotary_dim even, 2 .. 256;
+/* cos_sin[r] = the table row of position first + r, r < count.  Angles, sines and cosines
+ * are computed in 64 bits and rounded once, so far positions are as exact as near ones.  scaling: host pointer, NULL for none.  rotary_dim even, 2 .. 256;
  * theta > 0.  cos_sin 8-byte aligned. */
 int kr_rope_table(float *cos_sin, uint32_t first, uint32_t count, uint32_t rotary_dim, double theta,
                   const kr_rope_scaling *scaling, void *stream);

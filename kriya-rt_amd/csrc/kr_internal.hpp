@@ -334,7 +334,7 @@ struct RopeArgs {  // rotary_dim even, rows of the table 8-byte aligned
 inline bool rope_units_ok(const RopeArgs &a, uint32_t D) {
     return a.rotary_dim % 16 == 0 && D % 8 == 0 && (uintptr_t)a.cos_sin % 16 == 0;
 }
-hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, uint32_t count, float gain,
+hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, uint32_t count, double gain,
                              float *cos_sin, hipStream_t s);
 hipError_t launch_rope_apply(const RopeArgs &a, const void *x, size_t xs, void *y, size_t ys, int f32, uint32_t tokens,
                              uint32_t heads, uint32_t D, hipStream_t s);

@@ -112,7 +112,7 @@ int kr_rope_table(float *cos_sin, uint32_t first, uint32_t count, uint32_t rotar
         }
         f.turns[i] = w / pi2;
     }
-    return hip_status(launch_rope_table(f, rotary_dim / 2, first, count, (float)z.gain, cos_sin, (hipStream_t)stream),
+    return hip_status(launch_rope_table(f, rotary_dim / 2, first, count, z.gain, cos_sin, (hipStream_t)stream),
                       "kr_rope_table");
 }
 

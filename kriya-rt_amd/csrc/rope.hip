@@ -11,21 +11,20 @@
 namespace kr {
 
 // The angle of position p at f turns a position is p f turns, of which only the fraction counts.  p f is taken in 64
-// bits (an error of 2^-53 p f turns: 1e-11 at a million), the fraction by rint, and only the fraction's sine and
-// cosine in 32.  Bound by its launch: 3907 rows of 16 pairs 1.7 us.
+// bits (an error of 2^-53 p f turns: 1e-11 at a million), the fraction by rint; its sine and cosine are 64 bits too, so a table holds
+// the f32 nearest to them.  Bound by its launch: 3907 rows of 16 pairs 1.7 us.
 __global__ __launch_bounds__(256) void rope_table_kernel(RopeTurns f, uint32_t half, uint32_t first, uint32_t count,
-                                                         float gain, float *cos_sin) {
+                                                         double gain, float *cos_sin) {
     const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t r = (uint32_t)(at / half), i = (uint32_t)(at % half);
     if (r >= count) return;
     const double turns = ((double)first + (double)r) * f.turns[i];
-    const float frac = (float)(turns - rint(turns));
-    float s, c;
-    sincospif(2.0f * frac, &s, &c);
-    reinterpret_cast<float2 *>(cos_sin)[at] = make_float2(gain * c, gain * s);
+    double s, c;
+    sincospi(2.0 * (turns - rint(turns)), &s, &c);
+    reinterpret_cast<float2 *>(cos_sin)[at] = make_float2((float)(gain * c), (float)(gain * s));
 }
 
-hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, uint32_t count, float gain,
+hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, uint32_t count, double gain,
                              float *cos_sin, hipStream_t s) {
     const uint64_t blocks = ((uint64_t)count * half + 255) / 256;
     rope_table_kernel<<<dim3((uint32_t)blocks), 256, 0, s>>>(f, half, first, count, gain, cos_sin);

@@ -65,16 +65,19 @@ __device__ __forceinline__ float value_shift(const RowSums &r, float vlog) { ret
 // Whether a block whose largest score of the row is `top` passes what the row's base or d allow (one comparison once top is known);
 // both following it, and the factor of O.
 __device__ __forceinline__ bool row_passed(const RowSums &r, float top, float vlog) {
-    return top > r.base + fminf(8.0f, 15.0f - (vlog - r.d));
+    return top - r.base > fminf(8.0f, 15.0f - (vlog - r.d));
 }
 __device__ __forceinline__ float row_follow(RowSums &r, float top, float vlog) {
     const float base = fmaxf(r.base, top), down = r.base - base;
-    const float d = fmaxf(fmaxf(r.d + down, top + vlog - base - kTo), kLeast), od = down + (r.d - d);
+    const float d = fmaxf(fmaxf(r.d + down, (top - base) + vlog - kTo), kLeast), od = down + (r.d - d);
     r.base = base;
     r.d = d;
     r.l *= __builtin_amdgcn_exp2f(down);
     return __builtin_amdgcn_exp2f(od);
 }
+// Whether a base is so large that in its sum with an exponent beside it that exponent is off by more than 2^-14: then the scores'
+// differences from the base are taken first.  (A row that has seen no slot has no base.)
+__device__ __forceinline__ bool row_far(const RowSums &r) { return fabsf(r.base) > 0x1p10f && r.base > -9e37f; }
 
 // The row in fp16 times a power of two that brings its largest value to [2^14, 2^15): bf16 holds 8 bits of significand
 // and fp16 11, so every value down to 2^-28 of the largest is exact, and the rest are off by 2^-39 of it at
@@ -339,6 +342,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 #pragma unroll
         for (int i = 0; i < NS; ++i) o[i] = f32x16{};
         RowSums sums;
+        bool far = false;     // a row of the wave is row_far
         float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
         // what body n writes: this wave's pieces of keys n + 2 and values n + 1
         u32x4 piece[kUnits];
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
         };
         // The scores of the block in work, times c the exponents; its row maximum has been taken into `base`.
         f32x16 p;
-        float c;
+        float c, shift, org;  // shift: the exponent beside the probabilities; org: what the scores' exponents are taken from
         const auto key_steps = [&](f32x16 &s, const u32x4 (&kf)[2 * NS]) {
 #pragma unroll
             for (int j = 0; j < 2 * NS; ++j)
@@ -383,17 +387,21 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
         };
         // What a new block's scores change: slots that a row does not see get -infinity; the row's base and reference follow only when
         // they are passed (O is scaled down a few times in all).
-        // Returns the exponent beside the block's probabilities.
         const auto enter = [&](float top, float vscale, uint32_t p0) {
-            float vlog = __log2f(vscale);
+            float vlog = __log2f(vscale), ref = 0.0f;  // ref: what has been taken from the scores already
             const bool normal = __builtin_amdgcn_classf(vscale, 0x100);  // (log2 takes subnormal numbers for 0)
-            if (p0 + 32 > least || !normal) {
+            const bool special = p0 + 32 > least || !normal || far;
+            if (special) {
+#pragma clang fp contract(off)  // (the same bits for the maximum and for the difference from it)
                 const uint32_t room = limit > p0 ? limit - p0 : 0u;  // slots of this block that the row sees
 #pragma unroll
                 for (int i = 0; i < 16; ++i) p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < room ? p[i] * c : -INFINITY;
                 c = 1.0f;
                 top = row_top(p);
                 top = fmaxf(top, xchg32(top, lane));
+                ref = fmaxf(sums.base, top);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] -= ref;
                 if (!(vscale < INFINITY) && room) poison = __builtin_nanf("");
                 vlog = value_scale_log2(vscale);
             }
@@ -403,12 +411,21 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 for (int d = 0; d < NS; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= down;
+                far = __any(row_far(sums));
+                if (far && !special) {
+#pragma clang fp contract(off)
+                    ref = sums.base;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] = p[i] * c - ref;
+                    c = 1.0f;
+                }
             }
-            return value_shift(sums, vlog);
+            shift = value_shift(sums, vlog);
+            org = sums.base - ref;
         };
         // Body n.  One run of instructions, so that the vector unit takes the exponentials while the matrix cores multiply the
         // next keys, and the next row maximum while they multiply values.
-        const auto body = [&](auto more, uint32_t n, float shift) {
+        const auto body = [&](auto more, uint32_t n) {
             constexpr bool kMore = decltype(more)::value;
             u32x4 kf[2 * NS], vf[2 * NS];
             if constexpr (kMore) {
@@ -420,7 +437,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 #pragma unroll
             for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j][lane];
             // the values' scale joins the exponent, and l takes it out again
-            const float from = sums.base - shift;
+            const float from = org - shift;
             float sum = 0.0f;
             f16x8_t pf[2];
 #pragma unroll
@@ -445,9 +462,8 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 fetch_scales(n + 1);
                 float top = row_top(p) * c;
                 top = fmaxf(top, xchg32(top, lane));
-                return enter(top, vnext, (n + 1) * 32);
+                enter(top, vnext, (n + 1) * 32);
             }
-            return 0.0f;
         };
         if (first < end) {
             // keys first and first + 1, values first
@@ -457,7 +473,6 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
                 const uint8_t *from = (u / NS == 2 ? v : k) + (size_t)at * (32 * D) + 1024 * j + 16 * lane;
                 put(u / NS == 2 ? lds[1][first & 1] : lds[0][at & 1], j, *reinterpret_cast<const u32x4 *>(from));
             }
-            const float vfirst = uniform(vs[first]);
             c = score_scale(q.c, q.x, uniform(ks[first]));
             fetch(first);
             fetch_scales(first);
@@ -469,17 +484,17 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             key_steps(p, kf);
             float top = row_top(p) * c;
             top = fmaxf(top, xchg32(top, lane));
-            float shift = enter(top, vfirst, first * 32);
+            enter(top, uniform(vs[first]), first * 32);
             for (uint32_t n = first; n + 1 < end; ++n) {
                 // a wave in its body goes before one that is still at the barrier's end: 593 -> 570 us for 2048 tokens over 14000
                 // (32/4 heads, D 128); with one wave a SIMD there is none to go before
                 if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(0);
                 __syncthreads();
                 if constexpr (NS <= 4) __builtin_amdgcn_s_setprio(1);
-                shift = body(std::true_type{}, n, shift);
+                body(std::true_type{}, n);
             }
             __syncthreads();
-            body(std::false_type{}, end - 1, shift);
+            body(std::false_type{}, end - 1);
         }
         const float l = sums.l + xchg32(sums.l, lane);
         // (two factors: their product may be below the normal floats)
@@ -626,6 +641,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
 #pragma unroll
     for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
     RowSums sums;
+    bool far = false;     // a row of the wave is row_far
     float poison = 0.0f;  // NaN for a row that sees values that stand for NaN
     const auto step = [&](auto masked, const FewBlock<NS> &f, uint32_t blk) {
         constexpr bool kEdge = decltype(masked)::value;
@@ -646,6 +662,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+#pragma clang fp contract(off)  // (the same bits for the maximum and for the difference from it)
             float x = p[i >> 2][i & 3] * c;
             if (kEdge && 16 * (i >> 2) + 4 * g + (i & 3) >= room) x = -INFINITY;
             p[i >> 2][i & 3] = x;
@@ -657,8 +674,15 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
             const float down = row_follow(sums, top, vlog);
 #pragma unroll
             for (int d = 0; d < 2 * NS; ++d) o[d] *= down;
+            far = __any(row_far(sums));
         }
-        const float shift = value_shift(sums, vlog), from = sums.base - shift;
+        const float shift = value_shift(sums, vlog);
+        float from = sums.base - shift;
+        if (far) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i >> 2][i & 3] -= sums.base;
+            from = -shift;
+        }
         float sum = 0.0f;
         f16x8_t pf;
 #pragma unroll

@@ -107,3 +107,32 @@ def test_attention_and_weights_near_the_limits(kv8, m, q_gain, k_gain, scale, e4
     w = kv8.accumulate_weight(cache, q.cuda(), lse, lens, torch.zeros(1, 2, n, device="cuda"), starts=starts, scale=scale)
     tol = (4 * float(off.max()) + (n + 2 * m) * 2.0 ** -24 + 2.0 ** -20) * want + 1e-30
     assert ((w.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("power", [8, 12, 20, 30, 60, -30])
+@pytest.mark.parametrize("step", [40.0, -40.0, 9.0])
+@pytest.mark.parametrize("batch,m,n", [(1, 1, 160), (130, 1, 700), (1, 60, 160), (16, 60, 1600)])
+def test_equal_scores_of_any_size_over_values_of_many(kv8, batch, m, n, step, power):
+    """Every key the same, scores near 2^power (or -2^30): a plain average, whatever the blocks' scales of values are."""
+    g = torch.Generator().manual_seed(400 + n)
+    d = 64
+    block = torch.arange(n) // 32
+    v = _rand(g, batch, n, 1, d).double() * torch.exp2(step * (block % 3))[:, None, None]
+    k = torch.ones(batch, n, 1, d, dtype=BF)
+    q = torch.ones(batch * m, 2, d, dtype=BF)
+    scale = 2.0 ** (abs(power) - 6) * (1 if power > 0 else -1)
+    cache, lens = kv8.Kv8Cache(batch, 1, d, n), [n] * batch
+    kv8.append(cache, k.flatten(0, 1).cuda(), v.to(BF).flatten(0, 1).cuda(), _i32(lens), starts=_starts(lens))
+    out, lse = kv8.attention(cache, q.cuda(), _i32(lens), starts=_starts([m] * batch), scale=scale)
+    _, vv = ref.read(cache, n)
+    seen = torch.arange(m) + n - m + 1
+    cut = (torch.arange(n) < seen[:, None]).double() / seen[:, None]  # [m, n]
+    want, mass = cut @ vv[:, 0], cut @ vv[:, 0].abs()               # [batch, m, d]
+    most = vv[:, 0].abs().amax((1, 2))[:, None, None] / seen[:, None]
+    got = out.cpu().double().unflatten(0, (batch, m))
+    # the scores are the same bits, so only fp16's and bf16's half steps, sums of n in f32 and the exponents' 2^-14 (2^-15 of scores below 2^10)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -11 + 2.0 ** -13 + 2 * n * 2.0 ** -24) * mass + n * 2.0 ** -25 * most
+    assert ((got - want[:, :, None]).abs() <= tol[:, :, None]).all()
+    at = scale * 64 * float(ref.read(cache, 1)[0][0, 0, 0, 0])
+    wl = at + torch.log(seen.double())[:, None]
+    assert ((lse.cpu().double().unflatten(0, (batch, m)) - wl).abs() <= (d + 8) * 2.0 ** -24 * abs(at) + n * 2.0 ** -24 + 2.0 ** -22 * (1 + abs(at))).all()

@@ -33,7 +33,11 @@ extern "C" {
 #define KR_ROPE_SCALE_NTK 2    /* theta replaced by theta * factor^(rotary_dim / (rotary_dim - 2)) */
 #define KR_ROPE_SCALE_PARTS 3  /* by parts: with r = original_ctx f_i / (2 pi) turns over the trained
                                 * context and g = clamp((r - slow) / (fast - slow), 0, 1):
-                                * f_i (g + (1 - g) / factor) (YaRN's interpolation by parts)      */
+                                * f_i (g + (1 - g) / factor): the YaRN paper's interpolation by
+                                * parts, a ramp over turns.  Checkpoints stretched by its authors'
+                                * program ramp over i between whole numbers instead (theta 1e6,
+                                * 128 dims, 32768, factor 4: frequencies up to 71 % apart): make
+                                * their table by their formula, the rotations take any table.     */
 typedef struct kr_rope_scaling {
     int kind;             /* KR_ROPE_SCALE_*                                                  */
     double factor;        /* > 0; how much longer than trained                                */
@@ -139,7 +143,8 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
  * weight f32 [batch, kv_heads, max_ctx]: for every slot p < lengths[b] of every kv head
  *   weight[p] = decay * (p < n - m ? weight[p] : 0) + sum over the m new tokens and the heads of the group of e^(scale q . K_p - lse)
  * with the lse that kr_kv8_attention gave for the same q (slots of the new tokens start at zero: no initial contents are
- * needed; slots from lengths[b] on are left as they were).  Sums in f32, in a fixed order.  tokens == 0 does nothing.
+ * needed; slots from lengths[b] on are left as they were).  Sums in f32, in a fixed order.  tokens == 0 does nothing.  lse is f32, so a
+ * weight is off by half a step of its row's score: little up to scores of 2^12, all of it from 2^24 on.
  * The codes enter the matrix cores as bf16 (exact), as q does; the scores are f32.
  * workspace: kr_kv8_weight_workspace_bytes(cache, q_heads, tokens) bytes (none for few rows, else about the size of weight), 16-byte
  * aligned, no initial contents; calls sharing it must not overlap in time. */

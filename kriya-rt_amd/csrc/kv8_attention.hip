@@ -9,7 +9,8 @@
 //   s_rp = (q'_r . k_p) (c_r ks),   m_r = max_p s_rp,   l_r = sum_p 2^(s_rp - m_r),
 //   out_r = 2^d_r sum_p 2^(s_rp - m_r + log2 vs - d_r) v_p / l_r
 // with k_p, v_p the codes.  One pass over the slots: m_r only grows, and sums made under an older m_r are scaled down.  What enters
-// the second product is fp16, so its exponent has a reference of its own for each row: d_r follows the largest product of a
+// the second product is fp16 (the matrix cores take f32 at a fraction of its rate; half a step is 2^-11 where the bf16 output's own is
+// 2^-8), so its exponent has a reference of its own for each row: d_r follows the largest product of a
 // probability and its block's scale of values, so that a block of large values that a row hardly sees takes no bits from the others.
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T, on v_mfma_f32_32x32x16_f16: a lane then holds one
 // query row (column l & 31) and the slots 8 i + 4 (l >> 5) + j of a block, its m_r and l_r are plain registers, and after
@@ -290,7 +291,7 @@ __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_
 // cores take), each as the 16 bytes a lane that an operand load takes.  Body n of the loop takes block n's softmax and second
 // product and block n + 1's first; it reads keys n + 1 and values n, and writes keys n + 2 and values n + 1 into the other
 // halves, so that one barrier a block is enough.  Bound by what the matrix cores and the vector unit cannot overlap: 2048 tokens
-// over 14000, 32/4 heads, int8: D 128 870 TFLOP/s, D 256 865, D 64 680; a prompt of 3907 of 16/2 heads of 128 102 us (610: the
+// after 14000, 32/4 heads, int8: D 128 930 TFLOP/s, D 256 875, D 64 710; a prompt of 3907 of 16/2 heads of 128 97 us (645: the
 // diagonal's tiles are of unequal length).
 constexpr uint32_t kManyRows = 128;
 
@@ -762,7 +763,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
 // Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
 // of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile (four waves: with 16, which
 // find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).  Bound by latency (work count,
-// maxima, parts): 16 rows in 512 parts 6.5 us, 1536 rows in a few 8.4, 6000 rows of 256 10.3 for 34 MB.
+// maxima, parts): 16 rows in 256 parts 6.5 us, 1536 rows in a few 8.3, 6000 rows of 256 10.3 for 34 MB.
 constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;
 template <int NS, bool kMany, bool kWide>
 __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split,

@@ -8,6 +8,9 @@ sequences have other than one new token, `starts` (int32 [batch + 1]: their rows
     lengths += 1
     kv8.append(cache, k, v, lengths, q=q, q_out=q, cos_sin=table, positions=lengths - 1)
     out, lse = kv8.attention(cache, q, lengths)
+
+Calls run on `stream` (a torch.cuda.Stream or a raw one), the current stream where None.  What a call allocates for itself or its
+caller is of that stream's memory; inputs and given outputs are the caller's to order and to keep, as with any stream.
 """
 from __future__ import annotations
 

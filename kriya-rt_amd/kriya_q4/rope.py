@@ -29,7 +29,8 @@ class kr_rope(ctypes.Structure):
 @dataclasses.dataclass(frozen=True)
 class Scaling:
     """How the frequencies are stretched: "none", "linear" (position interpolation), "ntk" (a larger theta) or "parts"
-    (by parts, between `slow` and `fast` turns over the trained context).  gain multiplies cos and sin; None takes 1,
+    (by parts, between `slow` and `fast` turns over the trained context, as in the YaRN paper; checkpoints that ramp over the index of a
+    frequency between whole numbers need a table made so, which every call here takes).  gain multiplies cos and sin; None takes 1,
     and 0.1 ln(factor) + 1 for "parts" with a factor above 1."""
     kind: str = "none"
     factor: float = 1.0

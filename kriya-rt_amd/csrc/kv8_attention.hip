@@ -727,21 +727,18 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
         float M = sm[0][row], L = 0.0f;
 #pragma unroll
         for (uint32_t x = 1; x < kFewWaves; ++x) M = fmaxf(M, sm[x][row]);
-        f32x4 acc = {0, 0, 0, 0};
-        bool nan = false;
+        float wx[kFewWaves];
 #pragma unroll
         for (uint32_t x = 0; x < kFewWaves; ++x) {
             const float lx = sl[x][row];
-            nan |= lx != lx;
-            if (lx > 0.0f) {  // a wave that saw no slot has nothing to add
-                const float wx = lx * __builtin_amdgcn_exp2f(sm[x][row] - M);
-                L += wx;
-                acc += wx * *reinterpret_cast<const f32x4 *>(&so[x][row][d]);
-            }
+            wx[x] = lx == 0.0f ? 0.0f : lx * __builtin_amdgcn_exp2f(sm[x][row] - M);  // NaN stays
+            L += wx[x];
         }
-        if (nan) L = __builtin_nanf("");
+        // the weights before the values, which may be near the largest float
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-        acc *= inv;
+        f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t x = 0; x < kFewWaves; ++x) acc += wx[x] * inv * *reinterpret_cast<const f32x4 *>(&so[x][row][d]);
         if (w.parts == 1) {
             const uint32_t tt = s.t0 + rr / a.group, hh = head * a.group + rr % a.group;
             const size_t at = (size_t)tt * a.q_heads + hh;
@@ -809,27 +806,35 @@ __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_jo
                 wl[p] = f;
                 sum += f;
             }
-            L += wave_sum(sum);
-            if constexpr (kWide) __syncthreads();
-            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            // the weights are divided by L before they meet values, which may be near the largest float
+            sum = wave_sum(sum);
+            if constexpr (kWide) {
+                if (lane == 0) red[1][wave] = sum;
+                __syncthreads();
+                sum = red[1][0];
+#pragma unroll
+                for (uint32_t i = 1; i < kJoinThreads / 64; ++i) sum += red[1][i];
+            } else {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+            const float before = L;
+            L += sum;
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            if (p0) acc *= before * inv;
             if (way < kWays) {
 #pragma unroll 8
                 for (uint32_t p = way; p < n; p += kWays)
-                    acc += wl[p] * *reinterpret_cast<const f32x4 *>(o + part_row(p0 + p) * D);
+                    acc += wl[p] * inv * *reinterpret_cast<const f32x4 *>(o + part_row(p0 + p) * D);
             }
             if constexpr (!kWide) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         if constexpr (kWide) {
             if (way < kWays) so[way][quad] = acc;
-            if (lane == 0) red[1][wave] = L;
             __syncthreads();
             if (tid >= kQuads) return;
             acc = so[0][tid];
 #pragma unroll
             for (uint32_t i = 1; i < kWays; ++i) acc += so[i][tid];
-            L = red[1][0];
-#pragma unroll
-            for (uint32_t i = 1; i < kJoinThreads / 64; ++i) L += red[1][i];
         } else {
 #pragma unroll
             for (uint32_t i = 1; i < kWays; ++i)
@@ -840,7 +845,6 @@ __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_jo
                 }
         }
         if (tid < kQuads) {
-            acc *= L == 0.0f ? 0.0f : 1.0f / L;
             const size_t to = (size_t)(w.s.t0 + r / a.group) * a.q_heads + head * a.group + r % a.group;
             const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
             *reinterpret_cast<u32x2 *>(a.out + to * D + 4 * tid) = y;

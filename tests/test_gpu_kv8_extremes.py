@@ -136,3 +136,18 @@ def test_equal_scores_of_any_size_over_values_of_many(kv8, batch, m, n, step, po
     at = scale * 64 * float(ref.read(cache, 1)[0][0, 0, 0, 0])
     wl = at + torch.log(seen.double())[:, None]
     assert ((lse.cpu().double().unflatten(0, (batch, m)) - wl).abs() <= (d + 8) * 2.0 ** -24 * abs(at) + n * 2.0 ** -24 + 2.0 ** -22 * (1 + abs(at))).all()
+
+
+@pytest.mark.parametrize("e4m3", [0, 1])
+@pytest.mark.parametrize("batch,m,n", [(1, 1, 33), (1, 1, 160), (1, 2, 5000), (3, 1, 40000), (1, 60, 160), (1, 60, 5000), (1, 600, 4000)])
+def test_values_near_the_largest(kv8, batch, m, n, e4m3):
+    """Values up to 2^127: their averages are finite, however many waves and parts they are joined from."""
+    g = torch.Generator().manual_seed(500 + n)
+    d, lens = 64, [n] * batch
+    k = _rand(g, batch * n, 1, d)
+    v = ((torch.rand(batch * n, 1, d, generator=g) - 0.25) * 2.0 ** 127).to(BF)
+    cache = kv8.Kv8Cache(batch, 1, d, n, format=e4m3)
+    kv8.append(cache, k.cuda(), v.cuda(), _i32(lens), starts=_starts(lens))
+    q = _rand(g, batch * m, 2, d, gain=0.5)
+    out, lse, _, _ = _check_attention(kv8, cache, q, _starts([m] * batch), _i32(lens))
+    assert out.isfinite().all() and lse.isfinite().all()

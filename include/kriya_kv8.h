@@ -126,8 +126,8 @@ int kr_kv8_dequant(const kr_kv8_cache *cache, const uint32_t *lengths, const uin
  * with K_p, V_p the values that the cache's codes stand for.  The codes enter the matrix cores as fp16 (exact), q as
  * fp16 times a power of two of its row (exact down to 2^-29 of the row's largest), the probabilities times
  * their block's scale of values as fp16 (half a step, and at most 2^-32 of the largest such product of the row);
- * sums, maxima and the softmax are f32, for which |scale| sum |q| |K_p| must stay below 2^126.  A row that sees no slot gives
- * zeros and lse = -infinity.  A row whose q is infinite or NaN, or that sees a block that stands for NaN, gives NaN.
+ * sums, maxima and the softmax are f32, for which |scale| sum |q| |K_p| must stay below 2^126; values may be of any size.  A row that
+ * sees no slot gives zeros and lse = -infinity.  A row whose q is infinite or NaN, or that sees a block that stands for NaN, gives NaN.
  *   q, out: bf16 [tokens, q_heads, head_dim], q tokens q_stride elements apart (a multiple of 8), out contiguous; both 16-byte
  *   aligned and apart from each other; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
  *   be negative or 0).

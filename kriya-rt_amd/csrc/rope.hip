@@ -12,7 +12,7 @@ namespace kr {
 
 // The angle of position p at f turns a position is p f turns, of which only the fraction counts.  p f is taken in 64
 // bits (an error of 2^-53 p f turns: 1e-11 at a million), the fraction by rint; its sine and cosine are 64 bits too, so a table holds
-// the f32 nearest to them.  Bound by its launch: 3907 rows of 16 pairs 1.7 us.
+// the f32 nearest to them.  Bound by its launch: 3907 rows of 16 pairs 2.2 us.
 __global__ __launch_bounds__(256) void rope_table_kernel(RopeTurns f, uint32_t half, uint32_t first, uint32_t count,
                                                          double gain, float *cos_sin) {
     const size_t at = (size_t)blockIdx.x * 256 + threadIdx.x;

@@ -339,6 +339,12 @@ hipError_t launch_rope_table(const RopeTurns &f, uint32_t half, uint32_t first, 
 hipError_t launch_rope_apply(const RopeArgs &a, const void *x, size_t xs, void *y, size_t ys, int f32, uint32_t tokens,
                              uint32_t heads, uint32_t D, hipStream_t s);
 
+struct RaggedStep {          // the new tokens of a step over a cache
+    const uint32_t *starts;  // [batch + 1], nullptr: one token each
+    const uint32_t *lengths; // [batch]
+    uint32_t batch, tokens;
+};
+
 // ---- 8-bit key/value cache (kv8_cache.hip, kv8_attention.hip; layout in include/kriya_kv8.h)
 constexpr uint32_t kKv8Block = 32;
 struct Kv8 {
@@ -348,14 +354,9 @@ struct Kv8 {
     uint32_t batch, heads, D, max_ctx, blocks;
     int e4m3;
 };
-struct Kv8Step {             // the new tokens of a step
-    const uint32_t *starts;  // [batch + 1], nullptr: one token each
-    const uint32_t *lengths; // [batch]
-    uint32_t batch, tokens;
-};
 struct Kv8AppendArgs {
     Kv8 c;
-    Kv8Step step;
+    RaggedStep step;
     RopeArgs rope;           // cos_sin == nullptr: none
     int rope_units;          // the rotation in 8-dim units (rope_units_ok)
     const uint16_t *k, *v, *q;
@@ -368,7 +369,7 @@ hipError_t launch_kv8_dequant(const Kv8 &c, const uint32_t *lengths, const uint3
                               void *v_out, int f32, hipStream_t s);
 struct Kv8AttnArgs {
     Kv8 c;
-    Kv8Step step;
+    RaggedStep step;
     const uint16_t *q;
     size_t q_stride;
     uint32_t q_heads, group;
@@ -377,6 +378,8 @@ struct Kv8AttnArgs {
     float *lse;              // may be nullptr (attention); in (weights)
     float *part;             // workspace
     float decay, *weight;    // weights
+    // a row may see all new tokens of its sequence
+    __host__ __device__ bool sees_all() const { return false; }
 };
 uint64_t kv8_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);  // workgroups
 size_t kv8_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
@@ -392,5 +395,61 @@ struct Kv8EvictArgs {
     uint32_t *kept, *to_lengths;
 };
 hipError_t launch_kv8_evict(const Kv8EvictArgs &a, hipStream_t s);
+
+// ---- key/value cache in pages (paged_cache.hip, paged_attention.hip, paged_tree.hip; layout in include/kriya_paged.h)
+constexpr uint32_t kPagedUnit = 16;      // slots whose order is one block of operands
+constexpr uint32_t kTreeNodes = 4096;    // of a sequence that a plan or a commit looks at
+struct Paged {
+    uint16_t *k, *v;                     // of the layer
+    const uint32_t *table;               // [batch, max_pages]
+    uint32_t pages, max_pages, shift;    // 2^shift units a page
+    uint32_t batch, heads, D, max_ctx;   // max_ctx: max_pages pages of slots
+};
+struct PagedAppendArgs {
+    Paged c;
+    RaggedStep step;
+    RopeArgs rope;                       // cos_sin == nullptr: none
+    const uint16_t *q_norm, *k_norm;     // nullptr: not normalised
+    float eps;
+    const uint16_t *k, *v, *q;
+    uint16_t *q_out;
+    size_t kv_stride, q_stride;
+    uint32_t q_heads;
+};
+uint64_t paged_append_groups(const PagedAppendArgs &a);  // workgroups
+hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s);
+hipError_t launch_paged_read(const Paged &c, const RaggedStep &step, const uint32_t *first, uint32_t count, void *k_out,
+                             void *v_out, int f32, hipStream_t s);
+struct PagedAttnArgs {
+    Paged c;
+    RaggedStep step;
+    const uint16_t *q;
+    size_t q_stride;
+    uint32_t q_heads, group;
+    const uint32_t *mask;                // nullptr: causal
+    uint32_t words;
+    float scale_log2;
+    uint16_t *out;
+    float *lse;                          // may be nullptr
+    float *part;                         // workspace
+    // a row may see all new tokens of its sequence
+    __host__ __device__ bool sees_all() const { return mask != nullptr; }
+};
+uint64_t paged_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
+size_t paged_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
+hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);
+hipError_t launch_tree_plan(const int32_t *parents, const RaggedStep &step, uint32_t words, uint32_t *mask, uint32_t *positions,
+                            hipStream_t s);
+struct PagedCommitArgs {
+    Paged c;                             // of the first layer
+    uint32_t layers;
+    RaggedStep step;
+    const int32_t *drafted, *parents, *targets;
+    uint32_t max_path;
+    uint32_t *path, *counts;
+    int32_t *next;
+    uint32_t *new_lengths;
+};
+hipError_t launch_paged_commit(const PagedCommitArgs &a, hipStream_t s);
 
 }  // namespace kr

@@ -1,16 +1,10 @@
 // kv8_api.hip — the C ABI of include/kriya_kv8.h: argument checks and dispatch.
 #include <math.h>
 
-#include "kriya_kv8.h"
-#include "kr_internal.hpp"
+#include "api_checks.hpp"
 
 namespace kr {
 namespace {
-
-// A launch has fewer than 2^32 threads in a dimension: this many workgroups of 256.
-constexpr uint64_t kMostGroups = 0xFFFFFFFFull / 256;
-
-bool on(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 
 int check_cache(const kr_kv8_cache *c, const char *name) {
     if (!c) return fail(KR_E_INVALID, "%s: descriptor is NULL", name);
@@ -41,21 +35,6 @@ int check_step(const kr_kv8_cache *c, uint32_t tokens, const uint32_t *starts, c
     return KR_OK;
 }
 
-int check_rope(const kr_rope *r, uint32_t head_dim) {
-    if (!r->cos_sin || !r->positions) return fail(KR_E_INVALID, "rope: NULL pointer");
-    if (r->layout != KR_ROPE_HALF && r->layout != KR_ROPE_INTERLEAVED) return fail(KR_E_INVALID, "rope: layout %d", r->layout);
-    if (r->inverse != 0 && r->inverse != 1) return fail(KR_E_INVALID, "rope: inverse must be 0 or 1");
-    if (r->rows == 0) return fail(KR_E_SHAPE, "rope: the table has no rows");
-    if (r->rotary_dim == 0 || r->rotary_dim % 2 || r->rotary_dim > head_dim)
-        return fail(KR_E_SHAPE, "rope: rotary_dim=%u is not even, 2 .. head_dim=%u", r->rotary_dim, head_dim);
-    if (!on(r->cos_sin, 8) || !on(r->positions, 4)) return fail(KR_E_ALIGN, "rope: cos_sin must be 8-byte aligned");
-    return KR_OK;
-}
-
-RopeArgs to_rope(const kr_rope *r) {
-    return RopeArgs{r->cos_sin, r->positions, r->rows, r->rotary_dim, r->layout == KR_ROPE_INTERLEAVED, r->inverse};
-}
-
 int check_queries(const kr_kv8_cache *c, const uint16_t *q, size_t q_stride, uint32_t q_heads, uint32_t tokens) {
     if (q_heads == 0 || q_heads % c->kv_heads)
         return fail(KR_E_SHAPE, "q_heads=%u is not a positive multiple of kv_heads=%u", q_heads, c->kv_heads);
@@ -67,8 +46,6 @@ int check_queries(const kr_kv8_cache *c, const uint16_t *q, size_t q_stride, uin
     if (!on(q, 16)) return fail(KR_E_ALIGN, "q must be 16-byte aligned");
     return KR_OK;
 }
-
-constexpr float kMaxScale = 0x1p100f;  // times log2(e) a float
 
 bool finite_positive(double v) { return v > 0.0 && v < INFINITY; }
 
@@ -162,7 +139,7 @@ int kr_kv8_append(const kr_kv8_cache *cache, const kr_rope *rope, const uint16_t
         return fail(KR_E_SHAPE, "too many tokens for one launch");
     Kv8AppendArgs a{};
     a.c = to_kv8(cache);
-    a.step = Kv8Step{starts, lengths, cache->batch, tokens};
+    a.step = RaggedStep{starts, lengths, cache->batch, tokens};
     if (rope) {
         a.rope = to_rope(rope);
         a.rope_units = rope_units_ok(a.rope, cache->head_dim);
@@ -218,7 +195,7 @@ int kr_kv8_attention(const kr_kv8_cache *cache, const uint16_t *q, size_t q_stri
     if (!on(workspace, 16)) return fail(KR_E_ALIGN, "workspace must be 16-byte aligned");
     Kv8AttnArgs a{};
     a.c = to_kv8(cache);
-    a.step = Kv8Step{starts, lengths, cache->batch, tokens};
+    a.step = RaggedStep{starts, lengths, cache->batch, tokens};
     a.q = q;
     a.q_stride = q_stride;
     a.q_heads = q_heads;
@@ -254,7 +231,7 @@ int kr_kv8_accumulate_weight(const kr_kv8_cache *cache, const uint16_t *q, size_
     if (!on(workspace, 16)) return fail(KR_E_ALIGN, "workspace must be 16-byte aligned");
     Kv8AttnArgs a{};
     a.c = to_kv8(cache);
-    a.step = Kv8Step{starts, lengths, cache->batch, tokens};
+    a.step = RaggedStep{starts, lengths, cache->batch, tokens};
     a.q = q;
     a.q_stride = q_stride;
     a.q_heads = q_heads;

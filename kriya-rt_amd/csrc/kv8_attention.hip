@@ -17,13 +17,12 @@
 // rounding to fp16 those probabilities are the second product's operand as they lie (see kv8.hpp for the order of v).
 #include <algorithm>
 
+#include "attn_work.hpp"
 #include "kv8.hpp"
 
 namespace kr {
 
 namespace {
-
-constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // The power of two that brings a row to [2^14, 2^15), from the bf16 bits of its largest |q|; 2^126 at most, which is exact too: rows
 // below 2^-112 are multiples of 2^-133 and become multiples of 2^-7.
@@ -119,169 +118,6 @@ __device__ __forceinline__ void load_units(u32x4 (&w)[NS], const uint8_t *blk) {
     for (int j = 0; j < NS; ++j) w[j] = *reinterpret_cast<const u32x4 *>(blk + 1024 * j + 16 * __lane_id());
 }
 
-// Row r of sequence span s: the slots that it sees, 0 for a row past the end.
-__device__ __forceinline__ uint32_t row_limit(const Kv8Span &s, uint32_t r, uint32_t group, uint32_t max_ctx) {
-    const uint32_t i = r / group;
-    if (i >= s.m || s.n < s.m - i) return 0u;
-    return min(s.n - s.m + i + 1, max_ctx);
-}
-
-// ---- the work of a launch
-//
-// Few rows: tiles of `rows` query rows; the context of a tile is split into parts of `per` blocks, so that the workgroups have
-// about the same to do whatever the lengths are: `per` is the launch's blocks, counted on the device, over the workgroups wanted.
-// A sequence's tiles all have as many parts as its longest: workgroup sum_{b' < b} tiles parts + part tiles + tile, and
-// those past a shorter tile's end have nothing to do.  (The tile varies first: workgroups go round the XCDs in turn, and
-// with the part first one XCD would get all the empty ones.)
-struct Split {
-    uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
-    uint32_t rows;    // of a tile
-    uint32_t unit;    // few rows: `per` is a multiple of it; many: workgroups that a compute unit holds
-};
-__device__ __forceinline__ uint32_t tiles_of(const Kv8AttnArgs &a, const Split &w, const Kv8Span &s) {
-    return (s.m * a.group + w.rows - 1) / w.rows;
-}
-__device__ __forceinline__ uint32_t blocks_of(const Kv8AttnArgs &a, const Kv8Span &s) {
-    return (min(s.n, a.c.max_ctx) + 31) / 32;
-}
-__device__ __forceinline__ uint32_t parts_of(uint32_t blocks, uint32_t per) { return max((blocks + per - 1) / per, 1u); }
-
-// total / target, rounded up
-__device__ __forceinline__ unsigned long long fair_share(unsigned long long total, uint32_t target) {
-    return total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
-}
-
-// Blocks of a part.  Every wave computes it alike.
-__device__ __forceinline__ uint32_t split_per(const Kv8AttnArgs &a, const Split &w) {
-    unsigned long long total = 0;
-    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
-        const Kv8Span s = kv8_span(a.step, b);
-        total += (unsigned long long)tiles_of(a, w, s) * blocks_of(a, s);
-    }
-    const unsigned long long fair = fair_share(wave_sum_u64(total), w.target);
-    return max((uint32_t)((fair + w.unit - 1) / w.unit) * w.unit, w.unit);
-}
-
-// What workgroup `idx` of a head does.
-struct Work {
-    Kv8Span s;
-    uint32_t b, tile, part, parts, per;  // parts: of this tile, at least 1
-    uint32_t rows, most;                 // query rows of the sequence; slots that the tile's last row sees
-};
-__device__ __forceinline__ void fill_work(const Kv8AttnArgs &a, const Split &w, Work &o) {
-    o.s = kv8_span(a.step, o.b);
-    o.rows = o.s.m * a.group;
-    o.most = row_limit(o.s, min(w.rows * (o.tile + 1), o.rows) - 1, a.group, a.c.max_ctx);
-}
-__device__ __forceinline__ bool find_work(const Kv8AttnArgs &a, const Split &w, uint32_t idx, Work &o) {
-    o.per = split_per(a, w);
-    uint32_t item;
-    const auto count = [&](uint32_t i) {
-        const Kv8Span s = kv8_span(a.step, i);
-        return tiles_of(a, w, s) * parts_of(blocks_of(a, s), o.per);
-    };
-    if (!kv8_find(idx, a.c.batch, count, o.b, item)) return false;
-    const uint32_t tiles = tiles_of(a, w, kv8_span(a.step, o.b));
-    o.tile = item % tiles;
-    o.part = item / tiles;
-    fill_work(a, w, o);
-    o.parts = parts_of((o.most + 31) / 32, o.per);
-    return o.part < o.parts;
-}
-
-// Many rows: where there are fewer tiles than compute units, the tiles' blocks stand in one line, tile after tile, and a workgroup
-// takes an equal share of it: the end of a tile, whole ones, the beginning of the next.  (Parts of equal length, of which a whole
-// number fits a tile, leave the longest workgroup a quarter more than the mean: 600 tokens over up to 12000 in four sequences,
-// 10/2 heads, D 256: 124 -> 113 us.)  A tile's blocks are those that its sequence's last row sees.
-// Parts cost about 14 blocks' time (O through memory, and the join), and a tile alone on a compute unit is faster than one of
-// several: where the longest tile has no more blocks than 14 and the shares that a compute unit would hold, tiles stay whole
-// (16/2 heads, split and whole, us.  D 128: 500 tokens 26 and 23, 1000 31 and 34, 2000 58 and 58, 200 over 1000 25 and 38;
-// D 256: 1000 tokens 47 and 55; D 64: 31 and 26).
-__device__ __forceinline__ uint32_t tile_blocks(const Kv8AttnArgs &a, const Kv8Span &s) {
-    return max(blocks_of(a, s), 1u);  // (a tile that sees nothing is written too)
-}
-// A workgroup's share, in blocks; 0: a workgroup takes a tile.
-__device__ __forceinline__ uint32_t share_of(const Kv8AttnArgs &a, const Split &w) {
-    if (w.target == 0) return 0;
-    uint32_t total = 0, most = 0;  // (the host splits no launch whose blocks pass 2^31)
-    for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
-        const Kv8Span s = kv8_span(a.step, b);
-        const uint32_t tiles = tiles_of(a, w, s), blocks = tile_blocks(a, s);
-        total += tiles * blocks;
-        if (tiles) most = max(most, blocks);
-    }
-    const uint32_t share = max((wave_sum_u32(total) + w.target - 1) / w.target, 1u);
-    return wave_max_u32(most) <= 14 + w.unit * share ? 0 : share;
-}
-// The tile in which place `at` of the line falls, and where in it.
-__device__ __forceinline__ bool find_place(const Kv8AttnArgs &a, const Split &w, uint32_t at, Work &o, uint32_t &block, uint32_t &blocks) {
-    uint32_t item;
-    const auto count = [&](uint32_t i) {
-        const Kv8Span s = kv8_span(a.step, i);
-        return tiles_of(a, w, s) * tile_blocks(a, s);
-    };
-    if (!kv8_find(at, a.c.batch, count, o.b, item)) return false;
-    blocks = tile_blocks(a, kv8_span(a.step, o.b));
-    o.tile = item / blocks;
-    block = item % blocks;
-    fill_work(a, w, o);
-    return true;
-}
-
-// For the joins: the tile-th tile of all, false past the last, and where its parts lie in the workspace: slot `slot` + (part 0: `odd`) +
-// part * `step`.  Of a tile that is in one part (o.parts) nothing lies there.
-template <bool kMany>
-__device__ __forceinline__ bool find_tile(const Kv8AttnArgs &a, const Split &w, uint32_t tile, Work &o, uint32_t &slot,
-                                          uint32_t &odd, uint32_t &step) {
-    if (!kv8_find(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, kv8_span(a.step, i)); }, o.b, o.tile)) return false;
-    fill_work(a, w, o);
-    uint32_t share = 0;
-    if constexpr (kMany) {
-        share = share_of(a, w);
-        if (share == 0) {
-            o.parts = 1;
-            slot = odd = 0;
-            step = 1;
-            return true;
-        }
-    } else {
-        o.per = split_per(a, w);
-    }
-    uint32_t before = 0;
-    for (uint32_t i = __lane_id(); i < o.b; i += 64) {
-        const Kv8Span s = kv8_span(a.step, i);
-        before += tiles_of(a, w, s) * (kMany ? tile_blocks(a, s) : parts_of(blocks_of(a, s), o.per));
-    }
-    before = wave_sum_u32(before);
-    if constexpr (kMany) {
-        const uint32_t from = before + o.tile * tile_blocks(a, o.s), seen = max((o.most + 31) / 32, 1u);
-        const uint32_t first = from / share, last = (from + seen - 1) / share;
-        o.parts = last - first + 1;
-        slot = 2 * first;  // a workgroup's first piece in the even slot, its last one in the odd
-        odd = first * share < from;
-        step = 2;
-    } else {
-        o.parts = parts_of((o.most + 31) / 32, o.per);
-        slot = before + o.tile;
-        odd = 0;
-        step = tiles_of(a, w, o.s);
-    }
-    return true;
-}
-// parts of a tile of few rows: at most `target` and one, and target is at most 1024
-constexpr uint32_t kMostParts = 1056;
-// Where a part's normalised O of a row lies in the workspace, in rows; m and l of all rows lie behind them, in pairs.
-__device__ __forceinline__ size_t part_at(const Kv8AttnArgs &a, const Split &w, uint32_t idx, uint32_t head, uint32_t row) {
-    return ((size_t)idx * a.c.heads + head) * w.rows + row;
-}
-
-// A value that every lane holds, in a scalar register.
-__device__ __forceinline__ float uniform(float v) {
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
-}
-
-__device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_max_u32(~v); }
-
 }  // namespace
 
 // ---- many rows: prompts and chunks
@@ -323,12 +159,12 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
             if (first && first >= seen) continue;
             if (odd) __syncthreads();  // the last piece's bytes have been read
         } else {
-            if (odd || !kv8_find(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, kv8_span(a.step, i)); }, w.b, w.tile)) return;
-            w.tile = tiles_of(a, split, kv8_span(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
+            if (odd || !find_item(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, span_of(a.step, i)); }, w.b, w.tile)) return;
+            w.tile = tiles_of(a, split, span_of(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
             fill_work(a, split, w);
             end = (w.most + 31) / 32;
         }
-        const Kv8Span &s = w.s;
+        const Span &s = w.s;
         const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + (lane & 31);
         const bool live = r < w.rows;
         const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
@@ -537,7 +373,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void kv8_many_kernel(Kv8AttnA
 //
 // A workgroup takes one tile of 16 query rows and one part of the sequence's blocks, its four waves every fourth block of
 // the part; each wave keeps its own m, l and O, and they are joined in LDS. With more than one part the normalised
-// O_s and (m_s, l_s) go to the workspace and kv8_join_kernel joins the parts in order:
+// O_s and (m_s, l_s) go to the workspace and attn_join_kernel joins the parts in order:
 //   out = sum_s 2^(m_s - M) l_s O_s / L,   L = sum_s 2^(m_s - M) l_s
 // On v_mfma_f32_16x16x32_f16: lane (column l & 15, g = l >> 4) holds slots 16 t + 4 g + j after the first product, and
 // needs of dim d the slots 16 s + 4 g + j for the second, eight bytes of v's order (h = g & 1, a = g >> 1).
@@ -617,7 +453,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
     const uint32_t head = blockIdx.y, idx = blockIdx.x;
     Work w;
     if (!find_work(a, split, idx, w)) return;
-    const Kv8Span &s = w.s;
+    const Span &s = w.s;
     const uint32_t r0 = kFewRows * w.tile, r = r0 + r16;
     const bool live = r < w.rows;
     const uint32_t limit = live ? row_limit(s, r, a.group, a.c.max_ctx) : 0u;
@@ -757,102 +593,6 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
     }
 }
 
-// Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
-// of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile (four waves: with 16, which
-// find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).  Bound by latency (work count,
-// maxima, parts): 16 rows in 256 parts 6.5 us, 1536 rows in a few 8.3, 6000 rows of 256 10.3 for 34 MB.
-constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;
-template <int NS, bool kMany, bool kWide>
-__global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void kv8_join_kernel(Kv8AttnArgs a, Split split,
-                                                                                          uint32_t slots, uint32_t per_group) {
-    constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
-    __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
-    __shared__ float ws[kWide ? kMostParts : kJoinRowThreads], red[2][kJoinThreads / 64];
-    const uint32_t lane = __lane_id(), head = blockIdx.y, wave = threadIdx.x >> 6, tid = kWide ? threadIdx.x : lane;
-    const uint32_t groups = split.rows / per_group;
-    Work w;
-    uint32_t slot, odd, slot_step;
-    if (!find_tile<kMany>(a, split, blockIdx.x / groups, w, slot, odd, slot_step)) return;
-    // (starts that decrease can make more parts than the launch has: none behind its last.  Counted before the exit, beside the loads
-    // that it waits for: 5 sequences up to 3000 13.8 us, not 14.1)
-    if (slot < slots) w.parts = min(w.parts, (slots - slot + slot_step - 1) / slot_step);
-    if (w.parts == 1 || slot >= slots) return;
-    const size_t slot_rows = (size_t)a.c.heads * split.rows, step = slot_step * slot_rows;  // between parts, in rows
-    const auto part_row = [&](uint32_t p) { return p * step + (p == 0 ? odd * slot_rows : 0); };
-    const float *all_ml = a.part + slots * slot_rows * D;
-    const uint32_t way = tid / kQuads, quad = tid % kQuads, row0 = blockIdx.x % groups * per_group;
-    for (uint32_t row = row0 + (kWide ? 0 : wave); row < row0 + per_group; row += kWide ? 1 : kJoinRowThreads / 64) {
-        const uint32_t r = split.rows * w.tile + row;
-        if (r >= w.rows) return;
-        const size_t at = part_at(a, split, slot, head, row);
-        const float2 *ml = reinterpret_cast<const float2 *>(all_ml) + at;
-        f32x4 acc = {0, 0, 0, 0};
-        float M = -INFINITY, L = 0.0f;
-        for (uint32_t p = tid; p < w.parts; p += kThreads) M = fmaxf(M, ml[part_row(p)].x);
-        M = wave_max(M);
-        if constexpr (kWide) {
-            if (lane == 0) red[0][wave] = M;
-            __syncthreads();
-#pragma unroll
-            for (uint32_t i = 0; i < kJoinThreads / 64; ++i) M = fmaxf(M, red[0][i]);
-        }
-        const float *o = a.part + at * D + 4 * quad;
-        for (uint32_t p0 = 0; p0 < w.parts; p0 += kWide ? kMostParts : 64) {  // (kWide: once)
-            const uint32_t n = min(w.parts - p0, kWide ? kMostParts : 64u);
-            float *wl = kWide ? ws : ws + 64 * wave, sum = 0.0f;
-            for (uint32_t p = tid; p < n; p += kThreads) {
-                const float2 x = ml[part_row(p0 + p)];
-                const float f = x.y == 0.0f ? 0.0f : x.y * __builtin_amdgcn_exp2f(x.x - M);  // NaN stays
-                wl[p] = f;
-                sum += f;
-            }
-            // the weights are divided by L before they meet values, which may be near the largest float
-            sum = wave_sum(sum);
-            if constexpr (kWide) {
-                if (lane == 0) red[1][wave] = sum;
-                __syncthreads();
-                sum = red[1][0];
-#pragma unroll
-                for (uint32_t i = 1; i < kJoinThreads / 64; ++i) sum += red[1][i];
-            } else {
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            }
-            const float before = L;
-            L += sum;
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            if (p0) acc *= before * inv;
-            if (way < kWays) {
-#pragma unroll 8
-                for (uint32_t p = way; p < n; p += kWays)
-                    acc += wl[p] * inv * *reinterpret_cast<const f32x4 *>(o + part_row(p0 + p) * D);
-            }
-            if constexpr (!kWide) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-        if constexpr (kWide) {
-            if (way < kWays) so[way][quad] = acc;
-            __syncthreads();
-            if (tid >= kQuads) return;
-            acc = so[0][tid];
-#pragma unroll
-            for (uint32_t i = 1; i < kWays; ++i) acc += so[i][tid];
-        } else {
-#pragma unroll
-            for (uint32_t i = 1; i < kWays; ++i)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const float other = __shfl(acc[x], (lane + i * kQuads) & 63);
-                    acc[x] += lane < kQuads ? other : 0.0f;
-                }
-        }
-        if (tid < kQuads) {
-            const size_t to = (size_t)(w.s.t0 + r / a.group) * a.q_heads + head * a.group + r % a.group;
-            const u32x2 y = {pack_bf16_rne(acc.x, acc.y), pack_bf16_rne(acc.z, acc.w)};
-            *reinterpret_cast<u32x2 *>(a.out + to * D + 4 * tid) = y;
-            if (a.lse && tid == 0) a.lse[to] = L == 0.0f ? -INFINITY : (M + __log2f(L)) * kLn2;
-        }
-    }
-}
-
 // ---- attention weights of the slots
 //
 // Column sums of the attention matrix, from K and the rows' lse alone: weight_p += sum_r 2^(c s_rp - lse_r).  The products are taken
@@ -870,14 +610,14 @@ constexpr uint32_t weight_rows(bool few) { return few ? 32 : 64; }
 
 template <bool kFew>
 struct WeightSpan {
-    Kv8Span s;
+    Span s;
     uint32_t n, chunks, rows, tiles;  // slots in the cache, chunks of 128 of them; query rows, tiles of them
 };
 template <bool kFew>
 __device__ __forceinline__ WeightSpan<kFew> weight_span(const Kv8AttnArgs &a, uint32_t b) {
     constexpr uint32_t kRows = weight_rows(kFew);
     WeightSpan<kFew> w;
-    w.s = kv8_span(a.step, b);
+    w.s = span_of(a.step, b);
     w.n = min(w.s.n, a.c.max_ctx);
     w.chunks = (w.n + kWeightSlots - 1) / kWeightSlots;
     w.rows = w.s.m * a.group;
@@ -934,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void kv8_weight_kernel(Kv8AttnArgs a, uint3
     };
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {
         uint32_t b, item;
-        if (!kv8_find(idx, a.c.batch, count, b, item)) return;
+        if (!find_item(idx, a.c.batch, count, b, item)) return;
         const auto w = weight_span<kFew>(a, b);
         // the chunks of every other part in reverse: late ones see fewer rows, and workgroups go round the XCDs in turn
         const uint32_t part = item / w.chunks, chunk = part & 1 ? w.chunks - 1 - item % w.chunks : item % w.chunks;
@@ -1065,7 +805,7 @@ __global__ __launch_bounds__(kWeightSlots) void kv8_weight_join_kernel(Kv8AttnAr
     const uint32_t head = blockIdx.y, per = weight_per<false>(a, target);
     for (uint32_t idx = blockIdx.x;; idx += gridDim.x) {  // chunks
         uint32_t b, chunk;
-        if (!kv8_find(idx, a.c.batch, [&](uint32_t i) { return weight_span<false>(a, i).chunks; }, b, chunk)) return;
+        if (!find_item(idx, a.c.batch, [&](uint32_t i) { return weight_span<false>(a, i).chunks; }, b, chunk)) return;
         const auto w = weight_span<false>(a, b);
         const uint32_t parts = weight_parts(w.tiles, per), p = chunk * kWeightSlots + threadIdx.x;
         if (parts == 1) continue;
@@ -1162,13 +902,13 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 256) {
-            kv8_join_kernel<NS, false, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
+            attn_join_kernel<Kv8AttnArgs, NS, false, true, false><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
         } else {
             uint32_t per_group = kJoinRowThreads / 64;
             while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 2048) per_group *= 2;
             const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
-            if (p.few) kv8_join_kernel<NS, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
-            else kv8_join_kernel<NS, true, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            if (p.few) attn_join_kernel<Kv8AttnArgs, NS, false, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            else attn_join_kernel<Kv8AttnArgs, NS, true, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     });

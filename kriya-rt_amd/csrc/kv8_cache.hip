@@ -54,12 +54,12 @@ __device__ __forceinline__ void put_codes(uint8_t *blk, bool values, GroupAt at,
 
 // The blocks that sequence b's new tokens fall into: `first` .. `last` (slots n0 .. end - 1 are new).
 struct AppendSpan {
-    Kv8Span s;
+    Span s;
     uint32_t n0, end, first, last, items;
 };
 __device__ __forceinline__ AppendSpan append_span(const Kv8AppendArgs &a, uint32_t b) {
     AppendSpan r;
-    r.s = kv8_span(a.step, b);
+    r.s = span_of(a.step, b);
     r.n0 = r.s.n > r.s.m ? r.s.n - r.s.m : 0u;
     r.end = min(r.s.n, a.c.max_ctx);
     r.items = 0;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a, uint32
     }
     const uint32_t head = blockIdx.x % a.c.heads;
     uint32_t b, item;
-    if (!kv8_find(blockIdx.x / a.c.heads, a.c.batch, [&](uint32_t i) { return append_span(a, i).items; }, b, item)) return;
+    if (!find_item(blockIdx.x / a.c.heads, a.c.batch, [&](uint32_t i) { return append_span(a, i).items; }, b, item)) return;
     const AppendSpan s = append_span(a, b);
     const bool values = __builtin_amdgcn_readfirstlane(threadIdx.x >= per_side);
     const uint32_t tid = values ? threadIdx.x - per_side : threadIdx.x;

@@ -124,6 +124,12 @@ def lib():
             "kr_kv8_accumulate_weight": (i32, [vp, vp, sz, u32, u32, vp, vp, ctypes.c_float, vp, ctypes.c_float, vp, vp,
                                                sz, vp]),
             "kr_kv8_evict": (i32, [vp, vp, vp, u32, u32, u32, vp, vp, vp, vp, vp]),
+            "kr_paged_append": (i32, [vp, u32, vp, vp, vp, vp, vp, sz, vp, vp, sz, u32, u32, vp]),
+            "kr_paged_read": (i32, [vp, u32, vp, vp, u32, vp, vp, i32, vp]),
+            "kr_paged_attention_workspace_bytes": (sz, [vp, vp, u32, u32]),
+            "kr_paged_attention": (i32, [vp, u32, vp, vp, sz, u32, u32, vp, u32, ctypes.c_float, vp, vp, vp, sz, vp]),
+            "kr_tree_plan": (i32, [vp, u32, vp, vp, u32, u32, vp, vp, vp]),
+            "kr_paged_commit": (i32, [vp, vp, vp, vp, vp, u32, u32, vp, vp, vp, vp, vp]),
             "kr_rope_attention_q4_out": (i32, [vp, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp, u32, M, vp, i32, vp, sz,
                                                vp]),
         }

@@ -21,9 +21,12 @@ __device__ __forceinline__ uint32_t page_of(const Paged &c, uint32_t b, uint32_t
     const uint32_t p = u >> c.shift;
     return p < c.max_pages ? c.table[(size_t)b * c.max_pages + p] : 0xFFFFFFFFu;
 }
-// Where unit u lies in its page: elements from the pool's start.
+// Where unit u lies: units from the pool's start (below 2^32), and elements.
+__device__ __forceinline__ uint32_t unit_place(const Paged &c, uint32_t page, uint32_t head, uint32_t u) {
+    return ((page * c.heads + head) << c.shift) + (u & ((1u << c.shift) - 1));
+}
 __device__ __forceinline__ size_t unit_at(const Paged &c, uint32_t page, uint32_t head, uint32_t u) {
-    return ((((size_t)page * c.heads + head) << c.shift) + (u & ((1u << c.shift) - 1))) * (size_t)(kPagedUnit * c.D);
+    return (size_t)unit_place(c, page, head, u) * (kPagedUnit * c.D);
 }
 
 }  // namespace kr

@@ -16,6 +16,8 @@ int check_cache(const kr_paged_cache *c, uint32_t layer) {
     if (c->kv_heads == 0 || c->kv_heads > 65535) return fail(KR_E_SHAPE, "cache: kv_heads=%u is not 1 .. 65535", c->kv_heads);
     if (c->pages == 0 || c->pages > 0x7FFFFFFFu) return fail(KR_E_SHAPE, "cache: pages=%u is not 1 .. 2^31 - 1", c->pages);
     if (c->layers == 0 || c->layers > 65535) return fail(KR_E_SHAPE, "cache: layers=%u is not 1 .. 65535", c->layers);
+    if ((uint64_t)c->pages * c->kv_heads > 0xFFFFFFFFull / (c->page / kPagedUnit))
+        return fail(KR_E_SHAPE, "cache: pages=%u of %u heads and %u slots are more than 2^32 units of 16 slots", c->pages, c->kv_heads, c->page);
     if (layer >= c->layers) return fail(KR_E_SHAPE, "layer=%u of %u", layer, c->layers);
     if (!c->k || !c->v) return fail(KR_E_INVALID, "cache: NULL pointer");
     if (!on(c->k, 16) || !on(c->v, 16)) return fail(KR_E_ALIGN, "cache: k and v must be 16-byte aligned");

@@ -69,15 +69,31 @@ __device__ __forceinline__ uint32_t clear_of(const PagedAttnArgs &a, const Span 
     return a.mask ? min(s.n > s.m ? s.n - s.m : 0u, a.c.max_ctx) : row_limit(s, r0, a.group, a.c.max_ctx);
 }
 
-// The pages of a wave's units in the order in which it asks for them, 64 at a time and the next 64 on their way: lane l of a set
-// holds the page of the unit that the wave reads l-th.
+// Where a wave's units lie, in the order in which it asks for them, 64 at a time and the next 64 on their way: lane l of a set holds
+// the place, in units from the pool's start, of the l-th (a unit of no page: the first of the pool, and its bit in `holes`).
 template <class F>
-struct Pages {
-    F load;  // the pages of set i: a value a lane
-    uint32_t now, next;
-    __device__ __forceinline__ explicit Pages(F f) : load(f), now(f(0)), next(f(1)) {}
+struct Units {
+    F page;  // of the i-th unit
+    const Paged &c;
+    uint32_t head;
+    struct Set {
+        uint32_t at;
+        unsigned long long holes;
+    } now, next;
+    __device__ __forceinline__ Set load(uint32_t set) const {
+        uint32_t unit;
+        const uint32_t p = page(64 * set + __lane_id(), unit);
+        const bool hole = p >= c.pages;
+        return Set{hole ? 0u : unit_place(c, p, head, unit), __ballot(hole)};
+    }
+    __device__ __forceinline__ Units(F f, const Paged &c, uint32_t head) : page(f), c(c), head(head) {
+        now = load(0);
+        next = load(1);
+    }
     // of the i-th unit; units in rising order, each set entered at its first
-    __device__ __forceinline__ uint32_t at(uint32_t i) const { return (uint32_t)__builtin_amdgcn_readlane((int)now, (int)(i & 63)); }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return (uint32_t)__builtin_amdgcn_readlane((int)now.at, (int)(i & 63)); }
+    // whether the n units from i on have no page, as bits
+    __device__ __forceinline__ uint32_t holes(uint32_t i, uint32_t n) const { return (uint32_t)(now.holes >> (i & 63)) & ((1u << n) - 1); }
     __device__ __forceinline__ void enter(uint32_t i) {
         if ((i & 63) == 0 && i) {
             now = next;
@@ -104,12 +120,12 @@ __device__ __forceinline__ float row_follow(RowSums &r, float top) {
 // A product with a probability of 0 would bring them into those rows.  In a block that some row does not see whole, they are
 // therefore taken out of the operand, and added to the rows that see them one slot at a time.
 
-// Takes them out of a 16-byte piece of values; `bad` gets bit 15 and 31 of a word where its low and high value is one.
-__device__ __forceinline__ void take_out(u32x4 &v, u32x4 &bad) {
+// Takes them out of a 16-byte piece of values; returns bit 15 and 31 of a word where its low and high value is one.
+__device__ __forceinline__ u32x4 take_out(u32x4 &v) {
     // an exponent of all ones, and no other, carries into the sign's bit; from there over its half
     const u32x4 m = ((v & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
     v &= ~((m << 1) - (m >> 15));
-    bad |= m;
+    return m;
 }
 // The slots of a piece's bad words: bits 8 a + j.
 __device__ __forceinline__ uint32_t bad_slots(const u32x4 &bad) {
@@ -149,21 +165,43 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 // ---- many rows: prompts, chunks, large trees
 constexpr uint32_t kManyRows = 128;
 
-// 16 bytes a lane into LDS, past the registers: lane l's go to lds + 16 l.  lds the same in all lanes.
-__device__ __forceinline__ void to_lds(const void *from, void *lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+// N KB into LDS, past the registers: 16 bytes a lane and instruction, lane l's of the n-th go to byte lds + 1024 n + 16 l, lds the same in
+// all lanes (the instruction's offset counts on both sides).  In assembly, since the compiler would have every later read of LDS wait for
+// it: whoever reads what it writes waits for vmcnt(0) and a barrier first.
+template <int N>
+__device__ __forceinline__ void to_lds(const void *from, uint32_t lds) {
+    static_assert(N >= 1 && N <= 8);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, off offset:1024" ::"v"(from) : "memory");
+    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, off offset:2048" ::"v"(from) : "memory");
+    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, off offset:3072" ::"v"(from) : "memory");
+    if constexpr (N > 4) to_lds<N - 4>((const char *)from + 4096, lds + 4096);
 }
 
+// All but the last N of this wave's have landed (loads end in order).
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Groups of four waves: two where the registers hold two waves a SIMD, over every other pair of blocks each.
 template <int NS>
-__global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedAttnArgs a, Split split, uint32_t slots) {
-    constexpr uint32_t D = 32 * NS;
-    __shared__ u32x4 lds[2][2][2][NS][64];  // [keys, values][block & 1][unit][1 KB piece][lane]
-    const uint32_t lane = __lane_id(), r32 = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+constexpr uint32_t kManyGroups = NS <= 4 ? 2 : 1;
+
+template <int NS>
+__global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(PagedAttnArgs a, Split split, uint32_t slots) {
+    constexpr uint32_t D = 32 * NS, G = kManyGroups<NS>;
+    // A stage is G chunks of 64 slots, one a group: four units of NS pieces of 1 KB.  [keys, values][stage & 1][group][unit][piece]
+    constexpr uint32_t kPiece = 1024, kUnit = NS * kPiece, kChunk = 4 * kUnit, kStage = G * kChunk, kKind = 2 * kStage;
+    constexpr int kProducts = 4 * NS;  // of a chunk: of its scores, and of its values
+    __shared__ __align__(16) char lds[2 * kKind];
+    __shared__ float2 lds_ml[4][32];
+    __shared__ uint32_t lds_bad[2][G][2];  // [stage & 1][group]: slots of values that were taken out
+    const auto lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const uint32_t lane = __lane_id(), r32 = lane & 31, h = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     // heads side by side: with eight of them each XCD's L2 keeps the keys and values of one
-    // every second round of 256 workgroups mirrored: a compute unit's add up to about the same
-    uint32_t at = blockIdx.x;
-    if (at / 256 & 1) at = at / 256 * 256 + min(gridDim.x - at / 256 * 256, 256u) - 1 - at % 256;
-    const uint32_t head = at % a.c.heads, idx = at / a.c.heads;
+    const uint32_t head = blockIdx.x % a.c.heads, idx = blockIdx.x / a.c.heads;
     const uint32_t share = share_of(a, split);
     uint32_t place = idx * share, left = share;
     const float c = score_factor(a.scale_log2);
@@ -181,7 +219,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedA
             end = min(first + take, seen);
             whole = first == 0 && end == seen;
             if (first && first >= seen) continue;
-            if (odd) __syncthreads();  // the last piece's blocks have been read
+            if (odd) __syncthreads();  // LDS has been read
         } else {
             if (odd || !find_item(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, span_of(a.step, i)); }, w.b, w.tile)) return;
             w.tile = tiles_of(a, split, span_of(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
@@ -192,7 +230,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedA
         const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + r32;
         const bool live = r < w.rows;
         const Sight sight = sight_of(a, s, r, live);
-        const uint32_t clear = clear_of(a, s, r0 + 32 * wave);  // (rows past the end need nothing)
+        const uint32_t clear = r0 + 32 * wave < w.rows ? clear_of(a, s, r0 + 32 * wave) : kAll;  // (of rows past the end nothing counts)
         const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
         bf16x8_t q[2 * NS];
 #pragma unroll
@@ -201,140 +239,246 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedA
 #pragma unroll
         for (int i = 0; i < NS; ++i) o[i] = f32x16{};
         RowSums sums;
-        // the pages of units 2 first ..
-        Pages pages([&](uint32_t set) { return page_of(a.c, b, 2 * first + 64 * set + lane); });
-        // This wave's pieces of a block's keys or values, into side n & 1.
-        const auto request = [&](uint32_t kind, uint32_t n, uint32_t p0, uint32_t p1) {
-            const uint16_t *pool = kind ? a.c.v : a.c.k;
+        // stage i: blocks first + 2 G i ..; the group's own two from block_of(i) on
+        const uint32_t stages = first < end ? (end - first + 2 * G - 1) / (2 * G) : 0;
+        const auto block_of = [&](uint32_t i) { return first + 2 * (G * i + group); };
+        Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * first + i); }, a.c, head);
+        const uint32_t clear_tile = clear_of(a, s, r0);
+        // A wave brings one of the four units, its keys or its values, into LDS: `unit` where it lies in the pool.
+        const auto request = [&](uint32_t kind, uint32_t unit, uint32_t to) {
+            const uint16_t *from = (kind ? a.c.v : a.c.k) + (size_t)unit * (kPagedUnit * D) + 8 * lane;
+            to_lds<NS>(from, lds_base + kind * kKind + to + group * kChunk + wave * kUnit);
+        };
+        // Octet 2 j + h of slot r32 of two units, 256 bytes an octet, is the j-th operand of keys; 16 bytes of lane (dim, h) of a unit
+        // and 32 dims are an operand of values.
+        const char *key_at = lds + group * kChunk + (r32 >> 4) * kUnit + h * 256 + (r32 & 15) * 16;
+        const char *value_at = lds + kKind + group * kChunk + lane * 16;
+        // operand m of a chunk: of keys block m / 2 NS, dims 16 (m % 2 NS) ..; of values unit m / NS, 32 dims m % NS
+        const auto key = [&](uint32_t from, int m) { return *reinterpret_cast<const bf16x8_t *>(key_at + from + 512 * (m % (2 * NS)) + 2 * kUnit * (m / (2 * NS))); };
+        const auto value = [&](uint32_t from, int m) { return *reinterpret_cast<const u32x4 *>(value_at + from + kUnit * (m / NS) + kPiece * (m % NS)); };
+        f32x16 p[2], y[2];          // scores of the two blocks: in work, and of the next stage
+        u32x4 pf[4];                // probabilities of the four units
+        uint32_t seen[2];           // the slots of y's blocks that the row sees
+        float s0 = 0.0f, s1 = 0.0f;
+
+        // The pair k of the scores, 2 elements of 32: exponentials, then their sums and rounding.
+        float e[2][2];
+        const auto exponent = [&](int k) {
 #pragma unroll
-            for (int i = 0; i < (2 * NS + 3) / 4; ++i) {
-                const uint32_t j = min(wave + 4 * i, 2u * NS - 1), unit = j / NS, piece = j % NS;  // (the same one twice where they do not divide)
-                const uint32_t page = unit ? p1 : p0;
-                const uint16_t *from = pool + unit_at(a.c, page < a.c.pages ? page : 0u, head, 2 * n + unit) + 512 * piece + 8 * lane;
-                to_lds(from, &lds[kind][n & 1][unit][piece][0]);
+            for (int x = 0; x < 2; ++x) e[k & 1][x] = __builtin_amdgcn_exp2f(fmaf(p[k / 8][2 * (k % 8) + x], c, -sums.base));
+        };
+        const auto round = [&](int k) {
+            s0 += e[k & 1][0];
+            s1 += e[k & 1][1];
+            pf[k / 4][k % 4] = pack_bf16_rne(e[k & 1][0], e[k & 1][1]);
+        };
+        // A look ahead of kLook operands in registers.  Between the products, `also(m)` gives the vector unit its share.
+        constexpr int kLook = 4;
+        const auto scores = [&](uint32_t from, auto &&also) {
+            bf16x8_t kf[kLook];
+#pragma unroll
+            for (int m = 0; m < kLook; ++m) kf[m] = key(from, m);
+#pragma unroll
+            for (int m = 0; m < kProducts; ++m) {
+                f32x16 &to = y[m / (2 * NS)];
+                if (m % (2 * NS) == 0) to = f32x16{};
+                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % kLook], q[m % (2 * NS)], to, 0, 0, 0);
+                if (m + kLook < kProducts) kf[m % kLook] = key(from, m + kLook);
+                also(m);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        uint32_t pg[3][2];  // pages of blocks n, n + 1 and n + 2
-        const auto pages_of = [&](uint32_t n, uint32_t (&p)[2]) {
-            if (n >= end) {  // past the end: nothing reads it
-                p[0] = p[1] = 0;
-                return;
-            }
-            const uint32_t i = 2 * (n - first);
-            pages.enter(i);
-            p[0] = pages.at(i);
-            p[1] = pages.at(i + 1);
+        const auto product = [&](int m, const u32x4 &v) {
+            o[m % NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pf[m / NS]), o[m % NS], 0, 0, 0);
         };
-        f32x16 p;
-        bool edge = false;  // the block in work is not seen whole by every row of the wave
-        uint32_t seen = 0;  // its slots that the row sees, where it is
-        const auto key_steps = [&](uint32_t n) {
-            f32x16 x = {};
+        const auto average = [&](uint32_t from, auto &&also) {
+            u32x4 vf[kLook];
 #pragma unroll
-            for (int j = 0; j < 2 * NS; ++j) {
-                // octet 2 j + h of slot r32: 256 bytes an octet
-                const u32x4 k = lds[0][n & 1][r32 >> 4][j / 2][(j & 1) * 32 + h * 16 + (r32 & 15)];
-                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), q[j], x, 0, 0, 0);
-            }
-            return x;
-        };
-        const auto enter = [&](uint32_t n, const uint32_t (&pn)[2]) {
-            const bool hole0 = pn[0] >= a.c.pages, hole1 = pn[1] >= a.c.pages;
-            edge = 32 * n + 32 > clear || hole0 || hole1;
-            if (edge) {
-                seen = sight.bits(32 * n) & ~((hole0 ? 0xFFFFu : 0u) | (hole1 ? 0xFFFF0000u : 0u));
+            for (int m = 0; m < kLook; ++m) vf[m] = value(from, m);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = seen >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1 ? p[i] : -INFINITY;
-            }
-            float top = fmaxf(fmaxf(p[0], p[1]), p[2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) top = fmaxf(fmaxf(top, p[i]), p[i + 1]);
-            top = fmaxf(top, p[15]) * c;
-            top = fmaxf(top, xchg32(top, lane));
-            if (!edge || seen) top = fmaxf(top, kLowBase);
-            if (__any(top > sums.base + kLag)) {
-                const float down = row_follow(sums, top);
-#pragma unroll
-                for (int d = 0; d < NS; ++d) o[d] *= down;
+            for (int m = 0; m < kProducts; ++m) {
+                product(m, vf[m % kLook]);
+                if (m + kLook < kProducts) vf[m % kLook] = value(from, m + kLook);
+                also(m);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        const auto body = [&](auto more, uint32_t n, const uint32_t (&pn)[2]) {
-            constexpr bool kMore = decltype(more)::value;
-            float sum = 0.0f;
-            u32x4 pf[2];
-            const bool edge_now = edge;
-            const uint32_t seen_now = seen;
+        // A stage that some row of the tile does not see whole, and a chunk that some row of the wave does not (n blocks, holes of their
+        // units).
+        const auto has_edge = [&](uint32_t from, uint32_t n, uint32_t sees, uint32_t holes) { return from + n > end || 32 * (from + n) > sees || holes; };
+        const auto stage_edge = [&](uint32_t i, uint32_t holes) { return has_edge(first + 2 * G * i, 2 * G, clear_tile, holes); };
+        // Takes infinities and NaN out of a stage's values in LDS, once all have landed; `clean` before that, a barrier after it.
+        const auto clean = [&](uint32_t i) {
+            if (threadIdx.x % 256 < 2) lds_bad[i & 1][group][threadIdx.x % 256] = 0;
+        };
+        const auto take_out_all = [&](uint32_t i, uint32_t from) {
+            // a thread a 16-byte piece of each KB that its wave brought: all of unit `wave`, slots 8 a + 4 h + j
+            u32x4 words = {};
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(fmaf(p[i], c, -sums.base)), e1 = __builtin_amdgcn_exp2f(fmaf(p[i + 1], c, -sums.base));
-                sum += e0;
-                sum += e1;
-                pf[i >> 3][(i & 7) >> 1] = pack_bf16_rne(e0, e1);
+            for (int d = 0; d < NS; ++d) {
+                u32x4 *v = reinterpret_cast<u32x4 *>(lds + kKind + from + group * kChunk + wave * kUnit + kPiece * d) + lane;
+                u32x4 x = *v;
+                words |= take_out(x);
+                *v = x;
             }
-            sums.l += sum;
-            if constexpr (kMore) p = key_steps(n + 1);
-            u32x4 vf[2 * NS];
-#pragma unroll
-            for (int j = 0; j < 2 * NS; ++j) vf[j] = lds[1][n & 1][j & 1][j >> 1][lane];
-            uint32_t bad = 0;
-            if (edge_now) {
-                u32x4 words[2] = {};
-#pragma unroll
-                for (int j = 0; j < 2 * NS; ++j) take_out(vf[j], words[j & 1]);
-                bad = (bad_slots(words[0]) | bad_slots(words[1]) << 16) << (4 * h);
-                if (__any(bad)) bad &= wave_or(seen_now);  // (what no row sees is left out)
-            }
-#pragma unroll
-            for (int d = 0; d < NS; ++d)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[2 * d + x]),
-                                                                   __builtin_bit_cast(bf16x8_t, pf[x]), o[d], 0, 0, 0);
-            if (edge_now && __any(bad)) {
-                for (uint32_t left = wave_or(bad); left; left &= left - 1) {
-                    const uint32_t slot = (uint32_t)__builtin_ctz(left), page = slot < 16 ? pn[0] : pn[1];
-                    const uint16_t *v = a.c.v + unit_at(a.c, page, head, 2 * n + slot / 16) + paged_value_at(slot % 16, 4 * h);
+            const uint32_t bad = bad_slots(words) << (16 * (wave & 1) + 4 * h);
+            if (bad) atomicOr(&lds_bad[i & 1][group][wave >> 1], bad);
+        };
+        // ... and gives them to the rows that see them; seen_by: the chunk's slots that the row sees.
+        const auto put_back_all = [&](uint32_t i, const uint32_t (&seen_by)[2]) {
+#pragma unroll 1
+            for (uint32_t y = 0; y < 2; ++y) {
+                const uint32_t sees = y ? seen_by[1] : seen_by[0];
+                uint32_t rest = lds_bad[i & 1][group][y];
+                if (rest) rest &= wave_or(sees);  // (what no row sees is left out)
+                for (rest = __builtin_amdgcn_readfirstlane(rest); rest; rest &= rest - 1) {
+                    const uint32_t slot = (uint32_t)__builtin_ctz(rest), unit = 2 * (block_of(i) + y) + slot / 16;
+                    const uint16_t *v = a.c.v + unit_at(a.c, page_of(a.c, b, unit), head, unit) + paged_value_at(slot % 16, 4 * h);
 #pragma unroll
                     for (int d = 0; d < NS; ++d) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[d][i] = put_back(o[d][i], v[512 * d + 8 * (8 * (i >> 2) + (i & 3))], seen_now >> slot & 1);
+                        for (int x = 0; x < 16; ++x) o[d][x] = put_back(o[d][x], v[512 * d + 8 * (8 * (x >> 2) + (x & 3))], sees >> slot & 1);
                         __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
                     }
                 }
             }
         };
-        if (first < end) {
-            // keys first and first + 1, values first
-            pages_of(first, pg[0]);
-            pages_of(first + 1, pg[1]);
-            request(0, first, pg[0][0], pg[0][1]);
-            if (first + 1 < end) request(0, first + 1, pg[1][0], pg[1][1]);
-            request(1, first, pg[0][0], pg[0][1]);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            p = key_steps(first);
-            enter(first, pg[0]);
-            for (uint32_t n = first; n + 1 < end; ++n) {
-                // what body n reads has landed, what it overwrites has been read
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                __syncthreads();
-                pages_of(n + 2, pg[2]);
-                if (n + 2 < end) request(0, n + 2, pg[2][0], pg[2][1]);
-                request(1, n + 1, pg[1][0], pg[1][1]);
-                body(std::true_type{}, n, pg[0]);
-                enter(n + 1, pg[1]);
+        // Of the next stage's scores: slots that a row does not see get -infinity.
+        const auto hide = [&](uint32_t i, uint32_t holes) {
+            const uint32_t n = block_of(i);
+            holes = holes >> (4 * group) & 15;
+            seen[0] = seen[1] = kAll;
+            if (!has_edge(n, 2, clear, holes)) return;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    pg[0][x] = pg[1][x];
-                    pg[1][x] = pg[2][x];
-                }
+            for (uint32_t k = 0; k < 2; ++k) {
+                const uint32_t none = (holes >> (2 * k) & 1 ? 0xFFFFu : 0u) | (holes >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
+                seen[k] = n + k < end ? sight.bits(32 * (n + k)) & ~none : 0u;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) y[k][x] = seen[k] >> (8 * (x >> 2) + 4 * h + (x & 3)) & 1 ? y[k][x] : -INFINITY;
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        };
+        // Their maximum, in eight steps of two; the row's base follows where it is passed.
+        float top[2];
+        const auto highest = [&](int k) {
+            if (k == 0) top[0] = top[1] = -INFINITY;
+#pragma unroll
+            for (int z = 0; z < 2; ++z) top[z] = fmaxf(fmaxf(top[z], y[z][2 * k]), y[z][2 * k + 1]);
+        };
+        const auto follow = [&] {
+            float m = fmaxf(top[0], top[1]) * c;
+            m = fmaxf(m, xchg32(m, lane));
+            if (seen[0] | seen[1]) m = fmaxf(m, kLowBase);
+            if (__any(m > sums.base + kLag)) {
+                const float down = row_follow(sums, m);
+                s0 *= down;
+                s1 *= down;
+#pragma unroll
+                for (int d = 0; d < NS; ++d) o[d] *= down;
+            }
+            p[0] = y[0];
+            p[1] = y[1];
+        };
+        if (stages) {
+            // keys of stages 0 and 1, values of 0
+            constexpr uint32_t kOfStage = 4 * G;
+            uint32_t holes = units.holes(0, kOfStage), unit = units.at(4 * group + wave);
+            request(0, unit, 0);
+            request(1, unit, 0);
+            uint32_t next_holes = units.holes(kOfStage, kOfStage);
+            unit = units.at(kOfStage + 4 * group + wave);
+            if (stages > 1) {
+                request(0, unit, kStage);
+                landed<NS>();
+            } else {
+                landed<0>();
+            }
+            bool edge = stage_edge(0, holes);
+            if (edge) clean(0);
             __syncthreads();
-            body(std::false_type{}, end - 1, pg[0]);
+            scores(0, [](int) {});
+            hide(0, holes);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) highest(k);
+            follow();
+            uint32_t now = 0;  // the buffers of stage i
+            for (uint32_t i = 0; i + 1 < stages; ++i) {
+                // keys i + 1 and values i have landed, and what is overwritten has been read
+                landed<0>();
+                __syncthreads();
+                if (edge) {
+                    take_out_all(i, now);
+                    __syncthreads();
+                }
+                const uint32_t other = now ^ kStage;
+                request(1, unit, other);
+                units.enter(kOfStage * (i + 2));
+                holes = next_holes;
+                next_holes = units.holes(kOfStage * (i + 2), kOfStage);
+                unit = units.at(kOfStage * (i + 2) + 4 * group + wave);
+                if (i + 2 < stages) request(0, unit, now);
+                // the scores of the next stage beside the exponentials of this one, and the products of this one's values beside the next
+                // one's maxima
+                scores(other, [&](int m) {
+#pragma unroll
+                    for (int k = 16 * m / kProducts; k < 16 * (m + 1) / kProducts; ++k) {
+                        exponent(k);
+                        if (k) round(k - 1);
+                    }
+                });
+                round(15);
+                const uint32_t seen_now[2] = {seen[0], seen[1]};
+                hide(i + 1, holes);
+                average(now, [&](int m) {
+#pragma unroll
+                    for (int k = 8 * m / kProducts; k < 8 * (m + 1) / kProducts; ++k) highest(k);
+                });
+                if (edge) put_back_all(i, seen_now);
+                follow();
+                edge = stage_edge(i + 1, holes);
+                if (edge) clean(i + 1);
+                now = other;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                exponent(k);
+                round(k);
+            }
+            landed<0>();
+            __syncthreads();
+            if (edge) {
+                take_out_all(stages - 1, now);
+                __syncthreads();
+            }
+            average(now, [](int) {});
+            if (edge) put_back_all(stages - 1, seen);
         }
-        const float l = sums.l + xchg32(sums.l, lane);
+        sums.l = s0 + s1;
+        float l = sums.l + xchg32(sums.l, lane);
+        if constexpr (G == 2) {  // the second group's sums join the first's
+            __syncthreads();
+                f32x4 *other = reinterpret_cast<f32x4 *>(lds) + wave * (4 * NS * 64) + lane;
+            if (group == 1) {
+                if (h == 0) lds_ml[wave][r32] = make_float2(sums.base, l);
+#pragma unroll
+                for (int d = 0; d < NS; ++d)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) other[(4 * d + x) * 64] = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+            }
+            __syncthreads();
+            if (group == 1) continue;
+            const float2 ml = lds_ml[wave][r32];
+            const float base = fmaxf(sums.base, ml.x), f0 = __builtin_amdgcn_exp2f(sums.base - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
+            sums.base = base;
+            l = l * f0 + ml.y * f1;
+#pragma unroll
+            for (int d = 0; d < NS; ++d)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const f32x4 y = other[(4 * d + x) * 64];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[d][4 * x + k] = fmaf(o[d][4 * x + k], f0, y[k] * f1);
+                }
+        }
         const float norm = l == 0.0f ? 0.0f : 1.0f / l;
         const bool nan = l == 0.0f && sums.base > kSeenBase;  // saw slots, all with scores of -infinity
 #pragma unroll
@@ -345,7 +489,7 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedA
 #pragma unroll
                 for (int d = 0; d < NS; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] = __builtin_nanf("");
+                    for (int x = 0; x < 16; ++x) o[d][x] = __builtin_nanf("");
             }
             const size_t to = (size_t)t * a.q_heads + qh;
             if (a.lse && h == 0) a.lse[to] = l == 0.0f ? (nan ? __builtin_nanf("") : -INFINITY) : (sums.base + __log2f(l)) * kLn2;
@@ -353,16 +497,16 @@ __global__ __launch_bounds__(256, NS <= 4 ? 2 : 1) void paged_many_kernel(PagedA
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * i + 4 * h) = pack4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * x + 4 * h) = pack4(o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]);
         } else {
             const size_t to = part_at(a, split, 2 * idx + odd, head, r - r0);
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4 *>(a.part + to * D + 32 * d + 8 * i + 4 * h) =
-                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<f32x4 *>(a.part + to * D + 32 * d + 8 * x + 4 * h) =
+                        f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
             if (h == 0) {
                 float *ml = a.part + (size_t)slots * a.c.heads * kManyRows * D + 2 * to;
                 ml[0] = sums.base;
@@ -393,13 +537,14 @@ struct FewBlock {
     u32x4 v[NS][2];  // [32 dims][16 of them]
     uint32_t holes;  // slots without a page
 };
+// Units at u0 and u1.
 template <int NS>
-__device__ __forceinline__ void load_few(FewBlock<NS> &f, const PagedAttnArgs &a, uint32_t head, uint32_t blk, uint32_t p0, uint32_t p1) {
+__device__ __forceinline__ void load_few(FewBlock<NS> &f, const Paged &c, uint32_t u0, uint32_t u1, uint32_t holes) {
+    constexpr size_t kSize = kPagedUnit * 32 * NS;
     const uint32_t lane = __lane_id(), r = lane & 15, g = lane >> 4;
-    f.holes = (p0 < a.c.pages ? 0u : 0xFFFFu) | (p1 < a.c.pages ? 0u : 0xFFFF0000u);
-    const size_t at0 = unit_at(a.c, p0 < a.c.pages ? p0 : 0u, head, 2 * blk), at1 = unit_at(a.c, p1 < a.c.pages ? p1 : 0u, head, 2 * blk + 1);
-    const uint16_t *k = a.c.k + (r >> 3 ? at1 : at0) + 128 * g + 8 * (r & 7);
-    const uint16_t *v = a.c.v + (g >> 1 ? at1 : at0) + 256 * (g & 1) + 8 * r;
+    f.holes = (holes & 1 ? 0xFFFFu : 0u) | (holes & 2 ? 0xFFFF0000u : 0u);
+    const uint16_t *k = c.k + (r >> 3 ? u1 : u0) * kSize + 128 * g + 8 * (r & 7);
+    const uint16_t *v = c.v + (g >> 1 ? u1 : u0) * kSize + 256 * (g & 1) + 8 * r;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -431,16 +576,16 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
     constexpr uint32_t kAhead = kFewAhead<NS>;
     FewBlock<NS> f[kAhead];
     // unit i of the wave: half i % 2 of its i / 2-th block
-    Pages pages([&](uint32_t set) { return page_of(a.c, b, 2 * (first + wave + kFewWaves * (32 * set + lane / 2)) + lane % 2); });
+    Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * (first + wave + kFewWaves * (i / 2)) + i % 2); }, a.c, head);
     uint32_t asked = 0;
-    const auto ask = [&](FewBlock<NS> &f, uint32_t blk) {
-        pages.enter(asked);
-        load_few<NS>(f, a, head, blk, pages.at(asked), pages.at(asked + 1));
+    const auto ask = [&](FewBlock<NS> &f) {
+        units.enter(asked);
+        load_few<NS>(f, a.c, units.at(asked), units.at(asked + 1), units.holes(asked, 2));
         asked += 2;
     };
 #pragma unroll
     for (uint32_t i = 0; i < kAhead; ++i)
-        if (blk + i * kFewWaves < end) ask(f[i], blk + i * kFewWaves);
+        if (blk + i * kFewWaves < end) ask(f[i]);
     const uint32_t sign = query_sign(a.scale_log2);
     const float c = score_factor(a.scale_log2);
     bf16x8_t q[NS];
@@ -490,7 +635,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
         if (edge) {
             u32x4 words = {};
 #pragma unroll
-            for (int d = 0; d < 2 * NS; ++d) take_out(f.v[d >> 1][d & 1], words);
+            for (int d = 0; d < 2 * NS; ++d) words |= take_out(f.v[d >> 1][d & 1]);
             bad = bad_slots(words) << (16 * (g >> 1) + 4 * (g & 1));
         }
 #pragma unroll
@@ -516,7 +661,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             const uint32_t at = blk + i * kFewWaves;
             if (at >= end) break;
             step(f[i], at);
-            if (at + kAhead * kFewWaves < end) ask(f[i], at + kAhead * kFewWaves);
+            if (at + kAhead * kFewWaves < end) ask(f[i]);
         }
     }
     float l = sums.l + xchg32(sums.l, lane);
@@ -588,7 +733,7 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
         p.slots = p.grid = p.split.target + p.tiles;
     } else {
         // as many workgroups as the card holds at once
-        p.split.unit = D <= 128 ? 2 : 1;
+        p.split.unit = 1;
         const bool split = (uint64_t)p.tiles * kv_heads < 256 && (uint64_t)p.tiles * ((max_ctx + 31) / 32) < 1ull << 31;
         p.split.target = split ? 256 * p.split.unit / kv_heads : 0;  // at least `tiles`
         p.grid = p.split.target ? p.split.target : p.tiles;
@@ -614,7 +759,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
     const auto launch = [&](auto ns) -> hipError_t {
         constexpr int NS = decltype(ns)::value;
         if (p.few) paged_few_kernel<NS><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
-        else paged_many_kernel<NS><<<dim3(p.grid * a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
+        else paged_many_kernel<NS><<<dim3(p.grid * a.c.heads), 256 * kManyGroups<NS>, 0, s>>>(a, p.split, p.slots);
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 256) {

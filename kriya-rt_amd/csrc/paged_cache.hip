@@ -26,134 +26,180 @@ __device__ __forceinline__ UnitSpan unit_span(const PagedAppendArgs &a, uint32_t
     return r;
 }
 
-constexpr uint32_t kRows = kPagedUnit, kMaxDim = 256;
+// Heads of a unit that a workgroup takes: as many as make about 512 dims.
+__host__ __device__ constexpr uint32_t chunk_heads(uint32_t D) { return 512 / D; }
+// Threads of a row, each with two pieces of 8 dims: the power of two from D / 16 on.
+__host__ __device__ constexpr uint32_t row_threads(uint32_t D) { return D <= 64 ? 4 : (D <= 128 ? 8 : 16); }
+
+enum RopeKind : int { kNone, kHalf, kNeighbours, kAny };  // kHalf, kNeighbours: rotary_dim a multiple of 16
+
+// Dim d's partner in its pair, whether d is the pair's first, and its place in the table's row.
+struct Pair {
+    uint32_t other, at;
+    bool first;
+};
+__device__ __forceinline__ Pair pair_of(const RopeArgs &r, uint32_t d) {
+    if (r.interleaved) return Pair{d ^ 1, d / 2, d % 2 == 0};
+    const uint32_t half = r.rotary_dim / 2;
+    return d < half ? Pair{d + half, d, true} : Pair{d - half, d - half, false};
+}
 
 }  // namespace
 
-// Workgroups: (unit, kv head, keys or values), then (token, 16 query heads).  Each stages its up to 16 rows in LDS.  Keys and queries:
-// as f32, with the rows' sums of squares, then every thread normalises and turns 8 dims of a row, whatever the pairing, and
-// rounds them once.  Values: as they are, then every thread collects the 8 slots of a dim that lie together.  16-byte pieces whose
-// slots are not all new are written slot by slot: the others hold older tokens.
+// Workgroups: values of (unit, chunk of kv heads), keys of the same, then query rows.
+// Values come through LDS: a thread then collects the 8 slots of a dim that lie together.  16-byte pieces whose slots are not all new
+// are written slot by slot: the others hold older tokens.
+// Keys and queries: row_threads(D) threads a row, each with the two pieces of 8 dims that its rotation pairs (neighbouring ones
+// without), so that norm, rotation and rounding stay in registers; the row's sum of squares goes over its lanes.  kAny pairs dims that
+// lie anywhere: their partners are read one by one.
+template <uint32_t D, int kRope>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, uint32_t items) {
-    __shared__ __align__(16) float xs[kRows][kMaxDim];
-    __shared__ float squares[kRows][kMaxDim / 8];
-    const uint32_t D = a.c.D, units = D / 8;
-    const uint32_t kv_groups = items * a.c.heads * 2;
-    const uint16_t *src, *weight;
-    size_t stride;             // between rows
-    uint32_t rows, t0, t_step; // row i is of token t0 + i t_step
-    uint32_t r0 = 0;           // slot of row 0 in its unit
-    uint16_t *dst;
-    bool values = false, query = blockIdx.x >= kv_groups;
-    if (query) {
-        const uint32_t chunks = (a.q_heads + kRows - 1) / kRows, i = blockIdx.x - kv_groups, h0 = i % chunks * kRows;
-        t0 = i / chunks;
-        t_step = 0;
-        if (a.step.starts && (t0 < a.step.starts[0] || t0 >= a.step.starts[a.c.batch])) return;  // nobody's row
-        src = a.q + t0 * a.q_stride + (size_t)h0 * D;
-        dst = a.q_out + t0 * a.q_stride + (size_t)h0 * D;
-        stride = D;
-        rows = min(kRows, a.q_heads - h0);
-        weight = a.q_norm;
-    } else {
-        values = blockIdx.x & 1;
-        const uint32_t head = blockIdx.x / 2 % a.c.heads;
+    constexpr uint32_t kUnits = D / 8, kChunk = chunk_heads(D), kLanes = row_threads(D), kRowsAtOnce = 256 / kLanes;
+    __shared__ __align__(16) uint16_t vs[kPagedUnit][kChunk * D];
+    const uint32_t chunks = (a.c.heads + kChunk - 1) / kChunk, groups = items * chunks;
+    const bool query = blockIdx.x >= 2 * groups;
+    UnitSpan s{};
+    uint32_t u = 0, h0 = 0, heads = 0, from = 0, count = 0, t0 = 0, r0 = 0;  // slots `from` .., count of them; tokens t0 ..; r0: in the unit
+    size_t base = 0, head_step = 0;
+    if (!query) {
+        const uint32_t i = blockIdx.x % groups;
         uint32_t b, item;
-        if (!find_item(blockIdx.x / 2 / a.c.heads, a.c.batch, [&](uint32_t i) { return unit_span(a, i).items; }, b, item)) return;
-        const UnitSpan s = unit_span(a, b);
-        const uint32_t u = s.first + item, page = page_of(a.c, b, u);
+        if (!find_item(i / chunks, a.c.batch, [&](uint32_t x) { return unit_span(a, x).items; }, b, item)) return;
+        s = unit_span(a, b);
+        u = s.first + item;
+        const uint32_t page = page_of(a.c, b, u);
         if (page >= a.c.pages) return;
-        const uint32_t from = max(s.n0, u * kPagedUnit), to = min(s.end, (u + 1) * kPagedUnit);
+        h0 = i % chunks * kChunk;
+        heads = min(kChunk, a.c.heads - h0);
+        from = max(s.n0, u * kPagedUnit);
+        count = min(s.end, (u + 1) * kPagedUnit) - from;
         r0 = from % kPagedUnit;
-        rows = to - from;
         t0 = s.s.t0 + (from + s.s.m - s.s.n);
-        t_step = 1;
-        stride = a.kv_stride;
-        src = (values ? a.v : a.k) + t0 * a.kv_stride + (size_t)head * D;
-        dst = (values ? a.c.v : a.c.k) + unit_at(a.c, page, head, u);
-        weight = a.k_norm;
+        base = unit_at(a.c, page, h0, u);
+        head_step = (size_t)(kPagedUnit << a.c.shift) * D;
     }
-    if (values) {
-        uint16_t *vs = reinterpret_cast<uint16_t *>(&xs[0][0]);
-        for (uint32_t i = threadIdx.x; i < rows * units; i += 256) {
-            const uint32_t r = i / units, c = i % units;
-            *reinterpret_cast<u32x4 *>(vs + (r0 + r) * D + 8 * c) = *reinterpret_cast<const u32x4 *>(src + r * stride + 8 * c);
+    if (blockIdx.x < groups) {
+        const uint32_t width = heads * kUnits;  // pieces of a token
+        const uint16_t *src = a.v + t0 * a.kv_stride + (size_t)h0 * D;
+        for (uint32_t i = threadIdx.x; i < count * width; i += 256) {
+            const uint32_t r = i / width, x = i % width;
+            *reinterpret_cast<u32x4 *>(&vs[r0 + r][8 * x]) = *reinterpret_cast<const u32x4 *>(src + r * a.kv_stride + 8 * x);
         }
         __syncthreads();
-        // piece i: dims i / 64 32 + i % 32, half h = i / 32 % 2: slots 4 h + j and 8 + 4 h + j
-        for (uint32_t i = threadIdx.x; i < 2 * D; i += 256) {
-            const uint32_t h = i / 32 % 2, d = i / 64 * 32 + i % 32;
-            uint16_t e[8];
-            bool all = true;
+        // piece i of a head: dims i / 64 32 + i % 32, half h = i / 32 % 2: slots 4 h + j and 8 + 4 h + j
+        for (uint32_t i = threadIdx.x; i < heads * 2 * D; i += 256) {
+            const uint32_t head = i / (2 * D), p = i % (2 * D), h = p / 32 % 2, d = head * D + p / 64 * 32 + p % 32;
+            uint16_t *to = a.c.v + base + head * head_step + 8 * p;
+            uint32_t e[8];
 #pragma unroll
-            for (uint32_t x = 0; x < 8; ++x) {
-                const uint32_t r = x / 4 * 8 + 4 * h + x % 4;
-                const bool fresh = r - r0 < rows;
-                all = all && fresh;
-                e[x] = vs[r * D + d];
-                if (!fresh) e[x] = 0;
-            }
-            uint16_t *to = dst + 8 * i;
-            if (all) {
-                *reinterpret_cast<u32x4 *>(to) = u32x4{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                                                       e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16};
+            for (uint32_t x = 0; x < 8; ++x) e[x] = vs[x / 4 * 8 + 4 * h + x % 4][d];
+            if (count == kPagedUnit) {
+                *reinterpret_cast<u32x4 *>(to) = u32x4{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
             } else {
 #pragma unroll
                 for (uint32_t x = 0; x < 8; ++x)
-                    if (x / 4 * 8 + 4 * h + x % 4 - r0 < rows) to[x] = e[x];
+                    if (x / 4 * 8 + 4 * h + x % 4 - r0 < count) to[x] = (uint16_t)e[x];
             }
         }
         return;
     }
-    const bool turn = a.rope.cos_sin != nullptr;
-    if (!turn && !weight) {  // as they are
-        for (uint32_t i = threadIdx.x; i < rows * units; i += 256) {
-            const uint32_t r = i / units, c = i % units;
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(src + r * stride + 8 * c);
-            *reinterpret_cast<u32x4 *>(query ? dst + r * stride + 8 * c : dst + paged_key_at(r0 + r, 8 * c)) = v;
-        }
-        return;
+    // rows: (slot, head) of a unit's keys, or (token, head) of the queries
+    const uint32_t of = query ? a.q_heads : heads;  // rows of a token
+    uint32_t row = threadIdx.x / kLanes, end = count * heads;
+    size_t first_row = 0;
+    if (query) {
+        first_row = (size_t)(blockIdx.x - 2 * groups) * kRowsAtOnce;
+        const size_t rows = (size_t)a.step.tokens * a.q_heads;
+        end = (uint32_t)min((size_t)kRowsAtOnce, rows - first_row);
     }
-    for (uint32_t i = threadIdx.x; i < rows * units; i += 256) {
-        const uint32_t r = i / units, c = i % units;
-        float v[8], sum = 0.0f;
-        load8(src + r * stride + 8 * c, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], v[e], sum);
-        store8(&xs[r][8 * c], v);
-        squares[r][c] = sum;
+    const uint16_t *weight = query ? a.q_norm : a.k_norm;
+    const uint32_t p = threadIdx.x % kLanes, R = a.rope.rotary_dim;
+    // the thread's pieces
+    uint32_t u0 = 2 * p, u1 = 2 * p + 1;
+    bool turns = kRope == kNeighbours ? 16 * p < R : false;
+    if constexpr (kRope == kHalf) {
+        turns = 16 * p < R;
+        u0 = turns ? p : 2 * p;
+        u1 = turns ? p + R / 16 : 2 * p + 1;
     }
-    __syncthreads();
-    const uint32_t R = turn ? a.rope.rotary_dim : 0u, half = R / 2;
-    for (uint32_t i = threadIdx.x; i < rows * units; i += 256) {
-        const uint32_t r = i / units, c = i % units;
+    const bool mine = 16 * p < D;
+    for (; row < (end + kRowsAtOnce - 1) / kRowsAtOnce * kRowsAtOnce; row += kRowsAtOnce) {
+        const bool live = row < end && mine;
+        const size_t at = first_row + min(row, end - 1);
+        const uint32_t t = query ? (uint32_t)(at / of) : t0 + (uint32_t)at / of, head = (uint32_t)(at % of);
+        const bool nobody = query && a.step.starts && (t < a.step.starts[0] || t >= a.step.starts[a.c.batch]);
+        const uint16_t *src = query ? a.q + t * a.q_stride + (size_t)head * D : a.k + t * a.kv_stride + (size_t)(h0 + head) * D;
+        float lo[8], hi[8];
+        load8(src + (mine ? 8 * u0 : 0u), lo);
+        load8(src + (mine ? 8 * u1 : 0u), hi);
         float f = 1.0f;
         if (weight) {
             float sum = 0.0f;
-            for (uint32_t x = 0; x < units; ++x) sum += squares[r][x];
-            f = rsqrtf(sum / (float)D + a.eps);
-        }
-        const auto at = [&](uint32_t d) {
-            const float x = xs[r][d];
-            return weight ? x * f * bf16_to_f32(weight[d]) : x;
-        };
-        const uint32_t pos = turn ? a.rope.positions[t0 + r * t_step] : 0u;
-        const float *cs = pos < a.rope.rows ? a.rope.cos_sin + (size_t)pos * R : nullptr;
-        float y[8];
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-            const uint32_t d = 8 * c + e;
-            y[e] = at(d);
-            if (cs && d < R) {
-                const bool low = a.rope.interleaved ? d % 2 == 0 : d < half;
-                const uint32_t p = a.rope.interleaved ? d / 2 : (low ? d : d - half);
-                const float other = at(a.rope.interleaved ? d ^ 1 : (low ? d + half : d - half));
-                float y0, y1;
-                rope_pair(low ? y[e] : other, low ? other : y[e], cs[2 * p], cs[2 * p + 1], y0, y1);
-                y[e] = low ? y0 : y1;
+            for (int e = 0; e < 8; ++e) sum = fmaf(lo[e], lo[e], fmaf(hi[e], hi[e], sum));
+            if (!mine) sum = 0.0f;
+#pragma unroll
+            for (uint32_t x = 1; x < kLanes; x *= 2) sum += __shfl_xor(sum, (int)x);
+            f = rsqrtf(sum * (1.0f / D) + a.eps);
+            float w0[8], w1[8];
+            load8(weight + (mine ? 8 * u0 : 0u), w0);
+            load8(weight + (mine ? 8 * u1 : 0u), w1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lo[e] = lo[e] * f * w0[e];
+                hi[e] = hi[e] * f * w1[e];
             }
         }
-        store8(query ? dst + r * stride + 8 * c : dst + paged_key_at(r0 + r, 8 * c), y);
+        if constexpr (kRope != kNone) {
+            const uint32_t pos = a.rope.positions[t];
+            const float *cs = a.rope.cos_sin + (size_t)(pos < a.rope.rows ? pos : 0u) * R;
+            if constexpr (kRope == kAny) {
+                if (pos < a.rope.rows) {
+                    const auto turn = [&](float (&y)[8], uint32_t u) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e) {
+                            const uint32_t d = 8 * u + e;
+                            if (d >= R || !mine) continue;
+                            const Pair x = pair_of(a.rope, d);
+                            float other = bf16_to_f32(src[x.other]), y0, y1;
+                            if (weight) other = other * f * bf16_to_f32(weight[x.other]);
+                            rope_pair(x.first ? y[e] : other, x.first ? other : y[e], cs[2 * x.at], cs[2 * x.at + 1], y0, y1);
+                            y[e] = x.first ? y0 : y1;
+                        }
+                    };
+                    turn(lo, u0);
+                    turn(hi, u1);
+                }
+            } else {
+                // 16 numbers of the table either way: dims 16 p .. of a row are pairs 8 p .. of its first half
+                float c[16];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<f32x4 *>(c + 4 * x) = *reinterpret_cast<const f32x4 *>(cs + (turns ? 16 * p + 4 * x : 0));
+                if (turns && pos < a.rope.rows) {
+                    if constexpr (kRope == kHalf) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) rope_pair(lo[e], hi[e], c[2 * e], c[2 * e + 1], lo[e], hi[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            rope_pair(lo[e], lo[e + 1], c[e], c[e + 1], lo[e], lo[e + 1]);
+                            rope_pair(hi[e], hi[e + 1], c[8 + e], c[9 + e], hi[e], hi[e + 1]);
+                        }
+                    }
+                }
+            }
+        }
+        if (!live || nobody) continue;
+        if (query) {
+            uint16_t *to = a.q_out + t * a.q_stride + (size_t)head * D;
+            store8(to + 8 * u0, lo);
+            store8(to + 8 * u1, hi);
+        } else {
+            uint16_t *to = a.c.k + base + head * head_step;
+            store8(to + paged_key_at(r0 + row / of, 8 * u0), lo);
+            store8(to + paged_key_at(r0 + row / of, 8 * u1), hi);
+        }
     }
 }
 
@@ -162,11 +208,29 @@ static uint64_t append_items(const PagedAppendArgs &a) {
     return a.step.starts ? (uint64_t)a.step.tokens / kPagedUnit + 2ull * std::min(a.c.batch, a.step.tokens) : a.c.batch;
 }
 uint64_t paged_append_groups(const PagedAppendArgs &a) {
-    const uint64_t chunks = a.q ? (a.q_heads + kRows - 1) / kRows : 0;
-    return append_items(a) * a.c.heads * 2 + a.step.tokens * chunks;
+    const uint32_t chunk = chunk_heads(a.c.D), rows = 256 / row_threads(a.c.D);
+    return 2 * append_items(a) * ((a.c.heads + chunk - 1) / chunk) + (a.q ? ((uint64_t)a.step.tokens * a.q_heads + rows - 1) / rows : 0);
 }
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s) {
-    paged_append_kernel<<<dim3((uint32_t)paged_append_groups(a)), 256, 0, s>>>(a, (uint32_t)append_items(a));
+    const dim3 grid((uint32_t)paged_append_groups(a));
+    const auto items = (uint32_t)append_items(a);
+    const int kind = !a.rope.cos_sin ? kNone : !rope_units_ok(a.rope, a.c.D) ? kAny : a.rope.interleaved ? kNeighbours : kHalf;
+    const auto launch = [&](auto d) {
+        constexpr uint32_t D = decltype(d)::value;
+        switch (kind) {
+            case kNone: paged_append_kernel<D, kNone><<<grid, 256, 0, s>>>(a, items); break;
+            case kHalf: paged_append_kernel<D, kHalf><<<grid, 256, 0, s>>>(a, items); break;
+            case kNeighbours: paged_append_kernel<D, kNeighbours><<<grid, 256, 0, s>>>(a, items); break;
+            default: paged_append_kernel<D, kAny><<<grid, 256, 0, s>>>(a, items); break;
+        }
+    };
+    switch (a.c.D) {
+        case 64: launch(std::integral_constant<uint32_t, 64>{}); break;
+        case 96: launch(std::integral_constant<uint32_t, 96>{}); break;
+        case 128: launch(std::integral_constant<uint32_t, 128>{}); break;
+        case 192: launch(std::integral_constant<uint32_t, 192>{}); break;
+        default: launch(std::integral_constant<uint32_t, 256>{}); break;
+    }
     return hipGetLastError();
 }
 

@@ -93,20 +93,22 @@ hipError_t launch_tree_plan(const int32_t *parents, const RaggedStep &step, uint
 }
 
 // Workgroup (layer, sequence).  Each finds the path for itself (a few hundred bytes from the L2; a launch of its own would cost more
-// than the walks), the first layer's writes it out.  A thread then moves one column, 8 dims of a head's keys or one dim of
-// its values, over the path's nodes: path[i] >= i and rising, so the rows of later nodes are never where an earlier one goes, and within
-// eight nodes all are loaded before one is stored.  No thread touches another's column.
-constexpr uint32_t kCommitThreads = 256;
+// than the walks), the first layer's writes it out.  A node is the next one of the path if its parent is the last one and its token the
+// choice there: for every node that is looked up at once, and the walk then searches LDS.  A thread moves columns, 8 dims of a head's
+// keys or one dim of its values, over the nodes that change places, 64 of the path at a time: path[i] >= i and rising, so the rows of
+// later nodes are never where an earlier one goes, and within eight nodes all are loaded before one is stored.  No thread touches
+// another's column.
+constexpr uint32_t kCommitThreads = 512, kNoNode = 0xFFFFu;
 __global__ __launch_bounds__(kCommitThreads) void paged_commit_kernel(PagedCommitArgs a) {
-    __shared__ int32_t par[kTreeNodes], tok[kTreeNodes];
-    __shared__ uint16_t path[kTreeNodes];
-    __shared__ uint32_t found;
+    __shared__ uint16_t follows[kTreeNodes], path[kTreeNodes];
+    __shared__ uint32_t found, moved;
+    __shared__ uint32_t from_page[64], to_page[64], from_slot[64], to_slot[64];  // places in a page
     const uint32_t b = blockIdx.y, lane = threadIdx.x & 63, D = a.c.D;
     const Span s = span_of(a.step, b);
     const uint32_t m = min(s.m, kTreeNodes), old = s.n > s.m ? s.n - s.m : 0u;
     for (uint32_t i = threadIdx.x; i < m; i += kCommitThreads) {
-        par[i] = parent_of(a.parents + s.t0, i);
-        tok[i] = a.drafted[s.t0 + i];
+        const int32_t p = parent_of(a.parents + s.t0, i);
+        follows[i] = (uint16_t)(p >= 0 && a.drafted[s.t0 + i] == a.targets[s.t0 + (uint32_t)max(p, 0)] ? (uint32_t)p : kNoNode);
     }
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -115,17 +117,15 @@ __global__ __launch_bounds__(kCommitThreads) void paged_commit_kernel(PagedCommi
             if (lane == 0) path[0] = 0;
             n = 1;
             while (n < a.max_path) {
-                const int32_t want = a.targets[s.t0 + at];
-                uint32_t next = kTreeNodes;
+                uint32_t next = kNoNode;
                 for (uint32_t i0 = (at + 1) & ~63u; i0 < m; i0 += 64) {
-                    const uint32_t i = i0 + lane;
-                    const unsigned long long hit = __ballot(i < m && par[i] == (int32_t)at && tok[i] == want);
+                    const unsigned long long hit = __ballot(i0 + lane < m && follows[i0 + lane] == at);
                     if (hit) {
                         next = i0 + (uint32_t)__builtin_ctzll(hit);
                         break;
                     }
                 }
-                if (next == kTreeNodes) break;
+                if (next == kNoNode) break;
                 if (lane == 0) path[n] = (uint16_t)next;
                 ++n;
                 at = next;
@@ -143,41 +143,59 @@ __global__ __launch_bounds__(kCommitThreads) void paged_commit_kernel(PagedCommi
     if (blockIdx.x == 0)
         for (uint32_t i = threadIdx.x; i < a.max_path; i += kCommitThreads) a.path[(size_t)b * a.max_path + i] = i < n ? path[i] : 0u;
     if (s.n < s.m) return;  // (a length that was cut off: its nodes have no slots)
-    const size_t layer = (size_t)blockIdx.x * a.c.pages * a.c.heads * ((size_t)kPagedUnit << a.c.shift) * D;
-    const uint32_t key_columns = a.c.heads * (D / 8), columns = key_columns + a.c.heads * D;
-    for (uint32_t c = threadIdx.x; c < columns; c += kCommitThreads) {
-        const bool values = c >= key_columns;
-        const uint32_t x = values ? c - key_columns : c, per = values ? D : D / 8, head = x / per, d = values ? x % per : x % per * 8;
-        const auto place = [&](uint32_t node, size_t &to) {
-            const uint32_t slot = old + node, u = slot / kPagedUnit, r = slot % kPagedUnit;
-            if (slot >= a.c.max_ctx) return false;
-            const uint32_t page = page_of(a.c, b, u);
-            to = layer + unit_at(a.c, page, head, u) + (values ? paged_value_at(r, d) : paged_key_at(r, d));
-            return page < a.c.pages;
-        };
-        for (uint32_t i0 = 0; i0 < n; i0 += 8) {
-            u32x4 wide[8];
-            uint16_t narrow[8];
-            size_t to[8];
-            bool moves[8];
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                size_t from = 0;
-                const uint32_t node = i0 + i < n ? path[i0 + i] : i0 + i;
-                moves[i] = node != i0 + i && place(node, from) && place(i0 + i, to[i]);
-                if (moves[i]) {
-                    if (values) narrow[i] = a.c.v[from];
-                    else wide[i] = *reinterpret_cast<const u32x4 *>(a.c.k + from);
-                }
+    const size_t page_size = (size_t)a.c.heads * (kPagedUnit << a.c.shift) * D, layer = (size_t)blockIdx.x * a.c.pages * page_size;
+    const uint32_t slots = kPagedUnit << a.c.shift, key_columns = a.c.heads * (D / 8), columns = key_columns + a.c.heads * D;
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
+        if (threadIdx.x < 64) {
+            const uint32_t i = i0 + lane, node = i < n ? path[i] : i, from = old + node, to = old + i;
+            uint32_t pf = 0, pt = 0;
+            bool moves = node != i && from < a.c.max_ctx;  // (to < from)
+            if (moves) {
+                pf = page_of(a.c, b, from / kPagedUnit);
+                pt = page_of(a.c, b, to / kPagedUnit);
+                moves = pf < a.c.pages && pt < a.c.pages;
             }
+            const unsigned long long all = __ballot(moves);
+            if (moves) {
+                const uint32_t x = (uint32_t)__popcll(all & ((1ull << lane) - 1));
+                from_page[x] = pf;
+                to_page[x] = pt;
+                from_slot[x] = from & (slots - 1);
+                to_slot[x] = to & (slots - 1);
+            }
+            if (lane == 0) moved = (uint32_t)__popcll(all);
+        }
+        __syncthreads();
+        const uint32_t count = moved;
+        for (uint32_t c = threadIdx.x; c < columns; c += kCommitThreads) {
+            const bool values = c >= key_columns;
+            const uint32_t x = values ? c - key_columns : c, per = values ? D : D / 8, head = x / per, d = values ? x % per : x % per * 8;
+            const size_t column = layer + (size_t)head * slots * D;
+            const auto place = [&](uint32_t page, uint32_t slot) {
+                const uint32_t r = slot % kPagedUnit;
+                return column + page * page_size + (size_t)(slot / kPagedUnit) * (kPagedUnit * D) + (values ? paged_value_at(r, d) : paged_key_at(r, d));
+            };
+            for (uint32_t k = 0; k < count; k += 8) {
+                // (past the last one: the last one again, which is not stored)
+                if (values) {
+                    uint16_t v[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                if (moves[i]) {
-                    if (values) a.c.v[to[i]] = narrow[i];
-                    else *reinterpret_cast<u32x4 *>(a.c.k + to[i]) = wide[i];
+                    for (uint32_t i = 0; i < 8; ++i) v[i] = a.c.v[place(from_page[min(k + i, count - 1)], from_slot[min(k + i, count - 1)])];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (k + i < count) a.c.v[place(to_page[k + i], to_slot[k + i])] = v[i];
+                } else {
+                    u32x4 v[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        v[i] = *reinterpret_cast<const u32x4 *>(a.c.k + place(from_page[min(k + i, count - 1)], from_slot[min(k + i, count - 1)]));
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (k + i < count) *reinterpret_cast<u32x4 *>(a.c.k + place(to_page[k + i], to_slot[k + i])) = v[i];
                 }
             }
         }
+        __syncthreads();
     }
 }
 

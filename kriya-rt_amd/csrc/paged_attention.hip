@@ -165,17 +165,13 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 // ---- many rows: prompts, chunks, large trees
 constexpr uint32_t kManyRows = 128;
 
-// N KB into LDS, past the registers: 16 bytes a lane and instruction, lane l's of the n-th go to byte lds + 1024 n + 16 l, lds the same in
-// all lanes (the instruction's offset counts on both sides).  In assembly, since the compiler would have every later read of LDS wait for
-// it: whoever reads what it writes waits for vmcnt(0) and a barrier first.
+// The n-th KB from `from` on into LDS, past the registers: 16 bytes a lane, lane l's to byte lds + 1024 n + 16 l, lds the same in all lanes
+// (the instruction's offset counts on both sides).  In assembly, since the compiler would have every later read of LDS wait for it:
+// whoever reads what it writes waits for vmcnt(0) and a barrier first.
 template <int N>
-__device__ __forceinline__ void to_lds(const void *from, uint32_t lds) {
-    static_assert(N >= 1 && N <= 8);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
-    if constexpr (N > 1) asm volatile("global_load_lds_dwordx4 %0, off offset:1024" ::"v"(from) : "memory");
-    if constexpr (N > 2) asm volatile("global_load_lds_dwordx4 %0, off offset:2048" ::"v"(from) : "memory");
-    if constexpr (N > 3) asm volatile("global_load_lds_dwordx4 %0, off offset:3072" ::"v"(from) : "memory");
-    if constexpr (N > 4) to_lds<N - 4>((const char *)from + 4096, lds + 4096);
+__device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
+                 ::"s"(lds + N / 4 * 4096), "v"(from + N / 4 * 2048), "n"(N % 4 * 1024) : "memory");
 }
 
 // All but the last N of this wave's have landed (loads end in order).
@@ -244,11 +240,15 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
         const auto block_of = [&](uint32_t i) { return first + 2 * (G * i + group); };
         Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * first + i); }, a.c, head);
         const uint32_t clear_tile = clear_of(a, s, r0);
-        // A wave brings one of the four units, its keys or its values, into LDS: `unit` where it lies in the pool.
-        const auto request = [&](uint32_t kind, uint32_t unit, uint32_t to) {
-            const uint16_t *from = (kind ? a.c.v : a.c.k) + (size_t)unit * (kPagedUnit * D) + 8 * lane;
-            to_lds<NS>(from, lds_base + kind * kKind + to + group * kChunk + wave * kUnit);
+        // A wave brings one of the four units, its keys or its values, into LDS, NS pieces: `unit` where it lies in the pool.
+        struct Request {
+            const uint16_t *from;
+            uint32_t to;
         };
+        const auto request = [&](uint32_t kind, uint32_t unit, uint32_t to) {
+            return Request{(kind ? a.c.v : a.c.k) + (size_t)unit * (kPagedUnit * D) + 8 * lane, lds_base + kind * kKind + to + group * kChunk + wave * kUnit};
+        };
+        const auto all_of = [&](const Request &x) { static_for<NS>([&](auto n) { to_lds<n>(x.from, x.to); }); };
         // Octet 2 j + h of slot r32 of two units, 256 bytes an octet, is the j-th operand of keys; 16 bytes of lane (dim, h) of a unit
         // and 32 dims are an operand of values.
         const char *key_at = lds + group * kChunk + (r32 >> 4) * kUnit + h * 256 + (r32 & 15) * 16;
@@ -256,9 +256,11 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
         // operand m of a chunk: of keys block m / 2 NS, dims 16 (m % 2 NS) ..; of values unit m / NS, 32 dims m % NS
         const auto key = [&](uint32_t from, int m) { return *reinterpret_cast<const bf16x8_t *>(key_at + from + 512 * (m % (2 * NS)) + 2 * kUnit * (m / (2 * NS))); };
         const auto value = [&](uint32_t from, int m) { return *reinterpret_cast<const u32x4 *>(value_at + from + kUnit * (m / NS) + kPiece * (m % NS)); };
-        f32x16 p[2], y[2];          // scores of the two blocks: in work, and of the next stage
-        u32x4 pf[4];                // probabilities of the four units
-        uint32_t seen[2];           // the slots of y's blocks that the row sees
+        // Scores of the chunk's two blocks, the second in p[0] and the first in p[1], and the next chunk's first block's: the next second
+        // block's take p[0]'s place, once its exponentials are under way, and z then p[1]'s.
+        f32x16 p[2], z;
+        u32x4 pf[4];       // probabilities of the four units
+        uint32_t seen[2];  // the slots of the next chunk's blocks that the row sees
         float s0 = 0.0f, s1 = 0.0f;
 
         // The pair k of the scores, 2 elements of 32: exponentials, then their sums and rounding.
@@ -270,38 +272,38 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
         const auto round = [&](int k) {
             s0 += e[k & 1][0];
             s1 += e[k & 1][1];
-            pf[k / 4][k % 4] = pack_bf16_rne(e[k & 1][0], e[k & 1][1]);
+            uint32_t both = pack_bf16_rne(e[k & 1][0], e[k & 1][1]);
+            asm volatile("" : "+v"(both), "+v"(s0), "+v"(s1));  // (here: not where the compiler would put it, in one run before its use)
+            pf[(k / 4 + 2) % 4][k % 4] = both;
         };
         // A look ahead of kLook operands in registers.  Between the products, `also(m)` gives the vector unit its share.
-        constexpr int kLook = 4;
+        constexpr int kLook = NS <= 4 ? 4 : 8;
         const auto scores = [&](uint32_t from, auto &&also) {
             bf16x8_t kf[kLook];
 #pragma unroll
             for (int m = 0; m < kLook; ++m) kf[m] = key(from, m);
-#pragma unroll
-            for (int m = 0; m < kProducts; ++m) {
-                f32x16 &to = y[m / (2 * NS)];
-                if (m % (2 * NS) == 0) to = f32x16{};
+            static_for<kProducts>([&](auto at) {
+                constexpr int m = at;
+                f32x16 &to = m < 2 * NS ? z : p[0];
+                if constexpr (m % (2 * NS) == 0) to = f32x16{};
                 to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % kLook], q[m % (2 * NS)], to, 0, 0, 0);
-                if (m + kLook < kProducts) kf[m % kLook] = key(from, m + kLook);
-                also(m);
+                if constexpr (m + kLook < kProducts) kf[m % kLook] = key(from, m + kLook);
+                also(at);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        const auto product = [&](int m, const u32x4 &v) {
-            o[m % NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pf[m / NS]), o[m % NS], 0, 0, 0);
+            });
         };
         const auto average = [&](uint32_t from, auto &&also) {
             u32x4 vf[kLook];
 #pragma unroll
             for (int m = 0; m < kLook; ++m) vf[m] = value(from, m);
-#pragma unroll
-            for (int m = 0; m < kProducts; ++m) {
-                product(m, vf[m % kLook]);
-                if (m + kLook < kProducts) vf[m % kLook] = value(from, m + kLook);
-                also(m);
+            static_for<kProducts>([&](auto at) {
+                constexpr int m = at;
+                o[m % NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[m % kLook]), __builtin_bit_cast(bf16x8_t, pf[m / NS]),
+                                                                    o[m % NS], 0, 0, 0);
+                if constexpr (m + kLook < kProducts) vf[m % kLook] = value(from, m + kLook);
+                also(at);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+            });
         };
         // A stage that some row of the tile does not see whole, and a chunk that some row of the wave does not (n blocks, holes of their
         // units).
@@ -349,20 +351,21 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
             holes = holes >> (4 * group) & 15;
             seen[0] = seen[1] = kAll;
             if (!has_edge(n, 2, clear, holes)) return;
-#pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
+            static_for<2>([&](auto at) {
+                constexpr uint32_t k = at;
+                f32x16 &y = k ? p[0] : p[1];
                 const uint32_t none = (holes >> (2 * k) & 1 ? 0xFFFFu : 0u) | (holes >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
                 seen[k] = n + k < end ? sight.bits(32 * (n + k)) & ~none : 0u;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) y[k][x] = seen[k] >> (8 * (x >> 2) + 4 * h + (x & 3)) & 1 ? y[k][x] : -INFINITY;
-            }
+                for (int x = 0; x < 16; ++x) y[x] = seen[k] >> (8 * (x >> 2) + 4 * h + (x & 3)) & 1 ? y[x] : -INFINITY;
+            });
         };
         // Their maximum, in eight steps of two; the row's base follows where it is passed.
         float top[2];
         const auto highest = [&](int k) {
             if (k == 0) top[0] = top[1] = -INFINITY;
 #pragma unroll
-            for (int z = 0; z < 2; ++z) top[z] = fmaxf(fmaxf(top[z], y[z][2 * k]), y[z][2 * k + 1]);
+            for (int x = 0; x < 2; ++x) top[x] = fmaxf(fmaxf(top[x], p[x][2 * k]), p[x][2 * k + 1]);
         };
         const auto follow = [&] {
             float m = fmaxf(top[0], top[1]) * c;
@@ -375,34 +378,52 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
 #pragma unroll
                 for (int d = 0; d < NS; ++d) o[d] *= down;
             }
-            p[0] = y[0];
-            p[1] = y[1];
         };
         if (stages) {
-            // keys of stages 0 and 1, values of 0
+            // The loop of a wave: next scores beside exponentials, values' products beside the next maxima.  Of a SIMD's two waves the
+            // second group's is half a stage ahead: one is at the exponentials, which take the vector unit longer than the matrix
+            // cores take the products beside them, while the other one's products want little else.  Its keys come a stage earlier.
             constexpr uint32_t kOfStage = 4 * G;
-            uint32_t holes = units.holes(0, kOfStage), unit = units.at(4 * group + wave);
-            request(0, unit, 0);
-            request(1, unit, 0);
-            uint32_t next_holes = units.holes(kOfStage, kOfStage);
-            unit = units.at(kOfStage + 4 * group + wave);
-            if (stages > 1) {
-                request(0, unit, kStage);
-                landed<NS>();
-            } else {
-                landed<0>();
-            }
-            bool edge = stage_edge(0, holes);
+            const auto unit_of = [&](uint32_t i) { return units.at(kOfStage * i + 4 * group + wave); };
+            const auto holes_of = [&](uint32_t i) { return units.holes(kOfStage * i, kOfStage); };
+            const auto next_scores = [&](uint32_t from, auto &&also) {
+                scores(from, [&](auto at) {
+                    constexpr int m = at;
+                    static_for<16 * (m + 1) / kProducts - 16 * m / kProducts>([&](auto x) {
+                        constexpr int k = 16 * m / kProducts + x;
+                        exponent(k);
+                        if constexpr (k > 0) round(k - 1);
+                    });
+                    also(at);
+                });
+                round(15);
+                p[1] = z;
+            };
+            // keys of stages 0 and 1, values of 0
+            uint32_t u0 = unit_of(0), u1 = unit_of(1), u2 = unit_of(2), h0 = holes_of(0), h1 = holes_of(1), h2 = holes_of(2);
+            all_of(request(0, u0, 0));
+            all_of(request(1, u0, 0));
+            all_of(request(0, u1, kStage));  // (past the last stage: a unit that nothing reads)
+            bool edge = stage_edge(0, h0);
             if (edge) clean(0);
+            landed<0>();
             __syncthreads();
-            scores(0, [](int) {});
-            hide(0, holes);
+            scores(0, [](auto) {});
+            p[1] = z;
+            hide(0, h0);
 #pragma unroll
             for (int k = 0; k < 8; ++k) highest(k);
             follow();
+            if constexpr (G == 2) {
+                __syncthreads();  // keys 0 have been read
+                if (group == 1) {
+                    all_of(request(0, u2, 0));
+                    next_scores(kStage, [](auto) {});
+                }
+            }
             uint32_t now = 0;  // the buffers of stage i
             for (uint32_t i = 0; i + 1 < stages; ++i) {
-                // keys i + 1 and values i have landed, and what is overwritten has been read
+                // what this stage reads has landed, and what is overwritten has been read
                 landed<0>();
                 __syncthreads();
                 if (edge) {
@@ -410,38 +431,43 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
                     __syncthreads();
                 }
                 const uint32_t other = now ^ kStage;
-                request(1, unit, other);
-                units.enter(kOfStage * (i + 2));
-                holes = next_holes;
-                next_holes = units.holes(kOfStage * (i + 2), kOfStage);
-                unit = units.at(kOfStage * (i + 2) + 4 * group + wave);
-                if (i + 2 < stages) request(0, unit, now);
-                // the scores of the next stage beside the exponentials of this one, and the products of this one's values beside the next
-                // one's maxima
-                scores(other, [&](int m) {
-#pragma unroll
-                    for (int k = 16 * m / kProducts; k < 16 * (m + 1) / kProducts; ++k) {
-                        exponent(k);
-                        if (k) round(k - 1);
-                    }
-                });
-                round(15);
+                units.enter(kOfStage * (i + 3));
+                const uint32_t u3 = unit_of(i + 3), h3 = holes_of(i + 3);
+                const Request values = request(1, u1, other), keys = group ? request(0, u3, other) : request(0, u2, now);
+                // a KB for the stages after with every few products
+                if (group == 0) {
+                    next_scores(other, [&](auto at) {
+                        if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
+                    });
+                }
                 const uint32_t seen_now[2] = {seen[0], seen[1]};
-                hide(i + 1, holes);
-                average(now, [&](int m) {
-#pragma unroll
-                    for (int k = 8 * m / kProducts; k < 8 * (m + 1) / kProducts; ++k) highest(k);
+                hide(i + 1, h1);
+                average(now, [&](auto at) {
+                    constexpr int m = at;
+                    static_for<8 * (m + 1) / kProducts - 8 * m / kProducts>([&](auto x) { highest(8 * m / kProducts + x); });
+                    if constexpr (m % 4 == 1) to_lds<m / 4>(keys.from, keys.to);
                 });
                 if (edge) put_back_all(i, seen_now);
                 follow();
-                edge = stage_edge(i + 1, holes);
+                if (G == 2 && group == 1) {
+                    next_scores(now, [&](auto at) {
+                        if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
+                    });
+                }
+                edge = stage_edge(i + 1, h1);
                 if (edge) clean(i + 1);
+                u1 = u2;
+                u2 = u3;
+                h1 = h2;
+                h2 = h3;
                 now = other;
             }
+            if (group == 0) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                exponent(k);
-                round(k);
+                for (int k = 0; k < 16; ++k) {
+                    exponent(k);
+                    round(k);
+                }
             }
             landed<0>();
             __syncthreads();
@@ -449,7 +475,7 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
                 take_out_all(stages - 1, now);
                 __syncthreads();
             }
-            average(now, [](int) {});
+            average(now, [](auto) {});
             if (edge) put_back_all(stages - 1, seen);
         }
         sums.l = s0 + s1;

@@ -25,8 +25,11 @@ __device__ __forceinline__ uint32_t row_limit(const Span &s, uint32_t r, uint32_
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
     uint32_t rows;    // of a tile
-    uint32_t unit;    // few rows: `per` is a multiple of it; many: workgroups that a compute unit holds
+    uint32_t unit;    // `per` is a multiple of it; shares: workgroups that a compute unit holds
 };
+// How tiles are split: few rows as above (at most target + tiles parts); many rows in shares of one line, below; or many rows in even
+// parts, at most `target` of them.
+enum class Parts { few, shares, even };
 template <class A>
 __device__ __forceinline__ uint32_t tiles_of(const A &a, const Split &w, const Span &s) {
     return (s.m * a.group + w.rows - 1) / w.rows;
@@ -42,9 +45,42 @@ __device__ __forceinline__ unsigned long long fair_share(unsigned long long tota
     return total >> 31 ? (total + target - 1) / target : ((uint32_t)total + target - 1) / target;
 }
 
-// Blocks of a part.  Every wave computes it alike.
+// Even parts: the fewest blocks, in whole units, of which `target` parts are enough, so that a workgroup has one.  (Shares of one line,
+// as below, are even to a block, but a second piece costs a workgroup another start and end, as much as 18 blocks of 128 rows and D 128:
+// 250 tokens over up to 5000 in eight sequences, 16/2 heads of 128, took 43 us, not 33; two rounds of smaller parts won nothing
+// either.)  A tile that is not split saves the way of its O through memory, about 14 blocks' time: where the longest has no more than
+// that past a part, tiles stay whole.
 template <class A>
+__device__ __forceinline__ uint32_t even_per(const A &a, const Split &w) {
+    const auto tiles = [&](uint32_t b) { return tiles_of(a, w, span_of(a.step, b)); };
+    const auto blocks = [&](uint32_t b) { return blocks_of(a, span_of(a.step, b)); };
+    const uint32_t lane = __lane_id(), tiles0 = lane < a.c.batch ? tiles(lane) : 0u, blocks0 = lane < a.c.batch ? blocks(lane) : 0u;
+    unsigned long long total = (unsigned long long)tiles0 * blocks0;
+    uint32_t most = tiles0 ? blocks0 : 0u;
+    for (uint32_t b = lane + 64; b < a.c.batch; b += 64) {
+        total += (unsigned long long)tiles(b) * blocks(b);
+        if (tiles(b)) most = max(most, blocks(b));
+    }
+    most = max(wave_max_u32(most), 1u);
+    uint32_t per = (uint32_t)min(fair_share(wave_sum_u64(total), w.target), 1ull << 27);
+    for (;; per += max(per / 16, 1u)) {
+        per = max((per + w.unit - 1) / w.unit, 1u) * w.unit;
+        if (most <= 14 + per) return most;
+        uint32_t parts = tiles0 * parts_of(blocks0, per);
+        for (uint32_t b = lane + 64; b < a.c.batch; b += 64) parts += tiles(b) * parts_of(blocks(b), per);
+        if (wave_sum_u32(parts) <= w.target) return per;
+    }
+}
+
+// Blocks of a part.  Every wave computes it alike.
+template <Parts kParts, class A>
 __device__ __forceinline__ uint32_t split_per(const A &a, const Split &w) {
+    if constexpr (kParts == Parts::even) {
+        const uint32_t per = even_per(a, w);
+        // for the join: its many small workgroups would take longer over it than over the rows
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.per = per;
+        return per;
+    }
     unsigned long long total = 0;
     for (uint32_t b = __lane_id(); b < a.c.batch; b += 64) {
         const Span s = span_of(a.step, b);
@@ -66,9 +102,9 @@ __device__ __forceinline__ void fill_work(const A &a, const Split &w, Work &o) {
     o.rows = o.s.m * a.group;
     o.most = a.sees_all() ? min(o.s.n, a.c.max_ctx) : row_limit(o.s, min(w.rows * (o.tile + 1), o.rows) - 1, a.group, a.c.max_ctx);
 }
+// By o.per: the part and tile that `idx` falls to, false past the last of a launch (past the shorter tile's own last, o.part is o.parts).
 template <class A>
-__device__ __forceinline__ bool find_work(const A &a, const Split &w, uint32_t idx, Work &o) {
-    o.per = split_per(a, w);
+__device__ __forceinline__ bool find_part(const A &a, const Split &w, uint32_t idx, Work &o) {
     uint32_t item;
     const auto count = [&](uint32_t i) {
         const Span s = span_of(a.step, i);
@@ -80,7 +116,12 @@ __device__ __forceinline__ bool find_work(const A &a, const Split &w, uint32_t i
     o.part = item / tiles;
     fill_work(a, w, o);
     o.parts = parts_of((o.most + 31) / 32, o.per);
-    return o.part < o.parts;
+    return true;
+}
+template <Parts kParts, class A>
+__device__ __forceinline__ bool find_work(const A &a, const Split &w, uint32_t idx, Work &o) {
+    o.per = split_per<kParts>(a, w);
+    return find_part(a, w, idx, o) && o.part < o.parts;
 }
 
 // Many rows: where there are fewer tiles than compute units, the tiles' blocks stand in one line, tile after tile, and a workgroup
@@ -127,13 +168,13 @@ __device__ __forceinline__ bool find_place(const A &a, const Split &w, uint32_t 
 
 // For the joins: the tile-th tile of all, false past the last, and where its parts lie in the workspace: slot `slot` + (part 0: `odd`) +
 // part * `step`.  Of a tile that is in one part (o.parts) nothing lies there.
-template <bool kMany, class A>
+template <Parts kParts, class A>
 __device__ __forceinline__ bool find_tile(const A &a, const Split &w, uint32_t tile, Work &o, uint32_t &slot,
                                           uint32_t &odd, uint32_t &step) {
     if (!find_item(tile, a.c.batch, [&](uint32_t i) { return tiles_of(a, w, span_of(a.step, i)); }, o.b, o.tile)) return false;
     fill_work(a, w, o);
     uint32_t share = 0;
-    if constexpr (kMany) {
+    if constexpr (kParts == Parts::shares) {
         share = share_of(a, w);
         if (share == 0) {
             o.parts = 1;
@@ -141,16 +182,18 @@ __device__ __forceinline__ bool find_tile(const A &a, const Split &w, uint32_t t
             step = 1;
             return true;
         }
+    } else if constexpr (kParts == Parts::even) {
+        o.per = *a.per;
     } else {
-        o.per = split_per(a, w);
+        o.per = split_per<kParts>(a, w);
     }
     uint32_t before = 0;
     for (uint32_t i = __lane_id(); i < o.b; i += 64) {
         const Span s = span_of(a.step, i);
-        before += tiles_of(a, w, s) * (kMany ? tile_blocks(a, s) : parts_of(blocks_of(a, s), o.per));
+        before += tiles_of(a, w, s) * (kParts == Parts::shares ? tile_blocks(a, s) : parts_of(blocks_of(a, s), o.per));
     }
     before = wave_sum_u32(before);
-    if constexpr (kMany) {
+    if constexpr (kParts == Parts::shares) {
         const uint32_t from = before + o.tile * tile_blocks(a, o.s), seen = max((o.most + 31) / 32, 1u);
         const uint32_t first = from / share, last = (from + seen - 1) / share;
         o.parts = last - first + 1;
@@ -187,7 +230,7 @@ __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_
 // kNanRows: rows whose L is 0 although they saw slots (all their scores -infinity) give NaN: a base above kSeenBase says so.
 constexpr float kSeenBase = -1.5e38f;
 constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;
-template <class A, int NS, bool kMany, bool kWide, bool kNanRows>
+template <class A, int NS, Parts kParts, bool kWide, bool kNanRows>
 __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void attn_join_kernel(A a, Split split,
                                                                                           uint32_t slots, uint32_t per_group) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
@@ -197,7 +240,7 @@ __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void attn_j
     const uint32_t groups = split.rows / per_group;
     Work w;
     uint32_t slot, odd, slot_step;
-    if (!find_tile<kMany>(a, split, blockIdx.x / groups, w, slot, odd, slot_step)) return;
+    if (!find_tile<kParts>(a, split, blockIdx.x / groups, w, slot, odd, slot_step)) return;
     // (starts that decrease can make more parts than the launch has: none behind its last.  Counted before the exit, beside the loads
     // that it waits for: 5 sequences up to 3000 13.8 us, not 14.1)
     if (slot < slots) w.parts = min(w.parts, (slots - slot + slot_step - 1) / slot_step);

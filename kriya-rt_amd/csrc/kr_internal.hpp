@@ -432,6 +432,7 @@ struct PagedAttnArgs {
     uint16_t *out;
     float *lse;                          // may be nullptr
     float *part;                         // workspace
+    uint32_t *per;                       // and behind it, for the join: blocks of a part
     // a row may see all new tokens of its sequence
     __host__ __device__ bool sees_all() const { return mask != nullptr; }
 };

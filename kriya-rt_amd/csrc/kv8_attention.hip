@@ -452,7 +452,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void kv8_few_kernel(Kv8AttnArg
     const uint32_t lane = __lane_id(), r16 = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
     const uint32_t head = blockIdx.y, idx = blockIdx.x;
     Work w;
-    if (!find_work(a, split, idx, w)) return;
+    if (!find_work<Parts::few>(a, split, idx, w)) return;
     const Span &s = w.s;
     const uint32_t r0 = kFewRows * w.tile, r = r0 + r16;
     const bool live = r < w.rows;
@@ -902,13 +902,13 @@ hipError_t launch_kv8_attention(const Kv8AttnArgs &a, hipStream_t s) {
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 256) {
-            attn_join_kernel<Kv8AttnArgs, NS, false, true, false><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
+            attn_join_kernel<Kv8AttnArgs, NS, Parts::few, true, false><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
         } else {
             uint32_t per_group = kJoinRowThreads / 64;
             while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 2048) per_group *= 2;
             const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
-            if (p.few) attn_join_kernel<Kv8AttnArgs, NS, false, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
-            else attn_join_kernel<Kv8AttnArgs, NS, true, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            if (p.few) attn_join_kernel<Kv8AttnArgs, NS, Parts::few, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            else attn_join_kernel<Kv8AttnArgs, NS, Parts::shares, false, false><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     });

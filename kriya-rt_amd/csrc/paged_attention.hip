@@ -198,346 +198,337 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % 4, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     // heads side by side: with eight of them each XCD's L2 keeps the keys and values of one
     const uint32_t head = blockIdx.x % a.c.heads, idx = blockIdx.x / a.c.heads;
-    const uint32_t share = share_of(a, split);
-    uint32_t place = idx * share, left = share;
     const float c = score_factor(a.scale_log2);
     const uint32_t sign = query_sign(a.scale_log2);
-    for (uint32_t odd = 0;; odd = 1) {  // the pieces of this workgroup's share
-        Work w;
-        uint32_t first = 0, end;
-        bool whole = true;
-        if (share) {
-            uint32_t blocks;
-            if (left == 0 || !find_place(a, split, place, w, first, blocks)) return;
-            const uint32_t take = min(left, blocks - first), seen = (w.most + 31) / 32;
-            left -= take;
-            place += take;
-            end = min(first + take, seen);
-            whole = first == 0 && end == seen;
-            if (first && first >= seen) continue;
-            if (odd) __syncthreads();  // LDS has been read
-        } else {
-            if (odd || !find_item(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, span_of(a.step, i)); }, w.b, w.tile)) return;
-            w.tile = tiles_of(a, split, span_of(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
-            fill_work(a, split, w);
-            end = (w.most + 31) / 32;
-        }
-        const Span &s = w.s;
-        const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + r32;
-        const bool live = r < w.rows;
-        const Sight sight = sight_of(a, s, r, live);
-        const uint32_t clear = r0 + 32 * wave < w.rows ? clear_of(a, s, r0 + 32 * wave) : kAll;  // (of rows past the end nothing counts)
-        const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
-        bf16x8_t q[2 * NS];
+    Work w;
+    uint32_t first = 0, end;
+    bool whole = true;
+    if (split.target) {
+        if (!find_work<Parts::even>(a, split, idx, w)) return;
+        first = w.part * w.per;
+        end = min(first + w.per, (w.most + 31) / 32);
+        whole = w.parts == 1;
+    } else {
+        if (!find_item(idx, a.c.batch, [&](uint32_t i) { return tiles_of(a, split, span_of(a.step, i)); }, w.b, w.tile)) return;
+        w.tile = tiles_of(a, split, span_of(a.step, w.b)) - 1 - w.tile;  // the tiles that see the most first
+        fill_work(a, split, w);
+        end = (w.most + 31) / 32;
+    }
+    const Span &s = w.s;
+    const uint32_t r0 = kManyRows * w.tile, r = r0 + 32 * wave + r32;
+    const bool live = r < w.rows;
+    const Sight sight = sight_of(a, s, r, live);
+    const uint32_t clear = r0 + 32 * wave < w.rows ? clear_of(a, s, r0 + 32 * wave) : kAll;  // (of rows past the end nothing counts)
+    const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
+    bf16x8_t q[2 * NS];
 #pragma unroll
-        for (int i = 0; i < 2 * NS; ++i) q[i] = query_unit(a.q + t * a.q_stride + (size_t)qh * D + 16 * i + 8 * h, live, sign);
-        f32x16 o[NS];
+    for (int i = 0; i < 2 * NS; ++i) q[i] = query_unit(a.q + t * a.q_stride + (size_t)qh * D + 16 * i + 8 * h, live, sign);
+    f32x16 o[NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) o[i] = f32x16{};
-        RowSums sums;
-        // stage i: blocks first + 2 G i ..; the group's own two from block_of(i) on
-        const uint32_t stages = first < end ? (end - first + 2 * G - 1) / (2 * G) : 0;
-        const auto block_of = [&](uint32_t i) { return first + 2 * (G * i + group); };
-        Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * first + i); }, a.c, head);
-        const uint32_t clear_tile = clear_of(a, s, r0);
-        // A wave brings one of the four units, its keys or its values, into LDS, NS pieces: `unit` where it lies in the pool.
-        struct Request {
-            const uint16_t *from;
-            uint32_t to;
-        };
-        const auto request = [&](uint32_t kind, uint32_t unit, uint32_t to) {
-            return Request{(kind ? a.c.v : a.c.k) + (size_t)unit * (kPagedUnit * D) + 8 * lane, lds_base + kind * kKind + to + group * kChunk + wave * kUnit};
-        };
-        const auto all_of = [&](const Request &x) { static_for<NS>([&](auto n) { to_lds<n>(x.from, x.to); }); };
-        // Octet 2 j + h of slot r32 of two units, 256 bytes an octet, is the j-th operand of keys; 16 bytes of lane (dim, h) of a unit
-        // and 32 dims are an operand of values.
-        const char *key_at = lds + group * kChunk + (r32 >> 4) * kUnit + h * 256 + (r32 & 15) * 16;
-        const char *value_at = lds + kKind + group * kChunk + lane * 16;
-        // operand m of a chunk: of keys block m / 2 NS, dims 16 (m % 2 NS) ..; of values unit m / NS, 32 dims m % NS
-        const auto key = [&](uint32_t from, int m) { return *reinterpret_cast<const bf16x8_t *>(key_at + from + 512 * (m % (2 * NS)) + 2 * kUnit * (m / (2 * NS))); };
-        const auto value = [&](uint32_t from, int m) { return *reinterpret_cast<const u32x4 *>(value_at + from + kUnit * (m / NS) + kPiece * (m % NS)); };
-        // Scores of the chunk's two blocks, the second in p[0] and the first in p[1], and the next chunk's first block's: the next second
-        // block's take p[0]'s place, once its exponentials are under way, and z then p[1]'s.
-        f32x16 p[2], z;
-        u32x4 pf[4];       // probabilities of the four units
-        uint32_t seen[2];  // the slots of the next chunk's blocks that the row sees
-        float s0 = 0.0f, s1 = 0.0f;
+    for (int i = 0; i < NS; ++i) o[i] = f32x16{};
+    RowSums sums;
+    // stage i: blocks first + 2 G i ..; the group's own two from block_of(i) on
+    const uint32_t stages = first < end ? (end - first + 2 * G - 1) / (2 * G) : 0;
+    const auto block_of = [&](uint32_t i) { return first + 2 * (G * i + group); };
+    Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * first + i); }, a.c, head);
+    const uint32_t clear_tile = clear_of(a, s, r0);
+    // A wave brings one of the four units, its keys or its values, into LDS, NS pieces: `unit` where it lies in the pool.
+    struct Request {
+        const uint16_t *from;
+        uint32_t to;
+    };
+    const auto request = [&](uint32_t kind, uint32_t unit, uint32_t to) {
+        return Request{(kind ? a.c.v : a.c.k) + (size_t)unit * (kPagedUnit * D) + 8 * lane, lds_base + kind * kKind + to + group * kChunk + wave * kUnit};
+    };
+    const auto all_of = [&](const Request &x) { static_for<NS>([&](auto n) { to_lds<n>(x.from, x.to); }); };
+    // Octet 2 j + h of slot r32 of two units, 256 bytes an octet, is the j-th operand of keys; 16 bytes of lane (dim, h) of a unit
+    // and 32 dims are an operand of values.
+    const char *key_at = lds + group * kChunk + (r32 >> 4) * kUnit + h * 256 + (r32 & 15) * 16;
+    const char *value_at = lds + kKind + group * kChunk + lane * 16;
+    // operand m of a chunk: of keys block m / 2 NS, dims 16 (m % 2 NS) ..; of values unit m / NS, 32 dims m % NS
+    const auto key = [&](uint32_t from, int m) { return *reinterpret_cast<const bf16x8_t *>(key_at + from + 512 * (m % (2 * NS)) + 2 * kUnit * (m / (2 * NS))); };
+    const auto value = [&](uint32_t from, int m) { return *reinterpret_cast<const u32x4 *>(value_at + from + kUnit * (m / NS) + kPiece * (m % NS)); };
+    // Scores of the chunk's two blocks, the second in p[0] and the first in p[1], and the next chunk's first block's: the next second
+    // block's take p[0]'s place, once its exponentials are under way, and z then p[1]'s.
+    f32x16 p[2], z;
+    u32x4 pf[4];       // probabilities of the four units
+    uint32_t seen[2];  // the slots of the next chunk's blocks that the row sees
+    float s0 = 0.0f, s1 = 0.0f;
 
-        // The pair k of the scores, 2 elements of 32: exponentials, then their sums and rounding.
-        float e[2][2];
-        const auto exponent = [&](int k) {
+    // The pair k of the scores, 2 elements of 32: exponentials, then their sums and rounding.
+    float e[2][2];
+    const auto exponent = [&](int k) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) e[k & 1][x] = __builtin_amdgcn_exp2f(fmaf(p[k / 8][2 * (k % 8) + x], c, -sums.base));
-        };
-        const auto round = [&](int k) {
-            s0 += e[k & 1][0];
-            s1 += e[k & 1][1];
-            uint32_t both = pack_bf16_rne(e[k & 1][0], e[k & 1][1]);
-            asm volatile("" : "+v"(both), "+v"(s0), "+v"(s1));  // (here: not where the compiler would put it, in one run before its use)
-            pf[(k / 4 + 2) % 4][k % 4] = both;
-        };
-        // A look ahead of kLook operands in registers.  Between the products, `also(m)` gives the vector unit its share.
-        constexpr int kLook = NS <= 4 ? 4 : 8;
-        const auto scores = [&](uint32_t from, auto &&also) {
-            bf16x8_t kf[kLook];
+        for (int x = 0; x < 2; ++x) e[k & 1][x] = __builtin_amdgcn_exp2f(fmaf(p[k / 8][2 * (k % 8) + x], c, -sums.base));
+    };
+    const auto round = [&](int k) {
+        s0 += e[k & 1][0];
+        s1 += e[k & 1][1];
+        uint32_t both = pack_bf16_rne(e[k & 1][0], e[k & 1][1]);
+        asm volatile("" : "+v"(both), "+v"(s0), "+v"(s1));  // (here: not where the compiler would put it, in one run before its use)
+        pf[(k / 4 + 2) % 4][k % 4] = both;
+    };
+    // A look ahead of kLook operands in registers.  Between the products, `also(m)` gives the vector unit its share.
+    constexpr int kLook = NS <= 4 ? 4 : 8;
+    const auto scores = [&](uint32_t from, auto &&also) {
+        bf16x8_t kf[kLook];
 #pragma unroll
-            for (int m = 0; m < kLook; ++m) kf[m] = key(from, m);
-            static_for<kProducts>([&](auto at) {
-                constexpr int m = at;
-                f32x16 &to = m < 2 * NS ? z : p[0];
-                if constexpr (m % (2 * NS) == 0) to = f32x16{};
-                to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % kLook], q[m % (2 * NS)], to, 0, 0, 0);
-                if constexpr (m + kLook < kProducts) kf[m % kLook] = key(from, m + kLook);
-                also(at);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        };
-        const auto average = [&](uint32_t from, auto &&also) {
-            u32x4 vf[kLook];
+        for (int m = 0; m < kLook; ++m) kf[m] = key(from, m);
+        static_for<kProducts>([&](auto at) {
+            constexpr int m = at;
+            f32x16 &to = m < 2 * NS ? z : p[0];
+            if constexpr (m % (2 * NS) == 0) to = f32x16{};
+            to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[m % kLook], q[m % (2 * NS)], to, 0, 0, 0);
+            if constexpr (m + kLook < kProducts) kf[m % kLook] = key(from, m + kLook);
+            also(at);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    const auto average = [&](uint32_t from, auto &&also) {
+        u32x4 vf[kLook];
 #pragma unroll
-            for (int m = 0; m < kLook; ++m) vf[m] = value(from, m);
-            static_for<kProducts>([&](auto at) {
-                constexpr int m = at;
-                o[m % NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[m % kLook]), __builtin_bit_cast(bf16x8_t, pf[m / NS]),
-                                                                    o[m % NS], 0, 0, 0);
-                if constexpr (m + kLook < kProducts) vf[m % kLook] = value(from, m + kLook);
-                also(at);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-        };
-        // A stage that some row of the tile does not see whole, and a chunk that some row of the wave does not (n blocks, holes of their
-        // units).
-        const auto has_edge = [&](uint32_t from, uint32_t n, uint32_t sees, uint32_t holes) { return from + n > end || 32 * (from + n) > sees || holes; };
-        const auto stage_edge = [&](uint32_t i, uint32_t holes) { return has_edge(first + 2 * G * i, 2 * G, clear_tile, holes); };
-        // Takes infinities and NaN out of a stage's values in LDS, once all have landed; `clean` before that, a barrier after it.
-        const auto clean = [&](uint32_t i) {
-            if (threadIdx.x % 256 < 2) lds_bad[i & 1][group][threadIdx.x % 256] = 0;
-        };
-        const auto take_out_all = [&](uint32_t i, uint32_t from) {
-            // a thread a 16-byte piece of each KB that its wave brought: all of unit `wave`, slots 8 a + 4 h + j
-            u32x4 words = {};
+        for (int m = 0; m < kLook; ++m) vf[m] = value(from, m);
+        static_for<kProducts>([&](auto at) {
+            constexpr int m = at;
+            o[m % NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vf[m % kLook]), __builtin_bit_cast(bf16x8_t, pf[m / NS]),
+                                                                o[m % NS], 0, 0, 0);
+            if constexpr (m + kLook < kProducts) vf[m % kLook] = value(from, m + kLook);
+            also(at);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // A stage that some row of the tile does not see whole, and a chunk that some row of the wave does not (n blocks, holes of their
+    // units).
+    const auto has_edge = [&](uint32_t from, uint32_t n, uint32_t sees, uint32_t holes) { return from + n > end || 32 * (from + n) > sees || holes; };
+    const auto stage_edge = [&](uint32_t i, uint32_t holes) { return has_edge(first + 2 * G * i, 2 * G, clear_tile, holes); };
+    // Takes infinities and NaN out of a stage's values in LDS, once all have landed; `clean` before that, a barrier after it.
+    const auto clean = [&](uint32_t i) {
+        if (threadIdx.x % 256 < 2) lds_bad[i & 1][group][threadIdx.x % 256] = 0;
+    };
+    const auto take_out_all = [&](uint32_t i, uint32_t from) {
+        // a thread a 16-byte piece of each KB that its wave brought: all of unit `wave`, slots 8 a + 4 h + j
+        u32x4 words = {};
 #pragma unroll
-            for (int d = 0; d < NS; ++d) {
-                u32x4 *v = reinterpret_cast<u32x4 *>(lds + kKind + from + group * kChunk + wave * kUnit + kPiece * d) + lane;
-                u32x4 x = *v;
-                words |= take_out(x);
-                *v = x;
-            }
-            const uint32_t bad = bad_slots(words) << (16 * (wave & 1) + 4 * h);
-            if (bad) atomicOr(&lds_bad[i & 1][group][wave >> 1], bad);
-        };
-        // ... and gives them to the rows that see them; seen_by: the chunk's slots that the row sees.
-        const auto put_back_all = [&](uint32_t i, const uint32_t (&seen_by)[2]) {
+        for (int d = 0; d < NS; ++d) {
+            u32x4 *v = reinterpret_cast<u32x4 *>(lds + kKind + from + group * kChunk + wave * kUnit + kPiece * d) + lane;
+            u32x4 x = *v;
+            words |= take_out(x);
+            *v = x;
+        }
+        const uint32_t bad = bad_slots(words) << (16 * (wave & 1) + 4 * h);
+        if (bad) atomicOr(&lds_bad[i & 1][group][wave >> 1], bad);
+    };
+    // ... and gives them to the rows that see them; seen_by: the chunk's slots that the row sees.
+    const auto put_back_all = [&](uint32_t i, const uint32_t (&seen_by)[2]) {
 #pragma unroll 1
-            for (uint32_t y = 0; y < 2; ++y) {
-                const uint32_t sees = y ? seen_by[1] : seen_by[0];
-                uint32_t rest = lds_bad[i & 1][group][y];
-                if (rest) rest &= wave_or(sees);  // (what no row sees is left out)
-                for (rest = __builtin_amdgcn_readfirstlane(rest); rest; rest &= rest - 1) {
-                    const uint32_t slot = (uint32_t)__builtin_ctz(rest), unit = 2 * (block_of(i) + y) + slot / 16;
-                    const uint16_t *v = a.c.v + unit_at(a.c, page_of(a.c, b, unit), head, unit) + paged_value_at(slot % 16, 4 * h);
+        for (uint32_t y = 0; y < 2; ++y) {
+            const uint32_t sees = y ? seen_by[1] : seen_by[0];
+            uint32_t rest = lds_bad[i & 1][group][y];
+            if (rest) rest &= wave_or(sees);  // (what no row sees is left out)
+            for (rest = __builtin_amdgcn_readfirstlane(rest); rest; rest &= rest - 1) {
+                const uint32_t slot = (uint32_t)__builtin_ctz(rest), unit = 2 * (block_of(i) + y) + slot / 16;
+                const uint16_t *v = a.c.v + unit_at(a.c, page_of(a.c, b, unit), head, unit) + paged_value_at(slot % 16, 4 * h);
 #pragma unroll
-                    for (int d = 0; d < NS; ++d) {
+                for (int d = 0; d < NS; ++d) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) o[d][x] = put_back(o[d][x], v[512 * d + 8 * (8 * (x >> 2) + (x & 3))], sees >> slot & 1);
-                        __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
-                    }
+                    for (int x = 0; x < 16; ++x) o[d][x] = put_back(o[d][x], v[512 * d + 8 * (8 * (x >> 2) + (x & 3))], sees >> slot & 1);
+                    __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers)
                 }
             }
-        };
-        // Of the next stage's scores: slots that a row does not see get -infinity.
-        const auto hide = [&](uint32_t i, uint32_t holes) {
-            const uint32_t n = block_of(i);
-            holes = holes >> (4 * group) & 15;
-            seen[0] = seen[1] = kAll;
-            if (!has_edge(n, 2, clear, holes)) return;
-            static_for<2>([&](auto at) {
-                constexpr uint32_t k = at;
-                f32x16 &y = k ? p[0] : p[1];
-                const uint32_t none = (holes >> (2 * k) & 1 ? 0xFFFFu : 0u) | (holes >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
-                seen[k] = n + k < end ? sight.bits(32 * (n + k)) & ~none : 0u;
+        }
+    };
+    // Of the next stage's scores: slots that a row does not see get -infinity.
+    const auto hide = [&](uint32_t i, uint32_t holes) {
+        const uint32_t n = block_of(i);
+        holes = holes >> (4 * group) & 15;
+        seen[0] = seen[1] = kAll;
+        if (!has_edge(n, 2, clear, holes)) return;
+        static_for<2>([&](auto at) {
+            constexpr uint32_t k = at;
+            f32x16 &y = k ? p[0] : p[1];
+            const uint32_t none = (holes >> (2 * k) & 1 ? 0xFFFFu : 0u) | (holes >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
+            seen[k] = n + k < end ? sight.bits(32 * (n + k)) & ~none : 0u;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) y[x] = seen[k] >> (8 * (x >> 2) + 4 * h + (x & 3)) & 1 ? y[x] : -INFINITY;
-            });
-        };
-        // Their maximum, in eight steps of two; the row's base follows where it is passed.
-        float top[2];
-        const auto highest = [&](int k) {
-            if (k == 0) top[0] = top[1] = -INFINITY;
+            for (int x = 0; x < 16; ++x) y[x] = seen[k] >> (8 * (x >> 2) + 4 * h + (x & 3)) & 1 ? y[x] : -INFINITY;
+        });
+    };
+    // Their maximum, in eight steps of two; the row's base follows where it is passed.
+    float top[2];
+    const auto highest = [&](int k) {
+        if (k == 0) top[0] = top[1] = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) top[x] = fmaxf(fmaxf(top[x], p[x][2 * k]), p[x][2 * k + 1]);
-        };
-        const auto follow = [&] {
-            float m = fmaxf(top[0], top[1]) * c;
-            m = fmaxf(m, xchg32(m, lane));
-            if (seen[0] | seen[1]) m = fmaxf(m, kLowBase);
-            if (__any(m > sums.base + kLag)) {
-                const float down = row_follow(sums, m);
-                s0 *= down;
-                s1 *= down;
+        for (int x = 0; x < 2; ++x) top[x] = fmaxf(fmaxf(top[x], p[x][2 * k]), p[x][2 * k + 1]);
+    };
+    const auto follow = [&] {
+        float m = fmaxf(top[0], top[1]) * c;
+        m = fmaxf(m, xchg32(m, lane));
+        if (seen[0] | seen[1]) m = fmaxf(m, kLowBase);
+        if (__any(m > sums.base + kLag)) {
+            const float down = row_follow(sums, m);
+            s0 *= down;
+            s1 *= down;
 #pragma unroll
-                for (int d = 0; d < NS; ++d) o[d] *= down;
-            }
-        };
-        if (stages) {
-            // The loop of a wave: next scores beside exponentials, values' products beside the next maxima.  Of a SIMD's two waves the
-            // second group's is half a stage ahead: one is at the exponentials, which take the vector unit longer than the matrix
-            // cores take the products beside them, while the other one's products want little else.  Its keys come a stage earlier.
-            constexpr uint32_t kOfStage = 4 * G;
-            const auto unit_of = [&](uint32_t i) { return units.at(kOfStage * i + 4 * group + wave); };
-            const auto holes_of = [&](uint32_t i) { return units.holes(kOfStage * i, kOfStage); };
-            const auto next_scores = [&](uint32_t from, auto &&also) {
-                scores(from, [&](auto at) {
-                    constexpr int m = at;
-                    static_for<16 * (m + 1) / kProducts - 16 * m / kProducts>([&](auto x) {
-                        constexpr int k = 16 * m / kProducts + x;
-                        exponent(k);
-                        if constexpr (k > 0) round(k - 1);
-                    });
-                    also(at);
-                });
-                round(15);
-                p[1] = z;
-            };
-            // keys of stages 0 and 1, values of 0
-            uint32_t u0 = unit_of(0), u1 = unit_of(1), u2 = unit_of(2), h0 = holes_of(0), h1 = holes_of(1), h2 = holes_of(2);
-            all_of(request(0, u0, 0));
-            all_of(request(1, u0, 0));
-            all_of(request(0, u1, kStage));  // (past the last stage: a unit that nothing reads)
-            bool edge = stage_edge(0, h0);
-            if (edge) clean(0);
-            landed<0>();
-            __syncthreads();
-            scores(0, [](auto) {});
-            p[1] = z;
-            hide(0, h0);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) highest(k);
-            follow();
-            if constexpr (G == 2) {
-                __syncthreads();  // keys 0 have been read
-                if (group == 1) {
-                    all_of(request(0, u2, 0));
-                    next_scores(kStage, [](auto) {});
-                }
-            }
-            uint32_t now = 0;  // the buffers of stage i
-            for (uint32_t i = 0; i + 1 < stages; ++i) {
-                // what this stage reads has landed, and what is overwritten has been read
-                landed<0>();
-                __syncthreads();
-                if (edge) {
-                    take_out_all(i, now);
-                    __syncthreads();
-                }
-                const uint32_t other = now ^ kStage;
-                units.enter(kOfStage * (i + 3));
-                const uint32_t u3 = unit_of(i + 3), h3 = holes_of(i + 3);
-                const Request values = request(1, u1, other), keys = group ? request(0, u3, other) : request(0, u2, now);
-                // a KB for the stages after with every few products
-                if (group == 0) {
-                    next_scores(other, [&](auto at) {
-                        if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
-                    });
-                }
-                const uint32_t seen_now[2] = {seen[0], seen[1]};
-                hide(i + 1, h1);
-                average(now, [&](auto at) {
-                    constexpr int m = at;
-                    static_for<8 * (m + 1) / kProducts - 8 * m / kProducts>([&](auto x) { highest(8 * m / kProducts + x); });
-                    if constexpr (m % 4 == 1) to_lds<m / 4>(keys.from, keys.to);
-                });
-                if (edge) put_back_all(i, seen_now);
-                follow();
-                if (G == 2 && group == 1) {
-                    next_scores(now, [&](auto at) {
-                        if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
-                    });
-                }
-                edge = stage_edge(i + 1, h1);
-                if (edge) clean(i + 1);
-                u1 = u2;
-                u2 = u3;
-                h1 = h2;
-                h2 = h3;
-                now = other;
-            }
-            if (group == 0) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
+            for (int d = 0; d < NS; ++d) o[d] *= down;
+        }
+    };
+    if (stages) {
+        // The loop of a wave: next scores beside exponentials, values' products beside the next maxima.  Of a SIMD's two waves the
+        // second group's is half a stage ahead: one is at the exponentials, which take the vector unit longer than the matrix
+        // cores take the products beside them, while the other one's products want little else.  Its keys come a stage earlier.
+        constexpr uint32_t kOfStage = 4 * G;
+        const auto unit_of = [&](uint32_t i) { return units.at(kOfStage * i + 4 * group + wave); };
+        const auto holes_of = [&](uint32_t i) { return units.holes(kOfStage * i, kOfStage); };
+        const auto next_scores = [&](uint32_t from, auto &&also) {
+            scores(from, [&](auto at) {
+                constexpr int m = at;
+                static_for<16 * (m + 1) / kProducts - 16 * m / kProducts>([&](auto x) {
+                    constexpr int k = 16 * m / kProducts + x;
                     exponent(k);
-                    round(k);
-                }
+                    if constexpr (k > 0) round(k - 1);
+                });
+                also(at);
+            });
+            round(15);
+            p[1] = z;
+        };
+        // keys of stages 0 and 1, values of 0
+        uint32_t u0 = unit_of(0), u1 = unit_of(1), u2 = unit_of(2), h0 = holes_of(0), h1 = holes_of(1), h2 = holes_of(2);
+        all_of(request(0, u0, 0));
+        all_of(request(1, u0, 0));
+        all_of(request(0, u1, kStage));  // (past the last stage: a unit that nothing reads)
+        bool edge = stage_edge(0, h0);
+        if (edge) clean(0);
+        landed<0>();
+        __syncthreads();
+        scores(0, [](auto) {});
+        p[1] = z;
+        hide(0, h0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) highest(k);
+        follow();
+        if constexpr (G == 2) {
+            __syncthreads();  // keys 0 have been read
+            if (group == 1) {
+                all_of(request(0, u2, 0));
+                next_scores(kStage, [](auto) {});
             }
+        }
+        uint32_t now = 0;  // the buffers of stage i
+        for (uint32_t i = 0; i + 1 < stages; ++i) {
+            // what this stage reads has landed, and what is overwritten has been read
             landed<0>();
             __syncthreads();
             if (edge) {
-                take_out_all(stages - 1, now);
+                take_out_all(i, now);
                 __syncthreads();
             }
-            average(now, [](auto) {});
-            if (edge) put_back_all(stages - 1, seen);
+            const uint32_t other = now ^ kStage;
+            units.enter(kOfStage * (i + 3));
+            const uint32_t u3 = unit_of(i + 3), h3 = holes_of(i + 3);
+            const Request values = request(1, u1, other), keys = group ? request(0, u3, other) : request(0, u2, now);
+            // a KB for the stages after with every few products
+            if (group == 0) {
+                next_scores(other, [&](auto at) {
+                    if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
+                });
+            }
+            const uint32_t seen_now[2] = {seen[0], seen[1]};
+            hide(i + 1, h1);
+            average(now, [&](auto at) {
+                constexpr int m = at;
+                static_for<8 * (m + 1) / kProducts - 8 * m / kProducts>([&](auto x) { highest(8 * m / kProducts + x); });
+                if constexpr (m % 4 == 1) to_lds<m / 4>(keys.from, keys.to);
+            });
+            if (edge) put_back_all(i, seen_now);
+            follow();
+            if (G == 2 && group == 1) {
+                next_scores(now, [&](auto at) {
+                    if constexpr (at % 4 == 1) to_lds<at / 4>(values.from, values.to);
+                });
+            }
+            edge = stage_edge(i + 1, h1);
+            if (edge) clean(i + 1);
+            u1 = u2;
+            u2 = u3;
+            h1 = h2;
+            h2 = h3;
+            now = other;
         }
-        sums.l = s0 + s1;
-        float l = sums.l + xchg32(sums.l, lane);
-        if constexpr (G == 2) {  // the second group's sums join the first's
-            __syncthreads();
-                f32x4 *other = reinterpret_cast<f32x4 *>(lds) + wave * (4 * NS * 64) + lane;
-            if (group == 1) {
-                if (h == 0) lds_ml[wave][r32] = make_float2(sums.base, l);
+        if (group == 0) {
 #pragma unroll
-                for (int d = 0; d < NS; ++d)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) other[(4 * d + x) * 64] = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+            for (int k = 0; k < 16; ++k) {
+                exponent(k);
+                round(k);
             }
-            __syncthreads();
-            if (group == 1) continue;
-            const float2 ml = lds_ml[wave][r32];
-            const float base = fmaxf(sums.base, ml.x), f0 = __builtin_amdgcn_exp2f(sums.base - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
-            sums.base = base;
-            l = l * f0 + ml.y * f1;
-#pragma unroll
-            for (int d = 0; d < NS; ++d)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const f32x4 y = other[(4 * d + x) * 64];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) o[d][4 * x + k] = fmaf(o[d][4 * x + k], f0, y[k] * f1);
-                }
         }
-        const float norm = l == 0.0f ? 0.0f : 1.0f / l;
-        const bool nan = l == 0.0f && sums.base > kSeenBase;  // saw slots, all with scores of -infinity
-#pragma unroll
-        for (int d = 0; d < NS; ++d) o[d] *= norm;
-        if (!live) {  // (a row past the sequence's)
-        } else if (whole) {
-            if (nan) {
-#pragma unroll
-                for (int d = 0; d < NS; ++d)
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) o[d][x] = __builtin_nanf("");
-            }
-            const size_t to = (size_t)t * a.q_heads + qh;
-            if (a.lse && h == 0) a.lse[to] = l == 0.0f ? (nan ? __builtin_nanf("") : -INFINITY) : (sums.base + __log2f(l)) * kLn2;
-            uint16_t *out = a.out + to * D;
-#pragma unroll
-            for (int d = 0; d < NS; ++d)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * x + 4 * h) = pack4(o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]);
-        } else {
-            const size_t to = part_at(a, split, 2 * idx + odd, head, r - r0);
+        landed<0>();
+        __syncthreads();
+        if (edge) {
+            take_out_all(stages - 1, now);
+            __syncthreads();
+        }
+        average(now, [](auto) {});
+        if (edge) put_back_all(stages - 1, seen);
+    }
+    sums.l = s0 + s1;
+    float l = sums.l + xchg32(sums.l, lane);
+    if constexpr (G == 2) {  // the second group's sums join the first's
+        __syncthreads();
+            f32x4 *other = reinterpret_cast<f32x4 *>(lds) + wave * (4 * NS * 64) + lane;
+        if (group == 1) {
+            if (h == 0) lds_ml[wave][r32] = make_float2(sums.base, l);
 #pragma unroll
             for (int d = 0; d < NS; ++d)
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    *reinterpret_cast<f32x4 *>(a.part + to * D + 32 * d + 8 * x + 4 * h) =
-                        f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
-            if (h == 0) {
-                float *ml = a.part + (size_t)slots * a.c.heads * kManyRows * D + 2 * to;
-                ml[0] = sums.base;
-                ml[1] = l;
+                for (int x = 0; x < 4; ++x) other[(4 * d + x) * 64] = f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+        }
+        __syncthreads();
+        if (group == 1) return;
+        const float2 ml = lds_ml[wave][r32];
+        const float base = fmaxf(sums.base, ml.x), f0 = __builtin_amdgcn_exp2f(sums.base - base), f1 = __builtin_amdgcn_exp2f(ml.x - base);
+        sums.base = base;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const f32x4 y = other[(4 * d + x) * 64];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[d][4 * x + k] = fmaf(o[d][4 * x + k], f0, y[k] * f1);
             }
+    }
+    const float norm = l == 0.0f ? 0.0f : 1.0f / l;
+    const bool nan = l == 0.0f && sums.base > kSeenBase;  // saw slots, all with scores of -infinity
+#pragma unroll
+    for (int d = 0; d < NS; ++d) o[d] *= norm;
+    if (!live) {  // (a row past the sequence's)
+    } else if (whole) {
+        if (nan) {
+#pragma unroll
+            for (int d = 0; d < NS; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[d][x] = __builtin_nanf("");
+        }
+        const size_t to = (size_t)t * a.q_heads + qh;
+        if (a.lse && h == 0) a.lse[to] = l == 0.0f ? (nan ? __builtin_nanf("") : -INFINITY) : (sums.base + __log2f(l)) * kLn2;
+        uint16_t *out = a.out + to * D;
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<u32x2 *>(out + 32 * d + 8 * x + 4 * h) = pack4(o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]);
+    } else {
+        const size_t to = part_at(a, split, idx, head, r - r0);
+#pragma unroll
+        for (int d = 0; d < NS; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                *reinterpret_cast<f32x4 *>(a.part + to * D + 32 * d + 8 * x + 4 * h) =
+                    f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+        if (h == 0) {
+            float *ml = a.part + (size_t)slots * a.c.heads * kManyRows * D + 2 * to;
+            ml[0] = sums.base;
+            ml[1] = l;
         }
     }
 }
@@ -589,7 +580,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
     const uint32_t lane = __lane_id(), r16 = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t head = blockIdx.y, idx = blockIdx.x;
     Work w;
-    if (!find_work(a, split, idx, w)) return;
+    if (!find_work<Parts::even>(a, split, idx, w)) return;
     const Span &s = w.s;
     const uint32_t r0 = kFewRows * w.tile, r = r0 + r16;
     const bool live = r < w.rows;
@@ -747,26 +738,29 @@ struct AttnPlan {
 };
 AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     AttnPlan p{};
-    p.few = (uint64_t)tokens * group <= (D <= 128 ? 48ull : 32ull) * batch;
+    const uint64_t rows = (uint64_t)tokens * group;
+    p.few = rows <= 16ull * batch || rows * kv_heads * max_ctx <= 3u << 19;
     p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
-    p.tiles = (uint32_t)((uint64_t)tokens * group / p.split.rows) + std::min(batch, tokens);
+    p.tiles = (uint32_t)(rows / p.split.rows) + std::min(batch, tokens);
     if (p.few) {
         p.split.unit = kFewWaves;
-        // as many workgroups as the card holds at once, less the half part that a tile has more than its share on average
+        // as many workgroups as the card holds at once, or where the tiles are as many already, twice that
         const uint32_t held = (D <= 64 ? 768 : (D <= 128 ? 512 : 256)) / kv_heads;
-        p.split.target = std::max(std::max(held - std::min(held, p.tiles / 2), held / 2), std::min(p.tiles, 1024u));
-        p.slots = p.grid = p.split.target + p.tiles;
+        p.split.target = p.tiles < held ? held : std::max(2 * held, std::min(p.tiles, 1024u));
+        p.slots = p.grid = std::max(p.split.target, p.tiles);
     } else {
-        // as many workgroups as the card holds at once
-        p.split.unit = 1;
-        const bool split = (uint64_t)p.tiles * kv_heads < 256 && (uint64_t)p.tiles * ((max_ctx + 31) / 32) < 1ull << 31;
-        p.split.target = split ? 256 * p.split.unit / kv_heads : 0;  // at least `tiles`
+        p.split.unit = D <= 128 ? 4 : 2;  // a stage
+        const uint32_t longest = (max_ctx + 31) / 32;
+        const bool split = (uint64_t)p.tiles * kv_heads < 256 && longest > 4096 / D;
+        p.split.target = split ? 256 / kv_heads : 0;  // as many workgroups as the card holds at once: at least `tiles`
         p.grid = p.split.target ? p.split.target : p.tiles;
-        p.slots = 2 * p.split.target;
+        p.slots = p.split.target;
     }
     return p;
 }
+
+size_t part_floats(const AttnPlan &p, uint32_t kv_heads, uint32_t D) { return (size_t)p.slots * kv_heads * p.split.rows * (D + 2); }
 
 }  // namespace
 
@@ -777,11 +771,13 @@ uint64_t paged_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t grou
 
 size_t paged_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens, max_ctx);
-    return (size_t)p.slots * kv_heads * p.split.rows * (D + 2) * sizeof(float);
+    return p.slots ? part_floats(p, kv_heads, D) * sizeof(float) + 16 : 0;
 }
 
-hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
+hipError_t launch_paged_attention(const PagedAttnArgs &args, hipStream_t s) {
+    PagedAttnArgs a = args;
     const AttnPlan p = plan_of(a.c.batch, a.c.heads, a.group, a.c.D, a.step.tokens, a.c.max_ctx);
+    a.per = reinterpret_cast<uint32_t *>(a.part + part_floats(p, a.c.heads, a.c.D));
     const auto launch = [&](auto ns) -> hipError_t {
         constexpr int NS = decltype(ns)::value;
         if (p.few) paged_few_kernel<NS><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
@@ -789,13 +785,13 @@ hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s) {
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;
         if (p.few && (uint64_t)p.tiles * p.split.rows * a.c.heads <= 256) {
-            attn_join_kernel<PagedAttnArgs, NS, false, true, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
+            attn_join_kernel<PagedAttnArgs, NS, Parts::even, true, true><<<dim3(p.tiles * p.split.rows, a.c.heads), kJoinThreads, 0, s>>>(a, p.split, p.slots, 1);
         } else {
             uint32_t per_group = kJoinRowThreads / 64;
             while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 2048) per_group *= 2;
             const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
-            if (p.few) attn_join_kernel<PagedAttnArgs, NS, false, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
-            else attn_join_kernel<PagedAttnArgs, NS, true, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            if (p.few) attn_join_kernel<PagedAttnArgs, NS, Parts::even, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            else attn_join_kernel<PagedAttnArgs, NS, Parts::even, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     };

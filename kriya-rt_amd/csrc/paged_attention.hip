@@ -646,8 +646,13 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             sum += e[i];
         }
         sums.l += sum;
-        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, u32x4{pack_bf16_rne(e[0], e[1]), pack_bf16_rne(e[2], e[3]), pack_bf16_rne(e[4], e[5]),
-                                                               pack_bf16_rne(e[6], e[7])});
+        // in two bf16 each, the second what the first leaves: to 2^-17 of them (one alone is off by as much as the result's own rounding)
+        u32x4 high, low;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            high[i] = pack_bf16_rne(e[2 * i], e[2 * i + 1]);
+            low[i] = pack_bf16_rne(e[2 * i] - __uint_as_float(high[i] << 16), e[2 * i + 1] - __uint_as_float(high[i] & 0xFFFF0000u));
+        }
         uint32_t bad = 0;
         if (edge) {
             u32x4 words = {};
@@ -656,8 +661,10 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             bad = bad_slots(words) << (16 * (g >> 1) + 4 * (g & 1));
         }
 #pragma unroll
-        for (int d = 0; d < 2 * NS; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f.v[d >> 1][d & 1]), pf, o[d], 0, 0, 0);
+        for (int d = 0; d < 2 * NS; ++d) {
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f.v[d >> 1][d & 1]), __builtin_bit_cast(bf16x8_t, high), o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f.v[d >> 1][d & 1]), __builtin_bit_cast(bf16x8_t, low), o[d], 0, 0, 0);
+        }
         if (edge && __any(bad)) {
             for (uint32_t left = wave_or(bad) & wave_or(seen); left; left &= left - 1) {  // (what no row sees is left out)
                 const uint32_t slot = (uint32_t)__builtin_ctz(left), page = page_of(a.c, b, 2 * blk + slot / 16);

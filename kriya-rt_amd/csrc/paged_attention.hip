@@ -69,35 +69,34 @@ __device__ __forceinline__ uint32_t clear_of(const PagedAttnArgs &a, const Span 
     return a.mask ? min(s.n > s.m ? s.n - s.m : 0u, a.c.max_ctx) : row_limit(s, r0, a.group, a.c.max_ctx);
 }
 
-// Where a wave's units lie, in the order in which it asks for them, 64 at a time and the next 64 on their way: lane l of a set holds
-// the place, in units from the pool's start, of the l-th (a unit of no page: the first of the pool, and its bit in `holes`).
+// Where a wave's units lie, in the order in which it asks for them, 64 at a time and the next 64's pages on their way: lane l holds
+// the place, in units from the pool's start, of a set's l-th (a unit of no page: the first of the pool, and its bit in `holes`).
 template <class F>
 struct Units {
-    F page;  // of the i-th unit
+    F unit;  // the sequence's unit that is the i-th
     const Paged &c;
-    uint32_t head;
-    struct Set {
-        uint32_t at;
-        unsigned long long holes;
-    } now, next;
-    __device__ __forceinline__ Set load(uint32_t set) const {
-        uint32_t unit;
-        const uint32_t p = page(64 * set + __lane_id(), unit);
+    uint32_t b, head, at_lane, ahead[2];
+    unsigned long long holes_now;
+    __device__ __forceinline__ uint32_t look(uint32_t set) const { return page_of(c, b, unit(64 * set + __lane_id())); }
+    __device__ __forceinline__ void take(uint32_t set, uint32_t p) {
         const bool hole = p >= c.pages;
-        return Set{hole ? 0u : unit_place(c, p, head, unit), __ballot(hole)};
+        at_lane = hole ? 0u : unit_place(c, p, head, unit(64 * set + __lane_id()));
+        holes_now = __ballot(hole);
     }
-    __device__ __forceinline__ Units(F f, const Paged &c, uint32_t head) : page(f), c(c), head(head) {
-        now = load(0);
-        next = load(1);
+    __device__ __forceinline__ Units(F f, const Paged &c, uint32_t b, uint32_t head) : unit(f), c(c), b(b), head(head) {
+        ahead[0] = look(0);
+        ahead[1] = look(1);
     }
+    // before the first use: what is loaded between has the pages' way to come as well
+    __device__ __forceinline__ void begin() { take(0, ahead[0]); }
     // of the i-th unit; units in rising order, each set entered at its first
-    __device__ __forceinline__ uint32_t at(uint32_t i) const { return (uint32_t)__builtin_amdgcn_readlane((int)now.at, (int)(i & 63)); }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return (uint32_t)__builtin_amdgcn_readlane((int)at_lane, (int)(i & 63)); }
     // whether the n units from i on have no page, as bits
-    __device__ __forceinline__ uint32_t holes(uint32_t i, uint32_t n) const { return (uint32_t)(now.holes >> (i & 63)) & ((1u << n) - 1); }
+    __device__ __forceinline__ uint32_t holes(uint32_t i, uint32_t n) const { return (uint32_t)(holes_now >> (i & 63)) & ((1u << n) - 1); }
     __device__ __forceinline__ void enter(uint32_t i) {
         if ((i & 63) == 0 && i) {
-            now = next;
-            next = load(i / 64 + 1);
+            take(i / 64, ahead[1]);
+            ahead[1] = look(i / 64 + 1);
         }
     }
 };
@@ -220,9 +219,6 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
     const Sight sight = sight_of(a, s, r, live);
     const uint32_t clear = r0 + 32 * wave < w.rows ? clear_of(a, s, r0 + 32 * wave) : kAll;  // (of rows past the end nothing counts)
     const uint32_t b = w.b, t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
-    bf16x8_t q[2 * NS];
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) q[i] = query_unit(a.q + t * a.q_stride + (size_t)qh * D + 16 * i + 8 * h, live, sign);
     f32x16 o[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) o[i] = f32x16{};
@@ -230,7 +226,14 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
     // stage i: blocks first + 2 G i ..; the group's own two from block_of(i) on
     const uint32_t stages = first < end ? (end - first + 2 * G - 1) / (2 * G) : 0;
     const auto block_of = [&](uint32_t i) { return first + 2 * (G * i + group); };
-    Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * first + i); }, a.c, head);
+    Units units([&](uint32_t i) { return 2 * first + i; }, a.c, b, head);
+    // (a row past the sequence's takes the tile's first one's query; nothing of it is written)
+    const uint32_t rq = live ? r : r0;
+    const uint16_t *query = a.q + (s.t0 + rq / a.group) * a.q_stride + (size_t)(head * a.group + rq % a.group) * D + 8 * h;
+    bf16x8_t q[2 * NS];
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) q[i] = *reinterpret_cast<const bf16x8_t *>(query + 16 * i);
+    units.begin();
     const uint32_t clear_tile = clear_of(a, s, r0);
     // A wave brings one of the four units, its keys or its values, into LDS, NS pieces: `unit` where it lies in the pool.
     struct Request {
@@ -400,6 +403,8 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
         if (edge) clean(0);
         landed<0>();
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) q[i] = __builtin_bit_cast(bf16x8_t, __builtin_bit_cast(u32x4, q[i]) ^ u32x4{sign, sign, sign, sign});
         scores(0, [](auto) {});
         p[1] = z;
         hide(0, h0);
@@ -593,7 +598,8 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
     constexpr uint32_t kAhead = kFewAhead<NS>;
     FewBlock<NS> f[kAhead];
     // unit i of the wave: half i % 2 of its i / 2-th block
-    Units units([&](uint32_t i, uint32_t &unit) { return page_of(a.c, b, unit = 2 * (first + wave + kFewWaves * (i / 2)) + i % 2); }, a.c, head);
+    Units units([&](uint32_t i) { return 2 * (first + wave + kFewWaves * (i / 2)) + i % 2; }, a.c, b, head);
+    units.begin();
     uint32_t asked = 0;
     const auto ask = [&](FewBlock<NS> &f) {
         units.enter(asked);

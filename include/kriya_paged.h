@@ -29,7 +29,7 @@ extern "C" {
  * The 16 slots of a unit stand in the order of the matrix instructions' operands (kr_paged_read reads them back):
  *   k [head_dim / 8, 16 slots, 8 dims]
  *   v [head_dim / 32, 2 (h), 32 dims, 2 (a), 4 (j)], slot 8 a + 4 h + j
- * page: 16, 32, 64, .. 4096 (a power of two); head_dim 64, 96, 128, 192 or 256.  No initial contents are needed: what lies in
+ * page: 16, 32, 64, .. 4096 (a power of two); head_dim 64, 96, 128, 192 or 256; pages * kv_heads * page / 16 below 2^32.  No initial contents are needed: what lies in
  * slots without a token is never seen, whatever its bits. */
 typedef struct kr_paged_cache {
     uint16_t *k, *v;
@@ -80,8 +80,9 @@ int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_st
  *   q: bf16 [tokens, q_heads, head_dim], tokens q_stride elements apart (a multiple of 8); out: bf16, contiguous; both 16-byte
  *   aligned and apart from each other; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
  *   be negative or 0).
- * Products are bf16 with sums in f32; the probabilities enter the second product as bf16 (half a step is 2^-8 of each); maxima, sums and
- * joins are f32, for which |scale| sum |q| |K_p| must stay below 2^125.  A row that sees no slot gives zeros and lse = -infinity.
+ * Products are bf16 with sums in f32; the probabilities enter the second product as bf16 (half a step is 2^-8 of each), where rows are
+ * few as two of them (2^-16); maxima, sums and joins are f32, for which |scale| sum |q| |K_p| must stay below 2^125 and finite values
+ * below 2^89.  A row that sees no slot gives zeros and lse = -infinity.
  * Infinities and NaN count in the rows that see them alone: such a row gives what the formula gives, an infinity or NaN.
  * workspace: kr_paged_attention_workspace_bytes(cache, step, q_heads, tokens) bytes (of step only batch and max_pages are
  * read), 16-byte aligned, no initial contents; calls sharing it must not overlap in time.  Results are the same bits from run

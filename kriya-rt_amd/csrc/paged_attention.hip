@@ -9,8 +9,8 @@
 //   s_rp = q_r . k_p,   m_r = max_p c s_rp,   l_r = sum_p 2^(c s_rp - m_r),   out_r = sum_p 2^(c s_rp - m_r) v_p / l_r
 // One pass over the slots: m_r only grows, and sums made under an older one are scaled down.  The exponents are one fused
 // multiply-add from the product's f32 sums, so that large scores cost no more than their own rounding.  Probabilities enter the second
-// product as bf16, as the values are (the matrix cores take f32 at a fraction of the rate, and fp16 cannot hold all values); l_r sums them
-// unrounded, in f32.
+// product as bf16, as the values are (the matrix cores take f32 at a fraction of the rate, and fp16 cannot hold all values), in tiles of
+// few rows, where the matrix cores wait for bytes, as two of them; l_r sums them unrounded, in f32.
 // The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane then holds one query row, its m_r and l_r are plain
 // registers, and after rounding its probabilities are the second product's operand as they lie (paged.hpp: the order of v).
 #include <algorithm>
@@ -162,6 +162,15 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 }  // namespace
 
 // ---- many rows: prompts, chunks, large trees
+//
+// A workgroup takes a tile of 128 query rows, 32 a wave, or one part of its slots, on v_mfma_f32_32x32x16_bf16.  Keys and values go from
+// memory to LDS past the registers, a stage ahead, with one barrier a stage; a wave's O, queries and scores stay in registers.  Bound by
+// the matrix cores, and per tile by its start.  Of a stage's time the products take 90 %: exponentials, maxima and rounding are laid
+// between them (apart they took 198 us for a prompt of 3907, 16/2 heads of 128, beside them 81), and up to D 128 a second group of four
+// waves, over other slots, half a stage apart, uses what the first leaves; above, the registers hold one wave a SIMD.  In the loop 1040
+// TFLOP/s at D 128 and 980 at D 256, where a library product of 8192^3 reaches 1151.  A tile's start and end are 11 us (work, pages,
+// queries and the first stage 6, sums of the groups 1, the next workgroup's launch 4): a prompt of 3907, 16/2 heads of 128, takes 80 us
+// (787 TFLOP/s), 600 tokens over up to 12000 in four sequences, 10/2 heads of 256, 98 and its join 10.
 constexpr uint32_t kManyRows = 128;
 
 // The n-th KB from `from` on into LDS, past the registers: 16 bytes a lane, lane l's to byte lds + 1024 n + 16 l, lds the same in all lanes
@@ -546,6 +555,8 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
 // On v_mfma_f32_16x16x32_bf16, keys and values straight from memory to the operands' registers, 16 bytes a lane in whole cache lines.
 // Tile t of a block's keys is slots 8 t .. 8 t + 7 of both units: a lane (column l & 15, g = l >> 4) then holds after the first product
 // the slots 8 t + 4 (g & 1) + j of unit g >> 1, of both tiles the 8 slots of one 16-byte piece of values.
+// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64, 114 us for 595 MB, one of 131072, 16/2 heads of 128, 26 us for 134 MB, both
+// 5.2 TB/s, as a copy; by latency where there are few: five sequences up to 3000 8.3 us.
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
 template <int NS>
 constexpr uint32_t kFewAhead = NS <= 4 ? 2 : 1;
@@ -752,18 +763,24 @@ struct AttnPlan {
 AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     AttnPlan p{};
     const uint64_t rows = (uint64_t)tokens * group;
+    // Few rows: one tile of 16 a sequence, or all the rows there are over so few slots that their latency counts (us, few and many.
+    // D 128, 2 heads: 16 tokens of 8 rows over 3000 14.9 and 18.4, 8 over 100000 69 and 35, 8 sequences of 8 over 300 12.6 and 16.9, over
+    // 3000 25.7 and 22.0; D 64, 8 heads: 8 sequences of 4 tokens of 4 rows 19.2 and 25.1, 32 of 8 tokens 68 and 41).
     p.few = rows <= 16ull * batch || rows * kv_heads * max_ctx <= 3u << 19;
     p.split.rows = p.few ? kFewRows : kManyRows;
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)(rows / p.split.rows) + std::min(batch, tokens);
     if (p.few) {
         p.split.unit = kFewWaves;
-        // as many workgroups as the card holds at once, or where the tiles are as many already, twice that
+        // as many workgroups as the card holds at once, or where the tiles are as many already, twice that (64 sequences up to 3000,
+        // 32/8 heads of 128, 89 us -> 81; below, a second round costs more: 40 of 4000 119 -> 125)
         const uint32_t held = (D <= 64 ? 768 : (D <= 128 ? 512 : 256)) / kv_heads;
         p.split.target = p.tiles < held ? held : std::max(2 * held, std::min(p.tiles, 1024u));
         p.slots = p.grid = std::max(p.split.target, p.tiles);
     } else {
         p.split.unit = D <= 128 ? 4 : 2;  // a stage
+        // Contexts that a table can hold in so few blocks are not split: the join's launch takes longer (split and whole, us, D 128, 2 heads:
+        // 1000 tokens 30 and 25, 200 over 1000 24 and 27; D 256: 500 tokens 29 and 26, 100 over 800 33 and 39).
         const uint32_t longest = (max_ctx + 31) / 32;
         const bool split = (uint64_t)p.tiles * kv_heads < 256 && longest > 4096 / D;
         p.split.target = split ? 256 / kv_heads : 0;  // as many workgroups as the card holds at once: at least `tiles`

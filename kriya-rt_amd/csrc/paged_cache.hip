@@ -52,6 +52,9 @@ __device__ __forceinline__ Pair pair_of(const RopeArgs &r, uint32_t d) {
 // Keys and queries: row_threads(D) threads a row, each with the two pieces of 8 dims that its rotation pairs (neighbouring ones
 // without), so that norm, rotation and rounding stay in registers; the row's sum of squares goes over its lanes.  kAny pairs dims that
 // lie anywhere: their partners are read one by one.
+// Bound by latency where tokens are few (16 tokens, 2 heads of 128, 16 queries: 4.0 us: lengths, rows and table, pages, stores) and by
+// bytes where they are many (3907 tokens, 8 heads of 64, 32 queries, norm and rotation: 12.6 us for 49 MB, 3.9 TB/s; rows that went
+// through LDS took 39).
 template <uint32_t D, int kRope>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, uint32_t items) {
     constexpr uint32_t kUnits = D / 8, kChunk = chunk_heads(D), kLanes = row_threads(D), kRowsAtOnce = 256 / kLanes;

@@ -32,6 +32,7 @@ __device__ __forceinline__ uint32_t wave_scan_max(uint32_t v) {
 // A workgroup a sequence, a thread a node.  A node's ancestors are found from it upwards, in order of falling place, so its
 // words are complete one after the other and written once.  Nodes whose parent is the node before them form runs: a run's bits are
 // set at once, so that a chain (a prompt given as a tree) takes a few steps and not its length.
+// Bound by latency: one tree of 24 nodes 2.8 us, 64 of up to some hundred 6.1.
 __global__ __launch_bounds__(256) void tree_plan_kernel(const int32_t *parents, RaggedStep step, uint32_t words, uint32_t *mask,
                                                         uint32_t *positions) {
     __shared__ int32_t par[kTreeNodes];
@@ -98,7 +99,10 @@ hipError_t launch_tree_plan(const int32_t *parents, const RaggedStep &step, uint
 // keys or one dim of its values, over the nodes that change places, 64 of the path at a time: path[i] >= i and rising, so the rows of
 // later nodes are never where an earlier one goes, and within eight nodes all are loaded before one is stored.  No thread touches
 // another's column.
-constexpr uint32_t kCommitThreads = 512, kNoNode = 0xFFFFu;
+// Bound by latency (lengths; nodes; the walk, a step of LDS a node; pages; rows) and by lines: a slot's values are 2 of each 16 bytes.
+// 4 sequences, 36 layers of 2 heads of 128: 6 us; 48 of about 60 nodes, 24 layers of 8 heads of 64: 13.7 for 14 MB (512 threads, of
+// which a compute unit holds four workgroups, 14.0; 640 16.3).  One lookup a node and LDS walks took it from 160.
+constexpr uint32_t kCommitThreads = 320, kNoNode = 0xFFFFu;
 __global__ __launch_bounds__(kCommitThreads) void paged_commit_kernel(PagedCommitArgs a) {
     __shared__ uint16_t follows[kTreeNodes], path[kTreeNodes];
     __shared__ uint32_t found, moved;

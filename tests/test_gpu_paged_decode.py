@@ -3,7 +3,7 @@ drafted trees, sequences that end; against a layer-by-layer restatement on the C
 
 Bar: max |gpu - cpu| <= 3e-2 * RMS(cpu) for logits, as for the decoder over the 8-bit cache and for its reasons: both sides round to
 bf16 at the same points, and a value near a tie may round the other way; the probabilities, bf16 here in tiles of many rows, are off
-by up to 2^-9 of a value, half of what one such rounding of the result is.  Two device paths that each keep it differ by at most twice that."""
+by up to 2^-8 of themselves, which moves a result by at most as much as its own rounding does.  Two device paths that each keep it differ by at most twice that."""
 import numpy as np
 import pytest
 import torch

@@ -100,7 +100,8 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
  *
  * The plan: mask (u32 [tokens, words]) gets the bits of a node's ancestors and its own, positions (u32 [tokens]) n - m plus the
  * number of its ancestors: the mask of kr_paged_attention and the positions of kr_rope, for every layer of the step.  starts,
- * lengths as in kr_paged_step.  words 1 .. 128; a sequence's nodes from 32 words on get no bits and position n - m. */
+ * lengths as in kr_paged_step.  words 1 .. 128; a sequence's nodes from 32 words on get no bits and position n - m.  mask and positions lie
+ * apart from each other and from what is read. */
 int kr_tree_plan(const int32_t *parents, uint32_t tokens, const uint32_t *starts, const uint32_t *lengths, uint32_t batch,
                  uint32_t words, uint32_t *mask, uint32_t *positions, void *stream);
 
@@ -110,7 +111,9 @@ int kr_tree_plan(const int32_t *parents, uint32_t tokens, const uint32_t *starts
  *   path        u32 [batch, max_path]: the path's nodes, then zeros
  *   counts      u32 [batch]: its length, 0 for a sequence without new tokens
  *   next        i32 [batch]: the model's choice after its last node: the next step's node 0 (a sequence without new tokens: left)
- *   new_lengths u32 [batch]: n - m + counts; must not be lengths
+ *   new_lengths u32 [batch]: n - m + counts
+ * All four lie apart from one another and from what is read (new_lengths is not lengths).  A node without a slot or a page has no keys
+ * to move: a server gives a step's slots their pages before it.
  * Rows beyond new_lengths keep their bits (nothing sees them).  drafted, parents, targets as far as 4096 nodes a sequence; max_path
  * 1 .. 4096.  One launch for all layers. */
 int kr_paged_commit(const kr_paged_cache *cache, const kr_paged_step *step, const int32_t *drafted, const int32_t *parents,

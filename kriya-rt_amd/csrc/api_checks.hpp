@@ -1,6 +1,8 @@
 // api_checks.hpp — checks that the entry points of the caches share.
 #pragma once
 
+#include <initializer_list>
+
 #include "kriya_kv8.h"
 #include "kr_internal.hpp"
 
@@ -10,6 +12,27 @@ namespace kr {
 constexpr uint64_t kMostGroups = 0xFFFFFFFFull / 256;
 
 inline bool on(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
+
+// Memory of a call: what one argument points to.
+struct Range {
+    const char *name;
+    const void *at;
+    size_t bytes;
+};
+// Written memory must not be that of any other argument.
+inline int check_apart(std::initializer_list<Range> written, std::initializer_list<Range> read) {
+    const auto meet = [](const Range &x, const Range &y) {
+        const auto a = (uintptr_t)x.at, b = (uintptr_t)y.at;
+        return x.at && y.at && a < b + y.bytes && b < a + x.bytes;
+    };
+    for (auto x = written.begin(); x != written.end(); ++x) {
+        for (auto y = written.begin(); y != x; ++y)
+            if (meet(*x, *y)) return fail(KR_E_INVALID, "%s and %s overlap", y->name, x->name);
+        for (const Range &y : read)
+            if (meet(*x, y)) return fail(KR_E_INVALID, "%s overlaps %s", x->name, y.name);
+    }
+    return KR_OK;
+}
 
 inline int check_rope(const kr_rope *r, uint32_t head_dim) {
     if (!r->cos_sin || !r->positions) return fail(KR_E_INVALID, "rope: NULL pointer");

@@ -160,6 +160,11 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
     if (need && (!workspace || workspace_bytes < need))
         return fail(KR_E_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);
     if (!on(workspace, 16)) return fail(KR_E_ALIGN, "workspace must be 16-byte aligned");
+    const size_t rows = (size_t)tokens * q_heads;
+    if (int rc = check_apart({{"out", out, rows * cache->head_dim * 2}, {"lse", lse, rows * 4}, {"workspace", workspace, need}},
+                             {{"q", q, ((tokens - 1) * q_stride + (size_t)q_heads * cache->head_dim) * 2},
+                              {"mask", mask, (size_t)tokens * words * 4}}))
+        return rc;
     PagedAttnArgs a{};
     a.c = c;
     a.step = to_step(step, tokens);
@@ -184,6 +189,9 @@ int kr_tree_plan(const int32_t *parents, uint32_t tokens, const uint32_t *starts
     if (int rc = check_sequences(starts, lengths, batch, tokens)) return rc;
     if (!parents || !mask || !positions) return fail(KR_E_INVALID, "parents, mask and positions must not be NULL");
     if (!on(parents, 4) || !on(mask, 4) || !on(positions, 4)) return fail(KR_E_ALIGN, "parents, mask and positions must be 4-byte aligned");
+    if (int rc = check_apart({{"mask", mask, (size_t)tokens * words * 4}, {"positions", positions, (size_t)tokens * 4}},
+                             {{"parents", parents, (size_t)tokens * 4}, {"starts", starts, ((size_t)batch + 1) * 4}, {"lengths", lengths, (size_t)batch * 4}}))
+        return rc;
     return hip_status(launch_tree_plan(parents, RaggedStep{starts, lengths, batch, tokens}, words, mask, positions, (hipStream_t)stream),
                       "kr_tree_plan");
 }
@@ -200,7 +208,12 @@ int kr_paged_commit(const kr_paged_cache *cache, const kr_paged_step *step, cons
         return fail(KR_E_INVALID, "NULL pointer");
     if (!on(drafted, 4) || !on(parents, 4) || !on(targets, 4) || !on(path, 4) || !on(counts, 4) || !on(next, 4) || !on(new_lengths, 4))
         return fail(KR_E_ALIGN, "tokens, path, counts, next and new_lengths must be 4-byte aligned");
-    if (new_lengths == step->lengths) return fail(KR_E_INVALID, "new_lengths must not be lengths");
+    // (every layer's workgroups read what the first one's write)
+    const size_t all = (size_t)tokens * 4, each = (size_t)step->batch * 4;
+    if (int rc = check_apart({{"path", path, each * max_path}, {"counts", counts, each}, {"next", next, each}, {"new_lengths", new_lengths, each}},
+                             {{"tokens", drafted, all}, {"parents", parents, all}, {"targets", targets, all}, {"lengths", step->lengths, each},
+                              {"starts", step->starts, each + 4}, {"table", step->table, each * step->max_pages}}))
+        return rc;
     PagedCommitArgs a{};
     a.c = to_paged(cache, 0, step);
     a.layers = cache->layers;

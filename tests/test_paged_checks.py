@@ -148,6 +148,25 @@ def test_plan_and_commit_refusals(kq):
     assert _commit(L, c, s, lengths=0x40000) == kq.KR_E_INVALID  # the step's own
 
 
+def test_written_memory_lies_apart(kq):
+    """Outputs over inputs or one another: refused, by whole ranges (2 sequences, 2 tokens of 4 heads of 64)."""
+    L = kq.lib()
+    cache, step = ctypes.byref(_cache()), ctypes.byref(_step())
+    for change in (dict(out=X), dict(out=X + 1008), dict(out=X - 1008), dict(lse=X + 1020), dict(lse=0xA0000 + 1020), dict(ws=X - 16),
+                   dict(ws=0xB0000), dict(mask=0xA0000 + 1020, words=1), dict(mask=0xB0000, words=2)):
+        assert _attend(L, cache, step, **change) == kq.KR_E_INVALID, change
+    apart = dict(drafted=0x80000, parents=0x81000, targets=0x82000, path=0x83000, counts=0x84000, nxt=0x85000, lengths=0x86000)
+    for name, size in (("path", 32), ("counts", 8), ("nxt", 8), ("lengths", 8)):
+        for at in (0x80000, 0x81004, 0x82000, 0x40000, 0x30000 + 44):  # the inputs, the step's lengths, the table's last
+            assert _commit(L, cache, step, **dict(apart, **{name: at})) == kq.KR_E_INVALID, (name, hex(at))
+        for other in apart:
+            if other != name:
+                assert _commit(L, cache, step, **dict(apart, **{other: apart[name] + size - 4})) == kq.KR_E_INVALID, (name, other)
+    plan = lambda mask, positions: L.kr_tree_plan(0x80000, 10, 0x81000, 0x82000, 2, 2, mask, positions, None)  # noqa: E731
+    for mask, positions in ((0x80000, 0x90000), (0x90000, 0x80000 + 36), (0x90000, 0x90000 + 76), (0x81000 + 8, 0x90000), (0x90000, 0x82004)):
+        assert plan(mask, positions) == kq.KR_E_INVALID
+
+
 def test_workspace_is_bounded(kq):
     L = kq.lib()
     assert L.kr_paged_attention_workspace_bytes(None, ctypes.byref(_step()), 4, 2) == 0

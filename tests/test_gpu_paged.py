@@ -31,14 +31,30 @@ def _rand(g, *shape, gain=1.0):
     return (torch.randn(*shape, generator=g) * gain).to(BF)
 
 
-def _table(lens, page, seed=0, spare=2, extra=1):
+COLUMNS = 1  # of a table behind its longest sequence's pages
+
+
+@pytest.fixture(params=[1, 6000], ids=["narrow", "wide"])
+def table_of(request):
+    """The launch is planned by what a table could hold: in a wide one, many rows take tiles of 128 and may be split; in a narrow one
+    short contexts take tiles of 16, or whole ones of 128."""
+    global COLUMNS
+    COLUMNS = request.param
+    yield
+    COLUMNS = 1
+
+
+wide_and_narrow = pytest.mark.usefixtures("table_of")
+
+
+def _table(lens, page, seed=0, spare=2):
     """Scattered pages for sequences of these lengths: (table rows, pages of the pool)."""
     each = [-(-n // page) for n in lens]
     order = list(range(sum(each) + spare))
     random.Random(seed).shuffle(order)
     rows, at = [], 0
     for n in each:
-        rows.append(order[at: at + n] + [-1] * (max(each) - n + extra))
+        rows.append(order[at: at + n] + [-1] * (max(each) - n + COLUMNS))
         at += n
     return rows, len(order)
 
@@ -203,6 +219,7 @@ def test_append_without_starts_cuts_off_and_skips_missing_pages(paged):
 
 # ---- attention
 
+@wide_and_narrow
 @pytest.mark.parametrize("page", [16, 128])
 @pytest.mark.parametrize("d,kv,group", [(64, 2, 1), (96, 1, 8), (128, 2, 8), (128, 1, 3), (192, 2, 5), (256, 1, 17), (64, 1, 40)])
 def test_attention_one_token_each(paged, d, kv, group, page):
@@ -210,6 +227,7 @@ def test_attention_one_token_each(paged, d, kv, group, page):
     _check(f, paged, _rand(torch.Generator().manual_seed(2), 6, kv * group, d, gain=1.5), None)
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("d,kv,group,counts,lens,page", [
     (64, 2, 4, [40, 0, 1, 200], [40, 9, 500, 333], 16), (128, 1, 8, [130, 33, 1], [130, 900, 64], 32), (96, 3, 2, [65, 64], [65, 1000], 16),
     (192, 1, 6, [50, 3, 70], [51, 3, 400], 64), (256, 2, 5, [40, 90, 1, 0], [700, 90, 1000, 0], 16), (128, 2, 8, [17], [31], 16)])
@@ -218,6 +236,7 @@ def test_attention_ragged_chunks(paged, d, kv, group, counts, lens, page):
     _check(f, paged, _rand(torch.Generator().manual_seed(3), sum(counts), kv * group, d, gain=1.5), counts)
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("d,kv,group,lens", [(128, 2, 8, [700]), (64, 1, 4, [1300, 20]), (256, 1, 2, [300])])
 def test_attention_whole_prompts(paged, d, kv, group, lens):
     f = Filled(paged, lens, kv, d, 16, seed=d)
@@ -237,6 +256,7 @@ def _masks(rng, counts, words, kind):
     return rows
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("kind", ["tree", "any", "none"])
 @pytest.mark.parametrize("d,kv,group,counts,lens,words", [
     (128, 2, 8, [1, 5, 30], [1, 5, 400], 1), (64, 1, 2, [70, 33, 0], [100, 33, 64], 3), (96, 2, 4, [40, 64], [41, 1000], 2),
@@ -248,6 +268,20 @@ def test_attention_under_a_mask(paged, d, kv, group, counts, lens, words, kind):
     _check(f, paged, _rand(torch.Generator().manual_seed(5), sum(counts), kv * group, d, gain=1.5), counts, mask=mask)
 
 
+@wide_and_narrow
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("d,kv,group,counts,lens,page", [
+    (64, 1, 2, [70, 30], [2500, 900], 16), (96, 2, 3, [40, 50], [1700, 3000], 32), (128, 1, 8, [20, 17, 18], [1200, 3100, 5], 16),
+    (192, 1, 4, [33], [1500], 64), (256, 2, 2, [60, 9, 70], [640, 1300, 900], 16)])
+def test_attention_of_many_rows_over_long_contexts(paged, d, kv, group, counts, lens, page, masked):
+    """In a wide table, tiles of 128 rows in several parts; in a narrow one as the sizes have it."""
+    counts = [min(m, n) for m, n in zip(counts, lens)]
+    f = Filled(paged, lens, kv, d, page, seed=d + 1)
+    mask = _masks(random.Random(d), counts, 3, "tree") if masked else None
+    _check(f, paged, _rand(torch.Generator().manual_seed(12), sum(counts), kv * group, d, gain=1.5), counts, mask=mask)
+
+
+@wide_and_narrow
 def test_a_chain_under_a_mask_is_the_causal_call(paged):
     counts, lens = [90, 40, 1], [333, 40, 77]
     f = Filled(paged, lens, 2, 128, 16)
@@ -260,6 +294,7 @@ def test_a_chain_under_a_mask_is_the_causal_call(paged):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("masked", [False, True])
 @pytest.mark.parametrize("m", [1, 60])
 def test_lengths_below_the_new_tokens_and_past_the_table(paged, m, masked):
@@ -281,6 +316,7 @@ def test_lengths_below_the_new_tokens_and_past_the_table(paged, m, masked):
         assert torch.equal(torch.isneginf(lse[b * m: b * m + m]), torch.isinf(wl))
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("m", [1, 50])
 @pytest.mark.parametrize("holes", [[0], [1, 4], [2, 3, 5], [0, 1, 2, 3, 4, 5, 6]])
 def test_slots_without_a_page_are_not_seen(paged, m, holes):
@@ -300,6 +336,7 @@ def test_slots_without_a_page_are_not_seen(paged, m, holes):
     assert torch.equal(torch.isneginf(lse), torch.isinf(wl)) and ((lse.double() - wl).abs().nan_to_num(0.0) <= 2.0 ** -18).all()
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("d,m,masked", [(128, 1, False), (128, 60, False), (64, 3, True), (256, 40, True), (96, 90, False), (192, 2, False)])
@@ -337,6 +374,7 @@ def test_infinities_and_nan_stay_with_the_rows_that_see_them(paged, d, m, masked
             assert torch.isnan(got[hit][up]).all() and not torch.isnan(got[hit][~up]).any()
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("m", [1, 40])
 def test_queries_that_are_infinite_or_nan_and_rows_of_no_weight(paged, m):
     d, n = 128, 90
@@ -360,6 +398,7 @@ def test_queries_that_are_infinite_or_nan_and_rows_of_no_weight(paged, m):
     assert torch.isnan(out).all() and torch.isnan(lse).all()
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("scale", [-0.25, 0.0, 1.5])
 @pytest.mark.parametrize("m", [1, 50])
 def test_attention_at_any_scale(paged, scale, m):
@@ -367,6 +406,7 @@ def test_attention_at_any_scale(paged, scale, m):
     _check(f, paged, _rand(torch.Generator().manual_seed(11), 2 * m, 8, 64), [m, m], scale=scale)
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("gain", [1e-30, 1e30])
 @pytest.mark.parametrize("m", [1, 50])
 def test_attention_range_of_values_and_scores(paged, gain, m):
@@ -377,6 +417,7 @@ def test_attention_range_of_values_and_scores(paged, gain, m):
     _check(f, paged, (q.float() * 200).to(BF), [m])
 
 
+@wide_and_narrow
 def test_equal_scores_of_any_size_average(paged):
     """Keys alike: every weight is 1 / n, whatever the score (2^20 here, from block to block the same)."""
     for m in (1, 40):
@@ -394,6 +435,7 @@ def test_equal_scores_of_any_size_average(paged):
             assert abs(float(lse[i, 0]) - (2.0 ** 20 + math.log(n))) <= 0.25  # two f32 roundings at 2^20
 
 
+@wide_and_narrow
 def test_strided_queries_and_rows_of_nobody(paged, kq):
     """Queries inside the rows of a fused projection; rows before the first and behind the last sequence keep their results."""
     for counts, lens in (([3, 2], [900, 40]), ([90, 30], [200, 300])):
@@ -421,6 +463,7 @@ def test_strided_queries_and_rows_of_nobody(paged, kq):
         assert not torch.equal(before, f.cache.k)
 
 
+@wide_and_narrow
 @pytest.mark.parametrize("batch", [63, 65, 130])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_many_sequences(paged, batch, ragged):
@@ -431,6 +474,7 @@ def test_many_sequences(paged, batch, ragged):
     _check(f, paged, _rand(g, sum(counts) if ragged else batch, 4, 64), counts)
 
 
+@wide_and_narrow
 def test_sequences_share_pages(paged):
     """A prefix that several sequences have in common lies in the pool once."""
     f = Filled(paged, [100, 40, 40], 2, 64, 16, seed=17)
@@ -471,6 +515,7 @@ def test_pages_beyond_4_gib_and_a_long_context(paged):
     assert ((got[0][0][0].double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mass).all()
 
 
+@wide_and_narrow
 def test_calls_share_a_workspace_and_are_replayed(paged):
     """Eager calls of several shapes and captured ones, in turn over one workspace: every result as alone."""
     shapes = [([1, 1], [900, 40], False), ([30, 9], [400, 77], True), ([200, 1], [300, 3000], False), ([1, 0], [64, 9], False)]
@@ -509,6 +554,7 @@ def test_calls_share_a_workspace_and_are_replayed(paged):
             assert torch.equal(c[4], o) and torch.equal(c[5], l)
 
 
+@wide_and_narrow
 def test_other_streams(paged):
     f = Filled(paged, [3000, 2000], 2, 64, 16, seed=30)
     q, starts = _rand(torch.Generator().manual_seed(30), 400, 8, 64).cuda(), _starts([300, 100])

@@ -164,13 +164,14 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 // ---- many rows: prompts, chunks, large trees
 //
 // A workgroup takes a tile of 128 query rows, 32 a wave, or one part of its slots, on v_mfma_f32_32x32x16_bf16.  Keys and values go from
-// memory to LDS past the registers, a stage ahead, with one barrier a stage; a wave's O, queries and scores stay in registers.  Bound by
-// the matrix cores, and per tile by its start.  Of a stage's time the products take 90 %: exponentials, maxima and rounding are laid
-// between them (apart they took 198 us for a prompt of 3907, 16/2 heads of 128, beside them 81), and up to D 128 a second group of four
-// waves, over other slots, half a stage apart, uses what the first leaves; above, the registers hold one wave a SIMD.  In the loop 1040
-// TFLOP/s at D 128 and 980 at D 256, where a library product of 8192^3 reaches 1151.  A tile's start and end are 11 us (work, pages,
-// queries and the first stage 6, sums of the groups 1, the next workgroup's launch 4): a prompt of 3907, 16/2 heads of 128, takes 80 us
-// (787 TFLOP/s), 600 tokens over up to 12000 in four sequences, 10/2 heads of 256, 98 and its join 10.
+// memory to LDS past the registers, a stage ahead, with one barrier a stage; a wave's O, queries and scores stay in registers.
+// In the loop, 1040 TFLOP/s at D 128 and 980 at D 256 (a library product of 8192^3: 1151), no unit is full: the matrix cores and LDS
+// (every wave reads all of a chunk) are busy half of the cycles each, the vector unit a third, and an instruction of the first keeps the
+// last from issuing for 11 cycles.  So exponentials, maxima and rounding are laid between products (apart, a prompt of 3907, 16/2 heads of
+// 128, took 198 us), and up to D 128 a second group of four waves, over other slots and half a stage apart, takes what the first leaves;
+// above, the registers hold one wave a SIMD.  A tile's start and end are 11 us (work, pages, queries and the first stage 6, the groups'
+// sums 1, the next workgroup's launch 4): that prompt takes 78 us (804 TFLOP/s); 600 tokens over up to 12000 in four sequences, 10/2
+// heads of 256, 97 and their join 10; 250 nodes of trees over up to 5000 in eight, 16/2 heads of 128, 26 and 7.
 constexpr uint32_t kManyRows = 128;
 
 // The n-th KB from `from` on into LDS, past the registers: 16 bytes a lane, lane l's to byte lds + 1024 n + 16 l, lds the same in all lanes

@@ -234,6 +234,8 @@ template <class A, int NS, Parts kParts, bool kWide, bool kNanRows>
 __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void attn_join_kernel(A a, Split split,
                                                                                           uint32_t slots, uint32_t per_group) {
     constexpr uint32_t D = 32 * NS, kQuads = D / 4, kThreads = kWide ? kJoinThreads : 64, kWays = kThreads / kQuads;
+    // parts on their way: more take registers and so waves (6000 rows of 256, eight and two: 10.4 and 9.3 us; 1536 rows of 64 8.0 and 8.5)
+    constexpr int kLoads = NS <= 2 ? 8 : 2;
     __shared__ f32x4 so[kWide ? kWays : 1][kQuads];
     __shared__ float ws[kWide ? kMostParts : kJoinRowThreads], red[2][kJoinThreads / 64];
     const uint32_t lane = __lane_id(), head = blockIdx.y, wave = threadIdx.x >> 6, tid = kWide ? threadIdx.x : lane;
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(kWide ? kJoinThreads : kJoinRowThreads) void attn_j
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             if (p0) acc *= before * inv;
             if (way < kWays) {
-#pragma unroll 8
+#pragma unroll kLoads
                 for (uint32_t p = way; p < n; p += kWays)
                     acc += wl[p] * inv * *reinterpret_cast<const f32x4 *>(o + part_row(p0 + p) * D);
             }

@@ -171,7 +171,7 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 // 128, took 198 us), and up to D 128 a second group of four waves, over other slots and half a stage apart, takes what the first leaves;
 // above, the registers hold one wave a SIMD.  A tile's start and end are 11 us (work, pages, queries and the first stage 6, the groups'
 // sums 1, the next workgroup's launch 4): that prompt takes 78 us (804 TFLOP/s); 600 tokens over up to 12000 in four sequences, 10/2
-// heads of 256, 97 and their join 10; 250 nodes of trees over up to 5000 in eight, 16/2 heads of 128, 26 and 7.
+// heads of 256, 97 and their join 9; 250 nodes of trees over up to 5000 in eight, 16/2 heads of 128, 26 and 7.
 constexpr uint32_t kManyRows = 128;
 
 // The n-th KB from `from` on into LDS, past the registers: 16 bytes a lane, lane l's to byte lds + 1024 n + 16 l, lds the same in all lanes

@@ -572,8 +572,9 @@ struct FewBlock {
     uint32_t holes;  // slots without a page
 };
 // Units at u0 and u1.
-template <int NS>
+template <int NS, bool kOnce>
 __device__ __forceinline__ void load_few(FewBlock<NS> &f, const Paged &c, uint32_t u0, uint32_t u1, uint32_t holes) {
+    const auto load16 = [](const u32x4 *p) { return kOnce ? __builtin_nontemporal_load(p) : *p; };
     constexpr size_t kSize = kPagedUnit * 32 * NS;
     const uint32_t lane = __lane_id(), r = lane & 15, g = lane >> 4;
     f.holes = (holes & 1 ? 0xFFFFu : 0u) | (holes & 2 ? 0xFFFF0000u : 0u);
@@ -582,14 +583,15 @@ __device__ __forceinline__ void load_few(FewBlock<NS> &f, const Paged &c, uint32
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int j = 0; j < NS; ++j) f.k[t][j] = *reinterpret_cast<const u32x4 *>(k + 512 * j + 64 * t);
+        for (int j = 0; j < NS; ++j) f.k[t][j] = load16(reinterpret_cast<const u32x4 *>(k + 512 * j + 64 * t));
 #pragma unroll
     for (int d = 0; d < NS; ++d)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) f.v[d][x] = *reinterpret_cast<const u32x4 *>(v + 512 * d + 128 * x);
+        for (int x = 0; x < 2; ++x) f.v[d][x] = load16(reinterpret_cast<const u32x4 *>(v + 512 * d + 128 * x));
 }
 
-template <int NS>
+// kOnce: what is read is read once: past the caches (nontemporal).
+template <int NS, bool kOnce>
 __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAttnArgs a, Split split) {
     constexpr uint32_t D = 32 * NS;
     __shared__ float sm[kFewWaves][kFewRows], sl[kFewWaves][kFewRows];
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
     uint32_t asked = 0;
     const auto ask = [&](FewBlock<NS> &f) {
         units.enter(asked);
-        load_few<NS>(f, a.c, units.at(asked), units.at(asked + 1), units.holes(asked, 2));
+        load_few<NS, kOnce>(f, a.c, units.at(asked), units.at(asked + 1), units.holes(asked, 2));
         asked += 2;
     };
 #pragma unroll
@@ -757,7 +759,7 @@ namespace {
 
 // How a step is launched: tiles of 16 rows where the sequences have few query rows, else of 128.
 struct AttnPlan {
-    bool few;
+    bool few, once;
     Split split;
     uint32_t tiles, grid, slots;  // at most, a head; slots: of parts in the workspace
 };
@@ -772,6 +774,10 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)(rows / p.split.rows) + std::min(batch, tokens);
     if (p.few) {
+        // Keys and values that one tile reads, and more of them than may still be in the caches from the last call (us, with and without,
+        // over changing layers: 48 sequences up to 8000, 32/8 heads of 64, 110 and 122; 4 of 4000, 16/2 heads of 128, 16.0 and 16.3, one
+        // 14.4 and 13.6; 8 of 32 rows over 300 16.7 and 14.1).
+        p.once = rows <= 16ull * batch && (uint64_t)batch * max_ctx * kv_heads * D * 4 >= 1u << 24;
         p.split.unit = kFewWaves;
         // as many workgroups as the card holds at once, or where the tiles are as many already, twice that (64 sequences up to 3000,
         // 32/8 heads of 128, 89 us -> 81; below, a second round costs more: 40 of 4000 119 -> 125)
@@ -811,7 +817,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs &args, hipStream_t s) {
     a.per = reinterpret_cast<uint32_t *>(a.part + part_floats(p, a.c.heads, a.c.D));
     const auto launch = [&](auto ns) -> hipError_t {
         constexpr int NS = decltype(ns)::value;
-        if (p.few) paged_few_kernel<NS><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
+        if (p.few && p.once) paged_few_kernel<NS, true><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
+        else if (p.few) paged_few_kernel<NS, false><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
         else paged_many_kernel<NS><<<dim3(p.grid * a.c.heads), 256 * kManyGroups<NS>, 0, s>>>(a, p.split, p.slots);
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;

@@ -556,8 +556,8 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
 // On v_mfma_f32_16x16x32_bf16, keys and values straight from memory to the operands' registers, 16 bytes a lane in whole cache lines.
 // Tile t of a block's keys is slots 8 t .. 8 t + 7 of both units: a lane (column l & 15, g = l >> 4) then holds after the first product
 // the slots 8 t + 4 (g & 1) + j of unit g >> 1, of both tiles the 8 slots of one 16-byte piece of values.
-// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64, 114 us for 595 MB, one of 131072, 16/2 heads of 128, 26 us for 134 MB, both
-// 5.2 TB/s, as a copy; by latency where there are few: five sequences up to 3000 8.3 us.
+// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64, 102 us for 595 MB, 5.8 TB/s (a copy 5.2, a plain read 7.0); one of 131072,
+// 16/2 heads of 128, 25 us for 134 MB; by latency where there are few: five sequences up to 3000 8.4 us.
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
 template <int NS>
 constexpr uint32_t kFewAhead = NS <= 4 ? 2 : 1;

@@ -24,15 +24,15 @@ __device__ __forceinline__ uint32_t row_limit(const Span &s, uint32_t r, uint32_
 // with the part first one XCD would get all the empty ones.)
 struct Split {
     uint32_t target;  // workgroups wanted a kv head; 0: no tile is split
-    uint32_t rows;    // of a tile
-    uint32_t unit;    // `per` is a multiple of it; shares: workgroups that a compute unit holds
+    uint32_t rows;    // of a tile, a power of two
+    uint32_t unit;    // `per` is a multiple of it (even parts: a power of two); shares: workgroups that a compute unit holds
 };
 // How tiles are split: few rows as above (at most target + tiles parts); many rows in shares of one line, below; or many rows in even
 // parts, at most `target` of them.
 enum class Parts { few, shares, even };
 template <class A>
 __device__ __forceinline__ uint32_t tiles_of(const A &a, const Split &w, const Span &s) {
-    return (s.m * a.group + w.rows - 1) / w.rows;
+    return (s.m * a.group + w.rows - 1) >> __builtin_ctz(w.rows);
 }
 template <class A>
 __device__ __forceinline__ uint32_t blocks_of(const A &a, const Span &s) {
@@ -64,7 +64,7 @@ __device__ __forceinline__ uint32_t even_per(const A &a, const Split &w) {
     most = max(wave_max_u32(most), 1u);
     uint32_t per = (uint32_t)min(fair_share(wave_sum_u64(total), w.target), 1ull << 27);
     for (;; per += max(per / 16, 1u)) {
-        per = max((per + w.unit - 1) / w.unit, 1u) * w.unit;
+        per = (max(per, 1u) + w.unit - 1) & ~(w.unit - 1);
         if (most <= 14 + per) return most;
         uint32_t parts = tiles0 * parts_of(blocks0, per);
         for (uint32_t b = lane + 64; b < a.c.batch; b += 64) parts += tiles(b) * parts_of(blocks(b), per);

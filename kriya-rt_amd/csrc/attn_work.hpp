@@ -9,7 +9,8 @@ namespace kr {
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // Row r of sequence span s: the slots that it sees, 0 for a row past the end.
-__device__ __forceinline__ uint32_t row_limit(const Span &s, uint32_t r, uint32_t group, uint32_t max_ctx) {
+template <class Group>
+__device__ __forceinline__ uint32_t row_limit(const Span &s, uint32_t r, const Group &group, uint32_t max_ctx) {
     const uint32_t i = r / group;
     if (i >= s.m || s.n < s.m - i) return 0u;
     return min(s.n - s.m + i + 1, max_ctx);

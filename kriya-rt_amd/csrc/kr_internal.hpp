@@ -420,12 +420,27 @@ uint64_t paged_append_groups(const PagedAppendArgs &a);  // workgroups
 hipError_t launch_paged_append(const PagedAppendArgs &a, hipStream_t s);
 hipError_t launch_paged_read(const Paged &c, const RaggedStep &step, const uint32_t *first, uint32_t count, void *k_out,
                              void *v_out, int f32, hipStream_t s);
+// Division of numbers below 2^31 by one that the host knows: with 2^(l-1) < d <= 2^l and m = floor(2^(31+l) / d) + 1, which is below
+// 2^32 + 1 / d, the product n m / 2^(31+l) is above n / d by less than 1 / d.
+struct Divisor {
+    uint32_t d = 1, m = 0, shift = 0;
+    Divisor() = default;
+    explicit Divisor(uint32_t d) : d(d), shift(31) {
+        while (1ull << (shift - 31) < d) ++shift;
+        m = (uint32_t)((1ull << shift) / d + 1);
+    }
+    __host__ __device__ operator uint32_t() const { return d; }
+};
+__host__ __device__ inline uint32_t operator/(uint32_t n, const Divisor &x) { return (uint32_t)(((uint64_t)n * x.m) >> x.shift); }
+__host__ __device__ inline uint32_t operator%(uint32_t n, const Divisor &x) { return n - n / x * x.d; }
+
 struct PagedAttnArgs {
     Paged c;
     RaggedStep step;
     const uint16_t *q;
     size_t q_stride;
-    uint32_t q_heads, group;
+    uint32_t q_heads;
+    Divisor group;
     const uint32_t *mask;                // nullptr: causal
     uint32_t words;
     float scale_log2;

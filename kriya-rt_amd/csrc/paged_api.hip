@@ -171,7 +171,7 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
     a.q = q;
     a.q_stride = q_stride;
     a.q_heads = q_heads;
-    a.group = q_heads / c.heads;
+    a.group = Divisor(q_heads / c.heads);
     a.mask = mask;
     a.words = words;
     a.scale_log2 = scale * 1.44269504f;

@@ -56,19 +56,26 @@ __device__ __forceinline__ uint32_t even_per(const A &a, const Split &w) {
     const auto tiles = [&](uint32_t b) { return tiles_of(a, w, span_of(a.step, b)); };
     const auto blocks = [&](uint32_t b) { return blocks_of(a, span_of(a.step, b)); };
     const uint32_t lane = __lane_id(), tiles0 = lane < a.c.batch ? tiles(lane) : 0u, blocks0 = lane < a.c.batch ? blocks(lane) : 0u;
-    unsigned long long total = (unsigned long long)tiles0 * blocks0;
+    float total = (float)tiles0 * (float)blocks0;  // (where the search begins: it need not be exact)
     uint32_t most = tiles0 ? blocks0 : 0u;
     for (uint32_t b = lane + 64; b < a.c.batch; b += 64) {
-        total += (unsigned long long)tiles(b) * blocks(b);
+        total += (float)tiles(b) * (float)blocks(b);
         if (tiles(b)) most = max(most, blocks(b));
     }
     most = max(wave_max_u32(most), 1u);
-    uint32_t per = (uint32_t)min(fair_share(wave_sum_u64(total), w.target), 1ull << 27);
+    uint32_t per = (uint32_t)fminf(wave_sum(total) / (float)w.target, 0x1p27f);
     for (;; per += max(per / 16, 1u)) {
         per = (max(per, 1u) + w.unit - 1) & ~(w.unit - 1);
         if (most <= 14 + per) return most;
-        uint32_t parts = tiles0 * parts_of(blocks0, per);
-        for (uint32_t b = lane + 64; b < a.c.batch; b += 64) parts += tiles(b) * parts_of(blocks(b), per);
+        const float inv = __builtin_amdgcn_rcpf((float)per);
+        // parts_of(n, per): the product is off by less than one below 2^21, and beyond there are too many
+        const auto parts_by = [&](uint32_t n) {
+            const uint32_t x = n + per - 1, q = (uint32_t)((float)x * inv);
+            const int32_t rest = (int32_t)(x - q * per);
+            return max(q + (rest >= (int32_t)per) - (rest < 0), 1u);
+        };
+        uint32_t parts = tiles0 * parts_by(blocks0);
+        for (uint32_t b = lane + 64; b < a.c.batch; b += 64) parts += tiles(b) * parts_by(blocks(b));
         if (wave_sum_u32(parts) <= w.target) return per;
     }
 }

@@ -234,7 +234,7 @@ __device__ __forceinline__ uint32_t wave_min_uniform(uint32_t v) { return ~wave_
 // Joins the parts of the rows that were split.  kWide: a workgroup of 16 waves a row, thread (i, j) taking parts i, i + n, ...
 // of four dims, for few rows in many parts; else a wave a row, its workgroup `per_group` rows of a tile (four waves: with 16, which
 // find the work once for more rows, 400 tokens over 20000 in three sequences took 110 us, not 106).  Bound by latency (work count,
-// maxima, parts): 16 rows in 256 parts 6.5 us, 1536 rows in a few 8.3, 6000 rows of 256 10.3 for 34 MB.
+// maxima, parts): 16 rows in 256 parts 6.1 us, 1536 rows in a few 7, 6000 rows of 256 9 for 34 MB.
 // kNanRows: rows whose L is 0 although they saw slots (all their scores -infinity) give NaN: a base above kSeenBase says so.
 constexpr float kSeenBase = -1.5e38f;
 constexpr uint32_t kJoinThreads = 1024, kJoinRowThreads = 256;

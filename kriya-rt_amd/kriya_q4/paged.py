@@ -117,6 +117,11 @@ def _heads(cache: PagedCache, name: str, x: torch.Tensor) -> int:
     return stride
 
 
+def _alike(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether what holds for y holds for x: quicker than the checks again (0.3 us of a call of 9)."""
+    return x.shape == y.shape and x.stride() == y.stride() and x.dtype is y.dtype and x.get_device() == y.get_device()
+
+
 def append(cache: PagedCache, step: Step, k: torch.Tensor, v: torch.Tensor, layer: int = 0, q: Optional[torch.Tensor] = None,
            q_out: Optional[torch.Tensor] = None, cos_sin: Optional[torch.Tensor] = None,
            positions: Optional[torch.Tensor] = None, layout: int = _rope.HALF, q_norm: Optional[torch.Tensor] = None,
@@ -126,7 +131,7 @@ def append(cache: PagedCache, step: Step, k: torch.Tensor, v: torch.Tensor, laye
     (kr_paged_append)."""
     _together(cache, step)
     stride = _heads(cache, "k", k)
-    if v.shape != k.shape or _heads(cache, "v", v) != stride:
+    if not _alike(v, k) and (v.shape != k.shape or _heads(cache, "v", v) != stride):
         raise ValueError("k and v must have the same shape and strides")
     tokens, heads, d = k.shape
     if heads != cache.kv_heads:
@@ -144,7 +149,7 @@ def append(cache: PagedCache, step: Step, k: torch.Tensor, v: torch.Tensor, laye
     if q is not None:
         q_out = q if q_out is None else q_out
         qs, q_heads = _heads(cache, "q", q), q.shape[1]
-        if q.shape[0] != tokens or (q_out is not q and (q_out.shape != q.shape or _heads(cache, "q_out", q_out) != qs)):
+        if q.shape[0] != tokens or (not _alike(q_out, q) and (q_out.shape != q.shape or _heads(cache, "q_out", q_out) != qs)):
             raise ValueError("q and q_out must have the tokens of k, and the same shape and strides")
         qp, op = q.data_ptr(), q_out.data_ptr()
     with at(cache.k):

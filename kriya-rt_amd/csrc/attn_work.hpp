@@ -53,20 +53,28 @@ __device__ __forceinline__ unsigned long long fair_share(unsigned long long tota
 // that past a part, tiles stay whole.
 template <class A>
 __device__ __forceinline__ uint32_t even_per(const A &a, const Split &w) {
-    const auto tiles = [&](uint32_t b) { return tiles_of(a, w, span_of(a.step, b)); };
-    const auto blocks = [&](uint32_t b) { return blocks_of(a, span_of(a.step, b)); };
-    const uint32_t lane = __lane_id(), tiles0 = lane < a.c.batch ? tiles(lane) : 0u, blocks0 = lane < a.c.batch ? blocks(lane) : 0u;
-    float total = (float)tiles0 * (float)blocks0;  // (where the search begins: it need not be exact)
-    uint32_t most = tiles0 ? blocks0 : 0u;
-    for (uint32_t b = lane + 64; b < a.c.batch; b += 64) {
-        total += (float)tiles(b) * (float)blocks(b);
-        if (tiles(b)) most = max(most, blocks(b));
+    const uint32_t lane = __lane_id();
+    uint32_t tiles0 = 0, blocks0 = 0, tiles = 0, most = 0;
+    float total = 0.0f;  // (where the search begins, and with some more than its error where it ends)
+    for (uint32_t b = lane; b < a.c.batch; b += 64) {
+        const Span s = span_of(a.step, b);
+        tiles0 = tiles_of(a, w, s);
+        blocks0 = blocks_of(a, s);
+        tiles += tiles0;
+        total += (float)tiles0 * (float)blocks0;
+        if (tiles0) most = max(most, blocks0);
     }
     most = max(wave_max_u32(most), 1u);
-    uint32_t per = (uint32_t)fminf(wave_sum(total) / (float)w.target, 0x1p27f);
-    for (;; per += max(per / 16, 1u)) {
-        per = (max(per, 1u) + w.unit - 1) & ~(w.unit - 1);
+    tiles = wave_sum_u32(tiles);
+    total = wave_sum(total);
+    if (tiles >= w.target) return most;
+    const auto whole = [&](float per) { return ((uint32_t)fminf(per, 0x1p27f) + w.unit) & ~(w.unit - 1); };
+    const uint32_t last = whole(total / (float)(w.target - tiles) * 1.0001f);  // enough: a tile has less than a part more than its share
+    // (more sequences than lanes are read again for every step: longer ones)
+    const uint32_t step = a.c.batch > 64 ? 4 : 16;
+    for (uint32_t per = whole(total / (float)w.target);; per = min((per + max(per / step, 1u) + w.unit - 1) & ~(w.unit - 1), last)) {
         if (most <= 14 + per) return most;
+        if (per >= last) return per;
         const float inv = __builtin_amdgcn_rcpf((float)per);
         // parts_of(n, per): the product is off by less than one below 2^21, and beyond there are too many
         const auto parts_by = [&](uint32_t n) {
@@ -74,8 +82,15 @@ __device__ __forceinline__ uint32_t even_per(const A &a, const Split &w) {
             const int32_t rest = (int32_t)(x - q * per);
             return max(q + (rest >= (int32_t)per) - (rest < 0), 1u);
         };
-        uint32_t parts = tiles0 * parts_by(blocks0);
-        for (uint32_t b = lane + 64; b < a.c.batch; b += 64) parts += tiles(b) * parts_by(blocks(b));
+        uint32_t parts = 0;
+        if (a.c.batch <= 64) {
+            parts = tiles0 * parts_by(blocks0);
+        } else {
+            for (uint32_t b = lane; b < a.c.batch; b += 64) {
+                const Span s = span_of(a.step, b);
+                parts += tiles_of(a, w, s) * parts_by(blocks_of(a, s));
+            }
+        }
         if (wave_sum_u32(parts) <= w.target) return per;
     }
 }

@@ -464,7 +464,7 @@ def test_strided_queries_and_rows_of_nobody(paged, kq):
 
 
 @wide_and_narrow
-@pytest.mark.parametrize("batch", [63, 65, 130])
+@pytest.mark.parametrize("batch", [63, 65, 130, 1100])
 @pytest.mark.parametrize("ragged", [False, True])
 def test_many_sequences(paged, batch, ragged):
     g = torch.Generator().manual_seed(batch)
@@ -472,6 +472,17 @@ def test_many_sequences(paged, batch, ragged):
     counts = [min(n, c) for n, c in zip(lens, torch.randint(0, 9, (batch,), generator=g).tolist())] if ragged else None
     f = Filled(paged, lens, 1, 64, 16, seed=16)
     _check(f, paged, _rand(g, sum(counts) if ragged else batch, 4, 64), counts)
+
+
+@wide_and_narrow
+@pytest.mark.parametrize("m", [1, 40])
+def test_long_sequences_among_many(paged, m):
+    """More sequences than a wave has lanes, two of them long enough to be split."""
+    lens = [20 + i % 60 for i in range(90)]
+    lens[17], lens[80] = 3000, 2100
+    counts = [min(m if i % 9 == 8 else 1, n) for i, n in enumerate(lens)]
+    f = Filled(paged, lens, 1, 128, 16, seed=20)
+    _check(f, paged, _rand(torch.Generator().manual_seed(21), sum(counts), 4, 128, gain=1.5), counts)
 
 
 @wide_and_narrow

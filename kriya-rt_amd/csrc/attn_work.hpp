@@ -28,8 +28,8 @@ struct Split {
     uint32_t rows;    // of a tile, a power of two
     uint32_t unit;    // `per` is a multiple of it (even parts: a power of two); shares: workgroups that a compute unit holds
 };
-// How tiles are split: few rows as above (at most target + tiles parts); many rows in shares of one line, below; or many rows in even
-// parts, at most `target` of them.
+// How tiles are split: as above, in at most target + tiles parts; many rows in shares of one line, below; or in even parts, few rows and
+// many, at most `target` of them where there are not more tiles.
 enum class Parts { few, shares, even };
 template <class A>
 __device__ __forceinline__ uint32_t tiles_of(const A &a, const Split &w, const Span &s) {

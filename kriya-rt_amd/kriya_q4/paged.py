@@ -30,6 +30,7 @@ from . import rope as _rope
 from ._device import at, checked, new, stream_of
 
 UNIT = 16
+MAX_NODES = 4096  # of a sequence's tree
 _BF16 = (torch.bfloat16,)
 
 

@@ -17,13 +17,15 @@ import torch
 
 from . import (ACT_SWIGLU, DTYPE_BF16, DTYPE_F32, argmax, embedding, linear_workspace, paged, q4_linear, rmsnorm, rmsnorm_mlp,
                rmsnorm_mlp_workspace, rmsnorm_qkv, rope)
+from ._device import checked
 from .qwen_decode import QWEN25_3B, Layer, QwenConfig, QwenQ4Decoder
 
 
 class QwenPagedDecoder(QwenQ4Decoder):
     """`batch` sequences of up to max_ctx tokens over a pool of `pages` pages (as many as they could all fill where None), the first
     `ctx` tokens random as in QwenQ4Decoder.  Eager calls take pages from the pool as sequences grow; replays of a captured step
-    need theirs before (reserve): what they add beyond is lost, and refused by the next eager call.  All calls on one stream, or
+    need theirs before (reserve): what they add beyond is lost, and refused by the next eager call.  A prompt or a tree counts once all of
+    its pass has been enqueued: a call that is refused or fails leaves the sequences as they were.  All calls on one stream, or
     ordered by the caller."""
 
     def __init__(self, cfg: QwenConfig = QWEN25_3B, batch: int = 1, ctx: int = 512, seed: int = 3000,
@@ -134,20 +136,25 @@ class QwenPagedDecoder(QwenQ4Decoder):
         return self.next
 
     def _ragged(self, tokens: torch.Tensor, counts, what: str):
-        """A ragged batch: counts and starts on the device, after pages for it have been taken."""
-        m, device = int(tokens.numel()), tokens.device
+        """A ragged batch: counts, starts and the lengths after it on the device, after pages for it have been taken."""
+        m, device = int(tokens.numel()), self.lengths.device
         counts = [int(n) for n in counts]
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != m:
             raise ValueError(f"counts={counts} do not split {m} tokens over {self.batch} sequences")
         self._read_back(what)
-        self._grow(counts)
+        self._take([a + n for a, n in zip(self._used, counts)])
         n = torch.tensor(counts, dtype=torch.int32, device=device)
         starts = torch.zeros(self.batch + 1, dtype=torch.int32, device=device)
         torch.cumsum(n, 0, dtype=torch.int32, out=starts[1:])
-        return counts, n, starts
+        return counts, n, starts, self.lengths + n
+
+    def _counted(self, lengths, used) -> None:
+        """A ragged batch is part of its sequences."""
+        self.lengths.copy_(lengths)
+        self._used = used
 
     def _hidden(self, tokens, step, positions, mask) -> torch.Tensor:
-        """The last layer's output of a ragged batch whose lengths have been raised."""
+        """The last layer's output of a ragged batch."""
         c, m, device = self.cfg, int(tokens.numel()), tokens.device
 
         def rows(width, dtype=torch.bfloat16):
@@ -164,21 +171,22 @@ class QwenPagedDecoder(QwenQ4Decoder):
         """Appends counts[b] tokens to each sequence b (tokens int32, sequence after sequence; a count may be 0) in one ragged
         batch and sets `logits` and `tokens` of those that got any to what follows their last one; returns the next-token buffer.
         Reads the lengths back."""
-        counts, n, starts = self._ragged(tokens, counts, "prefill")
+        counts, n, starts, after = self._ragged(tokens, counts, "prefill")
         m = int(tokens.numel())
         if m == 0:
             return self.next
         place = torch.arange(m, dtype=torch.int32, device=tokens.device)
         seq = torch.repeat_interleave(torch.arange(self.batch, device=tokens.device), n, output_size=m)
         positions = self.positions[seq] + place - starts[seq]
-        self.lengths.add_(n)
-        h = self._hidden(tokens, paged.Step(self.table, self.lengths, starts), positions, None)
+        h = self._hidden(tokens, paged.Step(self.table, after, starts), positions, None)
         got = torch.tensor([b for b, n in enumerate(counts) if n], device=tokens.device)
         last = rmsnorm(h[(starts[1:][got] - 1).long()].contiguous(), self.ln_f, self.cfg.eps)
         logits = q4_linear(self.embed, last, out_dtype=DTYPE_F32)
+        chosen = argmax(logits)
         self.logits[got] = logits
-        self.tokens[got] = argmax(logits)
+        self.tokens[got] = chosen
         self.positions.add_(n)
+        self._counted(after, [a + n for a, n in zip(self._used, counts)])
         return self.next
 
     def verify(self, tokens: torch.Tensor, parents: torch.Tensor, counts):
@@ -188,19 +196,24 @@ class QwenPagedDecoder(QwenQ4Decoder):
         Returns (path int32 [batch, most nodes], counts int32 [batch]): the nodes kept.  Reads the lengths back."""
         if parents.shape != tokens.shape:
             raise ValueError(f"parents must be {tuple(tokens.shape)} like tokens, not {tuple(parents.shape)}")
-        counts, n, starts = self._ragged(tokens, counts, "verify")
-        most = max(counts)
+        if tokens.numel():
+            checked("tokens", tokens, torch.int32, (tokens.numel(),), self.lengths)
+            checked("parents", parents, torch.int32, (tokens.numel(),), self.lengths)
+        counts = [int(n) for n in counts]
+        most = max(counts, default=0)
+        if most > paged.MAX_NODES:
+            raise ValueError(f"a tree of {most} nodes, more than {paged.MAX_NODES}")
+        counts, n, starts, after = self._ragged(tokens, counts, "verify")
         if most == 0:
             return torch.zeros((self.batch, 1), dtype=torch.int32, device=n.device), torch.zeros_like(n)
-        self.lengths.add_(n)
-        step = paged.Step(self.table, self.lengths, starts)
-        mask, positions = paged.tree_plan(parents, self.lengths, starts, nodes=most)
+        step = paged.Step(self.table, after, starts)
+        mask, positions = paged.tree_plan(parents, after, starts, nodes=most)
         h = rmsnorm(self._hidden(tokens, step, positions, mask), self.ln_f, self.cfg.eps)
         logits = q4_linear(self.embed, h, out_dtype=DTYPE_F32)
-        path, kept, _, lengths = paged.commit(self.cache, step, tokens, parents, argmax(logits), next=self.tokens, max_path=most)
+        targets = argmax(logits)
+        path, kept, _, lengths = paged.commit(self.cache, step, tokens, parents, targets, next=self.tokens, max_path=most)
         got = torch.tensor([b for b, n in enumerate(counts) if n], device=n.device)
         self.logits[got] = logits[starts[:-1][got].long() + path[got, (kept[got] - 1).long()].long()]
-        self.lengths.copy_(lengths)
         self.positions.copy_(lengths)
-        self._used = lengths.tolist()
+        self._counted(lengths, lengths.tolist())
         return path, kept

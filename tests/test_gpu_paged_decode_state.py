@@ -1,0 +1,82 @@
+"""GPU: what the decoder over the paged cache keeps through refused calls, ended sequences and replays past their pages; against steps,
+and against the restatement of test_gpu_paged_decode under its bar."""
+import numpy as np
+import pytest
+import torch
+
+from _util import assert_rms_close
+from test_gpu_paged_decode import BAR, BATCH, forward_ref, make, stepped  # noqa: F401  (make: the fixture)
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=I32, device="cuda")
+
+
+def _state(m):
+    return [t.clone() for t in (m.lengths, m.positions, m.tokens, m.logits)] + [list(m._used)]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) if torch.is_tensor(x) else x == y for x, y in zip(a, b))
+
+
+def _captured(m):
+    """A captured step of m, not yet replayed."""
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(g, stream=side):
+            m.step()
+    torch.cuda.current_stream().wait_stream(side)
+    return g
+
+
+# ---- refused and failed calls
+
+def test_a_refused_verify_changes_nothing(make):
+    m = make()
+    m.step()
+    before, table = _state(m), m.table.clone()
+    ids, up = _i32([1, 2, 3]), _i32([-1, 0, -1])
+    wide = torch.zeros(3, 2, dtype=I32, device="cuda")
+    for tokens, parents, match in ((ids, up.long(), "parents must be torch.int32"), (ids.long(), up, "tokens must be torch.int32"),
+                                   (ids, wide[:, 0], "contiguous"), (wide[:, 0], up, "contiguous"), (ids.cpu(), up, "GPU"), (ids, up.cpu(), "GPU"),
+                                   (ids[None], up[None], "tokens must be")):
+        with pytest.raises(ValueError, match=match):
+            m.verify(tokens, parents, [2, 1, 0])
+        assert _same(_state(m), before) and torch.equal(m.table, table)
+    stepped(m)
+
+
+def test_a_tree_of_more_nodes_than_a_plan_takes(make):
+    m = make(max_ctx=6000)
+    before, table = _state(m), m.table.clone()
+    nodes = 4097
+    with pytest.raises(ValueError, match="4096"):
+        m.verify(torch.zeros(nodes, dtype=I32, device="cuda"), torch.arange(-1, nodes - 1, dtype=I32, device="cuda"), [nodes, 0, 0])
+    assert _same(_state(m), before) and torch.equal(m.table, table)
+    stepped(m)
+
+
+@pytest.mark.parametrize("late", [False, True])
+def test_a_pass_that_fails_changes_nothing(make, monkeypatch, late):
+    """An error in the middle of a pass (its first call, or the head's logits): the sequences are as they were."""
+    from kriya_q4 import qwen_paged
+
+    m, plain = make(), make()
+    m.step()
+    plain.step()
+    before = _state(m)
+    with monkeypatch.context() as patch:
+        def fails(*a, **kw):
+            raise RuntimeError("out of memory")
+        patch.setattr(qwen_paged, "argmax" if late else "embedding", fails)
+        for call in (lambda: m.prefill(_i32([1, 2, 3]), [2, 0, 1]), lambda: m.verify(_i32([1, 2, 3]), _i32([-1, 0, -1]), [2, 0, 1])):
+            with pytest.raises(RuntimeError, match="out of memory"):
+                call()
+            assert _same(_state(m)[:3] + [m._used], before[:3] + [before[4]])
+    assert torch.equal(m.step(), plain.step()) and torch.equal(m.logits, plain.logits)
+

@@ -210,10 +210,11 @@ class QwenPagedDecoder(QwenQ4Decoder):
         mask, positions = paged.tree_plan(parents, after, starts, nodes=most)
         h = rmsnorm(self._hidden(tokens, step, positions, mask), self.ln_f, self.cfg.eps)
         logits = q4_linear(self.embed, h, out_dtype=DTYPE_F32)
-        targets = argmax(logits)
-        path, kept, _, lengths = paged.commit(self.cache, step, tokens, parents, targets, next=self.tokens, max_path=most)
+        # (its next tokens beside `tokens`, which may be the nodes of this tree)
+        path, kept, chosen, lengths = paged.commit(self.cache, step, tokens, parents, argmax(logits), next=self.tokens.clone(), max_path=most)
         got = torch.tensor([b for b, n in enumerate(counts) if n], device=n.device)
         self.logits[got] = logits[starts[:-1][got].long() + path[got, (kept[got] - 1).long()].long()]
+        self.tokens.copy_(chosen)
         self.positions.copy_(lengths)
         self._counted(lengths, lengths.tolist())
         return path, kept

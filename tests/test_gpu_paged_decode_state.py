@@ -80,3 +80,22 @@ def test_a_pass_that_fails_changes_nothing(make, monkeypatch, late):
             assert _same(_state(m)[:3] + [m._used], before[:3] + [before[4]])
     assert torch.equal(m.step(), plain.step()) and torch.equal(m.logits, plain.logits)
 
+
+def test_verify_of_the_decoders_own_tokens(make):
+    """Trees of node 0 alone are a step: `tokens` themselves may be given."""
+    m, plain = make(), make()
+    path, kept = m.verify(m.tokens, torch.full((BATCH,), -1, dtype=I32, device="cuda"), [1] * BATCH)
+    plain.step()
+    assert kept.tolist() == [1] * BATCH and path.tolist() == [[0]] * BATCH
+    assert m.lengths.tolist() == [41] * BATCH == m.positions.tolist()
+    assert torch.equal(m.tokens, plain.tokens)
+    stepped(m)
+
+
+def test_a_prompt_of_the_decoders_own_tokens(make):
+    m, plain = make(), make()
+    m.prefill(m.tokens, [1] * BATCH)
+    plain.step()
+    assert torch.equal(m.tokens, plain.tokens) and m.lengths.tolist() == [41] * BATCH
+    stepped(m)
+

@@ -469,6 +469,8 @@ def moe_block(router: Q4Matrix, gate: Q4Matrix, up: Q4Matrix, down: Q4Matrix, ex
 
 def embedding(w: Q4Matrix, tokens: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """bf16 rows of the Q4 table for int32 token ids (transformer_glue.metal:122-152)."""
+    if tokens.dtype not in (torch.int32, torch.uint32) or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous torch.int32, not {tokens.dtype} with strides {tokens.stride()}")
     count = tokens.numel()
     if out is None:
         out = torch.empty((count, w.k), dtype=torch.bfloat16, device=tokens.device)

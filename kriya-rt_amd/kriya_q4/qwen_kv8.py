@@ -18,6 +18,7 @@ import torch
 
 from . import (ACT_SWIGLU, DTYPE_BF16, DTYPE_F32, argmax, embedding, kv8, linear_workspace, q4_linear, rmsnorm,
                rmsnorm_mlp, rmsnorm_mlp_workspace, rmsnorm_qkv, rope)
+from ._device import checked
 from .qwen_decode import QWEN25_3B, Layer, QwenConfig, QwenQ4Decoder
 
 
@@ -126,6 +127,7 @@ class QwenKv8Decoder(QwenQ4Decoder):
             raise ValueError(f"counts={counts} do not split {m} tokens over {self.batch} sequences")
         if m == 0:
             return self.next
+        checked("tokens", tokens, torch.int32, None, self.lengths)
         self._read_back("prefill")
         self._grow(counts)
         n = torch.tensor(counts, dtype=torch.int32, device=device)

@@ -141,6 +141,8 @@ class QwenPagedDecoder(QwenQ4Decoder):
         counts = [int(n) for n in counts]
         if len(counts) != self.batch or min(counts) < 0 or sum(counts) != m:
             raise ValueError(f"counts={counts} do not split {m} tokens over {self.batch} sequences")
+        if m:
+            checked("tokens", tokens, torch.int32, None, self.lengths)
         self._read_back(what)
         self._take([a + n for a, n in zip(self._used, counts)])
         n = torch.tensor(counts, dtype=torch.int32, device=device)

@@ -99,3 +99,16 @@ def test_a_prompt_of_the_decoders_own_tokens(make):
     assert torch.equal(m.tokens, plain.tokens) and m.lengths.tolist() == [41] * BATCH
     stepped(m)
 
+
+def test_prompts_of_other_types_are_refused(make):
+    m = make()
+    before = _state(m)
+    ids = torch.arange(6, device="cuda")
+    for tokens, match in ((ids, "torch.int32"), (ids.to(torch.int16), "torch.int32"), (ids.float(), "torch.int32"),
+                          (ids.to(I32)[::2].repeat(2)[::2], "contiguous"), (ids.to(I32).cpu(), "GPU")):
+        with pytest.raises(ValueError, match=match):
+            m.prefill(tokens, [tokens.numel(), 0, 0])
+        assert _same(_state(m), before)
+    stepped(m)
+
+

@@ -24,7 +24,8 @@ from .qwen_decode import QWEN25_3B, Layer, QwenConfig, QwenQ4Decoder
 class QwenPagedDecoder(QwenQ4Decoder):
     """`batch` sequences of up to max_ctx tokens over a pool of `pages` pages (as many as they could all fill where None), the first
     `ctx` tokens random as in QwenQ4Decoder.  Eager calls take pages from the pool as sequences grow; replays of a captured step
-    need theirs before (reserve): what they add beyond is lost, and refused by the next eager call.  A prompt or a tree counts once all of
+    need theirs before (reserve): what they add beyond is lost, and refused by the next eager call.  A released sequence takes no part in
+    steps, eager or replayed (its rows of `tokens` and `logits` mean nothing), until a prompt or a tree fills its place.  A prompt or a tree counts once all of
     its pass has been enqueued: a call that is refused or fails leaves the sequences as they were.  All calls on one stream, or
     ordered by the caller."""
 
@@ -41,6 +42,8 @@ class QwenPagedDecoder(QwenQ4Decoder):
         self.table = torch.full((batch, most), -1, dtype=torch.int32, device=device)
         # tokens in the pages, as far as the calls made here tell: replays of a captured step move the device's alone
         self._used, self._captured = [ctx] * batch, False
+        # 1 of sequences that take part in steps, on the device, where replays read it, and here
+        self.active, self._active = torch.ones(batch, dtype=torch.int32, device=device), [1] * batch
         self.lengths = torch.full((batch,), ctx, dtype=torch.int32, device=device)
         self._take([ctx] * batch)
         super().__init__(cfg, batch, ctx, seed, device)
@@ -89,19 +92,20 @@ class QwenPagedDecoder(QwenQ4Decoder):
         self._used = after
 
     def reserve(self, tokens: int) -> None:
-        """Gives every sequence the pages for `tokens` more: what so many replays of a captured step need.  Reads the lengths back."""
+        """Gives every sequence that has not ended the pages for `tokens` more: what so many replays of a captured step need.  Reads the
+        lengths back."""
         self._read_back("reserve")
-        self._take([n + tokens for n in self._used])
+        self._take([n + tokens * live for n, live in zip(self._used, self._active)])
 
     def release(self, sequence: int) -> None:
-        """Ends a sequence: its pages are free for others, its length is 0.  Reads the lengths back."""
+        """Ends a sequence: its pages are free for others, its length is 0 and stays so.  Reads the lengths back."""
         self._read_back("release")
         self._free += self._pages[sequence][::-1]
         self._pages[sequence] = []
         self.table[sequence].fill_(-1)
-        for t in (self.lengths, self.positions):
+        for t in (self.lengths, self.positions, self.active):
             t[sequence: sequence + 1].zero_()
-        self._used[sequence] = 0
+        self._used[sequence] = self._active[sequence] = 0
 
     def _layers(self, h, x, qkv, attn, lse, step, positions, mask, attn_ws, o_ws, mlp_ws, stream):
         c, m = self.cfg, h.shape[0]
@@ -115,8 +119,8 @@ class QwenPagedDecoder(QwenQ4Decoder):
             rmsnorm_mlp(L.gate, L.up, L.down, h, L.ln2, c.eps, activation=ACT_SWIGLU, workspace=mlp_ws, stream=stream)
 
     def step(self, stream=None) -> torch.Tensor:
-        """One greedy decode step of every sequence: `tokens` are appended at `positions`, both move on; returns the next-token
-        buffer.  stream: a torch.cuda.Stream.  Nothing returns to the host, so a step can be captured and replayed; once one has been,
+        """One greedy decode step of every sequence that has not ended: `tokens` are appended at `positions`, both move on; returns the
+        next-token buffer.  stream: a torch.cuda.Stream.  Nothing returns to the host, so a step can be captured and replayed; once one has been,
         eager ones read the lengths back first."""
         with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
             if torch.cuda.is_current_stream_capturing():
@@ -124,15 +128,16 @@ class QwenPagedDecoder(QwenQ4Decoder):
             else:
                 if self._captured:
                     self._read_back("an eager step")
-                self._grow([1] * self.batch)
-            self.lengths.add_(1)
+                self._grow(self._active)
+            # (one that has ended stays at 0 tokens, its new one without a slot: nothing is appended, and its row sees nothing)
+            self.lengths.add_(self.active)
             embedding(self.embed, self.tokens, out=self.h, stream=stream)
             self._layers(self.h, self.x, (self.q, self.k, self.v), self.attn, self.lse, self._step, self.positions, None,
                          self.attn_ws, self.o_ws, self.ws, stream)
             rmsnorm(self.h, self.ln_f, self.cfg.eps, out=self.x, stream=stream)
             q4_linear(self.embed, self.x, y=self.logits, out_dtype=DTYPE_F32, stream=stream)
             argmax(self.logits, out=self.next, workspace=self.argmax_ws, stream=stream)
-            self.positions.add_(1)
+            self.positions.add_(self.active)
         return self.next
 
     def _ragged(self, tokens: torch.Tensor, counts, what: str):
@@ -150,10 +155,14 @@ class QwenPagedDecoder(QwenQ4Decoder):
         torch.cumsum(n, 0, dtype=torch.int32, out=starts[1:])
         return counts, n, starts, self.lengths + n
 
-    def _counted(self, lengths, used) -> None:
+    def _counted(self, counts, lengths, used) -> None:
         """A ragged batch is part of its sequences."""
         self.lengths.copy_(lengths)
         self._used = used
+        for b, n in enumerate(counts):
+            if n and not self._active[b]:
+                self.active[b: b + 1].fill_(1)
+                self._active[b] = 1
 
     def _hidden(self, tokens, step, positions, mask) -> torch.Tensor:
         """The last layer's output of a ragged batch."""
@@ -188,7 +197,7 @@ class QwenPagedDecoder(QwenQ4Decoder):
         self.logits[got] = logits
         self.tokens[got] = chosen
         self.positions.add_(n)
-        self._counted(after, [a + n for a, n in zip(self._used, counts)])
+        self._counted(counts, after, [a + n for a, n in zip(self._used, counts)])
         return self.next
 
     def verify(self, tokens: torch.Tensor, parents: torch.Tensor, counts):
@@ -218,5 +227,5 @@ class QwenPagedDecoder(QwenQ4Decoder):
         self.logits[got] = logits[starts[:-1][got].long() + path[got, (kept[got] - 1).long()].long()]
         self.tokens.copy_(chosen)
         self.positions.copy_(lengths)
-        self._counted(lengths, lengths.tolist())
+        self._counted(counts, lengths, lengths.tolist())
         return path, kept

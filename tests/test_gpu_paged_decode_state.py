@@ -112,3 +112,82 @@ def test_prompts_of_other_types_are_refused(make):
     stepped(m)
 
 
+# ---- sequences that have ended
+
+def _rows(m, tokens, live, lengths, positions):
+    counts = [1 if b in live else 0 for b in range(BATCH)]
+    return forward_ref(m, tokens[live], counts, lengths, positions[live])
+
+
+def test_an_ended_sequence_takes_no_part_in_steps(make):
+    """Eager: it takes no page and grows no context; a prompt in its place starts from nothing."""
+    m = make()
+    m.release(1)
+    free = len(m._free)
+    for i in range(2):
+        tokens, positions = m.tokens.cpu().numpy().copy(), m.positions.cpu().clone()
+        m.step()
+        assert m.lengths.tolist() == [41 + i, 0, 41 + i] == m.positions.tolist()
+        want = _rows(m, tokens, [0, 2], [41 + i, 0, 41 + i], positions)
+        assert_rms_close(m.logits.cpu().numpy()[[0, 2]], want, rel=BAR, what="the others")
+    assert m.table[1].tolist() == [-1] * 8 and len(m._free) == free and torch.isfinite(m.logits).all()
+    ids = torch.randint(0, 512, (20,), dtype=I32, generator=torch.Generator().manual_seed(6))
+    m.prefill(ids.cuda(), [0, 20, 0])
+    assert m.lengths.tolist() == [42, 20, 42] == m.positions.tolist()
+    want = forward_ref(m, ids.numpy(), [0, 20, 0], [42, 20, 42], torch.arange(20, dtype=I32))
+    assert_rms_close(m.logits.cpu().numpy()[[1]], want[[19]], rel=BAR, what="prompt after the release")
+    stepped(m)
+    assert m.lengths.tolist() == [43, 21, 43]
+
+
+def test_ended_sequences_need_no_pages(make):
+    """A pool that is full but for one sequence's page goes on once the others have ended."""
+    m = make(pages=9)  # three pages each, of which 8 slots are left
+    for _ in range(8):
+        m.step()
+    with pytest.raises(ValueError, match="release"):
+        m.step()
+    m.release(0)
+    m.release(2)
+    for _ in range(20):
+        m.step()
+    m.reserve(10)
+    assert m.lengths.tolist() == [0, 68, 0] and [len(p) for p in m._pages] == [0, 5, 0]
+
+
+def test_captured_steps_after_a_release(make):
+    """Replays pass an ended sequence over, and take it along once a prompt has filled its place: all as eager steps do."""
+    m, eager = make(), make()
+    ids = torch.randint(0, 512, (20,), dtype=I32, generator=torch.Generator().manual_seed(7)).cuda()
+    m.step(), eager.step()
+    m.reserve(40)
+    g = _captured(m)
+
+    def both(n):
+        for _ in range(n):
+            g.replay()
+            eager.step()
+            torch.cuda.synchronize()
+            torch.ones(1000, device="cuda").sum().item()
+            assert torch.equal(m.lengths, eager.lengths) and torch.equal(m.positions, eager.positions)
+            live = m.lengths > 0
+            assert torch.equal(m.logits[live], eager.logits[live]) and torch.equal(m.tokens[live], eager.tokens[live])
+    both(2)
+    m.release(1), eager.release(1)
+    both(3)
+    assert m.lengths.tolist() == [46, 0, 46] and m.table[1].max() < 0
+    for x in (m, eager):
+        x.step()
+        x.prefill(ids, [0, 20, 0])
+    m.reserve(20)
+    both(12)
+    assert m.lengths.tolist() == [59, 32, 59]
+    stepped(m)
+
+
+def test_a_tree_starts_an_ended_sequence_again(make):
+    m = make()
+    m.release(2)
+    path, kept = m.verify(_i32([7, 9]), _i32([-1, -1]), [0, 0, 2])
+    assert kept.tolist() == [0, 0, 1] and m.lengths.tolist() == [40, 40, 1]
+    stepped(m)

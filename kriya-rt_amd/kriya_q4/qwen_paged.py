@@ -24,7 +24,7 @@ from .qwen_decode import QWEN25_3B, Layer, QwenConfig, QwenQ4Decoder
 class QwenPagedDecoder(QwenQ4Decoder):
     """`batch` sequences of up to max_ctx tokens over a pool of `pages` pages (as many as they could all fill where None), the first
     `ctx` tokens random as in QwenQ4Decoder.  Eager calls take pages from the pool as sequences grow; replays of a captured step
-    need theirs before (reserve): what they add beyond is lost, and refused by the next eager call.  A released sequence takes no part in
+    need theirs before (reserve): what they add beyond is lost, and the next eager calls are refused until that sequence is released.  A released sequence takes no part in
     steps, eager or replayed (its rows of `tokens` and `logits` mean nothing), until a prompt or a tree fills its place.  A prompt or a tree counts once all of
     its pass has been enqueued: a call that is refused or fails leaves the sequences as they were.  All calls on one stream, or
     ordered by the caller."""
@@ -76,14 +76,15 @@ class QwenPagedDecoder(QwenQ4Decoder):
                 self.table[b, have: have + n] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
                 self._pages[b] += new
 
-    def _read_back(self, what: str) -> None:
-        """The host's counts from the device's (a synchronization)."""
+    def _read_back(self, what: str, past: bool = False) -> None:
+        """The host's counts from the device's (a synchronization).  past: they may be past the sequences' pages."""
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what} counts pages on the host: it cannot be part of a capture")
         used = self.lengths.tolist()
         for b, n in enumerate(used):
-            if n > self.cache.page * len(self._pages[b]):
-                raise RuntimeError(f"replays have brought sequence {b} to {n} tokens, past its {len(self._pages[b])} pages: reserve before them")
+            if n > self.cache.page * len(self._pages[b]) and not past:
+                raise RuntimeError(f"replays have brought sequence {b} to {n} tokens, past its {len(self._pages[b])} pages: reserve before "
+                                   "them; now it can only be released")
         self._used = used
 
     def _grow(self, counts) -> None:
@@ -99,7 +100,7 @@ class QwenPagedDecoder(QwenQ4Decoder):
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages are free for others, its length is 0 and stays so.  Reads the lengths back."""
-        self._read_back("release")
+        self._read_back("release", past=True)
         self._free += self._pages[sequence][::-1]
         self._pages[sequence] = []
         self.table[sequence].fill_(-1)

@@ -185,6 +185,46 @@ def test_captured_steps_after_a_release(make):
     stepped(m)
 
 
+def test_a_sequence_past_its_pages_is_released_and_the_others_go_on(make):
+    m = make()
+    m.prefill(torch.arange(5, dtype=I32).cuda(), [5, 0, 0])
+    m.step()  # 46, 41, 41 tokens in three pages each
+    g = _captured(m)
+    for _ in range(4):
+        g.replay()
+    for call in (m.step, lambda: m.reserve(1), lambda: m.prefill(m.tokens[:1], [0, 1, 0])):
+        with pytest.raises(RuntimeError, match="reserve before"):
+            call()
+    m.release(0)
+    assert m.lengths.tolist() == [0, 45, 45] and m.table[0].max() < 0
+    tokens, positions = m.tokens.cpu().numpy().copy(), m.positions.cpu().clone()
+    m.step()
+    want = _rows(m, tokens, [1, 2], [0, 46, 46], positions)
+    assert_rms_close(m.logits.cpu().numpy()[[1, 2]], want, rel=BAR, what="the others")
+    m.prefill(torch.arange(9, dtype=I32).cuda(), [9, 0, 0])
+    m.reserve(4)
+    g.replay()
+    assert m.lengths.tolist() == [10, 47, 47]
+    stepped(m)
+    used = [p for row in m.table.tolist() for p in row if p >= 0]
+    assert len(used) == len(set(used)) and sorted(used + m._free) == list(range(m.cache.pages))
+
+
+def test_all_sequences_past_their_pages_are_released_one_by_one(make):
+    m = make()
+    m.step()
+    g = _captured(m)
+    for _ in range(8):
+        g.replay()
+    for b in range(BATCH):
+        with pytest.raises(RuntimeError, match="reserve before"):
+            m.reserve(1)
+        m.release(b)
+    assert m.lengths.tolist() == [0] * BATCH and len(m._free) == m.cache.pages
+    m.prefill(torch.arange(6, dtype=I32).cuda(), [1, 2, 3])
+    stepped(m)
+
+
 def test_a_tree_starts_an_ended_sequence_again(make):
     m = make()
     m.release(2)

@@ -100,6 +100,8 @@ class QwenPagedDecoder(QwenQ4Decoder):
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages are free for others, its length is 0 and stays so.  Reads the lengths back."""
+        if not 0 <= sequence < self.batch:
+            raise ValueError(f"sequence={sequence} is not 0 .. {self.batch - 1}")
         self._read_back("release", past=True)
         self._free += self._pages[sequence][::-1]
         self._pages[sequence] = []

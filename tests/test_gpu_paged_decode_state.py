@@ -231,3 +231,15 @@ def test_a_tree_starts_an_ended_sequence_again(make):
     path, kept = m.verify(_i32([7, 9]), _i32([-1, -1]), [0, 0, 2])
     assert kept.tolist() == [0, 0, 1] and m.lengths.tolist() == [40, 40, 1]
     stepped(m)
+
+
+def test_sequences_that_are_none(make):
+    m = make()
+    before = _state(m)
+    for b in (-1, BATCH, BATCH + 4):
+        with pytest.raises(ValueError, match="sequence"):
+            m.release(b)
+        assert _same(_state(m), before) and len(m._free) == m.cache.pages - 3 * BATCH
+    m.release(0)
+    m.release(0)  # nothing left to end
+    assert len(m._free) == m.cache.pages - 6 and m.lengths.tolist() == [0, 40, 40]

@@ -85,7 +85,7 @@ int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_st
  * below 2^89.  A row that sees no slot gives zeros and lse = -infinity.
  * Infinities and NaN count in the rows that see them alone: such a row gives what the formula gives, an infinity or NaN.
  * workspace: kr_paged_attention_workspace_bytes(cache, step, q_heads, tokens) bytes (of step only batch and max_pages are
- * read), 16-byte aligned, no initial contents; calls sharing it must not overlap in time.  Results are the same bits from run
+ * read; 0 for sizes that the call refuses), 16-byte aligned, no initial contents; calls sharing it must not overlap in time.  Results are the same bits from run
  * to run. */
 size_t kr_paged_attention_workspace_bytes(const kr_paged_cache *cache, const kr_paged_step *step, uint32_t q_heads,
                                           uint32_t tokens);

@@ -7,7 +7,7 @@
 namespace kr {
 namespace {
 
-int check_cache(const kr_paged_cache *c, uint32_t layer) {
+int check_sizes(const kr_paged_cache *c) {
     if (!c) return fail(KR_E_INVALID, "cache: descriptor is NULL");
     if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 192 && c->head_dim != 256)
         return fail(KR_E_UNSUPPORTED, "cache: head_dim=%u is not 64, 96, 128, 192 or 256", c->head_dim);
@@ -18,6 +18,10 @@ int check_cache(const kr_paged_cache *c, uint32_t layer) {
     if (c->layers == 0 || c->layers > 65535) return fail(KR_E_SHAPE, "cache: layers=%u is not 1 .. 65535", c->layers);
     if ((uint64_t)c->pages * c->kv_heads > 0xFFFFFFFFull / (c->page / kPagedUnit))
         return fail(KR_E_SHAPE, "cache: pages=%u of %u heads and %u slots are more than 2^32 units of 16 slots", c->pages, c->kv_heads, c->page);
+    return KR_OK;
+}
+int check_cache(const kr_paged_cache *c, uint32_t layer) {
+    if (int rc = check_sizes(c)) return rc;
     if (layer >= c->layers) return fail(KR_E_SHAPE, "layer=%u of %u", layer, c->layers);
     if (!c->k || !c->v) return fail(KR_E_INVALID, "cache: NULL pointer");
     if (!on(c->k, 16) || !on(c->v, 16)) return fail(KR_E_ALIGN, "cache: k and v must be 16-byte aligned");
@@ -53,11 +57,26 @@ Paged to_paged(const kr_paged_cache *c, uint32_t layer, const kr_paged_step *s) 
 }
 RaggedStep to_step(const kr_paged_step *s, uint32_t tokens) { return RaggedStep{s->starts, s->lengths, s->batch, tokens}; }
 
+int check_heads(const char *name, uint32_t heads) {
+    return heads == 0 || heads > 65535 ? fail(KR_E_SHAPE, "%s: %u heads are not 1 .. 65535", name, heads) : KR_OK;
+}
 int check_rows(const char *name, const uint16_t *x, size_t stride, uint32_t heads, uint32_t head_dim) {
-    if (heads == 0 || heads > 65535) return fail(KR_E_SHAPE, "%s: %u heads are not 1 .. 65535", name, heads);
+    if (int rc = check_heads(name, heads)) return rc;
     if (stride < (size_t)heads * head_dim || stride % 8)
         return fail(KR_E_SHAPE, "%s: a stride of %zu is not a multiple of 8, at least heads * head_dim", name, stride);
     if (!on(x, 16)) return fail(KR_E_ALIGN, "%s must be 16-byte aligned", name);
+    return KR_OK;
+}
+
+// The sizes of an attention call on a cache and step whose own are right.
+int check_attention(const kr_paged_cache *c, const kr_paged_step *s, uint32_t q_heads, uint32_t tokens) {
+    if (q_heads == 0 || q_heads % c->kv_heads)
+        return fail(KR_E_SHAPE, "q_heads=%u is not a positive multiple of kv_heads=%u", q_heads, c->kv_heads);
+    if ((uint64_t)tokens * q_heads > 0x7FFFFFFFull) return fail(KR_E_SHAPE, "tokens * q_heads exceeds 2^31 - 1");
+    if (tokens == 0 || s->batch == 0) return KR_OK;
+    if (int rc = check_heads("q", q_heads)) return rc;
+    if (paged_attention_groups(s->batch, c->kv_heads, q_heads / c->kv_heads, c->head_dim, tokens, s->max_pages * c->page) > kMostGroups)
+        return fail(KR_E_SHAPE, "tokens=%u of %u sequences and %u heads are too many for one launch", tokens, s->batch, q_heads);
     return KR_OK;
 }
 
@@ -131,7 +150,7 @@ int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_st
 
 size_t kr_paged_attention_workspace_bytes(const kr_paged_cache *cache, const kr_paged_step *step, uint32_t q_heads,
                                           uint32_t tokens) {
-    if (!cache || !step || cache->kv_heads == 0 || q_heads == 0 || q_heads % cache->kv_heads || tokens == 0 || step->batch == 0) return 0;
+    if (check_sizes(cache) || check_step(cache, step) || check_attention(cache, step, q_heads, tokens) || tokens == 0 || step->batch == 0) return 0;
     const size_t n = paged_attention_workspace_bytes(step->batch, cache->kv_heads, q_heads / cache->kv_heads, cache->head_dim,
                                                      tokens, step->max_pages * cache->page);
     return (n + 255) / 256 * 256;
@@ -142,9 +161,7 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
                        float scale, uint16_t *out, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = check_cache(cache, layer)) return rc;
     if (int rc = check_step(cache, step)) return rc;
-    if (q_heads == 0 || q_heads % cache->kv_heads)
-        return fail(KR_E_SHAPE, "q_heads=%u is not a positive multiple of kv_heads=%u", q_heads, cache->kv_heads);
-    if ((uint64_t)tokens * q_heads > 0x7FFFFFFFull) return fail(KR_E_SHAPE, "tokens * q_heads exceeds 2^31 - 1");
+    if (int rc = check_attention(cache, step, q_heads, tokens)) return rc;
     if (!(fabsf(scale) < kMaxScale)) return fail(KR_E_INVALID, "scale must be below 2^100 in size");
     if (mask && (words == 0 || words > (1u << 20))) return fail(KR_E_SHAPE, "mask: words=%u is not 1 .. 2^20", words);
     if (!on(mask, 4)) return fail(KR_E_ALIGN, "mask must be 4-byte aligned");
@@ -154,8 +171,6 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
     if (int rc = check_rows("q", q, q_stride, q_heads, cache->head_dim)) return rc;
     if (!on(out, 16) || !on(lse, 4)) return fail(KR_E_ALIGN, "out must be 16-byte aligned, lse 4-byte");
     const Paged c = to_paged(cache, layer, step);
-    if (paged_attention_groups(c.batch, c.heads, q_heads / c.heads, c.D, tokens, c.max_ctx) > kMostGroups)
-        return fail(KR_E_SHAPE, "tokens=%u of %u sequences and %u heads are too many for one launch", tokens, step->batch, q_heads);
     const size_t need = kr_paged_attention_workspace_bytes(cache, step, q_heads, tokens);
     if (need && (!workspace || workspace_bytes < need))
         return fail(KR_E_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace_bytes);

@@ -1,0 +1,27 @@
+"""CPU checks of the paged cache's entry points at the ends of their sizes, and of what their arguments may share (no GPU work here)."""
+import ctypes
+
+import pytest
+
+from test_paged_checks import _cache, _step, kq  # noqa: F401  (kq: the fixture)
+
+
+def _workspace(L, q_heads, tokens, cache=None, step=None):
+    return L.kr_paged_attention_workspace_bytes(ctypes.byref(_cache(**(cache or {}))), ctypes.byref(_step(**(step or {}))), q_heads, tokens)
+
+
+# ---- the workspace of attention
+
+@pytest.mark.parametrize("q_heads,tokens,step", [(4, 2, {}), (16, 200, dict(batch=1, max_pages=100000))], ids=["few", "many"])
+def test_no_workspace_for_what_the_call_refuses(kq, q_heads, tokens, step):
+    """Sizes that attention refuses give 0, and no arithmetic on them (a head_dim of 0 was divided by)."""
+    L = kq.lib()
+    assert _workspace(L, q_heads, tokens, {}, step) > 0
+    for cache in (dict(head_dim=0), dict(head_dim=80), dict(head_dim=512), dict(page=0), dict(page=48), dict(page=8192), dict(kv_heads=0),
+                  dict(kv_heads=65536), dict(pages=0), dict(pages=1 << 31), dict(layers=0)):
+        assert _workspace(L, q_heads, tokens, cache, step) == 0, cache
+    for change in (dict(max_pages=0), dict(max_pages=(1 << 26) + 1), dict(max_pages=1 << 28), dict(batch=65536)):  # 2^28 pages of 16: 2^32 slots
+        assert _workspace(L, q_heads, tokens, {}, dict(step, **change)) == 0, change
+    assert _workspace(L, 0, tokens, {}, step) == 0 and _workspace(L, 3, tokens, {}, step) == 0
+    assert _workspace(L, 65536, tokens, {}, step) == 0 and _workspace(L, q_heads, 1 << 30, {}, step) == 0
+    assert L.kr_paged_attention_workspace_bytes(None, None, q_heads, tokens) == 0

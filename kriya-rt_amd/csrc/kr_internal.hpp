@@ -451,6 +451,7 @@ struct PagedAttnArgs {
     // a row may see all new tokens of its sequence
     __host__ __device__ bool sees_all() const { return mask != nullptr; }
 };
+// 256 threads each
 uint64_t paged_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
 size_t paged_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx);
 hipError_t launch_paged_attention(const PagedAttnArgs &a, hipStream_t s);

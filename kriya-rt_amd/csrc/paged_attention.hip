@@ -190,8 +190,9 @@ __device__ __forceinline__ void landed() {
 }
 
 // Groups of four waves: two where the registers hold two waves a SIMD, over every other pair of blocks each.
+constexpr uint32_t many_groups(uint32_t D) { return D <= 128 ? 2 : 1; }
 template <int NS>
-constexpr uint32_t kManyGroups = NS <= 4 ? 2 : 1;
+constexpr uint32_t kManyGroups = many_groups(32 * NS);
 
 template <int NS>
 __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(PagedAttnArgs a, Split split, uint32_t slots) {
@@ -803,7 +804,7 @@ size_t part_floats(const AttnPlan &p, uint32_t kv_heads, uint32_t D) { return (s
 
 uint64_t paged_attention_groups(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {
     const AttnPlan p = plan_of(batch, kv_heads, group, D, tokens, max_ctx);
-    return (uint64_t)p.grid * (p.few ? 1 : kv_heads);  // (few: heads are another dimension)
+    return (uint64_t)p.grid * (p.few ? 1 : kv_heads * many_groups(D));  // (few: heads are another dimension)
 }
 
 size_t paged_attention_workspace_bytes(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, uint32_t tokens, uint32_t max_ctx) {

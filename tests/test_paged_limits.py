@@ -25,3 +25,18 @@ def test_no_workspace_for_what_the_call_refuses(kq, q_heads, tokens, step):
     assert _workspace(L, 0, tokens, {}, step) == 0 and _workspace(L, 3, tokens, {}, step) == 0
     assert _workspace(L, 65536, tokens, {}, step) == 0 and _workspace(L, q_heads, 1 << 30, {}, step) == 0
     assert L.kr_paged_attention_workspace_bytes(None, None, q_heads, tokens) == 0
+
+
+@pytest.mark.parametrize("d,tiles", [(64, 8388607), (128, 8388607), (192, 16777215), (256, 16777215)])
+def test_launches_of_too_many_threads_are_refused(kq, d, tiles):
+    """A launch has fewer than 2^32 threads: tiles of 128 rows by 512 threads up to a head_dim of 128, by 256 above.  (The call with
+    sizes that fit goes on to its pointers.)"""
+    L, c = kq.lib(), ctypes.byref(_cache(kv_heads=1, head_dim=d))
+    s = ctypes.byref(_step(batch=1, starts=0x50000))
+
+    def call(tokens):
+        return L.kr_paged_attention(c, 0, s, None, d, 1, tokens, None, 0, 0.125, None, None, None, 0, None)
+    rows = 128 * (tiles - 1)  # and one tile that is not full
+    assert call(rows) == call(rows + 127) == kq.KR_E_INVALID
+    if rows + 128 < 1 << 31:
+        assert call(rows + 128) == kq.KR_E_SHAPE

@@ -231,7 +231,7 @@ __device__ __forceinline__ bool find_tile(const A &a, const Split &w, uint32_t t
     }
     return true;
 }
-// parts of a tile of few rows: at most `target` and one, and target is at most 1024
+// parts of a tile in the wide join: at most `target` and one; that join is for so few tiles that target is at most 1024
 constexpr uint32_t kMostParts = 1056;
 // Where a part's normalised O of a row lies in the workspace, in rows; m and l of all rows lie behind them, in pairs.
 template <class A>

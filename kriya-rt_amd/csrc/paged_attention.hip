@@ -593,7 +593,7 @@ __device__ __forceinline__ void load_few(FewBlock<NS> &f, const Paged &c, uint32
 
 // kOnce: what is read is read once: past the caches (nontemporal).
 template <int NS, bool kOnce>
-__global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAttnArgs a, Split split) {
+__global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAttnArgs a, Split split, uint32_t slots) {
     constexpr uint32_t D = 32 * NS;
     __shared__ float sm[kFewWaves][kFewRows], sl[kFewWaves][kFewRows];
     __shared__ __align__(16) float so[kFewWaves][kFewRows][D + 4];
@@ -744,11 +744,11 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             if (L == 0.0f && M > kSeenBase) acc = f32x4{1, 1, 1, 1} * (none = __builtin_nanf(""));
             *reinterpret_cast<u32x2 *>(a.out + to * D + d) = pack4(acc.x, acc.y, acc.z, acc.w);
             if (a.lse && d == 0) a.lse[to] = L == 0.0f ? none : (M + __log2f(L)) * kLn2;
-        } else {
+        } else if (idx < slots) {  // (where the tiles are `target` and more, none is split: only `target` parts have a place)
             const size_t to = part_at(a, split, idx, head, row);
             *reinterpret_cast<f32x4 *>(a.part + to * D + d) = acc;
             if (d == 0) {
-                float *ml = a.part + (size_t)gridDim.x * a.c.heads * kFewRows * D + 2 * to;
+                float *ml = a.part + (size_t)slots * a.c.heads * kFewRows * D + 2 * to;
                 ml[0] = M;
                 ml[1] = L;
             }
@@ -784,7 +784,8 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
         // 32/8 heads of 128, 89 us -> 81; below, a second round costs more: 40 of 4000 119 -> 125)
         const uint32_t held = (D <= 64 ? 768 : (D <= 128 ? 512 : 256)) / kv_heads;
         p.split.target = p.tiles < held ? held : std::max(2 * held, std::min(p.tiles, 1024u));
-        p.slots = p.grid = std::max(p.split.target, p.tiles);
+        p.grid = std::max(p.split.target, p.tiles);
+        p.slots = p.split.target;
     } else {
         p.split.unit = D <= 128 ? 4 : 2;  // a stage
         // Contexts that a table can hold in so few blocks are not split: the join's launch takes longer (split and whole, us, D 128, 2 heads:
@@ -818,8 +819,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs &args, hipStream_t s) {
     a.per = reinterpret_cast<uint32_t *>(a.part + part_floats(p, a.c.heads, a.c.D));
     const auto launch = [&](auto ns) -> hipError_t {
         constexpr int NS = decltype(ns)::value;
-        if (p.few && p.once) paged_few_kernel<NS, true><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
-        else if (p.few) paged_few_kernel<NS, false><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
+        if (p.few && p.once) paged_few_kernel<NS, true><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
+        else if (p.few) paged_few_kernel<NS, false><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
         else paged_many_kernel<NS><<<dim3(p.grid * a.c.heads), 256 * kManyGroups<NS>, 0, s>>>(a, p.split, p.slots);
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;

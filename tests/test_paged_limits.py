@@ -40,3 +40,13 @@ def test_launches_of_too_many_threads_are_refused(kq, d, tiles):
     assert call(rows) == call(rows + 127) == kq.KR_E_INVALID
     if rows + 128 < 1 << 31:
         assert call(rows + 128) == kq.KR_E_SHAPE
+
+
+@pytest.mark.parametrize("batch", [64, 600, 1100, 4096, 16384, 65535])
+@pytest.mark.parametrize("kv,group,d", [(1, 4, 64), (8, 4, 128), (2, 8, 256), (8, 16, 64)])
+def test_the_workspace_of_a_large_batch_is_bounded(kq, batch, kv, group, d):
+    """One token each: no more parts have a place than a launch may split its tiles into (at most 1536 a kv head), however many
+    sequences there are."""
+    most = 1536 * kv * 16 * (d + 2) * 4 + 512
+    for starts in (None, 0x50000):
+        assert 0 < _workspace(kq.lib(), kv * group, batch, dict(kv_heads=kv, head_dim=d), dict(batch=batch, max_pages=1000, starts=starts)) <= most

@@ -145,8 +145,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, ui
             for (uint32_t x = 1; x < kLanes; x *= 2) sum += __shfl_xor(sum, (int)x);
             f = rsqrtf(sum * (1.0f / D) + a.eps);
             float w0[8], w1[8];
-            load8(weight + (mine ? 8 * u0 : 0u), w0);
-            load8(weight + (mine ? 8 * u1 : 0u), w1);
+            load8_at(weight + (mine ? 8 * u0 : 0u), w0);
+            load8_at(weight + (mine ? 8 * u1 : 0u), w1);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 lo[e] = lo[e] * f * w0[e];

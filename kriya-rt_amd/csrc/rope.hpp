@@ -12,14 +12,19 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c, float s, 
 }
 
 // Eight consecutive dims as floats, and back (bf16 rounded to nearest even).
-__device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+__device__ __forceinline__ void load8(const u32x4 &w, float (&v)[8]) {
     const uint32_t W[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         v[2 * e] = __uint_as_float(W[e] << 16);
         v[2 * e + 1] = __uint_as_float(W[e] & 0xFFFF0000u);
     }
+}
+__device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) { load8(*reinterpret_cast<const u32x4 *>(p), v); }
+// p: at any element (one load all the same: memory takes 16 bytes at any address)
+__device__ __forceinline__ void load8_at(const uint16_t *p, float (&v)[8]) {
+    typedef u32x4 Loose __attribute__((aligned(2)));
+    load8(*reinterpret_cast<const Loose *>(p), v);
 }
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
     const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];

@@ -12,7 +12,7 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c, float s, 
 }
 
 // Eight consecutive dims as floats, and back (bf16 rounded to nearest even).
-__device__ __forceinline__ void load8(const u32x4 &w, float (&v)[8]) {
+__device__ __forceinline__ void load8(u32x4 w, float (&v)[8]) {
     const uint32_t W[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

@@ -60,14 +60,16 @@ typedef struct kr_head_norm {
 /* Appends k, v (bf16 [tokens, kv_heads, head_dim], tokens kv_stride elements apart) to the pages of `layer`.  norm, rope (host
  * pointers, may be NULL): k is normalised, then rotated by the table row of its token's position (kr_rope as in kriya_kv8.h), in f32,
  * and rounded once; so is q (bf16 [tokens, q_heads, head_dim], q_stride elements apart; NULL: none) into q_out (the same stride;
- * may equal q).  One launch.  k, v, q, q_out 16-byte aligned, strides multiples of 8; q needs norm or rope; rope->inverse
+ * may equal q).  q_out and the layer's pages lie apart from each other and from all else that is read; rows may lie in one another's
+ * gaps (k, v and q of a fused projection).  One launch.  k, v, q, q_out 16-byte aligned, strides multiples of 8; q needs norm or rope; rope->inverse
  * must be 0. */
 int kr_paged_append(const kr_paged_cache *cache, uint32_t layer, const kr_paged_step *step, const kr_head_norm *norm,
                     const kr_rope *rope, const uint16_t *k, const uint16_t *v, size_t kv_stride, const uint16_t *q,
                     uint16_t *q_out, size_t q_stride, uint32_t q_heads, uint32_t tokens, void *stream);
 
 /* Reads slots first[b] .. first[b] + count - 1 of each sequence (first: u32 [batch], NULL for 0) into k_out, v_out [batch, count,
- * kv_heads, head_dim] of dtype (either may be NULL); slots at or beyond lengths[b], and those of no page, give zeros. */
+ * kv_heads, head_dim] of dtype (either may be NULL); slots at or beyond lengths[b], and those of no page, give zeros.  Both
+ * lie apart from each other and from what is read. */
 int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_step *step, const uint32_t *first,
                   uint32_t count, void *k_out, void *v_out, int dtype, void *stream);
 
@@ -78,7 +80,7 @@ int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_st
  * token's row of `mask` (u32 [tokens, words], bit j % 32 of word j / 32; nodes from 32 words on are not seen): a tree of drafted
  * tokens (kr_tree_plan makes its masks), a chain, or any other rule.
  *   q: bf16 [tokens, q_heads, head_dim], tokens q_stride elements apart (a multiple of 8); out: bf16, contiguous; both 16-byte
- *   aligned and apart from each other; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
+ *   aligned; out, lse and the workspace lie apart from one another and from what is read; lse f32 [tokens, q_heads] or NULL; q_heads a multiple of kv_heads; |scale| < 2^100 (may
  *   be negative or 0).
  * Products are bf16 with sums in f32; the probabilities enter the second product as bf16 (half a step is 2^-8 of each), where rows are
  * few as two of them (2^-16); maxima, sums and joins are f32, for which |scale| sum |q| |K_p| must stay below 2^125 and finite values

@@ -1,6 +1,7 @@
 // api_checks.hpp — checks that the entry points of the caches share.
 #pragma once
 
+#include <algorithm>
 #include <initializer_list>
 
 #include "kriya_kv8.h"
@@ -13,18 +14,31 @@ constexpr uint64_t kMostGroups = 0xFFFFFFFFull / 256;
 
 inline bool on(const void *p, size_t a) { return (uintptr_t)p % a == 0; }
 
-// Memory of a call: what one argument points to.
+// Memory of a call: what one argument points to, `bytes` of it, or of each of `rows` rows, `stride` bytes from one to the next.
 struct Range {
     const char *name;
     const void *at;
-    size_t bytes;
+    size_t bytes, rows = 1, stride = 0;
+    size_t whole() const { return (rows - 1) * stride + bytes; }
 };
+// Whether any byte is in both.
+inline bool meet(const Range &x, const Range &y) {
+    const auto a = (uintptr_t)x.at, b = (uintptr_t)y.at;
+    if (!x.at || !y.at || !x.bytes || !y.bytes || !x.rows || !y.rows || a >= b + y.whole() || b >= a + x.whole()) return false;
+    if (x.rows == 1 && y.rows == 1) return true;
+    if (x.rows > 1 && y.rows > 1 && x.stride != y.stride) {  // row by row
+        if (x.rows > y.rows) return meet(y, x);
+        for (size_t i = 0; i < x.rows; ++i)
+            if (meet(Range{x.name, (const char *)x.at + i * x.stride, x.bytes}, y)) return true;
+        return false;
+    }
+    // row i of x and row j of y meet where (i - j) stride lies between b - a - x.bytes and b - a + y.bytes
+    const auto step = (int64_t)(x.rows > 1 ? x.stride : y.stride), low = (int64_t)(b - a) - (int64_t)x.bytes, high = (int64_t)(b - a) + (int64_t)y.bytes;
+    const auto below = [&](int64_t v) { return v / step - (v % step < 0); };  // v / step, rounded down
+    return std::max(below(low) + 1, 1 - (int64_t)y.rows) <= std::min(-below(-high) - 1, (int64_t)x.rows - 1);
+}
 // Written memory must not be that of any other argument.
 inline int check_apart(std::initializer_list<Range> written, std::initializer_list<Range> read) {
-    const auto meet = [](const Range &x, const Range &y) {
-        const auto a = (uintptr_t)x.at, b = (uintptr_t)y.at;
-        return x.at && y.at && a < b + y.bytes && b < a + x.bytes;
-    };
     for (auto x = written.begin(); x != written.end(); ++x) {
         for (auto y = written.begin(); y != x; ++y)
             if (meet(*x, *y)) return fail(KR_E_INVALID, "%s and %s overlap", y->name, x->name);

@@ -49,6 +49,19 @@ int check_pointers(const kr_paged_step *s, uint32_t tokens) {
     return check_sequences(s->starts, s->lengths, s->batch, tokens);
 }
 
+// Keys or values of `layers` layers from one on.
+Range pool_of(const char *name, const uint16_t *at, const kr_paged_cache *c, uint32_t layer, uint32_t layers) {
+    const size_t each = (size_t)c->pages * c->kv_heads * c->page * c->head_dim;
+    return Range{name, at + layer * each, layers * each * 2};
+}
+// Rows of heads.
+Range rows_of(const char *name, const uint16_t *at, uint32_t rows, uint32_t heads, uint32_t head_dim, size_t stride) {
+    return Range{name, at, (size_t)heads * head_dim * 2, rows, stride * 2};
+}
+Range lengths_of(const kr_paged_step *s) { return Range{"lengths", s->lengths, (size_t)s->batch * 4}; }
+Range starts_of(const kr_paged_step *s) { return Range{"starts", s->starts, ((size_t)s->batch + 1) * 4}; }
+Range table_of(const kr_paged_step *s) { return Range{"table", s->table, (size_t)s->batch * s->max_pages * 4}; }
+
 Paged to_paged(const kr_paged_cache *c, uint32_t layer, const kr_paged_step *s) {
     const size_t at = (size_t)layer * c->pages * c->kv_heads * c->page * c->head_dim;
     uint32_t shift = 0;
@@ -128,6 +141,16 @@ int kr_paged_append(const kr_paged_cache *cache, uint32_t layer, const kr_paged_
     a.q_stride = q_stride;
     a.q_heads = q_heads;
     if (paged_append_groups(a) > kMostGroups) return fail(KR_E_SHAPE, "tokens=%u are too many for one launch", tokens);
+    // (a workgroup's rows are written while others read theirs)
+    const uint32_t D = cache->head_dim;
+    if (int rc = check_apart({rows_of("q_out", q ? q_out : nullptr, tokens, q_heads, D, q_stride),
+                              pool_of("cache k", cache->k, cache, layer, 1), pool_of("cache v", cache->v, cache, layer, 1)},
+                             {rows_of("q", q == q_out ? nullptr : q, tokens, q_heads, D, q_stride),
+                              rows_of("k", k, tokens, cache->kv_heads, D, kv_stride), rows_of("v", v, tokens, cache->kv_heads, D, kv_stride),
+                              {"q_weight", a.q_norm, D * 2ul}, {"k_weight", a.k_norm, D * 2ul},
+                              {"positions", a.rope.positions, tokens * 4ul}, {"cos_sin", a.rope.cos_sin, (size_t)a.rope.rows * a.rope.rotary_dim * 4},
+                              table_of(step), lengths_of(step), starts_of(step)}))
+        return rc;
     return hip_status(launch_paged_append(a, (hipStream_t)stream), "kr_paged_append");
 }
 
@@ -143,6 +166,11 @@ int kr_paged_read(const kr_paged_cache *cache, uint32_t layer, const kr_paged_st
     if (!on(first, 4)) return fail(KR_E_ALIGN, "first must be 4-byte aligned");
     if ((uint64_t)count * cache->kv_heads * (cache->head_dim / 8) > kMostGroups * 256)
         return fail(KR_E_SHAPE, "count=%u is too large for one launch", count);
+    const size_t bytes = (size_t)step->batch * count * cache->kv_heads * cache->head_dim * (dtype == KR_DTYPE_F32 ? 4 : 2);
+    if (int rc = check_apart({{"k_out", k_out, bytes}, {"v_out", v_out, bytes}},
+                             {pool_of("cache k", cache->k, cache, layer, 1), pool_of("cache v", cache->v, cache, layer, 1), table_of(step),
+                              lengths_of(step), {"first", first, step->batch * 4ul}}))
+        return rc;
     return hip_status(launch_paged_read(to_paged(cache, layer, step), to_step(step, 0), first, count, k_out, v_out,
                                         dtype == KR_DTYPE_F32, (hipStream_t)stream),
                       "kr_paged_read");
@@ -177,8 +205,9 @@ int kr_paged_attention(const kr_paged_cache *cache, uint32_t layer, const kr_pag
     if (!on(workspace, 16)) return fail(KR_E_ALIGN, "workspace must be 16-byte aligned");
     const size_t rows = (size_t)tokens * q_heads;
     if (int rc = check_apart({{"out", out, rows * cache->head_dim * 2}, {"lse", lse, rows * 4}, {"workspace", workspace, need}},
-                             {{"q", q, ((tokens - 1) * q_stride + (size_t)q_heads * cache->head_dim) * 2},
-                              {"mask", mask, (size_t)tokens * words * 4}}))
+                             {rows_of("q", q, tokens, q_heads, cache->head_dim, q_stride), {"mask", mask, (size_t)tokens * words * 4},
+                              pool_of("cache k", cache->k, cache, layer, 1), pool_of("cache v", cache->v, cache, layer, 1), table_of(step),
+                              lengths_of(step), starts_of(step)}))
         return rc;
     PagedAttnArgs a{};
     a.c = c;
@@ -226,8 +255,8 @@ int kr_paged_commit(const kr_paged_cache *cache, const kr_paged_step *step, cons
     // (every layer's workgroups read what the first one's write)
     const size_t all = (size_t)tokens * 4, each = (size_t)step->batch * 4;
     if (int rc = check_apart({{"path", path, each * max_path}, {"counts", counts, each}, {"next", next, each}, {"new_lengths", new_lengths, each}},
-                             {{"tokens", drafted, all}, {"parents", parents, all}, {"targets", targets, all}, {"lengths", step->lengths, each},
-                              {"starts", step->starts, each + 4}, {"table", step->table, each * step->max_pages}}))
+                             {{"tokens", drafted, all}, {"parents", parents, all}, {"targets", targets, all}, lengths_of(step), starts_of(step),
+                              table_of(step), pool_of("cache k", cache->k, cache, 0, cache->layers), pool_of("cache v", cache->v, cache, 0, cache->layers)}))
         return rc;
     PagedCommitArgs a{};
     a.c = to_paged(cache, 0, step);

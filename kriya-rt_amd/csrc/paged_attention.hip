@@ -177,11 +177,14 @@ constexpr uint32_t kManyRows = 128;
 // The n-th KB from `from` on into LDS, past the registers: 16 bytes a lane, lane l's to byte lds + 1024 n + 16 l, lds the same in all lanes
 // (the instruction's offset counts on both sides).  In assembly, since the compiler would have every later read of LDS wait for it:
 // whoever reads what it writes waits for vmcnt(0) and a barrier first.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is a register that the compiler uses for itself alone: that is why it is named)
 template <int N>
 __device__ __forceinline__ void to_lds(const uint16_t *from, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off offset:%2"
-                 ::"s"(lds + N / 4 * 4096), "v"(from + N / 4 * 2048), "n"(N % 4 * 1024) : "memory");
+                 ::"s"(lds + N / 4 * 4096), "v"(from + N / 4 * 2048), "n"(N % 4 * 1024) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 // All but the last N of this wave's have landed (loads end in order).
 template <int N>

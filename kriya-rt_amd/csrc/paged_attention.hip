@@ -89,6 +89,11 @@ struct Units {
     }
     // before the first use: what is loaded between has the pages' way to come as well
     __device__ __forceinline__ void begin() { take(0, ahead[0]); }
+    // ... of all once more
+    __device__ __forceinline__ void restart() {
+        ahead[1] = look(1);
+        begin();
+    }
     // of the i-th unit; units in rising order, each set entered at its first
     __device__ __forceinline__ uint32_t at(uint32_t i) const { return (uint32_t)__builtin_amdgcn_readlane((int)at_lane, (int)(i & 63)); }
     // whether the n units from i on have no page, as bits
@@ -117,7 +122,9 @@ __device__ __forceinline__ float row_follow(RowSums &r, float top) {
 // ---- values that are infinite or NaN in slots that some rows do not see
 //
 // A product with a probability of 0 would bring them into those rows.  In a block that some row does not see whole, they are
-// therefore taken out of the operand, and added to the rows that see them one slot at a time.
+// therefore taken out of the operand, and added to the rows that see them one slot at a time.  (Where probabilities are two bf16, the
+// second one, of either sign or 0, would make NaN of an infinity that every row sees, too: a wave that ends with a NaN takes its blocks
+// once more, all of them so.)
 
 // Takes them out of a 16-byte piece of values; returns bit 15 and 31 of a word where its low and high value is one.
 __device__ __forceinline__ u32x4 take_out(u32x4 &v) {
@@ -596,7 +603,7 @@ __device__ __forceinline__ void load_few(FewBlock<NS> &f, const Paged &c, uint32
 
 // kOnce: what is read is read once: past the caches (nontemporal).
 template <int NS, bool kOnce>
-__global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAttnArgs a, Split split, uint32_t slots) {
+__global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAttnArgs a, Split split) {
     constexpr uint32_t D = 32 * NS;
     __shared__ float sm[kFewWaves][kFewRows], sl[kFewWaves][kFewRows];
     __shared__ __align__(16) float so[kFewWaves][kFewRows][D + 4];
@@ -608,7 +615,7 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
     const uint32_t r0 = kFewRows * w.tile, r = r0 + r16;
     const bool live = r < w.rows;
     const Sight sight = sight_of(a, s, r, live);
-    const uint32_t clear = clear_of(a, s, r0);
+    uint32_t clear = clear_of(a, s, r0);
     const uint32_t first = w.part * w.per, end = min(first + w.per, (w.most + 31) / 32), b = w.b;
     const uint32_t t = s.t0 + r / a.group, qh = head * a.group + r % a.group;
     uint32_t blk = first + wave;
@@ -703,14 +710,30 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             }
         }
     };
-    for (; blk < end; blk += kAhead * kFewWaves) {
+    for (;;) {
+        for (; blk < end; blk += kAhead * kFewWaves) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t at = blk + i * kFewWaves;
-            if (at >= end) break;
-            step(f[i], at);
-            if (at + kAhead * kFewWaves < end) ask(f[i]);
+            for (uint32_t i = 0; i < kAhead; ++i) {
+                const uint32_t at = blk + i * kFewWaves;
+                if (at >= end) break;
+                step(f[i], at);
+                if (at + kAhead * kFewWaves < end) ask(f[i]);
+            }
         }
+        float nan = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) nan += (o[d][0] + o[d][1]) + (o[d][2] + o[d][3]);
+        if (__builtin_expect(clear == 0 || !__any(nan != nan), 1)) break;
+        clear = 0;  // every block as one that some row does not see whole
+        sums = RowSums{};
+#pragma unroll
+        for (int d = 0; d < 2 * NS; ++d) o[d] = f32x4{0, 0, 0, 0};
+        blk = first + wave;
+        asked = 0;
+        units.restart();
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i)
+            if (blk + i * kFewWaves < end) ask(f[i]);
     }
     float l = sums.l + xchg32(sums.l, lane);
     l += xchg16(l, lane);
@@ -747,11 +770,11 @@ __global__ __launch_bounds__(256, kFewGroups<NS>) void paged_few_kernel(PagedAtt
             if (L == 0.0f && M > kSeenBase) acc = f32x4{1, 1, 1, 1} * (none = __builtin_nanf(""));
             *reinterpret_cast<u32x2 *>(a.out + to * D + d) = pack4(acc.x, acc.y, acc.z, acc.w);
             if (a.lse && d == 0) a.lse[to] = L == 0.0f ? none : (M + __log2f(L)) * kLn2;
-        } else if (idx < slots) {  // (where the tiles are `target` and more, none is split: only `target` parts have a place)
+        } else if (idx < split.target) {  // (where the tiles are `target` and more, none is split: only `target` parts have a place)
             const size_t to = part_at(a, split, idx, head, row);
             *reinterpret_cast<f32x4 *>(a.part + to * D + d) = acc;
             if (d == 0) {
-                float *ml = a.part + (size_t)slots * a.c.heads * kFewRows * D + 2 * to;
+                float *ml = a.part + (size_t)split.target * a.c.heads * kFewRows * D + 2 * to;
                 ml[0] = M;
                 ml[1] = L;
             }
@@ -822,8 +845,8 @@ hipError_t launch_paged_attention(const PagedAttnArgs &args, hipStream_t s) {
     a.per = reinterpret_cast<uint32_t *>(a.part + part_floats(p, a.c.heads, a.c.D));
     const auto launch = [&](auto ns) -> hipError_t {
         constexpr int NS = decltype(ns)::value;
-        if (p.few && p.once) paged_few_kernel<NS, true><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
-        else if (p.few) paged_few_kernel<NS, false><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split, p.slots);
+        if (p.few && p.once) paged_few_kernel<NS, true><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
+        else if (p.few) paged_few_kernel<NS, false><<<dim3(p.grid, a.c.heads), 256, 0, s>>>(a, p.split);
         else paged_many_kernel<NS><<<dim3(p.grid * a.c.heads), 256 * kManyGroups<NS>, 0, s>>>(a, p.split, p.slots);
         if (hipError_t e = hipGetLastError()) return e;
         if (p.split.target == 0) return hipSuccess;

@@ -177,7 +177,7 @@ __device__ __forceinline__ uint32_t query_sign(float scale) { return scale < 0.0
 // last from issuing for 11 cycles.  So exponentials, maxima and rounding are laid between products (apart, a prompt of 3907, 16/2 heads of
 // 128, took 198 us), and up to D 128 a second group of four waves, over other slots and half a stage apart, takes what the first leaves;
 // above, the registers hold one wave a SIMD.  A tile's start and end are 11 us (work, pages, queries and the first stage 6, the groups'
-// sums 1, the next workgroup's launch 4): that prompt takes 78 us (804 TFLOP/s); 600 tokens over up to 12000 in four sequences, 10/2
+// sums 1, the next workgroup's launch 4): that prompt takes 78 to 81 us (804 to 771 TFLOP/s, from machine to machine); 600 tokens over up to 12000 in four sequences, 10/2
 // heads of 256, 97 and their join 9; 250 nodes of trees over up to 5000 in eight, 16/2 heads of 128, 26 and 7.
 constexpr uint32_t kManyRows = 128;
 
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(256 * kManyGroups<NS>, 1) void paged_many_kernel(Pa
 // On v_mfma_f32_16x16x32_bf16, keys and values straight from memory to the operands' registers, 16 bytes a lane in whole cache lines.
 // Tile t of a block's keys is slots 8 t .. 8 t + 7 of both units: a lane (column l & 15, g = l >> 4) then holds after the first product
 // the slots 8 t + 4 (g & 1) + j of unit g >> 1, of both tiles the 8 slots of one 16-byte piece of values.
-// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64, 102 us for 595 MB, 5.8 TB/s (a copy 5.2, a plain read 7.0); one of 131072,
+// Bound by bytes: 48 sequences up to 8000, 32/8 heads of 64, 103 us for 595 MB, 5.8 TB/s (a copy 5.2, a plain read 7.0); one of 131072,
 // 16/2 heads of 128, 25 us for 134 MB; by latency where there are few: five sequences up to 3000 8.4 us.
 constexpr uint32_t kFewRows = 16, kFewWaves = 4;
 template <int NS>
@@ -801,7 +801,9 @@ AttnPlan plan_of(uint32_t batch, uint32_t kv_heads, uint32_t group, uint32_t D, 
     // tiles of every sequence: at most one that is not full each
     p.tiles = (uint32_t)(rows / p.split.rows) + std::min(batch, tokens);
     if (p.few) {
-        // Keys and values that one tile reads, and more of them than may still be in the caches from the last call (us, with and without,
+        // Keys and values that one tile reads in the mean, and more of them than may still be in the caches from the last call (a chunk among
+        // decoded tokens reads its own once a tile all the same: 63 and one of 193, 32/8 heads of 64, contexts of 4000 to 8000, 259 us, in two
+        // calls 174.  us, with and without,
         // over changing layers: 48 sequences up to 8000, 32/8 heads of 64, 110 and 122; 4 of 4000, 16/2 heads of 128, 16.0 and 16.3, one
         // 14.4 and 13.6; 8 of 32 rows over 300 16.7 and 14.1).
         p.once = rows <= 16ull * batch && (uint64_t)batch * max_ctx * kv_heads * D * 4 >= 1u << 24;
@@ -856,8 +858,7 @@ hipError_t launch_paged_attention(const PagedAttnArgs &args, hipStream_t s) {
             uint32_t per_group = kJoinRowThreads / 64;
             while (per_group < p.split.rows && (uint64_t)p.tiles * a.c.heads * (p.split.rows / per_group) > 2048) per_group *= 2;
             const dim3 grid(p.tiles * (p.split.rows / per_group), a.c.heads);
-            if (p.few) attn_join_kernel<PagedAttnArgs, NS, Parts::even, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
-            else attn_join_kernel<PagedAttnArgs, NS, Parts::even, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
+            attn_join_kernel<PagedAttnArgs, NS, Parts::even, false, true><<<grid, kJoinRowThreads, 0, s>>>(a, p.split, p.slots, per_group);
         }
         return hipGetLastError();
     };

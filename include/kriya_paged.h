@@ -50,8 +50,8 @@ typedef struct kr_paged_step {
     const uint32_t *starts, *lengths;
 } kr_paged_step;
 
-/* RMS norm of each head before its rotation: x rsqrt(mean(x^2) + eps) w, w bf16 [head_dim], at any element of a tensor.  A weight may be
- * NULL: not normalised.  (fused_qknorm_rope_and_kv_append, paged_gqa_and_deltanet.metal:115-222) */
+/* RMS norm of each head before its rotation: x rsqrt(mean(x^2) + eps) w, the squares summed in f32, w bf16 [head_dim], at any element
+ * of a tensor.  A weight may be NULL: not normalised.  (fused_qknorm_rope_and_kv_append, paged_gqa_and_deltanet.metal:115-222) */
 typedef struct kr_head_norm {
     const uint16_t *q_weight, *k_weight;
     float eps;
